@@ -76,10 +76,29 @@ SIGNATURES = {
     "affb_sine_embed": [_p, _i64, _i64, _p, _p, _p, _i32, _p],
     "affb_relu_dropout_fwd": [_p, _i32, _i64, _f32, _u32, _p, _p],
     "affb_relu_dropout_bwd": [_p, _p, _i32, _i64, _f32, _p, _p],
+    "affb_linear_fwd": [_p, _p, _p, _i32, _p, _i32, _i32, _i32, _i64, _i64, _i64, _p, _i32, _p, _p, _i64, _p],
+    "affb_linear_bwd": [_p, _i32, _p, _p, _p, _i32, _i32, _i64, _i64, _i64, _p, _p, _p, _i32, _p, _i64, _p],
+    "affb_linear_e4m3": [_p, _p, _p, _p, _p, _p, _i32, _i32, _i64, _i64, _i64, _p, _i32, _p, _i64, _p],
+    "affb_linear_status": [_p],
+    "affb_rms_norm_fwd": [_p, _i32, _p, _i32, _p, _i64, _p, _f32, _i64, _i64, _p, _p, _p, _i32, _p, _p, _p],
+    "affb_quantize_e4m3": [_p, _i32, _i64, _i64, _p, _p, _p],
+    "affb_rms_norm_bwd": [_p, _i32, _p, _p, _i32, _p, _p, _p, _i64, _i64, _i64, _p, _p, _i32, _p, _p, _i64, _p],
+    "affb_bucket_bias_fwd": [_p, _i32, _p, _i32, _i32, _p, _p, _i32, _i32, _p, _i64, _i64, _i64, _i64, _i64, _p,
+                             _i32, _p],
+    "affb_bucket_bias_bwd": [_p, _i32, _p, _i32, _i32, _p, _p, _i32, _i32, _p, _i64, _i64, _i64, _i64, _i64, _p,
+                             _i32, _p, _i64, _p],
+}
+# workspace-size functions of the operators above -> argtypes (they return int64)
+SIZES = {
+    "affb_linear_fwd_workspace_bytes": [_i32, _i64, _i64, _i64],
+    "affb_linear_bwd_workspace_bytes": [_i32, _i64, _i64, _i64],
+    "affb_linear_e4m3_workspace_bytes": [_i64, _i64, _i64],
+    "affb_rms_norm_bwd_workspace_bytes": [_i64, _i64],
+    "affb_bucket_bias_bwd_workspace_bytes": [_i32, _i32, _i32, _i64, _i64, _i64, _i64],
 }
 OTHER_SYMBOLS = ["affb_last_error", "affb_abi_version", "affb_deform_workspace_bytes",
                  "affb_deform_noalloc_max_scratch_bytes", "affb_nbhd_attn_bwd_workspace_bytes",
-                 "affb_knn2d_workspace_bytes", "affb_nbhd_tile_plan_bytes"]
+                 "affb_knn2d_workspace_bytes", "affb_nbhd_tile_plan_bytes", *SIZES]
 
 
 def library_path() -> Path:
@@ -117,6 +136,10 @@ def lib():
             fn = getattr(l, name)
             fn.argtypes = args
             fn.restype = C.c_int
+        for name, args in SIZES.items():
+            fn = getattr(l, name)
+            fn.argtypes = args
+            fn.restype = _i64
         _lib = l
         return l
 
@@ -132,6 +155,28 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = lib().affb_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed (code {rc}): {msg}")
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with `device` current (kernels launch on the current device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
+
+
+def workspace(name: str, device, *args):
+    """Uninitialised device memory of the size the library's function `name`
+    asks for (None where it needs none), from the current stream's pool."""
+    n = getattr(lib(), name)(*args)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
+
+
+def dense(t: torch.Tensor) -> torch.Tensor:
+    """`t` contiguous and 16-byte aligned (itself where it already is)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def ptr(t):

@@ -1,0 +1,78 @@
+// Activations of the matrix product's epilogue and their derivatives, fp32.
+#pragma once
+
+#include "common.cuh"
+
+namespace affb {
+
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// Phi(-a) of the normal distribution for a >= 0 as 2^p(a): log2 Phi(-a) is
+// close to a parabola, and the degree-7 polynomial below (weighted least
+// squares on [0, 9], weight a Phi(-a)) leaves |a| * error <= 1.3e-7 and a
+// relative error of Phi below 1e-3 down to Phi(-9); the leading coefficient is
+// negative, so the tail goes to 0.  One exponential and 7 FMAs, against erff's
+// branches.
+__device__ __forceinline__ float normal_tail(float a) {
+  float p = -1.41679106e-06f;
+  p = fmaf(p, a, 5.36095686e-05f);
+  p = fmaf(p, a, -0.000875660044f);
+  p = fmaf(p, a, 0.00834226329f);
+  p = fmaf(p, a, -0.0537395962f);
+  p = fmaf(p, a, -0.458566278f);
+  p = fmaf(p, a, -1.15125847f);
+  p = fmaf(p, a, -0.999988079f);
+  return exp2_approx(p);
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+  if constexpr (ACT == AFFB_ACT_RELU) {
+    return max_nan(z, 0.f);
+  } else if constexpr (ACT == AFFB_ACT_GELU) {
+    // z Phi(z) = max(z, 0) - |z| Phi(-|z|); the clamp keeps inf * 0 out
+    const float a = min_nan(fabsf(z), 64.f);
+    return fmaf(-a, normal_tail(a), fmaxf(z, 0.f));
+  } else if constexpr (ACT == AFFB_ACT_SILU) {
+    return __fdividef(z, 1.f + exp2_approx(-LOG2E * z));
+  } else {
+    return z;
+  }
+}
+
+template <int ACT>
+__device__ __forceinline__ float activate_grad(float z) {
+  if constexpr (ACT == AFFB_ACT_RELU) {
+    return z > 0.f ? 1.f : 0.f;
+  } else if constexpr (ACT == AFFB_ACT_GELU) {
+    const float a = min_nan(fabsf(z), 64.f);
+    const float t = normal_tail(a);
+    // Phi(z) + z phi(z)
+    const float pdf = 0.3989422804014327f * exp2_approx(-0.5f * LOG2E * a * a);
+    return fmaf(copysignf(a, z), pdf, z > 0.f ? 1.f - t : t);
+  } else if constexpr (ACT == AFFB_ACT_SILU) {
+    const float s = __fdividef(1.f, 1.f + exp2_approx(-LOG2E * z));
+    return s > 0.f ? s * fmaf(z, 1.f - s, 1.f) : s;
+  } else {
+    return 1.f;
+  }
+}
+
+}  // namespace affb

@@ -1,0 +1,680 @@
+// Matrix product with bias, activation and residual in its epilogue:
+//   z = x w^T + b,  y = act(z) + residual,
+// its backward (dx = dz w, dw = dz^T x with dz = dy act'(z)) and its form for
+// e4m3 operands with one scale per row of each.
+//
+// One kernel computes D[m,n] = sum_k A[m,k] B[n,k] for all of them.  A and B
+// are brought in by TMA as 128-byte-swizzled tiles, K-major (rows of k) or
+// MN-major (rows of m or n, for the two products of the backward, which
+// contract over the other index of the stored matrices), and multiplied by
+// tcgen05.mma with the 128 x BN accumulator in tensor memory.  A block is
+// persistent and split by role: one warp issues the loads, one the products,
+// eight take the finished accumulator (two are in flight) through the
+// epilogue into shared memory, from where TMA stores write it.
+//
+// fp32 operands are split into three bf16 parts (8 mantissa bits each) and
+// the six leading products of parts are summed into the same accumulator,
+// smallest first; what is left out is of the order of 2^-24.
+//
+// Long contractions with few output tiles (the weight gradient sums over all
+// tokens) are split over blocks; partial products go to a workspace and are
+// summed in a fixed order, so results do not depend on timing.
+#include "activation.cuh"
+#include "linear.cuh"
+#include "tcgen05.cuh"
+
+#include <type_traits>
+
+namespace affb {
+
+using namespace tc5;
+
+constexpr int TILE_M = 128;
+constexpr int EPI_WARPS = 8;
+constexpr int LIN_THREADS = 64 + EPI_WARPS * 32;
+constexpr int A_BYTES = TILE_M * 128;
+constexpr int SMEM_MAX = 232448;     // 227 KB of a block
+constexpr int MAX_STAGES = 8;
+constexpr int STAGE_ROWS = 32;       // rows x columns of one warp's staging buffer
+constexpr int CHUNK = 32;
+constexpr int BAR_BYTES = 256;
+constexpr int COLS_BYTES = EPI_WARPS * 2 * CHUNK * 4;  // each epilogue warp's bias and column scales of a chunk
+
+// Set when a block's waits ran out; read by affb_linear_status.
+__device__ int g_linear_failed;
+
+struct GemmArgs {
+  int M, N, bn, mt, nt, splits;
+  int kblocks;       // 128-byte blocks of the contraction
+  int parts;         // pairs of operand parts summed (1, or 6 for fp32)
+  int stages;
+  int a_mn, b_mn, f8;
+  int b_bytes;
+  uint32_t idesc;
+  int direct;        // outputs not addressable by TMA: plain stores
+  int bufs;          // staging buffers of a warp (2, or 1 where fp32 outputs make them large)
+  int buf_bytes;     // one of them: out chunk, then z chunk
+  int z_off;
+  LinearEpilogue e;
+};
+
+// Parts of A and B of product i of an fp32 contraction, smallest first
+// (0: leading 8 bits, 1: next, 2: last).
+__device__ __forceinline__ int part_a(int i) { return (0x010120 >> (4 * i)) & 15; }
+__device__ __forceinline__ int part_b(int i) { return (0x001102 >> (4 * i)) & 15; }
+
+template <typename T> struct code_of;
+template <> struct code_of<float> { static constexpr int value = AFFB_F32; };
+template <> struct code_of<__half> { static constexpr int value = AFFB_F16; };
+template <> struct code_of<__nv_bfloat16> { static constexpr int value = AFFB_BF16; };
+
+// 32 columns of one row into a warp's staging buffer, in the swizzle that the
+// TMA store undoes (64-byte rows: 64B swizzle, 128-byte rows: 128B).
+template <typename T>
+__device__ __forceinline__ void stage_row(unsigned char* buf, int lane, const float* v) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+          make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      st8(reinterpret_cast<T*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)), v + 8 * j);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_row(T* p, int n, const float* v) {
+#pragma unroll
+  for (int i = 0; i < CHUNK; ++i)
+    if (i < n) stf(p + i, v[i]);
+}
+// 32 columns of a row of the residual added to v (n valid).
+template <typename T>
+__device__ __forceinline__ void add_row(const T* p, int n, float* v) {
+  if (n == CHUNK && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float r[8];
+      ld8(p + 8 * j, r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[8 * j + i] += r[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < CHUNK; ++i)
+      if (i < n) v[i] += ldf(p + i);
+  }
+}
+
+template <typename TO, int ACT>
+__global__ void __launch_bounds__(LIN_THREADS, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_z,
+                const __grid_constant__ GemmArgs p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+  const int stage_bytes = A_BYTES + p.b_bytes;
+  unsigned char* staging = smem + p.stages * stage_bytes;
+  float* cols = reinterpret_cast<float*>(staging + EPI_WARPS * p.bufs * p.buf_bytes);
+  unsigned char* bars = reinterpret_cast<unsigned char*>(cols) + COLS_BYTES;
+  const uint32_t full = smem_addr(bars), empty = full + 8 * MAX_STAGES;
+  const uint32_t acc_full = empty + 8 * MAX_STAGES, acc_empty = acc_full + 16, drain = acc_empty + 16;
+  volatile int* failed = reinterpret_cast<volatile int*>(bars + 200);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 208);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      bar_init(full + 8 * i, 1);
+      bar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(acc_full + 8 * i, 1);
+      bar_init(acc_empty + 8 * i, EPI_WARPS);
+    }
+    bar_init(drain, 1);
+    bar_init_fence();
+    *failed = 0;
+    tma_prefetch(&map_a);
+    tma_prefetch(&map_b);
+  }
+  if (warp == 1) tmem_alloc<512>(smem_addr(tmem_slot));
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+
+  const int units = p.mt * p.nt * p.splits;
+  const int total_k = p.kblocks * p.parts;
+  const int ke = p.f8 ? 128 : 64;  // elements of one k block
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const int tile = u % (p.mt * p.nt), s = u / (p.mt * p.nt);
+        const int m0 = tile / p.nt * TILE_M, n0 = tile % p.nt * p.bn;
+        const int kb0 = (int)((int64_t)total_k * s / p.splits), kb1 = (int)((int64_t)total_k * (s + 1) / p.splits);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % p.stages;
+          if (!(ok = bar_wait(empty + 8 * st, ((it / p.stages) & 1) ^ 1, failed))) break;
+          const int part = kb / p.kblocks, k0 = (kb - part * p.kblocks) * ke;
+          const int za = p.parts > 1 ? part_a(part) : 0, zb = p.parts > 1 ? part_b(part) : 0;
+          const uint32_t bar = full + 8 * st, a = smem_addr(smem + st * stage_bytes), b = a + A_BYTES;
+          bar_expect(bar, stage_bytes);
+          if (p.a_mn) {
+            tma_load(a, &map_a, m0, k0, za, bar);
+            tma_load(a + 8192, &map_a, m0 + 64, k0, za, bar);
+          } else {
+            tma_load(a, &map_a, k0, m0, za, bar);
+          }
+          if (p.b_mn) {
+            for (int j = 0; j * 8192 < p.b_bytes; ++j) tma_load(b + j * 8192, &map_b, n0 + 64 * j, k0, zb, bar);
+          } else {
+            tma_load(b, &map_b, k0, n0, zb, bar);
+          }
+        }
+      }
+      if (!ok)  // loads still in flight must land before the block's memory is given back
+        for (int i = it > p.stages ? it - p.stages : 0; i < it; ++i)
+          bar_drain(full + 8 * (i % p.stages), (i / p.stages) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int it = 0, acc_it = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++acc_it) {
+        const int s = u / (p.mt * p.nt);
+        const int kb0 = (int)((int64_t)total_k * s / p.splits), kb1 = (int)((int64_t)total_k * (s + 1) / p.splits);
+        const int acc = acc_it & 1;
+        if (!(ok = bar_wait(acc_empty + 8 * acc, ((acc_it >> 1) & 1) ^ 1, failed))) break;
+        fence_after();
+        const uint32_t d = tmem + acc * 256;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % p.stages;
+          if (!(ok = bar_wait(full + 8 * st, (it / p.stages) & 1, failed))) break;
+          fence_after();
+          const uint32_t a = smem_addr(smem + st * stage_bytes), b = a + A_BYTES;
+          // advance of 32 bytes along k (K-major) or of 16 k rows (MN-major)
+          const uint64_t da = smem_desc(a, p.a_mn ? 8192 : 0, 1024), db = smem_desc(b, p.b_mn ? 8192 : 0, 1024);
+          const uint64_t sa = p.a_mn ? 2048 >> 4 : 32 >> 4, sb = p.b_mn ? 2048 >> 4 : 32 >> 4;
+          if (p.f8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_f8(d, da + k * sa, db + k * sb, p.idesc, kb > kb0 || k > 0);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_f16(d, da + k * sa, db + k * sb, p.idesc, kb > kb0 || k > 0);
+          }
+          mma_commit(empty + 8 * st);
+        }
+        if (ok) mma_commit(acc_full + 8 * acc);
+      }
+      if (!ok) {
+        mma_commit(drain);
+        bar_drain(drain, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+    unsigned char* my = staging + ew * p.bufs * p.buf_bytes;
+    float* bias = cols + ew * 2 * CHUNK;
+    int acc_it = 0, buf = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x, ++acc_it) {
+      const int tile = u % (p.mt * p.nt), s = u / (p.mt * p.nt);
+      const int m0 = tile / p.nt * TILE_M, n0 = tile % p.nt * p.bn;
+      const int ncols = min(p.bn, p.N - n0);
+      const int acc = acc_it & 1;
+      const int m = m0 + quad * 32 + lane;
+      // the next chunk's bias and column scale of this lane's column
+      float nb = 0.f, ns = 1.f;
+      const auto fetch = [&](int c) {
+        if (c + lane >= ncols) return;
+        const int n = n0 + c + lane;
+        if (p.e.bias) {
+          if (p.e.bias_dtype == AFFB_F32) nb = ((const float*)p.e.bias)[n];
+          else if (p.e.bias_dtype == AFFB_BF16) nb = __bfloat162float(((const __nv_bfloat16*)p.e.bias)[n]);
+          else nb = __half2float(((const __half*)p.e.bias)[n]);
+        }
+        if (p.e.col_scale) ns = p.e.col_scale[n];
+      };
+      const bool per_col = p.e.bias || p.e.col_scale;
+      if (per_col) fetch(half * CHUNK);
+      const float rs = (p.e.row_scale && m < p.M) ? p.e.row_scale[m] : 1.f;
+      // all lanes of the warp leave together
+      if (__any_sync(0xffffffffu, !bar_wait(acc_full + 8 * acc, (acc_it >> 1) & 1, failed))) break;
+      fence_after();
+      for (int c = half * CHUNK; c < ncols; c += 2 * CHUNK) {
+        uint32_t r[32];
+        tmem_load32(tmem + acc * 256 + c + ((uint32_t)(quad * 32) << 16), r);
+        tmem_wait_load();
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        if (per_col) {
+          __syncwarp();  // the chunk before has been read
+          bias[lane] = nb;
+          bias[CHUNK + lane] = ns;
+          __syncwarp();
+          fetch(c + 2 * CHUNK);
+          if (p.e.col_scale) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= rs * bias[CHUNK + i];
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += bias[i];
+        }
+        const int n = min(CHUNK, ncols - c);
+        const int64_t off = ((int64_t)s * p.M + m) * p.N + n0 + c;
+        unsigned char* ob = my + buf * p.buf_bytes;
+        if (!p.direct) {  // the buffer's last store has been read
+          if (lane == 0) {
+            if (p.bufs == 2) store_wait_read<1>();
+            else store_wait_read<0>();
+          }
+          __syncwarp();
+        }
+        if (p.e.z) {
+          if (p.direct) {
+            if (m < p.M) {
+              if (p.e.z_dtype == AFFB_F32) store_row((float*)p.e.z + off, n, v);
+              else if (p.e.z_dtype == AFFB_BF16) store_row((__nv_bfloat16*)p.e.z + off, n, v);
+              else store_row((__half*)p.e.z + off, n, v);
+            }
+          } else {
+            if (p.e.z_dtype == AFFB_F32) stage_row<float>(ob + p.z_off, lane, v);
+            else if (p.e.z_dtype == AFFB_BF16) stage_row<__nv_bfloat16>(ob + p.z_off, lane, v);
+            else stage_row<__half>(ob + p.z_off, lane, v);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = activate<ACT>(v[i]);
+        if (p.e.residual && m < p.M) {
+          if (p.e.residual_dtype == AFFB_F32) add_row((const float*)p.e.residual + off, n, v);
+          else if (p.e.residual_dtype == AFFB_BF16) add_row((const __nv_bfloat16*)p.e.residual + off, n, v);
+          else add_row((const __half*)p.e.residual + off, n, v);
+        }
+        if (p.direct) {
+          if (m < p.M) store_row((TO*)p.e.out + off, n, v);
+        } else {
+          stage_row<TO>(ob, lane, v);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store(&map_out, smem_addr(ob), n0 + c, m0 + quad * 32, s);
+            if (p.e.z) tma_store(&map_z, smem_addr(ob + p.z_off), n0 + c, m0 + quad * 32, s);
+            store_commit();
+          }
+          if (p.bufs == 2) buf ^= 1;
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(acc_empty + 8 * acc);
+    }
+    if (lane == 0) store_wait_all();
+    __syncwarp();
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    tmem_free<512>(tmem);
+  }
+  if (threadIdx.x == 0 && *failed) atomicExch(&g_linear_failed, 1);
+}
+
+// ------------------------------------------------------------------ host --
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return (EncodeFn)f;
+  }();
+  return fn;
+}
+
+// A [planes][rows][cols] array with row pitch `ld` (elements).
+static int make_map(CUtensorMap* map, int dtype, const void* base, int64_t cols, int64_t rows, int64_t planes,
+                    int64_t ld, int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
+  const CUtensorMapDataType t = dtype == AFFB_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : dtype == AFFB_F16  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                : dtype == AFFB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)(ld * dtype_size(dtype)), (cuuint64_t)(rows * ld * dtype_size(dtype))};
+  const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, es[3] = {1, 1, 1};
+  EncodeFn fn = encode_fn();
+  AFFB_REQUIRE(fn, "linear: the driver has no tensor-map encoder");
+  const CUresult rc = fn(map, t, 3, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  AFFB_REQUIRE(rc == CUDA_SUCCESS, "linear: tensor map refused (code %d)", (int)rc);
+  return AFFB_OK;
+}
+
+// One operand of a product: [planes][rows][cols], contracted over cols
+// (K-major) or over rows (MN-major).
+struct Operand {
+  const void* p;
+  int64_t rows, cols, ld;
+  bool mn;
+};
+
+struct Shape {
+  int bn, nt, mt, splits;
+};
+
+// Tile width and split of the contraction.  Few, wide tiles feed the tensor
+// cores best; with fewer tiles than SMs narrower tiles (down to 64 columns)
+// and then a split contraction (at least 4 k blocks a part) fill the GPU.
+static Shape choose_shape(int64_t M, int64_t N, int64_t total_k) {
+  const int64_t sms = sm_count();
+  Shape s;
+  s.mt = (int)((M + TILE_M - 1) / TILE_M);
+  s.nt = (int)((N + 255) / 256);
+  while ((int64_t)s.mt * s.nt * 2 <= sms && (N + s.nt * 2 - 1) / (s.nt * 2) >= 64) s.nt *= 2;
+  const int64_t per = (N + s.nt - 1) / s.nt;
+  s.bn = (int)(s.nt == 1 ? round_up(per, 16) : round_up(per, 32));
+  s.nt = (int)((N + s.bn - 1) / s.bn);
+  const int64_t tiles = (int64_t)s.mt * s.nt;
+  int64_t sp = sms / tiles;
+  if (sp > total_k / 4) sp = total_k / 4;
+  s.splits = (int)(sp < 2 ? 1 : sp);
+  return s;
+}
+
+static int64_t partial_bytes(int64_t M, int64_t N, int64_t total_k) {
+  const Shape s = choose_shape(M, N, total_k);
+  return s.splits > 1 ? round_up((int64_t)s.splits * M * round_up(N, 4) * 4, 256) : 0;
+}
+
+// K blocks of a contraction of length K (all part pairs).
+static int64_t k_blocks(int dtype, int64_t K) {
+  const int64_t ke = dtype == AFFB_E4M3 ? 128 : 64;
+  return (K + ke - 1) / ke * (dtype == AFFB_F32 ? 6 : 1);
+}
+
+template <typename TO>
+static const void* kernel_of(int act) {
+  switch (act) {
+    case AFFB_ACT_RELU: return (const void*)gemm_kernel<TO, AFFB_ACT_RELU>;
+    case AFFB_ACT_GELU: return (const void*)gemm_kernel<TO, AFFB_ACT_GELU>;
+    case AFFB_ACT_SILU: return (const void*)gemm_kernel<TO, AFFB_ACT_SILU>;
+    default: return (const void*)gemm_kernel<TO, AFFB_ACT_NONE>;
+  }
+}
+
+static bool tma_rows(const void* p, int dtype, int64_t N) {
+  return aligned_to(p, 16) && N * dtype_size(dtype) % 16 == 0;
+}
+
+// D = A B^T over a contraction of length K, then the epilogue.  `dtype` names
+// the operands' type as the caller has them (fp32: three bf16 planes each);
+// `ws` holds partial_bytes(...).
+static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K, LinearEpilogue e,
+                unsigned char* ws, cudaStream_t st) {
+  const int64_t total_k = k_blocks(dtype, K);
+  const Shape s = choose_shape(M, N, total_k);
+  const int et = dtype == AFFB_F32 ? AFFB_BF16 : dtype;  // element type in memory
+  const int64_t planes = dtype == AFFB_F32 ? 3 : 1;
+  GemmArgs p{};
+  p.M = (int)M; p.N = (int)N;
+  p.bn = s.bn; p.mt = s.mt; p.nt = s.nt; p.splits = s.splits;
+  p.parts = dtype == AFFB_F32 ? 6 : 1;
+  p.kblocks = (int)(total_k / p.parts);
+  p.a_mn = a.mn; p.b_mn = b.mn; p.f8 = dtype == AFFB_E4M3;
+  p.b_bytes = b.mn ? (int)round_up(s.bn, 64) * 128 : s.bn * 128;
+  p.idesc = instr_desc(et == AFFB_BF16 ? 1 : 0, a.mn, b.mn, (uint32_t)s.bn);
+  LinearEpilogue full = e;
+  if (s.splits > 1) {
+    e = LinearEpilogue{};
+    e.out = ws;
+    e.out_dtype = AFFB_F32;
+    p.N = (int)round_up(N, 4);  // pitch of the partial products (columns past N hold zeros)
+  }
+  p.e = e;
+  p.direct = s.splits > 1 ? 0
+                          : !(tma_rows(e.out, e.out_dtype, N) && (!e.z || tma_rows(e.z, e.z_dtype, N)));
+  p.z_off = (int)dtype_size(e.out_dtype) * STAGE_ROWS * CHUNK;
+  p.buf_bytes = p.z_off + (e.z ? (int)dtype_size(e.z_dtype) * STAGE_ROWS * CHUNK : 0);
+  const int stage = A_BYTES + p.b_bytes;
+  p.bufs = p.buf_bytes > 4096 ? 1 : 2;
+  const int fixed = 1024 + EPI_WARPS * p.bufs * p.buf_bytes + COLS_BYTES + BAR_BYTES;
+  p.stages = (SMEM_MAX - fixed) / stage;
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  AFFB_REQUIRE(p.stages >= 2, "linear: no room for two stages");
+  const int smem = fixed + p.stages * stage;
+
+  CUtensorMap ma, mb, mo{}, mz{};
+  const int ke = p.f8 ? 128 : 64;
+  int rc;
+  if ((rc = make_map(&ma, et, a.p, a.cols, a.rows, planes, a.ld, a.mn ? 64 : ke, a.mn ? 64 : TILE_M,
+                     CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  if ((rc = make_map(&mb, et, b.p, b.cols, b.rows, planes, b.ld, b.mn ? 64 : ke, b.mn ? 64 : s.bn,
+                     CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  if (!p.direct) {
+    const auto sw = [](int t) { return t == AFFB_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B; };
+    if ((rc = make_map(&mo, e.out_dtype, e.out, p.N, M, s.splits, p.N, CHUNK, STAGE_ROWS, sw(e.out_dtype)))) return rc;
+    if (e.z && (rc = make_map(&mz, e.z_dtype, e.z, p.N, M, 1, p.N, CHUNK, STAGE_ROWS, sw(e.z_dtype)))) return rc;
+  }
+  const void* k = e.out_dtype == AFFB_F32    ? kernel_of<float>(e.act)
+                  : e.out_dtype == AFFB_BF16 ? kernel_of<__nv_bfloat16>(e.act)
+                                             : kernel_of<__half>(e.act);
+  cudaError_t err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+  if (err == cudaSuccess) {
+    const int64_t units = (int64_t)s.mt * s.nt * s.splits;
+    void* args[] = {&ma, &mb, &mo, &mz, &p};
+    err = cudaLaunchKernel(k, dim3((unsigned)imin64(units, sm_count())), dim3(LIN_THREADS), args, (size_t)smem, st);
+  }
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    set_error("linear: launch failed: %s", cudaGetErrorString(err));
+    return AFFB_ERR_CUDA;
+  }
+  if (s.splits > 1) return linear_sum((const float*)ws, s.splits, M, N, p.N, full, st);
+  return AFFB_OK;
+}
+
+// --------------------------------------------------------------- operands --
+// Row pitch of an operand as the product reads it: its own when TMA can
+// address it, else that of a packed copy.
+static int64_t pitch(int dtype, int64_t cols) { return round_up(cols, dtype == AFFB_E4M3 ? 16 : 8); }
+static bool needs_copy(int dtype, const void* p, int64_t cols) {
+  return dtype == AFFB_F32 || cols % (dtype == AFFB_E4M3 ? 16 : 8) != 0 || !aligned_to(p, 16);
+}
+// Bytes of an operand's copy where its shape (or `any`: other reasons) needs one.
+static int64_t copy_bytes(int dtype, int64_t rows, int64_t cols, bool any) {
+  if (!any && dtype != AFFB_F32 && cols % (dtype == AFFB_E4M3 ? 16 : 8) == 0) return 0;
+  return round_up(rows * pitch(dtype, cols) * (dtype == AFFB_F32 ? 6 : dtype_size(dtype)), 256);
+}
+struct Arena {
+  unsigned char* base;
+  int64_t used, size;
+  void* take(int64_t bytes) {
+    void* p = base + used;
+    used += round_up(bytes, 256);
+    return used <= size ? p : nullptr;
+  }
+};
+static int make_operand(int dtype, const void* src, int64_t rows, int64_t cols, bool mn, Arena* ws, Operand* o,
+                        cudaStream_t st) {
+  *o = Operand{src, rows, cols, cols, mn};
+  if (!needs_copy(dtype, src, cols)) return AFFB_OK;
+  o->ld = pitch(dtype, cols);
+  void* dst = ws->take(rows * o->ld * (dtype == AFFB_F32 ? 6 : dtype_size(dtype)));
+  AFFB_REQUIRE(dst, "linear: workspace too small (or an operand that is not 16-byte aligned)");
+  o->p = dst;
+  return dtype == AFFB_F32 ? linear_split((const float*)src, rows, cols, dst, o->ld, st)
+                           : linear_pack(src, dtype_size(dtype), rows, cols, dst, o->ld, st);
+}
+
+static int check_sizes(int64_t M, int64_t N, int64_t K) {
+  AFFB_REQUIRE(M >= 0 && N >= 1 && K >= 1, "linear: needs rows >= 0 and at least one input and one output channel");
+  const int64_t most = (1ll << 31) - 1024;
+  AFFB_REQUIRE(M < most && N < most && K < most, "linear: a dimension exceeds 2^31");
+  const int64_t mt = (M + TILE_M - 1) / TILE_M, nt = (N + 31) / 32, kt = (K + TILE_M - 1) / TILE_M;
+  AFFB_REQUIRE(mt * nt < most && mt * ((K + 31) / 32) < most && kt * nt < most, "linear: too many tiles");
+  return AFFB_OK;
+}
+
+static int forward(const void* x, const void* w, int dtype, int64_t M, int64_t N, int64_t K, const LinearEpilogue& e,
+                   void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+  if (M <= SMALL_ROWS) return linear_small(x, w, dtype, M, N, K, e, st);
+  Arena ws{(unsigned char*)workspace, 0, workspace ? workspace_bytes : 0};
+  Operand a, b;
+  int rc;
+  if ((rc = make_operand(dtype, x, M, K, false, &ws, &a, st))) return rc;
+  if ((rc = make_operand(dtype, w, N, K, false, &ws, &b, st))) return rc;
+  const int64_t part = partial_bytes(M, N, k_blocks(dtype, K));
+  unsigned char* pp = nullptr;
+  if (part) AFFB_REQUIRE(pp = (unsigned char*)ws.take(part), "linear: workspace too small");
+  return gemm(dtype, a, b, M, N, K, e, pp, st);
+}
+
+}  // namespace affb
+
+using namespace affb;
+
+extern "C" int affb_linear_status(int* failed) {
+  AFFB_REQUIRE(failed, "affb_linear_status: null pointer");
+  const cudaError_t e = cudaMemcpyFromSymbol(failed, g_linear_failed, sizeof(int));
+  if (e != cudaSuccess) {
+    set_error("affb_linear_status: %s", cudaGetErrorString(e));
+    return AFFB_ERR_CUDA;
+  }
+  return AFFB_OK;
+}
+
+extern "C" int64_t affb_linear_fwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+  if (M <= SMALL_ROWS || N < 1 || K < 1) return 0;
+  return copy_bytes(dtype, M, K, false) + copy_bytes(dtype, N, K, false) + partial_bytes(M, N, k_blocks(dtype, K));
+}
+
+extern "C" int64_t affb_linear_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  const int64_t strips = linear_dz_strips(M, N);
+  int64_t b = copy_bytes(dtype, M, N, true) + copy_bytes(dtype, N, K, false) + copy_bytes(dtype, M, K, false);
+  b += round_up(strips * N * 4, 256);
+  const int64_t p1 = partial_bytes(M, K, k_blocks(dtype, N)), p2 = partial_bytes(N, K, k_blocks(dtype, M));
+  return b + (p1 > p2 ? p1 : p2);
+}
+
+extern "C" int affb_linear_fwd(const void* x, const void* weight, const void* bias, int bias_dtype,
+                               const void* residual, int residual_dtype, int act, int dtype, int64_t M, int64_t N,
+                               int64_t K, void* out, int out_dtype, void* z, void* workspace, int64_t workspace_bytes,
+                               void* stream) {
+  int rc = check_sizes(M, N, K);
+  if (rc) return rc;
+  AFFB_REQUIRE(is_float_dtype(dtype), "linear: operands must be fp32, fp16 or bf16");
+  AFFB_REQUIRE(act >= AFFB_ACT_NONE && act <= AFFB_ACT_SILU, "linear: unknown activation %d", act);
+  AFFB_REQUIRE(out_dtype == dtype || out_dtype == AFFB_F32, "linear: the output is of the operands' type or fp32");
+  AFFB_REQUIRE(!bias || is_float_dtype(bias_dtype), "linear: unsupported bias dtype");
+  AFFB_REQUIRE(!residual || is_float_dtype(residual_dtype), "linear: unsupported residual dtype");
+  if (M == 0) return AFFB_OK;
+  AFFB_REQUIRE(x && weight && out, "linear: null pointer");
+  AFFB_REQUIRE(workspace || affb_linear_fwd_workspace_bytes(dtype, M, N, K) == 0, "linear: workspace missing");
+  LinearEpilogue e{nullptr, nullptr, bias, bias_dtype, residual, residual_dtype, act, out, out_dtype, z, dtype};
+  return forward(x, weight, dtype, M, N, K, e, workspace, workspace_bytes, as_stream(stream));
+}
+
+extern "C" int64_t affb_linear_e4m3_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  return affb_linear_fwd_workspace_bytes(AFFB_E4M3, M, N, K);
+}
+
+extern "C" int affb_linear_e4m3(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
+                                const float* bias, const void* residual, int residual_dtype, int act, int64_t M,
+                                int64_t N, int64_t K, void* out, int out_dtype, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+  int rc = check_sizes(M, N, K);
+  if (rc) return rc;
+  AFFB_REQUIRE(act >= AFFB_ACT_NONE && act <= AFFB_ACT_SILU, "linear_e4m3: unknown activation %d", act);
+  AFFB_REQUIRE(is_float_dtype(out_dtype), "linear_e4m3: the output must be fp32, fp16 or bf16");
+  AFFB_REQUIRE(!residual || is_float_dtype(residual_dtype), "linear_e4m3: unsupported residual dtype");
+  if (M == 0) return AFFB_OK;
+  AFFB_REQUIRE(x && x_scale && weight && weight_scale && out, "linear_e4m3: null pointer");
+  AFFB_REQUIRE(workspace || affb_linear_e4m3_workspace_bytes(M, N, K) == 0, "linear_e4m3: workspace missing");
+  LinearEpilogue e{x_scale, weight_scale, bias, AFFB_F32, residual, residual_dtype, act, out, out_dtype, nullptr, 0};
+  return forward(x, weight, AFFB_E4M3, M, N, K, e, workspace, workspace_bytes, as_stream(stream));
+}
+
+extern "C" int affb_linear_bwd(const void* dout, int dout_dtype, const void* z, const void* x, const void* weight,
+                               int act, int dtype, int64_t M, int64_t N, int64_t K, void* dx, void* dweight,
+                               void* dbias, int dbias_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = check_sizes(M, N, K);
+  if (rc) return rc;
+  AFFB_REQUIRE(is_float_dtype(dtype), "linear: operands must be fp32, fp16 or bf16");
+  AFFB_REQUIRE(act >= AFFB_ACT_NONE && act <= AFFB_ACT_SILU, "linear: unknown activation %d", act);
+  AFFB_REQUIRE(dout_dtype == dtype || dout_dtype == AFFB_F32, "linear: the gradient is of the operands' type or fp32");
+  AFFB_REQUIRE(!dbias || is_float_dtype(dbias_dtype), "linear: unsupported bias dtype");
+  cudaStream_t st = as_stream(stream);
+  if (M == 0) {  // sums over no rows
+    cudaError_t err = cudaSuccess;
+    if (dweight) err = cudaMemsetAsync(dweight, 0, (size_t)(N * K * dtype_size(dtype)), st);
+    if (dbias && err == cudaSuccess) err = cudaMemsetAsync(dbias, 0, (size_t)(N * dtype_size(dbias_dtype)), st);
+    if (err != cudaSuccess) {
+      set_error("linear: %s", cudaGetErrorString(err));
+      return AFFB_ERR_CUDA;
+    }
+    return AFFB_OK;
+  }
+  AFFB_REQUIRE(dout && (act == AFFB_ACT_NONE || z) && (!dx || weight) && (!dweight || x), "linear: null pointer");
+  AFFB_REQUIRE(workspace, "linear: workspace missing");
+  Arena ws{(unsigned char*)workspace, 0, workspace_bytes};
+
+  // dz: the output gradient itself when nothing changes it
+  Operand dz{dout, M, N, N, false};
+  const bool want_dz = dx || dweight;
+  const bool as_is = act == AFFB_ACT_NONE && dout_dtype == dtype && !needs_copy(dtype, dout, N);
+  void* dzp = nullptr;
+  if (want_dz && !as_is) {
+    dz.ld = pitch(dtype, N);
+    dzp = ws.take(M * dz.ld * (dtype == AFFB_F32 ? 6 : dtype_size(dtype)));
+    AFFB_REQUIRE(dzp, "linear: workspace too small");
+    dz.p = dzp;
+  }
+  float* part = nullptr;
+  const int64_t strips = linear_dz_strips(M, N);
+  if (dbias) AFFB_REQUIRE(part = (float*)ws.take(strips * N * 4), "linear: workspace too small");
+  if (dzp || part) {
+    if ((rc = linear_dz(dout, dout_dtype, z, act, dtype, M, N, dzp, dz.ld, part, st))) return rc;
+  }
+  if (dbias) {
+    LinearEpilogue e{};
+    e.out = dbias;
+    e.out_dtype = dbias_dtype;
+    if ((rc = linear_sum(part, strips, 1, N, N, e, st))) return rc;
+  }
+  LinearEpilogue e{};
+  e.out_dtype = dtype;
+  const int64_t p1 = dx ? partial_bytes(M, K, k_blocks(dtype, N)) : 0;
+  const int64_t p2 = dweight ? partial_bytes(N, K, k_blocks(dtype, M)) : 0;
+  unsigned char* pp = nullptr;
+  if (p1 || p2) AFFB_REQUIRE(pp = (unsigned char*)ws.take(p1 > p2 ? p1 : p2), "linear: workspace too small");
+  if (dx) {  // dx[m,k] = sum_n dz[m,n] w[n,k]
+    Operand b;
+    if ((rc = make_operand(dtype, weight, N, K, true, &ws, &b, st))) return rc;
+    dz.mn = false;
+    e.out = dx;
+    if ((rc = gemm(dtype, dz, b, M, K, N, e, pp, st))) return rc;
+  }
+  if (dweight) {  // dw[n,k] = sum_m dz[m,n] x[m,k]
+    Operand b;
+    if ((rc = make_operand(dtype, x, M, K, true, &ws, &b, st))) return rc;
+    dz.mn = true;
+    e.out = dweight;
+    if ((rc = gemm(dtype, dz, b, N, K, M, e, pp, st))) return rc;
+  }
+  return AFFB_OK;
+}

@@ -1,0 +1,249 @@
+// Side passes of the matrix product: operand packing for rows that TMA cannot
+// address, the fp32 -> 3 x bf16 split, the activation's gradient with the
+// bias gradient's column sums, and the sums of partial products.
+#include "activation.cuh"
+#include "linear.cuh"
+
+#include <type_traits>
+
+namespace affb {
+
+// ------------------------------------------------------------------ pack --
+template <typename U>
+__global__ void __launch_bounds__(256) pack_rows_kernel(const U* __restrict__ src, int64_t R, int64_t C,
+                                                        U* __restrict__ dst, int64_t ld) {
+  const int64_t n = R * C;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / C;
+    dst[r * ld + (i - r * C)] = src[i];
+  }
+}
+
+int linear_pack(const void* src, int64_t elem, int64_t R, int64_t C, void* dst, int64_t ld, cudaStream_t st) {
+  if (R * C == 0) return AFFB_OK;
+  const unsigned blocks = (unsigned)imin64((R * C + 255) / 256, (int64_t)sm_count() * 16);
+  if (elem == 1) pack_rows_kernel<uint8_t><<<blocks, 256, 0, st>>>((const uint8_t*)src, R, C, (uint8_t*)dst, ld);
+  else pack_rows_kernel<uint16_t><<<blocks, 256, 0, st>>>((const uint16_t*)src, R, C, (uint16_t*)dst, ld);
+  AFFB_LAUNCH_CHECK("linear: pack");
+  return AFFB_OK;
+}
+
+// Three bf16 parts of an fp32 value: each takes the next 8 bits of the
+// mantissa, so their sum is the value (up to bf16's exponent range).
+__device__ __forceinline__ void split3(float v, __nv_bfloat16* o) {
+  o[0] = __float2bfloat16_rn(v);
+  // the largest fp32 values would round up to infinity
+  if (isfinite(v) && !isfinite(__bfloat162float(o[0]))) o[0] = __float2bfloat16_rz(v);
+  // an infinity or NaN stays in the first part alone
+  const float r1 = isfinite(v) ? v - __bfloat162float(o[0]) : 0.f;
+  o[1] = __float2bfloat16_rn(r1);
+  o[2] = __float2bfloat16_rn(isfinite(r1) ? r1 - __bfloat162float(o[1]) : 0.f);
+}
+
+__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, int64_t R, int64_t C,
+                                                         __nv_bfloat16* __restrict__ dst, int64_t ld) {
+  const int64_t n = R * C, part = R * ld;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / C, o = r * ld + (i - r * C);
+    __nv_bfloat16 p[3];
+    split3(src[i], p);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) dst[o + k * part] = p[k];
+  }
+}
+
+int linear_split(const float* src, int64_t R, int64_t C, void* dst, int64_t ld, cudaStream_t st) {
+  if (R * C == 0) return AFFB_OK;
+  const unsigned blocks = (unsigned)imin64((R * C + 255) / 256, (int64_t)sm_count() * 16);
+  split_rows_kernel<<<blocks, 256, 0, st>>>(src, R, C, (__nv_bfloat16*)dst, ld);
+  AFFB_LAUNCH_CHECK("linear: split");
+  return AFFB_OK;
+}
+
+// ---------------------------------------------------- activation gradient --
+constexpr int DZ_THREADS = 256;
+constexpr int DZ_COLS = 256;   // columns of one block
+constexpr int DZ_MIN_ROWS = 64;
+
+int64_t linear_dz_strips(int64_t R, int64_t C) {
+  const int64_t cols = (C + DZ_COLS - 1) / DZ_COLS;
+  const int64_t want = ((int64_t)sm_count() * 8 + cols - 1) / cols;
+  const int64_t most = (R + DZ_MIN_ROWS - 1) / DZ_MIN_ROWS;
+  return want < most ? want : (most > 0 ? most : 1);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void ldn(const T* p, float* o) {
+  if constexpr (VEC == 8) {
+    ld8(p, o);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) o[k] = ldf(p + k);
+  }
+}
+
+// Block: DZ_COLS columns x one strip of rows.  A thread keeps VEC columns and
+// walks down the strip; the threads of a column group are summed in order, so
+// the sums do not depend on timing.
+template <typename TO, typename T, int ACT, int VEC>
+__global__ void __launch_bounds__(DZ_THREADS) dz_kernel(const TO* __restrict__ dout, const T* __restrict__ z, int64_t R,
+                                                        int64_t C, void* __restrict__ dz, int64_t ld, int64_t strip,
+                                                        float* __restrict__ part) {
+  constexpr bool SPLIT = std::is_same<T, float>::value;
+  __shared__ float red[DZ_THREADS * VEC];
+  const int64_t c0 = (int64_t)blockIdx.x * DZ_COLS;
+  const int cols = (int)imin64(DZ_COLS, C - c0);
+  const int cv = (cols + VEC - 1) / VEC;        // column groups
+  const int lanes = DZ_THREADS / cv;            // rows walked side by side
+  const int g = threadIdx.x % cv, rl = threadIdx.x / cv;
+  const int64_t r0 = (int64_t)blockIdx.y * strip, r1 = imin64(R, r0 + strip);
+  const int64_t c = c0 + (int64_t)g * VEC;
+  float sum[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
+  if (rl < lanes) {
+    for (int64_t r = r0 + rl; r < r1; r += lanes) {
+      float d[VEC];
+      ldn<TO, VEC>(dout + r * C + c, d);
+      if constexpr (ACT != AFFB_ACT_NONE) {
+        float zz[VEC];
+        ldn<T, VEC>(z + r * C + c, zz);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) d[k] *= activate_grad<ACT>(zz[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sum[k] += d[k];
+      if (dz) {
+        if constexpr (SPLIT) {
+          __nv_bfloat16* o = (__nv_bfloat16*)dz + r * ld + c;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            __nv_bfloat16 p[3];
+            split3(d[k], p);
+            o[k] = p[0];
+            o[k + R * ld] = p[1];
+            o[k + 2 * R * ld] = p[2];
+          }
+        } else {
+          T* o = (T*)dz + r * ld + c;
+          if constexpr (VEC == 8) {
+            st8(o, d);
+          } else {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) stf(o + k, d[k]);
+          }
+        }
+      }
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) red[k * DZ_THREADS + threadIdx.x] = sum[k];
+  __syncthreads();
+  for (int i = threadIdx.x; i < cols; i += DZ_THREADS) {
+    const int gg = i / VEC, k = i % VEC;
+    float s = 0.f;
+    for (int l = 0; l < lanes; ++l) s += red[k * DZ_THREADS + l * cv + gg];
+    part[(int64_t)blockIdx.y * C + c0 + i] = s;
+  }
+}
+
+template <typename TO, typename T, int ACT>
+static int dz_launch(const void* dout, const void* z, int64_t R, int64_t C, void* dz, int64_t ld, float* part,
+                     cudaStream_t st) {
+  const int64_t strips = linear_dz_strips(R, C);
+  const int64_t strip = (R + strips - 1) / strips;
+  const dim3 grid((unsigned)((C + DZ_COLS - 1) / DZ_COLS), (unsigned)strips);
+  const bool vec = C % 8 == 0 && aligned_to(dout, 16) && aligned_to(z, 16) && aligned_to(dz, 16) && ld % 8 == 0;
+  if (vec)
+    dz_kernel<TO, T, ACT, 8><<<grid, DZ_THREADS, 0, st>>>((const TO*)dout, (const T*)z, R, C, dz, ld, strip, part);
+  else
+    dz_kernel<TO, T, ACT, 1><<<grid, DZ_THREADS, 0, st>>>((const TO*)dout, (const T*)z, R, C, dz, ld, strip, part);
+  AFFB_LAUNCH_CHECK("linear: activation gradient");
+  return AFFB_OK;
+}
+
+template <typename TO, typename T>
+static int dz_act(int act, const void* dout, const void* z, int64_t R, int64_t C, void* dz, int64_t ld, float* part,
+                  cudaStream_t st) {
+  switch (act) {
+    case AFFB_ACT_RELU: return dz_launch<TO, T, AFFB_ACT_RELU>(dout, z, R, C, dz, ld, part, st);
+    case AFFB_ACT_GELU: return dz_launch<TO, T, AFFB_ACT_GELU>(dout, z, R, C, dz, ld, part, st);
+    case AFFB_ACT_SILU: return dz_launch<TO, T, AFFB_ACT_SILU>(dout, z, R, C, dz, ld, part, st);
+    default: return dz_launch<TO, T, AFFB_ACT_NONE>(dout, z, R, C, dz, ld, part, st);
+  }
+}
+
+int linear_dz(const void* dout, int dout_dtype, const void* z, int act, int dtype, int64_t R, int64_t C, void* dz,
+              int64_t ld, float* part, cudaStream_t st) {
+  if (dtype == AFFB_F32) return dz_act<float, float>(act, dout, z, R, C, dz, ld, part, st);
+  if (dtype == AFFB_BF16)
+    return dout_dtype == AFFB_F32 ? dz_act<float, __nv_bfloat16>(act, dout, z, R, C, dz, ld, part, st)
+                                  : dz_act<__nv_bfloat16, __nv_bfloat16>(act, dout, z, R, C, dz, ld, part, st);
+  return dout_dtype == AFFB_F32 ? dz_act<float, __half>(act, dout, z, R, C, dz, ld, part, st)
+                                : dz_act<__half, __half>(act, dout, z, R, C, dz, ld, part, st);
+}
+
+// ------------------------------------------------------- sums of partials --
+__device__ __forceinline__ float load_as(const void* p, int dtype, int64_t i) {
+  if (dtype == AFFB_F32) return ((const float*)p)[i];
+  if (dtype == AFFB_BF16) return __bfloat162float(((const __nv_bfloat16*)p)[i]);
+  return __half2float(((const __half*)p)[i]);
+}
+__device__ __forceinline__ void store_as(void* p, int dtype, int64_t i, float v) {
+  if (dtype == AFFB_F32) ((float*)p)[i] = v;
+  else if (dtype == AFFB_BF16) ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
+  else ((__half*)p)[i] = __float2half_rn(v);
+}
+__device__ __forceinline__ float activate_code(int act, float z) {
+  switch (act) {
+    case AFFB_ACT_RELU: return activate<AFFB_ACT_RELU>(z);
+    case AFFB_ACT_GELU: return activate<AFFB_ACT_GELU>(z);
+    case AFFB_ACT_SILU: return activate<AFFB_ACT_SILU>(z);
+    default: return z;
+  }
+}
+
+// Block: 32 consecutive elements x 8 lanes of parts, summed in a fixed order.
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ part, int64_t S, int64_t M, int64_t N,
+                                                        int64_t ld, LinearEpilogue e) {
+  __shared__ float red[8][33];
+  const int x = threadIdx.x & 31, l = threadIdx.x >> 5;
+  const int64_t n = M * N, plane = M * ld;
+  for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < n; i0 += (int64_t)gridDim.x * 32) {
+    const int64_t i = i0 + x;
+    const int64_t m = i < n ? i / N : 0, c = i < n ? i - m * N : 0;
+    const float* p = part + m * ld + c;
+    float s = 0.f;
+    if (i < n) {
+#pragma unroll 4
+      for (int64_t k = l; k < S; k += 8) s += __ldg(p + k * plane);
+    }
+    red[l][x] = s;
+    __syncthreads();
+    if (l == 0 && i < n) {
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v += red[k][x];
+      if (e.row_scale) v *= e.row_scale[m];
+      if (e.col_scale) v *= e.col_scale[c];
+      if (e.bias) v += load_as(e.bias, e.bias_dtype, c);
+      if (e.z) store_as(e.z, e.z_dtype, i, v);
+      v = activate_code(e.act, v);
+      if (e.residual) v += load_as(e.residual, e.residual_dtype, i);
+      store_as(e.out, e.out_dtype, i, v);
+    }
+    __syncthreads();
+  }
+}
+
+int linear_sum(const float* part, int64_t S, int64_t M, int64_t N, int64_t ld, const LinearEpilogue& e,
+               cudaStream_t st) {
+  if (M * N == 0) return AFFB_OK;
+  const unsigned blocks = (unsigned)imin64((M * N + 31) / 32, (int64_t)sm_count() * 16);
+  sum_parts_kernel<<<blocks, 256, 0, st>>>(part, S, M, N, ld, e);
+  AFFB_LAUNCH_CHECK("linear: sum of partial products");
+  return AFFB_OK;
+}
+
+}  // namespace affb

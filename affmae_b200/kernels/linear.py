@@ -1,0 +1,210 @@
+"""Matrix product with bias, activation and residual in its epilogue.
+
+* ``fused_linear(x, weight, bias, act, residual)`` computes
+  ``act(x W^T + bias) + residual`` in one kernel (tensor cores for fp16, bf16
+  and, as three bf16 parts, fp32; a streaming kernel for up to 8 rows), with
+  its backward;
+* ``FusedLinear`` is the ``nn.Linear`` of it, in the autocast dtype under CUDA
+  autocast;
+* ``linear_e4m3`` is the forward for 8-bit operands with one fp32 scale per
+  row (``quantize_e4m3`` makes them, as does ``rms_norm_e4m3``), and
+  ``LinearE4M3`` a layer that keeps its weight so.
+
+Sums are fp32.  Everything runs on the current stream; the gradients do not
+depend on timing.  In fp32 an infinite operand gives NaN.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from .. import _native as nat
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _act_code(act: str) -> int:
+    try:
+        return ACTIVATIONS[act]
+    except KeyError:
+        raise RuntimeError(f"unknown activation {act!r}; expected one of {sorted(ACTIVATIONS)}")
+
+
+def _check(x, weight, bias, residual):
+    nat.require_cuda(x, weight, bias, residual)
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise RuntimeError(f"linear: input {tuple(x.shape)} does not match weight {tuple(weight.shape)} [out, in]")
+    if bias is not None and (tuple(bias.shape) != (weight.shape[0],) or bias.dtype not in _FLOATS):
+        raise RuntimeError(f"linear: bias must be a float vector of {weight.shape[0]} values")
+    out_shape = (*x.shape[:-1], weight.shape[0])
+    if residual is not None and tuple(residual.shape) != out_shape:
+        raise RuntimeError(f"linear: residual {tuple(residual.shape)} does not have the output's shape {out_shape}")
+    for t in (weight, bias, residual):
+        if t is not None and t.device != x.device:
+            raise RuntimeError("linear: tensors are on different devices")
+    return out_shape
+
+
+class FusedLinearFunction(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        out_shape = (*x.shape[:-1], weight.shape[0])
+        N, K = weight.shape
+        M = x.numel() // K
+        dev = x.device
+        xc, wc = nat.dense(x), nat.dense(weight)
+        bc = bias.contiguous() if bias is not None else None
+        rc = residual.contiguous() if residual is not None else None
+        out = torch.empty(out_shape, device=dev, dtype=x.dtype if rc is None else rc.dtype)
+        # the backward needs the pre-activation sums; the sign of ReLU's output serves as well
+        z = None
+        if any(ctx.needs_input_grad[:3]) and act:
+            z = out if act == ACTIVATIONS["relu"] and rc is None else torch.empty(out_shape, device=dev, dtype=x.dtype)
+        dt = nat.dcode(xc)
+        ws = nat.workspace("affb_linear_fwd_workspace_bytes", dev, dt, M, N, K)
+        nat.call_on(dev, "affb_linear_fwd", nat.ptr(xc), nat.ptr(wc), nat.ptr(bc),
+                    nat.dcode(bc) if bc is not None else 0, nat.ptr(rc), nat.dcode(rc) if rc is not None else 0, act,
+                    dt, M, N, K, nat.ptr(out), nat.dcode(out), None if z is out else nat.ptr(z), nat.ptr(ws),
+                    ws.numel() if ws is not None else 0, nat.stream(dev))
+        ctx.save_for_backward(xc, wc, z)
+        ctx.meta = (act, M, N, K, x.shape, bias.dtype if bias is not None else None)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        xc, wc, z = ctx.saved_tensors
+        act, M, N, K, xshape, bdt = ctx.meta
+        dev = xc.device
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        g = nat.dense(dout)
+        dx = torch.empty(xshape, device=dev, dtype=xc.dtype) if need_x else None
+        dw = torch.empty((N, K), device=dev, dtype=wc.dtype) if need_w else None
+        db = torch.empty(N, device=dev, dtype=bdt) if need_b else None
+        if need_x or need_w or need_b:
+            dt = nat.dcode(xc)
+            ws = nat.workspace("affb_linear_bwd_workspace_bytes", dev, dt, M, N, K)
+            nat.call_on(dev, "affb_linear_bwd", nat.ptr(g), nat.dcode(g), nat.ptr(z), nat.ptr(xc), nat.ptr(wc), act, dt,
+                        M, N, K, nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.dcode(db) if db is not None else 0,
+                        nat.ptr(ws), ws.numel() if ws is not None else 0, nat.stream(dev))
+        return dx, dw, db, dout if need_r else None, None
+
+
+def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, act: str = "none",
+                 residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual``.
+
+    x [..., K] and weight [N, K] in one of fp32 / fp16 / bf16; bias [N] of any
+    of these; residual [..., N] in x's dtype or fp32.  The output has the
+    residual's dtype, else x's.  act: "none", "relu", "gelu" (exact) or
+    "silu".  Differentiable once in x, weight, bias and residual."""
+    code = _act_code(act)
+    _check(x, weight, bias, residual)
+    if x.dtype not in _FLOATS or weight.dtype != x.dtype:
+        raise RuntimeError(f"linear: input ({x.dtype}) and weight ({weight.dtype}) must share one of fp32, fp16, bf16")
+    if residual is not None and residual.dtype not in (x.dtype, torch.float32):
+        raise RuntimeError(f"linear: residual must be {x.dtype} or float32, got {residual.dtype}")
+    return FusedLinearFunction.apply(x, weight, bias, residual, code)
+
+
+class FusedLinear(nn.Linear):
+    """nn.Linear with an activation and a residual in the kernel's epilogue.
+    Under CUDA autocast the operands are in the autocast dtype; a residual
+    keeps its own dtype when that is fp32."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, act: str = "none", device=None,
+                 dtype=None):
+        super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
+        _act_code(act)
+        self.act = act
+
+    def forward(self, x, residual=None):
+        w, b = self.weight, self.bias
+        if torch.is_autocast_enabled("cuda"):
+            dt = torch.get_autocast_dtype("cuda")
+            x, w = x.to(dt), w.to(dt)
+            if residual is not None and residual.dtype not in (dt, torch.float32):
+                residual = residual.to(dt)
+        return fused_linear(x, w, b, self.act, residual)
+
+
+# ----------------------------------------------------------- 8-bit operands --
+
+def quantize_e4m3(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of x [..., C] as e4m3 values and the fp32 scale [...] of each row:
+    x ~ q * scale, scale = max|row| / 448 (1 for a zero row)."""
+    nat.require_cuda(x)
+    if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in _FLOATS:
+        raise RuntimeError("quantize_e4m3: needs fp32, fp16 or bf16 rows of at least one value")
+    xc = nat.dense(x.detach())
+    C = x.shape[-1]
+    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    nat.call_on(x.device, "affb_quantize_e4m3", nat.ptr(xc), nat.dcode(xc), xc.numel() // C, C, nat.ptr(q),
+                nat.ptr(scale), nat.stream(x.device))
+    return q, scale
+
+
+def linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                bias: torch.Tensor | None = None, act: str = "none", residual: torch.Tensor | None = None,
+                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``act((x * x_scale) @ (weight * weight_scale).T + bias) + residual`` for
+    e4m3 x [..., K] and weight [N, K] with fp32 scales per row ([...] and
+    [N]); bias fp32; residual of any float dtype; forward only."""
+    code = _act_code(act)
+    _check(x, weight, bias, residual)
+    if x.dtype != torch.float8_e4m3fn or weight.dtype != torch.float8_e4m3fn:
+        raise RuntimeError("linear_e4m3: input and weight must be float8_e4m3fn")
+    if out_dtype not in _FLOATS or (residual is not None and residual.dtype not in _FLOATS):
+        raise RuntimeError("linear_e4m3: output and residual must be fp32, fp16 or bf16")
+    N, K = weight.shape
+    if tuple(x_scale.shape) != tuple(x.shape[:-1]) or tuple(weight_scale.shape) != (N,):
+        raise RuntimeError("linear_e4m3: scales must have one value per row")
+    nat.require_cuda(x_scale, weight_scale)
+    dev = x.device
+    if x_scale.device != dev or weight_scale.device != dev:
+        raise RuntimeError("linear_e4m3: tensors are on different devices")
+    M = x.numel() // K
+    xc, wc = nat.dense(x), nat.dense(weight)
+    xs, wsc = x_scale.to(torch.float32).contiguous(), weight_scale.to(torch.float32).contiguous()
+    bc = bias.to(torch.float32).contiguous() if bias is not None else None
+    rc = residual.contiguous() if residual is not None else None
+    out = torch.empty((*x.shape[:-1], N), device=dev, dtype=out_dtype)
+    ws = nat.workspace("affb_linear_e4m3_workspace_bytes", dev, M, N, K)
+    nat.call_on(dev, "affb_linear_e4m3", nat.ptr(xc), nat.ptr(xs), nat.ptr(wc), nat.ptr(wsc), nat.ptr(bc), nat.ptr(rc),
+                nat.dcode(rc) if rc is not None else 0, code, M, N, K, nat.ptr(out), nat.dcode(out), nat.ptr(ws),
+                ws.numel() if ws is not None else 0, nat.stream(dev))
+    return out
+
+
+class LinearE4M3(nn.Module):
+    """A trained Linear kept as e4m3 rows for inference (``from_linear``);
+    forward takes the e4m3 rows and scales that ``rms_norm_e4m3`` writes."""
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None, act: str = "none"):
+        super().__init__()
+        _act_code(act)
+        q, scale = quantize_e4m3(weight)
+        self.act = act
+        self.register_buffer("weight", q)
+        self.register_buffer("weight_scale", scale)
+        self.register_buffer("bias", bias.detach().float() if bias is not None else None)
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, act: str | None = None) -> "LinearE4M3":
+        return cls(linear.weight, linear.bias, act if act is not None else getattr(linear, "act", "none"))
+
+    def forward(self, q, q_scale, residual=None, out_dtype=torch.bfloat16):
+        return linear_e4m3(q, q_scale, self.weight, self.weight_scale, self.bias, self.act, residual, out_dtype)
+
+
+def linear_status() -> bool:
+    """True unless a product on the current device gave up a bounded wait
+    (which leaves its output incomplete).  Synchronises."""
+    import ctypes
+    failed = ctypes.c_int(0)
+    nat.call("affb_linear_status", ctypes.addressof(failed))
+    return failed.value == 0

@@ -1,0 +1,144 @@
+"""Root-mean-square norm with the residual's addition, and its 8-bit output.
+
+* ``fused_rms_norm(x, weight, eps, delta, row_scale, out_dtype)``:
+  ``s = x + row_scale * delta`` (the residual stream, in x's dtype) and
+  ``y = s * rsqrt(mean(s^2) + eps) * weight`` in one pass, with the backward
+  in one pass over the gradients of both;
+* ``rms_norm_e4m3``: the same with y as e4m3 rows and one fp32 scale per row,
+  the operand of ``linear_e4m3`` (forward only);
+* ``FusedRMSNorm``: the module.
+
+Statistics are fp32, taken of the sum before it is rounded to x's dtype; the
+backward reads the rounded sum.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from .. import _native as nat
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _check(x, weight, delta, row_scale):
+    nat.require_cuda(x, weight, delta, row_scale)
+    if x.dim() < 1 or tuple(weight.shape) != (x.shape[-1],) or x.shape[-1] < 1:
+        raise RuntimeError(f"rms_norm: weight {tuple(weight.shape)} does not match the rows of {tuple(x.shape)}")
+    for t in (x, weight) + ((delta,) if delta is not None else ()):
+        if t.dtype not in _FLOATS:
+            raise RuntimeError(f"rms_norm: unsupported dtype {t.dtype}; expected float32, float16 or bfloat16")
+    if delta is not None and delta.shape != x.shape:
+        raise RuntimeError(f"rms_norm: delta {tuple(delta.shape)} does not have the shape {tuple(x.shape)} of x")
+    if row_scale is not None:
+        if delta is None:
+            raise RuntimeError("rms_norm: row_scale scales delta, which is missing")
+        rows = x.numel() // x.shape[-1]
+        if row_scale.dim() != 1 or row_scale.numel() < 1 or rows % row_scale.numel():
+            raise RuntimeError(f"rms_norm: row_scale [{row_scale.numel()}] does not divide {rows} rows")
+    for t in (weight, delta, row_scale):
+        if t is not None and t.device != x.device:
+            raise RuntimeError("rms_norm: tensors are on different devices")
+
+
+def _launch(x, delta, row_scale, weight, eps, out_dtype, keep, want_s):
+    """One forward pass; out_dtype None writes e4m3 rows and scales."""
+    C = x.shape[-1]
+    R = x.numel() // C
+    dev = x.device
+    xc = nat.dense(x)
+    dc = nat.dense(delta) if delta is not None else None
+    rs = row_scale.float().contiguous() if row_scale is not None else None
+    w = nat.dense(weight.detach().float())
+    s = torch.empty(x.shape, device=dev, dtype=x.dtype) if dc is not None and want_s else None
+    rstd = torch.empty(R, device=dev, dtype=torch.float32) if keep else None
+    y = q = scale = None
+    if out_dtype is None:
+        q = torch.empty(x.shape, device=dev, dtype=torch.float8_e4m3fn)
+        scale = torch.empty(x.shape[:-1], device=dev, dtype=torch.float32)
+    else:
+        y = torch.empty(x.shape, device=dev, dtype=out_dtype)
+    nat.call_on(dev, "affb_rms_norm_fwd", nat.ptr(xc), nat.dcode(xc), nat.ptr(dc),
+                nat.dcode(dc) if dc is not None else 0, nat.ptr(rs), rs.numel() if rs is not None else 0, nat.ptr(w),
+                float(eps), R, C, nat.ptr(s), nat.ptr(rstd), nat.ptr(y), nat.dcode(y) if y is not None else 0,
+                nat.ptr(q), nat.ptr(scale), nat.stream(dev))
+    return xc, rs, w, s, rstd, y, q, scale
+
+
+class FusedRMSNormFunction(Function):
+    @staticmethod
+    def forward(ctx, x, weight, delta, row_scale, eps, out_dtype):
+        ctx.set_materialize_grads(False)
+        keep = any(ctx.needs_input_grad[:3])
+        xc, rs, w, s, rstd, y, _, _ = _launch(x, delta, row_scale, weight, eps, out_dtype, keep, True)
+        if keep:
+            ctx.save_for_backward(xc if s is None else s, rstd, w, rs)
+            ctx.meta = (weight.dtype, delta.dtype if delta is not None else None, out_dtype)
+        return y if s is None else (s, y)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        s, rstd, w, rs = ctx.saved_tensors
+        wdt, ddt, ydt = ctx.meta
+        C = s.shape[-1]
+        R = s.numel() // C
+        dev = s.device
+        ds, dy = grads if ddt is not None else (None, grads[0])
+        ds = nat.dense(ds) if ds is not None else None
+        dy = nat.dense(dy) if dy is not None else None
+        need_x, need_w, need_d = ctx.needs_input_grad[:3]
+        dx = torch.empty(s.shape, device=dev, dtype=s.dtype) if need_x else None
+        dd = torch.empty(s.shape, device=dev, dtype=ddt) if need_d else None
+        dw = torch.empty(C, device=dev, dtype=torch.float32) if need_w else None
+        ws = nat.workspace("affb_rms_norm_bwd_workspace_bytes", dev, R, C) if need_w else None
+        nat.call_on(dev, "affb_rms_norm_bwd", nat.ptr(dy), nat.dcode(dy) if dy is not None else 0, nat.ptr(ds),
+                    nat.ptr(s), nat.dcode(s), nat.ptr(rstd), nat.ptr(w), nat.ptr(rs), rs.numel() if rs is not None else 0,
+                    R, C, nat.ptr(dx), nat.ptr(dd), nat.dcode(dd) if dd is not None else 0, nat.ptr(dw), nat.ptr(ws),
+                    ws.numel() if ws is not None else 0, nat.stream(dev))
+        return dx, dw.to(wdt) if need_w else None, dd, None, None, None
+
+
+def fused_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, delta: torch.Tensor | None = None,
+                   row_scale: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
+    """y, or (s, y) when ``delta`` is given: ``s = x + row_scale * delta`` in
+    x's dtype and ``y = s * rsqrt(mean(s^2) + eps) * weight`` in ``out_dtype``
+    (x's by default).
+
+    x [..., C] and delta of the same shape, each fp32 / fp16 / bf16;
+    row_scale [G]: one factor per G-th of the rows (stochastic depth per
+    sample), no gradient.  Differentiable once in x, weight and delta."""
+    _check(x, weight, delta, row_scale)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _FLOATS:
+        raise RuntimeError(f"rms_norm: unsupported output dtype {out_dtype}")
+    return FusedRMSNormFunction.apply(x, weight, delta, row_scale, eps, out_dtype)
+
+
+@torch.no_grad()
+def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, delta: torch.Tensor | None = None,
+                  row_scale: torch.Tensor | None = None):
+    """(q, scale), or (s, q, scale) when ``delta`` is given: the norm with its
+    output as e4m3 rows, ``y ~ q * scale``, ``scale = max|y| / 448`` of each
+    row (1 for a zero row).  No gradient."""
+    _check(x, weight, delta, row_scale)
+    _, _, _, s, _, _, q, scale = _launch(x, delta, row_scale, weight, eps, None, False, True)
+    return (q, scale) if delta is None else (s, q, scale)
+
+
+class FusedRMSNorm(nn.Module):
+    """``forward(x)`` -> y; ``forward(x, delta, row_scale)`` -> (s, y)."""
+
+    def __init__(self, dim: int, eps: float = 1e-6, device=None, dtype=None):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim, device=device, dtype=dtype))
+
+    def forward(self, x, delta=None, row_scale=None, out_dtype=None):
+        return fused_rms_norm(x, self.weight, self.eps, delta, row_scale, out_dtype)
+
+    def quantized(self, x, delta=None, row_scale=None):
+        """(q, scale) or (s, q, scale): ``rms_norm_e4m3`` with this weight."""
+        return rms_norm_e4m3(x, self.weight, self.eps, delta, row_scale)

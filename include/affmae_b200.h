@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-enum { AFFB_F32 = 0, AFFB_F16 = 1, AFFB_BF16 = 2 };
+enum { AFFB_F32 = 0, AFFB_F16 = 1, AFFB_BF16 = 2, AFFB_E4M3 = 3 };
 enum { AFFB_OK = 0, AFFB_ERR_INVALID = 1, AFFB_ERR_CUDA = 2 };
 
 /* Last error message of the calling thread ("" if none). */
@@ -357,6 +357,89 @@ int affb_mssample_bwd(const float* dw, const float* sl, const float* kv_pos,
  * dst[i] = (T) src[i] for n elements (fp32 accumulator -> storage dtype).
  * No counterpart in the reference (it casts with torch's .to()).           */
 int affb_cast_f32(const float* src, void* dst, int dtype, int64_t n, void* stream);
+
+/* ============================================ encoder-block operators ==
+ * No counterpart among the reference's kernels: the operators of an encoder
+ * block of root-mean-square norms around the neighbourhood attention.
+ *
+ * ---------------------------------------------------- matrix product --
+ * z = x w^T + bias, out = act(z) + residual.  x [M,K] T, weight [N,K] T,
+ * bias [N] bias_dtype or NULL, residual [M,N] residual_dtype or NULL,
+ * out [M,N] out_dtype (T or fp32), z [M,N] T or NULL: the pre-activation
+ * sums for the backward.  N, K >= 1, M >= 0.  x and weight 16-byte aligned.
+ * Sums are fp32; fp32 operands are multiplied as three bf16 parts each
+ * (error of the order of 2^-24; an infinite operand gives NaN).
+ * workspace: affb_linear_fwd_workspace_bytes(...) bytes, 256-byte aligned, no
+ * initial contents (NULL where that is 0).                                 */
+enum { AFFB_ACT_NONE = 0, AFFB_ACT_RELU = 1, AFFB_ACT_GELU = 2, AFFB_ACT_SILU = 3 };
+int64_t affb_linear_fwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+int affb_linear_fwd(const void* x, const void* weight, const void* bias, int bias_dtype, const void* residual,
+                    int residual_dtype, int act, int dtype, int64_t M, int64_t N, int64_t K, void* out,
+                    int out_dtype, void* z, void* workspace, int64_t workspace_bytes, void* stream);
+/* dz = dout act'(z); dx = dz w, dweight = dz^T x, dbias = column sums of dz.
+ * dout [M,N] dout_dtype (T or fp32); z as written by the forward (for ReLU
+ * without a residual its output will do; NULL without activation); dx [M,K]
+ * T, dweight [N,K] T, dbias [N] dbias_dtype, each written unless NULL.      */
+int64_t affb_linear_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+int affb_linear_bwd(const void* dout, int dout_dtype, const void* z, const void* x, const void* weight, int act,
+                    int dtype, int64_t M, int64_t N, int64_t K, void* dx, void* dweight, void* dbias, int dbias_dtype,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+/* The forward for e4m3 operands: z[m,n] = x_scale[m] weight_scale[n]
+ * sum_k x[m,k] weight[n,k] + bias[n].  x [M,K], weight [N,K] e4m3 bytes,
+ * scales and bias fp32, out of any float type.                             */
+int64_t affb_linear_e4m3_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int affb_linear_e4m3(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
+                     const float* bias, const void* residual, int residual_dtype, int act, int64_t M, int64_t N,
+                     int64_t K, void* out, int out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+/* 1 in *failed if a product on this device ever gave up one of its bounded
+ * waits (its output is then incomplete), else 0.  Synchronises.             */
+int affb_linear_status(int* failed);
+
+/* ------------------------------------------- root-mean-square norm --
+ * s = x + f delta, y = s (mean(s^2) + eps)^-1/2 weight over rows of C.
+ * x [R,C] x_dtype, delta [R,C] delta_dtype or NULL, row_scale [groups] fp32
+ * or NULL: f of each R / groups consecutive rows, weight [C] fp32;
+ * s [R,C] x_dtype (NULL: not wanted; only with delta), rstd [R] fp32 or NULL
+ * (kept for the backward).  Exactly one of y [R,C] y_dtype and q is written:
+ * q [R,C] e4m3 with q_scale [R] fp32, y = q q_scale,
+ * q_scale = max|y| / 448 of the row (1 for a zero row).                     */
+int affb_rms_norm_fwd(const void* x, int x_dtype, const void* delta, int delta_dtype, const float* row_scale,
+                      int64_t groups, const float* weight, float eps, int64_t R, int64_t C, void* s, float* rstd,
+                      void* y, int y_dtype, void* q, float* q_scale, void* stream);
+/* Rows of x [R,C] as e4m3 values q [R,C] with q_scale [R]: the scale above,
+ * of the rows themselves (weights and inputs of affb_linear_e4m3).          */
+int affb_quantize_e4m3(const void* x, int dtype, int64_t R, int64_t C, void* q, float* q_scale, void* stream);
+/* dy [R,C] y_dtype or NULL, ds [R,C] x_dtype or NULL: gradients of y and s;
+ * s [R,C] x_dtype: the forward's sum (x itself without delta).  dx [R,C]
+ * x_dtype, ddelta [R,C] delta_dtype, dweight [C] fp32, each written unless
+ * NULL.  workspace: affb_rms_norm_bwd_workspace_bytes(R, C) bytes.          */
+int64_t affb_rms_norm_bwd_workspace_bytes(int64_t R, int64_t C);
+int affb_rms_norm_bwd(const void* dy, int y_dtype, const void* ds, const void* s, int x_dtype, const float* rstd,
+                      const float* weight, const float* row_scale, int64_t groups, int64_t R, int64_t C, void* dx,
+                      void* ddelta, int delta_dtype, float* dweight, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+/* ------------------------------------- bucketed relative-position bias --
+ * out[b,h,i,m] = table[row, h], row from the offsets d = round(k_pos - q_pos)
+ * of the pair: with c(n) = number of edges <= n, an axis has index
+ * n_edges + sign(d) c(|d|), or one sided c(max(-d, 0)); two axes (x, y)
+ * combine as index(y) * n + index(x), n = 2 n_edges + 1 (n_edges + 1).
+ * edges: host array, ascending in [1, 2^30], at most 64 (32 with two axes);
+ * table [n^axes, H]; q_pos [B,Nq,axes], k_pos [B,Nk,axes] of pos_type;
+ * member_idx [B,Nq,M] int32 key indices, or NULL: all keys (M = Nk); an index
+ * outside [0, Nk) gives bias 0.  out [B,H,Nq,M].                            */
+enum { AFFB_POS_F32 = 0, AFFB_POS_I32 = 1, AFFB_POS_I64 = 2 };
+int affb_bucket_bias_fwd(const void* table, int table_dtype, const int32_t* edges, int n_edges, int one_sided,
+                         const void* q_pos, const void* k_pos, int pos_type, int axes, const int32_t* member_idx,
+                         int64_t B, int64_t H, int64_t Nq, int64_t Nk, int64_t M, void* out, int out_dtype,
+                         void* stream);
+/* dtable [n^axes, H] table_dtype (written).  Deterministic.                 */
+int64_t affb_bucket_bias_bwd_workspace_bytes(int n_edges, int one_sided, int axes, int64_t B, int64_t H, int64_t Nq,
+                                             int64_t M);
+int affb_bucket_bias_bwd(const void* dout, int dout_dtype, const int32_t* edges, int n_edges, int one_sided,
+                         const void* q_pos, const void* k_pos, int pos_type, int axes, const int32_t* member_idx,
+                         int64_t B, int64_t H, int64_t Nq, int64_t Nk, int64_t M, void* dtable, int table_dtype,
+                         void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
