@@ -54,58 +54,7 @@ def _check_edges(edges) -> tuple[int, ...]:
     return tuple(int(e) for e in edges)
 
 
-class BucketBiasFunction(Function):
-    @staticmethod
-    def forward(ctx, table, edges, q_pos, k_pos, member_idx, one_sided, dtype):
-        arr = (ctypes.c_int32 * len(edges))(*edges)
-        dev = table.device
-        B, Nq, axes = q_pos.shape
-        Nk = k_pos.shape[1]
-        H = table.shape[1]
-        M = member_idx.shape[2] if member_idx is not None else Nk
-        tab, qp, kp = table.contiguous(), q_pos.contiguous(), k_pos.contiguous()
-        mem = member_idx
-        if mem is not None:
-            if mem.dtype == torch.int64:  # an index beyond 32 bits stays out of range
-                mem = mem.clamp(-1, 2 ** 31 - 1).to(torch.int32)
-            mem = nat.dense(mem)
-        out = torch.empty((B, H, Nq, M), device=dev, dtype=dtype)
-        nat.call_on(dev, "affb_bucket_bias_fwd", nat.ptr(tab), nat.dcode(tab), ctypes.addressof(arr), len(edges),
-                    int(one_sided), nat.ptr(qp), nat.ptr(kp), _POS[qp.dtype], axes, nat.ptr(mem), B, H, Nq, Nk, M,
-                    nat.ptr(out), nat.dcode(out), nat.stream(dev))
-        ctx.save_for_backward(qp, kp, mem)
-        ctx.meta = (edges, bool(one_sided), H, M, table.dtype)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        qp, kp, mem = ctx.saved_tensors
-        edges, one_sided, H, M, dt = ctx.meta
-        arr = (ctypes.c_int32 * len(edges))(*edges)
-        dev = qp.device
-        B, Nq, axes = qp.shape
-        Nk = kp.shape[1]
-        g = nat.dense(dout)
-        dtable = torch.empty((bucket_count(edges, axes, one_sided), H), device=dev, dtype=dt)
-        ws = nat.workspace("affb_bucket_bias_bwd_workspace_bytes", dev, len(edges), int(one_sided), axes, B, H, Nq, M)
-        nat.call_on(dev, "affb_bucket_bias_bwd", nat.ptr(g), nat.dcode(g), ctypes.addressof(arr), len(edges),
-                    int(one_sided), nat.ptr(qp), nat.ptr(kp), _POS[qp.dtype], axes, nat.ptr(mem), B, H, Nq, Nk, M,
-                    nat.ptr(dtable), nat.dcode(dtable), nat.ptr(ws), ws.numel() if ws is not None else 0,
-                    nat.stream(dev))
-        return dtable, None, None, None, None, None, None
-
-
-def bucket_bias(table: torch.Tensor, edges, q_pos: torch.Tensor, k_pos: torch.Tensor,
-                member_idx: torch.Tensor | None = None, one_sided: bool = False,
-                dtype: torch.dtype | None = None) -> torch.Tensor:
-    """bias [B, H, Nq, M] in ``dtype`` (the table's by default).
-
-    table [bucket_count(edges, axes, one_sided), H] fp32 / fp16 / bf16;
-    q_pos [B, Nq, axes] and k_pos [B, Nk, axes] in fp32, int32 or int64 with 1
-    or 2 axes (x, y); member_idx [B, Nq, M]: the keys of each query (an index
-    outside [0, Nk) gives a bias of 0), or None: all keys, M = Nk.
-    Differentiable once in the table."""
+def _check(table, edges, q_pos, k_pos, member_idx, one_sided, dtype) -> tuple[int, ...]:
     edges = _check_edges(edges)
     nat.require_cuda(table, q_pos, k_pos, member_idx)
     if q_pos.dim() != 3 or k_pos.dim() != 3 or q_pos.shape[2] not in (1, 2) or q_pos.shape[2] != k_pos.shape[2] \
@@ -124,12 +73,81 @@ def bucket_bias(table: torch.Tensor, edges, q_pos: torch.Tensor, k_pos: torch.Te
                                    or member_idx.dtype not in (torch.int32, torch.int64)):
         raise RuntimeError(f"bucket_bias: member_idx must be an int32 or int64 array [B, Nq, M], got "
                            f"{tuple(member_idx.shape)} {member_idx.dtype}")
-    dtype = table.dtype if dtype is None else dtype
     if dtype not in _FLOATS:
         raise RuntimeError(f"bucket_bias: unsupported output dtype {dtype}")
     for t in (q_pos, k_pos, member_idx):
         if t is not None and t.device != table.device:
             raise RuntimeError("bucket_bias: tensors are on different devices")
+    return edges
+
+
+def _members(member_idx):
+    if member_idx is None:
+        return None
+    if member_idx.dtype == torch.int64:  # an index beyond 32 bits stays out of range
+        member_idx = member_idx.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    return nat.dense(member_idx)
+
+
+def bucket_bias_fwd(table, edges, q_pos, k_pos, member_idx, one_sided, dtype):
+    """bias [B,H,Nq,M]; dense inputs, int32 members."""
+    arr = (ctypes.c_int32 * len(edges))(*edges)
+    B, Nq, axes = q_pos.shape
+    Nk, H = k_pos.shape[1], table.shape[1]
+    M = member_idx.shape[2] if member_idx is not None else Nk
+    dev = table.device
+    out = torch.empty((B, H, Nq, M), device=dev, dtype=dtype)
+    nat.call_on(dev, "affb_bucket_bias_fwd", nat.ptr(table), nat.dcode(table), ctypes.addressof(arr), len(edges),
+                int(one_sided), nat.ptr(q_pos), nat.ptr(k_pos), _POS[q_pos.dtype], axes, nat.ptr(member_idx), B, H, Nq,
+                Nk, M, nat.ptr(out), nat.dcode(out), nat.stream(dev))
+    return out
+
+
+def bucket_bias_bwd(dout, edges, q_pos, k_pos, member_idx, one_sided, dtype):
+    """The table's gradient in `dtype`; dense inputs, int32 members."""
+    arr = (ctypes.c_int32 * len(edges))(*edges)
+    B, Nq, axes = q_pos.shape
+    _, H, _, M = dout.shape
+    dev = dout.device
+    dtable = torch.empty((bucket_count(edges, axes, one_sided), H), device=dev, dtype=dtype)
+    ws = nat.workspace("affb_bucket_bias_bwd_workspace_bytes", dev, len(edges), int(one_sided), axes, B, H, Nq, M)
+    nat.call_on(dev, "affb_bucket_bias_bwd", nat.ptr(dout), nat.dcode(dout), ctypes.addressof(arr), len(edges),
+                int(one_sided), nat.ptr(q_pos), nat.ptr(k_pos), _POS[q_pos.dtype], axes, nat.ptr(member_idx), B, H, Nq,
+                k_pos.shape[1], M, nat.ptr(dtable), nat.dcode(dtable), nat.ptr(ws), ws.numel() if ws is not None else 0,
+                nat.stream(dev))
+    return dtable
+
+
+class BucketBiasFunction(Function):
+    @staticmethod
+    def forward(ctx, table, edges, q_pos, k_pos, member_idx, one_sided, dtype):
+        qp, kp, mem = q_pos.contiguous(), k_pos.contiguous(), _members(member_idx)
+        out = bucket_bias_fwd(table.contiguous(), edges, qp, kp, mem, one_sided, dtype)
+        ctx.save_for_backward(qp, kp, mem)
+        ctx.meta = (edges, bool(one_sided), table.dtype)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        qp, kp, mem = ctx.saved_tensors
+        edges, one_sided, dt = ctx.meta
+        dtable = bucket_bias_bwd(nat.dense(dout), edges, qp, kp, mem, one_sided, dt)
+        return dtable, None, None, None, None, None, None
+
+
+def bucket_bias(table: torch.Tensor, edges, q_pos: torch.Tensor, k_pos: torch.Tensor,
+                member_idx: torch.Tensor | None = None, one_sided: bool = False,
+                dtype: torch.dtype | None = None) -> torch.Tensor:
+    """bias [B, H, Nq, M] in ``dtype`` (the table's by default).
+
+    table [bucket_count(edges, axes, one_sided), H] fp32 / fp16 / bf16;
+    q_pos [B, Nq, axes] and k_pos [B, Nk, axes] in fp32, int32 or int64 with 1
+    or 2 axes (x, y); member_idx [B, Nq, M]: the keys of each query (an index
+    outside [0, Nk) gives a bias of 0), or None: all keys, M = Nk.
+    Differentiable once in the table."""
+    dtype = table.dtype if dtype is None else dtype
+    edges = _check(table, edges, q_pos, k_pos, member_idx, one_sided, dtype)
     return BucketBiasFunction.apply(table, edges, q_pos, k_pos, member_idx, one_sided, dtype)
 
 

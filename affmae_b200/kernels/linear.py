@@ -45,51 +45,82 @@ def _check(x, weight, bias, residual):
     for t in (weight, bias, residual):
         if t is not None and t.device != x.device:
             raise RuntimeError("linear: tensors are on different devices")
-    return out_shape
+
+
+def _check_operands(x, weight, bias, residual):
+    _check(x, weight, bias, residual)
+    if x.dtype not in _FLOATS or weight.dtype != x.dtype:
+        raise RuntimeError(f"linear: input ({x.dtype}) and weight ({weight.dtype}) must share one of fp32, fp16, bf16")
+    if residual is not None and residual.dtype not in (x.dtype, torch.float32):
+        raise RuntimeError(f"linear: residual must be {x.dtype} or float32, got {residual.dtype}")
+
+
+def linear_fwd(x, weight, bias, residual, act: int, save: bool):
+    """(out, z): the product and, where `save` asks for them and the output
+    does not serve (``linear_saves``), the pre-activation sums, else None.
+    x and weight dense."""
+    N, K = weight.shape
+    M = x.numel() // K
+    dev = x.device
+    out_shape = (*x.shape[:-1], N)
+    bc = bias.contiguous() if bias is not None else None
+    rc = residual.contiguous() if residual is not None else None
+    out = torch.empty(out_shape, device=dev, dtype=x.dtype if rc is None else rc.dtype)
+    z = torch.empty(out_shape, device=dev, dtype=x.dtype) if save and linear_saves(act, rc) else None
+    dt = nat.dcode(x)
+    ws = nat.workspace("affb_linear_fwd_workspace_bytes", dev, dt, M, N, K)
+    nat.call_on(dev, "affb_linear_fwd", nat.ptr(x), nat.ptr(weight), nat.ptr(bc),
+                nat.dcode(bc) if bc is not None else 0, nat.ptr(rc), nat.dcode(rc) if rc is not None else 0, act, dt,
+                M, N, K, nat.ptr(out), nat.dcode(out), nat.ptr(z), nat.ptr(ws), ws.numel() if ws is not None else 0,
+                nat.stream(dev))
+    return out, z
+
+
+def linear_saves(act: int, residual) -> bool:
+    """Whether the backward needs the pre-activation sums: not without an
+    activation, and the sign of ReLU's output serves as well as theirs."""
+    return act != 0 and not (act == ACTIVATIONS["relu"] and residual is None)
+
+
+def linear_bwd(dout, z, x, weight, act: int, need_x: bool, need_w: bool, bias_dtype):
+    """(dx, dw, db), None where not needed (`bias_dtype` None: no db).  dout,
+    x and weight dense; z as saved (the output itself for ReLU without a
+    residual)."""
+    N, K = weight.shape
+    M = x.numel() // K
+    dev = x.device
+    dx = torch.empty_like(x) if need_x else None
+    dw = torch.empty_like(weight) if need_w else None
+    db = torch.empty(N, device=dev, dtype=bias_dtype) if bias_dtype is not None else None
+    if need_x or need_w or db is not None:
+        dt = nat.dcode(x)
+        ws = nat.workspace("affb_linear_bwd_workspace_bytes", dev, dt, M, N, K)
+        nat.call_on(dev, "affb_linear_bwd", nat.ptr(dout), nat.dcode(dout), nat.ptr(z), nat.ptr(x), nat.ptr(weight), act,
+                    dt, M, N, K, nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.dcode(db) if db is not None else 0,
+                    nat.ptr(ws), ws.numel() if ws is not None else 0, nat.stream(dev))
+    return dx, dw, db
 
 
 class FusedLinearFunction(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        out_shape = (*x.shape[:-1], weight.shape[0])
-        N, K = weight.shape
-        M = x.numel() // K
-        dev = x.device
+        save = any(ctx.needs_input_grad[:3])
         xc, wc = nat.dense(x), nat.dense(weight)
-        bc = bias.contiguous() if bias is not None else None
-        rc = residual.contiguous() if residual is not None else None
-        out = torch.empty(out_shape, device=dev, dtype=x.dtype if rc is None else rc.dtype)
-        # the backward needs the pre-activation sums; the sign of ReLU's output serves as well
-        z = None
-        if any(ctx.needs_input_grad[:3]) and act:
-            z = out if act == ACTIVATIONS["relu"] and rc is None else torch.empty(out_shape, device=dev, dtype=x.dtype)
-        dt = nat.dcode(xc)
-        ws = nat.workspace("affb_linear_fwd_workspace_bytes", dev, dt, M, N, K)
-        nat.call_on(dev, "affb_linear_fwd", nat.ptr(xc), nat.ptr(wc), nat.ptr(bc),
-                    nat.dcode(bc) if bc is not None else 0, nat.ptr(rc), nat.dcode(rc) if rc is not None else 0, act,
-                    dt, M, N, K, nat.ptr(out), nat.dcode(out), None if z is out else nat.ptr(z), nat.ptr(ws),
-                    ws.numel() if ws is not None else 0, nat.stream(dev))
-        ctx.save_for_backward(xc, wc, z)
-        ctx.meta = (act, M, N, K, x.shape, bias.dtype if bias is not None else None)
+        out, z = linear_fwd(xc, wc, bias, residual, act, save)
+        if save:
+            ctx.save_for_backward(xc, wc, z if linear_saves(act, residual) else out if act else None)
+            ctx.meta = (act, bias.dtype if bias is not None else None)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        xc, wc, z = ctx.saved_tensors
-        act, M, N, K, xshape, bdt = ctx.meta
-        dev = xc.device
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
-        g = nat.dense(dout)
-        dx = torch.empty(xshape, device=dev, dtype=xc.dtype) if need_x else None
-        dw = torch.empty((N, K), device=dev, dtype=wc.dtype) if need_w else None
-        db = torch.empty(N, device=dev, dtype=bdt) if need_b else None
+        dx = dw = db = None
         if need_x or need_w or need_b:
-            dt = nat.dcode(xc)
-            ws = nat.workspace("affb_linear_bwd_workspace_bytes", dev, dt, M, N, K)
-            nat.call_on(dev, "affb_linear_bwd", nat.ptr(g), nat.dcode(g), nat.ptr(z), nat.ptr(xc), nat.ptr(wc), act, dt,
-                        M, N, K, nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.dcode(db) if db is not None else 0,
-                        nat.ptr(ws), ws.numel() if ws is not None else 0, nat.stream(dev))
+            xc, wc, z = ctx.saved_tensors
+            act, bdt = ctx.meta
+            dx, dw, db = linear_bwd(nat.dense(dout), z, xc, wc, act, need_x, need_w, bdt if need_b else None)
         return dx, dw, db, dout if need_r else None, None
 
 
@@ -102,11 +133,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     residual's dtype, else x's.  act: "none", "relu", "gelu" (exact) or
     "silu".  Differentiable once in x, weight, bias and residual."""
     code = _act_code(act)
-    _check(x, weight, bias, residual)
-    if x.dtype not in _FLOATS or weight.dtype != x.dtype:
-        raise RuntimeError(f"linear: input ({x.dtype}) and weight ({weight.dtype}) must share one of fp32, fp16, bf16")
-    if residual is not None and residual.dtype not in (x.dtype, torch.float32):
-        raise RuntimeError(f"linear: residual must be {x.dtype} or float32, got {residual.dtype}")
+    _check_operands(x, weight, bias, residual)
     return FusedLinearFunction.apply(x, weight, bias, residual, code)
 
 

@@ -43,8 +43,10 @@ def _check(x, weight, delta, row_scale):
             raise RuntimeError("rms_norm: tensors are on different devices")
 
 
-def _launch(x, delta, row_scale, weight, eps, out_dtype, keep, want_s):
-    """One forward pass; out_dtype None writes e4m3 rows and scales."""
+def _launch(x, delta, row_scale, weight, eps, out_dtype, keep):
+    """One forward pass: (x, row_scale, weight as the kernel read them, s, rstd,
+    y, q, scale).  out_dtype None writes e4m3 rows and scales; rstd only with
+    `keep`, s only with delta."""
     C = x.shape[-1]
     R = x.numel() // C
     dev = x.device
@@ -52,7 +54,7 @@ def _launch(x, delta, row_scale, weight, eps, out_dtype, keep, want_s):
     dc = nat.dense(delta) if delta is not None else None
     rs = row_scale.float().contiguous() if row_scale is not None else None
     w = nat.dense(weight.detach().float())
-    s = torch.empty(x.shape, device=dev, dtype=x.dtype) if dc is not None and want_s else None
+    s = torch.empty(x.shape, device=dev, dtype=x.dtype) if dc is not None else None
     rstd = torch.empty(R, device=dev, dtype=torch.float32) if keep else None
     y = q = scale = None
     if out_dtype is None:
@@ -67,37 +69,44 @@ def _launch(x, delta, row_scale, weight, eps, out_dtype, keep, want_s):
     return xc, rs, w, s, rstd, y, q, scale
 
 
+def rms_norm_bwd(dy, ds, s, rstd, weight, row_scale, need_x: bool, need_w: bool, delta_dtype):
+    """(dx, dw, ddelta), None where not needed (`delta_dtype` None: no
+    ddelta); weight, row_scale, dw fp32; dy or ds may be None."""
+    C = s.shape[-1]
+    R = s.numel() // C
+    dev = s.device
+    dx = torch.empty_like(s) if need_x else None
+    dd = torch.empty(s.shape, device=dev, dtype=delta_dtype) if delta_dtype is not None else None
+    dw = torch.empty(C, device=dev, dtype=torch.float32) if need_w else None
+    ws = nat.workspace("affb_rms_norm_bwd_workspace_bytes", dev, R, C) if need_w else None
+    nat.call_on(dev, "affb_rms_norm_bwd", nat.ptr(dy), nat.dcode(dy) if dy is not None else 0, nat.ptr(ds), nat.ptr(s),
+                nat.dcode(s), nat.ptr(rstd), nat.ptr(weight), nat.ptr(row_scale),
+                row_scale.numel() if row_scale is not None else 0, R, C, nat.ptr(dx), nat.ptr(dd),
+                nat.dcode(dd) if dd is not None else 0, nat.ptr(dw), nat.ptr(ws), ws.numel() if ws is not None else 0,
+                nat.stream(dev))
+    return dx, dw, dd
+
+
 class FusedRMSNormFunction(Function):
     @staticmethod
     def forward(ctx, x, weight, delta, row_scale, eps, out_dtype):
         ctx.set_materialize_grads(False)
         keep = any(ctx.needs_input_grad[:3])
-        xc, rs, w, s, rstd, y, _, _ = _launch(x, delta, row_scale, weight, eps, out_dtype, keep, True)
+        xc, rs, w, s, rstd, y, _, _ = _launch(x, delta, row_scale, weight, eps, out_dtype, keep)
         if keep:
             ctx.save_for_backward(xc if s is None else s, rstd, w, rs)
-            ctx.meta = (weight.dtype, delta.dtype if delta is not None else None, out_dtype)
+            ctx.meta = (weight.dtype, delta.dtype if delta is not None else None)
         return y if s is None else (s, y)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
         s, rstd, w, rs = ctx.saved_tensors
-        wdt, ddt, ydt = ctx.meta
-        C = s.shape[-1]
-        R = s.numel() // C
-        dev = s.device
+        wdt, ddt = ctx.meta
         ds, dy = grads if ddt is not None else (None, grads[0])
-        ds = nat.dense(ds) if ds is not None else None
-        dy = nat.dense(dy) if dy is not None else None
         need_x, need_w, need_d = ctx.needs_input_grad[:3]
-        dx = torch.empty(s.shape, device=dev, dtype=s.dtype) if need_x else None
-        dd = torch.empty(s.shape, device=dev, dtype=ddt) if need_d else None
-        dw = torch.empty(C, device=dev, dtype=torch.float32) if need_w else None
-        ws = nat.workspace("affb_rms_norm_bwd_workspace_bytes", dev, R, C) if need_w else None
-        nat.call_on(dev, "affb_rms_norm_bwd", nat.ptr(dy), nat.dcode(dy) if dy is not None else 0, nat.ptr(ds),
-                    nat.ptr(s), nat.dcode(s), nat.ptr(rstd), nat.ptr(w), nat.ptr(rs), rs.numel() if rs is not None else 0,
-                    R, C, nat.ptr(dx), nat.ptr(dd), nat.dcode(dd) if dd is not None else 0, nat.ptr(dw), nat.ptr(ws),
-                    ws.numel() if ws is not None else 0, nat.stream(dev))
+        dx, dw, dd = rms_norm_bwd(nat.dense(dy) if dy is not None else None, nat.dense(ds) if ds is not None else None,
+                                  s, rstd, w, rs, need_x, need_w, ddt if need_d else None)
         return dx, dw.to(wdt) if need_w else None, dd, None, None, None
 
 
@@ -124,7 +133,7 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, delt
     output as e4m3 rows, ``y ~ q * scale``, ``scale = max|y| / 448`` of each
     row (1 for a zero row).  No gradient."""
     _check(x, weight, delta, row_scale)
-    _, _, _, s, _, _, q, scale = _launch(x, delta, row_scale, weight, eps, None, False, True)
+    _, _, _, s, _, _, q, scale = _launch(x, delta, row_scale, weight, eps, None, False)
     return (q, scale) if delta is None else (s, q, scale)
 
 

@@ -36,14 +36,17 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _native as nat
+from .kernels.bucket_bias import BucketBias
 from .kernels.fused_deform_attn import (fused_knn_deformable_cross_attention,
                                         fused_knn_deformable_self_attention)
 from .kernels.head_layout import merge_heads, split_heads
 from .kernels.knn import knn
 from .kernels.layer_norm import FusedLayerNorm
+from .kernels.linear import FusedLinear, LinearE4M3
 from .kernels.local_attn import FlashLocalAttentionFunction
 from .kernels.pos_bias import pos_bias_gather, rel_pos_bias
 from .kernels.relu_dropout import relu_dropout
+from .kernels.rms_norm import FusedRMSNorm
 from .kernels.token_mask import apply_token_mask
 from .kernels.weighted_features import weighted_features
 from .workloads import REL_POS_WIDTH, TABLE_WIDTH, relative_position_table
@@ -69,6 +72,10 @@ class MAEConfig:
     decoder_heads: int = 6
     decoder_dropout: float = 0.1
     loss_weights: tuple = field(default=(0.05, 0.12, 1.0))  # res5, res4, res2 heads
+    # encoder blocks: "layer" (the reference's) or "rms" (root-mean-square
+    # norms, fused matrix products, bucketed position bias)
+    block: str = "layer"
+    bias_edges: tuple = (1, 2, 3, 4, 7, 13, 24)             # distances in tokens where a bias bucket begins
 
 
 # ------------------------------------------------------------- clustering --
@@ -286,6 +293,98 @@ class ClusterBlock(nn.Module):
         return feat, (self.fc2(F.gelu(self.fc1(h))), self.drop_path.factor(B, feat.device))
 
 
+class BucketAttention(nn.Module):
+    """Neighbourhood attention with a bucketed relative-position bias and a
+    per-head blank token, on the fused matrix products."""
+
+    def __init__(self, dim: int, heads: int, edges: tuple):
+        super().__init__()
+        self.heads = heads
+        self.scale = (dim // heads) ** -0.5
+        self.q = FusedLinear(dim, dim)
+        self.kv = FusedLinear(dim, 2 * dim)
+        self.blank_k = nn.Parameter(torch.randn(dim) * 0.2)
+        self.blank_v = nn.Parameter(torch.randn(dim) * 0.2)
+        self.bias = BucketBias(heads, edges)
+        self.proj = FusedLinear(dim, dim)
+
+    def forward(self, q, kv, member_idx, mask, pos, global_attn: bool = False, residual=None):
+        """q [B,N,C] and kv [B,N,2C] as projected; the output projection adds
+        `residual` (None: nothing) in its epilogue."""
+        B, N, C = q.shape
+        H, d = self.heads, C // self.heads
+        q = split_heads(q, H)
+        k, v = split_heads(kv, H, 2)
+        bk, bv = self.blank_k.view(H, d), self.blank_v.view(H, d)
+        if global_attn:  # every token and the blank one, whose bias is zero (PyTorch's attention, library code)
+            bias = F.pad(self.bias(pos, pos, dtype=q.dtype), (0, 1))
+            bk, bv = (t.view(1, H, 1, d).expand(B, -1, -1, -1).to(q.dtype) for t in (bk, bv))
+            out = F.scaled_dot_product_attention(q, torch.cat([k, bk], 2), torch.cat([v, bv], 2), attn_mask=bias)
+            return self.proj(merge_heads(out.contiguous()), residual)
+        bias = self.bias(pos, pos, member_idx, q.dtype)
+        out = FlashLocalAttentionFunction.apply(q, k, v, member_idx, bias, None if mask is None else mask[:, None],
+                                                bk, bv, float(self.scale))
+        return self.proj(merge_heads(out), residual)
+
+
+class RMSClusterBlock(nn.Module):
+    """Pre-norm encoder block on the fused operators: root-mean-square norms
+    that add the residual branch, bucketed position bias, matrix products with
+    GELU or the residual in their epilogue.
+
+    A branch that stochastic depth scales is added by the next norm, which
+    takes the per-sample factor; any other is added to the stream by the
+    product's epilogue.  After ``quantize()`` (inference) the projections that
+    read a norm run on e4m3 operands."""
+
+    def __init__(self, dim: int, heads: int, mlp_ratio: float, drop_path: float, edges: tuple):
+        super().__init__()
+        self.norm1 = FusedRMSNorm(dim)
+        self.attn = BucketAttention(dim, heads, edges)
+        self.norm2 = FusedRMSNorm(dim)
+        hidden = int(dim * mlp_ratio)
+        self.fc1 = FusedLinear(dim, hidden, act="gelu")
+        self.fc2 = FusedLinear(hidden, dim)
+        self.drop_path = DropPath(drop_path)
+        self.eight_bit = None
+
+    def quantize(self):
+        """Keep e4m3 copies of the weights that read a norm and use them in
+        eval mode.  Returns self."""
+        self.eight_bit = nn.ModuleDict({n: LinearE4M3.from_linear(m) for n, m in
+                                        (("q", self.attn.q), ("kv", self.attn.kv), ("fc1", self.fc1))})
+        return self
+
+    def _project(self, norm, x, delta, factor, layers, names):
+        """The stream (x, or x + factor * delta) and its norm through `layers`."""
+        dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+        if self.eight_bit is not None and not self.training:
+            *s, q, scale = norm.quantized(x, delta, factor)
+            outs = [self.eight_bit[n](q, scale, out_dtype=dt) for n in names]
+        else:
+            y = norm(x, delta, factor, dt)
+            s, y = ((), y) if delta is None else ((y[0],), y[1])
+            outs = [m(y) for m in layers]
+        return s[0] if s else x, outs
+
+    def forward(self, feat, member_idx, mask, pos, global_attn: bool = False, pending=None):
+        """Returns (feat, pending) as ClusterBlock does."""
+        if pending is None and torch.is_autocast_enabled("cuda"):
+            feat = feat.float()  # the residual stream
+        delta, f = (None, None) if pending is None else pending
+        feat, (q, kv) = self._project(self.norm1, feat, delta, f, (self.attn.q, self.attn.kv), ("q", "kv"))
+        f = self.drop_path.factor(feat.shape[0], feat.device)
+        if f is None:
+            feat, delta = self.attn(q, kv, member_idx, mask, pos, global_attn, residual=feat), None
+        else:
+            delta = self.attn(q, kv, member_idx, mask, pos, global_attn)
+        feat, (h,) = self._project(self.norm2, feat, delta, f, (self.fc1,), ("fc1",))
+        f = self.drop_path.factor(feat.shape[0], feat.device)
+        if f is None:
+            return self.fc2(h, residual=feat), None
+        return feat, (self.fc2(h), f)
+
+
 def add_pending(feat, pending):
     """feat + factor * delta for a residual add left pending by ClusterBlock."""
     if pending is None:
@@ -340,7 +439,11 @@ class Stage(nn.Module):
     def __init__(self, dim, out_dim, depth, heads, cfg: MAEConfig, drop_paths):
         super().__init__()
         self.cfg = cfg
-        self.blocks = nn.ModuleList(ClusterBlock(dim, heads, cfg.mlp_ratio, dp) for dp in drop_paths)
+        if cfg.block not in ("layer", "rms"):
+            raise ValueError(f"unknown encoder block {cfg.block!r}; expected 'layer' or 'rms'")
+        self.blocks = nn.ModuleList(
+            RMSClusterBlock(dim, heads, cfg.mlp_ratio, dp, cfg.bias_edges) if cfg.block == "rms" else
+            ClusterBlock(dim, heads, cfg.mlp_ratio, dp) for dp in drop_paths)
         self.merge = None
         if out_dim is not None:
             self.prob_net = Linear(dim, 1)
@@ -353,8 +456,9 @@ class Stage(nn.Module):
         feat = feat.gather(1, order[..., None].expand(-1, -1, C))
         member, mask, pe_idx = neighbourhood(pos, means, cmask, self.cfg.nbhd_size, m)
         global_attn = self.cfg.nbhd_size >= n  # BasicLayer.forward, aff.py:421-424
-        att_pe = pe_idx
-        if global_attn:  # relative indices of every token pair (aff.py:458-459)
+        rms = self.cfg.block == "rms"
+        att_pe = pos if rms else pe_idx
+        if global_attn and not rms:  # relative indices of every token pair (aff.py:458-459)
             rel = ((pos[:, None, :, :] + REL_POS_WIDTH) - pos[:, :, None, :]).clamp(0, TABLE_WIDTH - 1)
             att_pe = (rel[..., 1] * TABLE_WIDTH + rel[..., 0]).long()
         pending = None
@@ -433,7 +537,12 @@ class Encoder(nn.Module):
                 nn.init.trunc_normal_(mod.kv.weight, std=0.02)
                 nn.init.xavier_uniform_(mod.pos_embed.weight)
                 nn.init.xavier_uniform_(mod.proj.weight)
-            elif isinstance(mod, ClusterBlock):
+            elif isinstance(mod, BucketAttention):
+                nn.init.trunc_normal_(mod.q.weight, std=0.02)
+                nn.init.trunc_normal_(mod.kv.weight, std=0.02)
+                nn.init.trunc_normal_(mod.bias.table, std=0.02)
+                nn.init.xavier_uniform_(mod.proj.weight)
+            elif isinstance(mod, (ClusterBlock, RMSClusterBlock)):
                 nn.init.xavier_uniform_(mod.fc1.weight)
                 nn.init.kaiming_uniform_(mod.fc2.weight, a=math.sqrt(5))
             elif isinstance(mod, ClusterMerging):
@@ -640,6 +749,17 @@ class AFFMaskedAutoEncoder(nn.Module):
         self.head_res5 = PredictionHead(D, out)
         self.head_res4 = PredictionHead(D, out)
         self.head_res2 = PredictionHead(D, out)
+
+    def quantize_encoder(self):
+        """Inference with 8-bit operands: every "rms" encoder block keeps e4m3
+        copies of the projections that read a norm (used in eval mode; call
+        again after a change of the weights).  Returns self."""
+        if self.cfg.block != "rms":
+            raise RuntimeError('quantize_encoder needs MAEConfig(block="rms")')
+        for mod in self.modules():
+            if isinstance(mod, RMSClusterBlock):
+                mod.quantize()
+        return self
 
     def patchify(self, imgs):
         p, c = self.cfg.patch_size, self.cfg.in_chans

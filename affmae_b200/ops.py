@@ -24,9 +24,13 @@ import torch
 from torch import Tensor
 from torch.library import custom_op
 
+from . import _native as _nat
+from .kernels import bucket_bias as _bb
 from .kernels import fused_deform_attn as _fd
 from .kernels import knn as _knn
+from .kernels import linear as _li
 from .kernels import local_attn as _la
+from .kernels import rms_norm as _rn
 from .kernels import weighted_features as _wf
 
 _EMPTY = (0,)
@@ -178,3 +182,170 @@ def _deform_backward(ctx, grad_out, grad_idx, grad_d2):
 
 
 deform_cross_fwd.register_autograd(_deform_backward, setup_context=_deform_setup)
+
+
+# --------------------------------------------------------- matrix product --
+@custom_op("affb200::linear_fwd", mutates_args=())
+def linear_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, residual: Optional[Tensor]
+               ) -> tuple[Tensor, Tensor]:
+    """(out, z): z holds the pre-activation sums, empty where the backward needs none."""
+    code = _li._act_code(act)
+    _li._check_operands(x, weight, bias, residual)
+    out, z = _li.linear_fwd(_nat.dense(x), _nat.dense(weight), bias, residual, code, True)
+    return out, (z if z is not None else x.new_empty(_EMPTY))
+
+
+@linear_fwd.register_fake
+def _(x, weight, bias, act, residual):
+    shape = (*x.shape[:-1], weight.shape[0])
+    saves = _li.linear_saves(_li._act_code(act), residual)
+    return (x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype),
+            x.new_empty(shape if saves else _EMPTY))
+
+
+@custom_op("affb200::linear_bwd", mutates_args=())
+def linear_bwd(dout: Tensor, z: Tensor, x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str
+               ) -> tuple[Tensor, Tensor, Tensor]:
+    dx, dw, db = _li.linear_bwd(_nat.dense(dout), _none_if_empty(z), _nat.dense(x), _nat.dense(weight),
+                                _li._act_code(act), True, True, bias.dtype if bias is not None else None)
+    return dx, dw, (db if db is not None else x.new_empty(_EMPTY))
+
+
+@linear_bwd.register_fake
+def _(dout, z, x, weight, bias, act):
+    return (x.new_empty(x.shape), weight.new_empty(weight.shape),
+            bias.new_empty(bias.shape) if bias is not None else x.new_empty(_EMPTY))
+
+
+def _linear_setup(ctx, inputs, output):
+    x, weight, bias, act, residual = inputs
+    out, z = output
+    code = _li._act_code(act)
+    ctx.save_for_backward(x, weight, bias, z if _li.linear_saves(code, residual) or not code else out)
+    ctx.act, ctx.residual = act, residual is not None
+
+
+def _linear_backward(ctx, grad_out, grad_z):
+    x, weight, bias, z = ctx.saved_tensors
+    dx, dw, db = linear_bwd(grad_out.contiguous(), z, x, weight, bias, ctx.act)
+    return dx, dw, _none_if_empty(db), None, grad_out if ctx.residual else None
+
+
+linear_fwd.register_autograd(_linear_backward, setup_context=_linear_setup)
+
+
+@custom_op("affb200::linear_e4m3", mutates_args=())
+def linear_e4m3(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor], act: str,
+                residual: Optional[Tensor], out_dtype: torch.dtype) -> Tensor:
+    return _li.linear_e4m3(x, x_scale, weight, weight_scale, bias, act, residual, out_dtype)
+
+
+@linear_e4m3.register_fake
+def _(x, x_scale, weight, weight_scale, bias, act, residual, out_dtype):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=out_dtype)
+
+
+# ---------------------------------------------------------------- RMS norm --
+@custom_op("affb200::rms_norm_fwd", mutates_args=())
+def rms_norm_fwd(x: Tensor, weight: Tensor, eps: float, delta: Optional[Tensor], row_scale: Optional[Tensor],
+                 out_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
+    """(s, y, rstd): s is empty without delta."""
+    _rn._check(x, weight, delta, row_scale)
+    _, _, _, s, rstd, y, _, _ = _rn._launch(x, delta, row_scale, weight, eps, out_dtype, True)
+    return (s if s is not None else x.new_empty(_EMPTY)), y, rstd
+
+
+@rms_norm_fwd.register_fake
+def _(x, weight, eps, delta, row_scale, out_dtype):
+    return (x.new_empty(x.shape if delta is not None else _EMPTY), x.new_empty(x.shape, dtype=out_dtype),
+            x.new_empty((x.numel() // x.shape[-1],), dtype=torch.float32))
+
+
+@custom_op("affb200::rms_norm_bwd", mutates_args=())
+def rms_norm_bwd(dy: Optional[Tensor], ds: Optional[Tensor], s: Tensor, rstd: Tensor, weight: Tensor,
+                 row_scale: Optional[Tensor], delta: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
+    dx, dw, dd = _rn.rms_norm_bwd(_nat.dense(dy) if dy is not None else None,
+                                  _nat.dense(ds) if ds is not None else None, _nat.dense(s), rstd,
+                                  _nat.dense(weight.float()),
+                                  row_scale.float().contiguous() if row_scale is not None else None, True, True,
+                                  delta.dtype if delta is not None else None)
+    return dx, dw.to(weight.dtype), (dd if dd is not None else s.new_empty(_EMPTY))
+
+
+@rms_norm_bwd.register_fake
+def _(dy, ds, s, rstd, weight, row_scale, delta):
+    return s.new_empty(s.shape), weight.new_empty(weight.shape), \
+        (delta.new_empty(delta.shape) if delta is not None else s.new_empty(_EMPTY))
+
+
+def _rms_setup(ctx, inputs, output):
+    x, weight, eps, delta, row_scale, out_dtype = inputs
+    s, y, rstd = output
+    ctx.save_for_backward(x if delta is None else s, rstd, weight, row_scale, delta)
+    ctx.set_materialize_grads(False)
+
+
+def _rms_backward(ctx, grad_s, grad_y, grad_rstd):
+    s, rstd, weight, row_scale, delta = ctx.saved_tensors
+    dx, dw, dd = rms_norm_bwd(grad_y, grad_s if delta is not None else None, s, rstd, weight, row_scale, delta)
+    return dx, dw, None, _none_if_empty(dd), None, None
+
+
+rms_norm_fwd.register_autograd(_rms_backward, setup_context=_rms_setup)
+
+
+@custom_op("affb200::rms_norm_e4m3", mutates_args=())
+def rms_norm_e4m3(x: Tensor, weight: Tensor, eps: float, delta: Optional[Tensor], row_scale: Optional[Tensor]
+                  ) -> tuple[Tensor, Tensor, Tensor]:
+    """(s, q, scale): s is empty without delta."""
+    got = _rn.rms_norm_e4m3(x, weight, eps, delta, row_scale)
+    return got if delta is not None else (x.new_empty(_EMPTY), *got)
+
+
+@rms_norm_e4m3.register_fake
+def _(x, weight, eps, delta, row_scale):
+    return (x.new_empty(x.shape if delta is not None else _EMPTY),
+            x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(x.shape[:-1], dtype=torch.float32))
+
+
+# ------------------------------------------------------------- bucket bias --
+@custom_op("affb200::bucket_bias_fwd", mutates_args=())
+def bucket_bias_fwd(table: Tensor, edges: list[int], q_pos: Tensor, k_pos: Tensor, member_idx: Optional[Tensor],
+                    one_sided: bool, dtype: torch.dtype) -> Tensor:
+    edges = _bb._check(table, edges, q_pos, k_pos, member_idx, one_sided, dtype)
+    return _bb.bucket_bias_fwd(table.contiguous(), edges, q_pos.contiguous(), k_pos.contiguous(),
+                               _bb._members(member_idx), one_sided, dtype)
+
+
+@bucket_bias_fwd.register_fake
+def _(table, edges, q_pos, k_pos, member_idx, one_sided, dtype):
+    M = member_idx.shape[2] if member_idx is not None else k_pos.shape[1]
+    return table.new_empty((q_pos.shape[0], table.shape[1], q_pos.shape[1], M), dtype=dtype)
+
+
+@custom_op("affb200::bucket_bias_bwd", mutates_args=())
+def bucket_bias_bwd(dout: Tensor, edges: list[int], q_pos: Tensor, k_pos: Tensor, member_idx: Optional[Tensor],
+                    one_sided: bool, dtype: torch.dtype) -> Tensor:
+    return _bb.bucket_bias_bwd(_nat.dense(dout), tuple(edges), q_pos.contiguous(), k_pos.contiguous(),
+                               _bb._members(member_idx), one_sided, dtype)
+
+
+@bucket_bias_bwd.register_fake
+def _(dout, edges, q_pos, k_pos, member_idx, one_sided, dtype):
+    return dout.new_empty((_bb.bucket_count(edges, q_pos.shape[2], one_sided), dout.shape[1]), dtype=dtype)
+
+
+def _bias_setup(ctx, inputs, output):
+    table, edges, q_pos, k_pos, member_idx, one_sided, _ = inputs
+    ctx.save_for_backward(q_pos, k_pos, member_idx)
+    ctx.meta = (edges, one_sided, table.dtype)
+
+
+def _bias_backward(ctx, grad):
+    q_pos, k_pos, member_idx = ctx.saved_tensors
+    edges, one_sided, dt = ctx.meta
+    return bucket_bias_bwd(grad.contiguous(), edges, q_pos, k_pos, member_idx, one_sided, dt), None, None, None, \
+        None, None, None
+
+
+bucket_bias_fwd.register_autograd(_bias_backward, setup_context=_bias_setup)
