@@ -8,6 +8,7 @@ used for device memory and streams only.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import threading
 from pathlib import Path
 
@@ -157,22 +158,6 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name} failed (code {rc}): {msg}")
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """``call`` with `device` current (kernels launch on the current device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        call(name, *args)
-    else:
-        with torch.cuda.device(device):
-            call(name, *args)
-
-
-def workspace(name: str, device, *args):
-    """Uninitialised device memory of the size the library's function `name`
-    asks for (None where it needs none), from the current stream's pool."""
-    n = getattr(lib(), name)(*args)
-    return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
-
-
 def dense(t: torch.Tensor) -> torch.Tensor:
     """`t` contiguous and 16-byte aligned (itself where it already is)."""
     t = t.contiguous()
@@ -192,6 +177,35 @@ def dcode(t: torch.Tensor) -> int:
 
 def stream(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with `device` current (kernels launch on the current device)
+    and that device's current stream as the last argument."""
+    index = device.index
+    if index == _current_device():
+        call(name, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, _raw_stream(torch.cuda.current_device()))
+
+
+# the interpreter-level queries behind torch.cuda.current_device() / current_stream(), without their wrappers
+# (a call of a few microseconds spends a third of its time there)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", stream)
+
+
+@functools.lru_cache(maxsize=4096)
+def _size(name: str, *args) -> int:
+    return getattr(lib(), name)(*args)
+
+
+def workspace(name: str, device, *args):
+    """Uninitialised device memory of the size the library's function `name`
+    asks for (None where it needs none), from the current stream's pool."""
+    n = _size(name, *args)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
 
 
 def require_cuda(*tensors) -> None:

@@ -8,9 +8,14 @@
 //   bias[b,h,i,m] = table[index, h],   dtable[index, h] = sum of dbias.
 // Keys are those of member_idx [B,Nq,M], or all Nk of the sequence.
 //
-// Forward: bound by the bytes of the lists read and the biases written; a
-// thread takes eight consecutive pairs, so that every access is 16 bytes or
-// more, and finds buckets by a byte table in shared memory.
+// The bytes that have to move are the lists and the biases; what bounds the
+// kernels is the load/store unit.  A lane takes two consecutive pairs (one
+// where rows of the output are not aligned for two), so that the lists, the
+// positions of a run of keys and the biases are read and written by
+// neighbouring lanes, and four such steps are in flight.  The table lies in
+// shared memory with four heads side by side (one access a pair and four
+// heads).  Where the distances up to the last edge are few it is expanded to
+// one entry per offset, so no bucket is looked up at all.
 //
 // Backward: bins in shared memory.  Float atomics would make the sums depend
 // on timing, so a block takes 2048 pairs at a time, scales their gradients by
@@ -22,15 +27,13 @@
 namespace affb {
 
 constexpr int BB_THREADS = 256;
-constexpr int BB_VEC = 8;
-constexpr int BB_TILE = BB_THREADS * BB_VEC;
-constexpr int BB_HEADS = 4;          // heads of one backward block
+constexpr int BB_STEPS = 4;          // steps of BB_THREADS * PAIRS pairs in a tile
+constexpr int BB_HEADS = 4;          // heads side by side in shared memory; heads of one backward block
 constexpr int BB_MAX_EDGES = 64;
-constexpr int BB_MAX_ROWS = 4225;    // 65 x 65
-constexpr int BB_LUT = 8192;         // distances answered by the byte table
+constexpr int BB_LUT = 8192;         // distances answered by a byte table, else the edges are searched
 constexpr int BB_BITS = 19;          // 2^19 * 2048 terms stay below 2^31
-constexpr int BB_NO_ROW = 0xFFFF;
 constexpr int BB_BLOCKS_PER_SM = 4;
+constexpr int BB_TABLE_SMEM = 64 * 1024;   // of one block's heads
 
 struct BucketArgs {
   int edges[BB_MAX_EDGES];
@@ -40,12 +43,23 @@ struct BucketArgs {
   int axes;
   int per_axis;         // index values of one axis
   int rows;             // rows of the table
+  int span;             // offsets of one axis up to the last edge: 2 last + 1 (one sided: last + 1)
   const void* q_pos;    // [B,Nq,axes]
   const void* k_pos;    // [B,Nk,axes]
   const int* member;    // [B,Nq,M] or null (M = Nk)
   int B, H;
   int64_t Nq, Nk, M, NM;
+  uint32_t div_mul, div_shift;  // n / M for n < 2^31 (div_shift 32: not usable)
 };
+
+// n / M by a multiplication (n < 2^31) where M allows it.
+__device__ __forceinline__ int64_t query_of(const BucketArgs& a, int64_t nm) {
+  if (a.div_shift < 32) {
+    const uint32_t n = (uint32_t)nm;
+    return (__umulhi(a.div_mul, n) + n) >> a.div_shift;
+  }
+  return nm / a.M;
+}
 
 __device__ __forceinline__ int offset_of(float k, float q) {
   const int d = __float2int_rn(k - q);  // saturates; NaN counts as 0
@@ -83,77 +97,143 @@ __device__ __forceinline__ int axis_index(const BucketArgs& a, const uint8_t* lu
   const int c = a.lut ? lut[min(n, a.lut - 1)] : search_edges(a, n);
   return a.one_sided ? c : d < 0 ? a.k - c : a.k + c;
 }
-// Table row of the pair (query qi, key ki) of one batch element.
-template <typename P>
-__device__ __forceinline__ int pair_row(const BucketArgs& a, const uint8_t* lut, const P* q, const P* kp, int64_t ki) {
-  if (ki < 0 || ki >= a.Nk) return BB_NO_ROW;
-  if (a.axes == 1) return axis_index(a, lut, offset_of(kp[ki], q[0]));
-  const P* p = kp + 2 * ki;
-  return axis_index(a, lut, offset_of(p[1], q[1])) * a.per_axis + axis_index(a, lut, offset_of(p[0], q[0]));
+// Index of an offset cut off at the last edge: [0, span).
+__device__ __forceinline__ int clipped(const BucketArgs& a, int d) {
+  const int last = a.lut - 1;
+  return a.one_sided ? min(max(-d, 0), last) : max(-last, min(last, d)) + last;
+}
+// The offset that `clipped` index i stands for.
+__device__ __forceinline__ int unclipped(const BucketArgs& a, int i) { return a.one_sided ? -i : i - (a.lut - 1); }
+
+// Entry of a pair in the table in shared memory: its row, or (BY_OFFSET) the
+// combined clipped offset.
+template <typename P, bool BY_OFFSET>
+__device__ __forceinline__ int entry1(const BucketArgs& a, const uint8_t* lut, P q, P k) {
+  const int d = offset_of(k, q);
+  return BY_OFFSET ? clipped(a, d) : axis_index(a, lut, d);
+}
+template <typename P, bool BY_OFFSET>
+__device__ __forceinline__ int entry2(const BucketArgs& a, const uint8_t* lut, P qx, P qy, P kx, P ky) {
+  const int dx = offset_of(kx, qx), dy = offset_of(ky, qy);
+  return BY_OFFSET ? clipped(a, dy) * a.span + clipped(a, dx)
+                   : axis_index(a, lut, dy) * a.per_axis + axis_index(a, lut, dx);
 }
 
-// Rows of BB_VEC consecutive pairs of batch element b starting at nm.
-template <typename P, bool VEC>
-__device__ __forceinline__ void pair_rows(const BucketArgs& a, const uint8_t* lut, int b, int64_t nm, int* row) {
-  const P* qb = (const P*)a.q_pos + (int64_t)b * a.Nq * a.axes;
-  const P* kb = (const P*)a.k_pos + (int64_t)b * a.Nk * a.axes;
-  if constexpr (VEC) {  // M % 8 == 0: one query
-    const int64_t i = nm / a.M, m = nm - i * a.M;
-    const P* q = qb + i * a.axes;
-    if (a.member) {
-      const int4* mp = reinterpret_cast<const int4*>(a.member + (int64_t)b * a.NM + nm);
-      const int4 u = __ldg(mp), v = __ldg(mp + 1);
-      const int id[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+template <typename P> struct alignas(2 * sizeof(P)) Pos2 { P x, y; };
+
+// Entries of the pairs nm .. nm + PAIRS - 1 of batch element b (`none` where
+// there is no such pair or the list names no key).  PAIRS == 2: nm and M even.
+template <typename P, int AXES, int PAIRS, bool BY_OFFSET>
+__device__ __forceinline__ void pair_entries(const BucketArgs& a, const uint8_t* lut, int b, int64_t nm, int none,
+                                             int* e) {
 #pragma unroll
-      for (int j = 0; j < BB_VEC; ++j) row[j] = pair_row(a, lut, q, kb, (int64_t)id[j]);
+  for (int j = 0; j < PAIRS; ++j) e[j] = none;
+  if (nm >= a.NM) return;
+  const int64_t i = query_of(a, nm), m = nm - i * a.M;
+  int64_t id[PAIRS];
+  if (a.member) {
+    const int* mp = a.member + (int64_t)b * a.NM + nm;
+    if constexpr (PAIRS == 2) {
+      const int2 u = __ldg(reinterpret_cast<const int2*>(mp));
+      id[0] = u.x;
+      id[1] = u.y;
     } else {
-#pragma unroll
-      for (int j = 0; j < BB_VEC; ++j) row[j] = pair_row(a, lut, q, kb, m + j);
+      id[0] = __ldg(mp);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < BB_VEC; ++j) {
-      row[j] = BB_NO_ROW;
-      if (nm + j < a.NM) {
-        const int64_t i = (nm + j) / a.M, m = nm + j - i * a.M;
-        const int64_t ki = a.member ? (int64_t)a.member[(int64_t)b * a.NM + nm + j] : m;
-        row[j] = pair_row(a, lut, qb + i * a.axes, kb, ki);
+    for (int j = 0; j < PAIRS; ++j) id[j] = m + j;
+  }
+  const P* qb = (const P*)a.q_pos + ((int64_t)b * a.Nq + i) * AXES;
+  const P* kb = (const P*)a.k_pos + (int64_t)b * a.Nk * AXES;
+  if constexpr (AXES == 1) {
+    const P q = __ldg(qb);
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j)
+      if (id[j] >= 0 && id[j] < a.Nk) e[j] = entry1<P, BY_OFFSET>(a, lut, q, __ldg(kb + id[j]));
+  } else {
+    const Pos2<P> q = *reinterpret_cast<const Pos2<P>*>(qb);
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j)
+      if (id[j] >= 0 && id[j] < a.Nk) {
+        const Pos2<P> k = *reinterpret_cast<const Pos2<P>*>(kb + 2 * id[j]);
+        e[j] = entry2<P, BY_OFFSET>(a, lut, q.x, q.y, k.x, k.y);
       }
-    }
   }
 }
 
-template <typename T, typename TB, typename P, bool VEC>
-__global__ void __launch_bounds__(BB_THREADS) bucket_fwd_kernel(const __grid_constant__ BucketArgs a,
-                                                                const TB* __restrict__ table, int in_smem,
-                                                                T* __restrict__ out) {
+// Four heads of one table entry, in the output's type.
+template <typename T> struct Heads4 { using type = uint2; };
+template <> struct Heads4<float> { using type = float4; };
+__device__ __forceinline__ uint32_t head_bits(const uint2& v, int h) {
+  const uint32_t w = h < 2 ? v.x : v.y;
+  return h & 1 ? w >> 16 : w & 0xffffu;
+}
+__device__ __forceinline__ float head_value(const float4& v, int h) {
+  return h == 0 ? v.x : h == 1 ? v.y : h == 2 ? v.z : v.w;
+}
+
+// Block (x: tiles taken in turn, y: chunk of `groups` groups of four heads).
+template <typename T, typename TB, typename P, int AXES, int PAIRS, bool BY_OFFSET>
+__global__ void __launch_bounds__(BB_THREADS, 4)
+    bucket_fwd_kernel(const __grid_constant__ BucketArgs a, const TB* __restrict__ table, int groups,
+                      T* __restrict__ out) {
+  using V = typename Heads4<T>::type;
   extern __shared__ unsigned char sm[];
-  uint8_t* lut = sm;
-  float* tab = reinterpret_cast<float*>(sm + BB_LUT);  // [H][rows]
+  const int entries = BY_OFFSET ? (AXES == 2 ? a.span * a.span : a.span) : a.rows;
+  V* tab = reinterpret_cast<V*>(sm);                                        // [groups][entries + 1]
+  uint8_t* lut = sm + (size_t)groups * (entries + 1) * sizeof(V);
+  const int h0 = blockIdx.y * groups * BB_HEADS, nh = min(groups * BB_HEADS, a.H - h0);
   fill_lut(a, lut);
-  if (in_smem)
-    for (int i = threadIdx.x; i < a.rows * a.H; i += BB_THREADS) tab[(i % a.H) * a.rows + i / a.H] = ldf(table + i);
   __syncthreads();
-  const int64_t per = (a.NM + BB_VEC - 1) / BB_VEC, total = per * a.B;
-  for (int64_t v = (int64_t)blockIdx.x * BB_THREADS + threadIdx.x; v < total; v += (int64_t)gridDim.x * BB_THREADS) {
-    const int b = (int)(v / per);
-    const int64_t nm = (v - b * per) * BB_VEC;
-    int row[BB_VEC];
-    pair_rows<P, VEC>(a, lut, b, nm, row);
-    for (int h = 0; h < a.H; ++h) {
-      float o[BB_VEC];
+  for (int i = threadIdx.x; i <= entries; i += BB_THREADS) {  // the last entry is zero
+    int row = i;
+    if (BY_OFFSET && i < entries) {
+      row = axis_index(a, lut, unclipped(a, AXES == 2 ? i % a.span : i));
+      if (AXES == 2) row += axis_index(a, lut, unclipped(a, i / a.span)) * a.per_axis;
+    }
+    for (int h = 0; h < groups * BB_HEADS; ++h) {
+      const float v = i < entries && h < nh ? ldf(table + (int64_t)row * a.H + h0 + h) : 0.f;
+      stf(reinterpret_cast<T*>(tab + (h / BB_HEADS) * (entries + 1) + i) + h % BB_HEADS, v);
+    }
+  }
+  __syncthreads();
+  constexpr int STEP = BB_THREADS * PAIRS, TILE = STEP * BB_STEPS;
+  const int64_t per = (a.NM + TILE - 1) / TILE, total = per * a.B;
+  for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
+    const int b = total < (1ll << 31) ? (int)((uint32_t)t / (uint32_t)per) : (int)(t / per);
+    const int64_t nm = (t - b * per) * TILE + threadIdx.x * PAIRS;
+    int e[BB_STEPS][PAIRS];
 #pragma unroll
-      for (int j = 0; j < BB_VEC; ++j) {
-        if (row[j] == BB_NO_ROW) o[j] = 0.f;
-        else o[j] = in_smem ? tab[h * a.rows + row[j]] : ldf(table + (int64_t)row[j] * a.H + h);
-      }
-      T* p = out + ((int64_t)b * a.H + h) * a.NM + nm;
-      if constexpr (VEC) {
-        st8(p, o);
-      } else {
+    for (int u = 0; u < BB_STEPS; ++u)
+      pair_entries<P, AXES, PAIRS, BY_OFFSET>(a, lut, b, nm + u * STEP, entries, e[u]);
+    for (int g = 0; g < groups; ++g) {
+      const V* tg = tab + g * (entries + 1);
+      T* o = out + ((int64_t)b * a.H + h0 + g * BB_HEADS) * a.NM + nm;
+      V v[BB_STEPS][PAIRS];
 #pragma unroll
-        for (int j = 0; j < BB_VEC; ++j)
-          if (nm + j < a.NM) stf(p + j, o[j]);
+      for (int u = 0; u < BB_STEPS; ++u)
+#pragma unroll
+        for (int j = 0; j < PAIRS; ++j) v[u][j] = tg[e[u][j]];
+#pragma unroll
+      for (int h = 0; h < BB_HEADS; ++h) {
+        if (g * BB_HEADS + h >= nh) break;
+#pragma unroll
+        for (int u = 0; u < BB_STEPS; ++u) {
+          if (nm + u * STEP >= a.NM) break;
+          T* p = o + h * a.NM + u * STEP;
+          if constexpr (sizeof(T) == 2) {
+            if constexpr (PAIRS == 2)
+              *reinterpret_cast<uint32_t*>(p) = head_bits(v[u][0], h) | (head_bits(v[u][1], h) << 16);
+            else
+              *reinterpret_cast<uint16_t*>(p) = (uint16_t)head_bits(v[u][0], h);
+          } else {
+            if constexpr (PAIRS == 2)
+              *reinterpret_cast<float2*>(p) = make_float2(head_value(v[u][0], h), head_value(v[u][1], h));
+            else
+              *p = head_value(v[u][0], h);
+          }
+        }
       }
     }
   }
@@ -166,53 +246,77 @@ __device__ __forceinline__ float bb_max_nan(float a, float b) {
 }
 
 // Block (x: tiles taken in turn, y: group of BB_HEADS heads).
-template <typename T, typename P, bool VEC>
-__global__ void __launch_bounds__(BB_THREADS) bucket_bwd_kernel(const __grid_constant__ BucketArgs a,
-                                                                const T* __restrict__ dout,
-                                                                float* __restrict__ part) {
+template <typename T, typename P, int AXES, int PAIRS, bool BY_OFFSET>
+__global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
+    bucket_bwd_kernel(const __grid_constant__ BucketArgs a, const T* __restrict__ dout, float* __restrict__ part) {
+  constexpr int STEP = BB_THREADS * PAIRS, TILE = STEP * BB_STEPS, PER = BB_STEPS * PAIRS;
   extern __shared__ unsigned char sm[];
   __shared__ float wmax[BB_HEADS][BB_THREADS / 32];
-  __shared__ float raw[BB_TILE];
-  __shared__ uint16_t raw_row[BB_TILE];
-  uint8_t* lut = sm;
-  float* acc = reinterpret_cast<float*>(sm + BB_LUT);                   // [BB_HEADS][rows]
+  const int none = a.rows;
+  float* acc = reinterpret_cast<float*>(sm);                            // [BB_HEADS][rows]
   int* bins = reinterpret_cast<int*>(acc + BB_HEADS * a.rows);          // [BB_HEADS][rows]
+  float* raw = reinterpret_cast<float*>(bins + BB_HEADS * a.rows);      // [TILE] values, only of an odd tile
+  uint16_t* raw_row = reinterpret_cast<uint16_t*>(raw + TILE);          // [TILE]
+  // BY_OFFSET: the row of every combined clipped offset, and `none` last
+  const int offsets = AXES == 2 ? a.span * a.span : a.span;
+  uint16_t* rows = raw_row + TILE;
+  uint8_t* lut = reinterpret_cast<uint8_t*>(rows + (BY_OFFSET ? (offsets + 2) & ~1 : 0));
   const int h0 = blockIdx.y * BB_HEADS, nh = min(BB_HEADS, a.H - h0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   fill_lut(a, lut);
+  __syncthreads();
+  if (BY_OFFSET) {
+    for (int i = threadIdx.x; i <= offsets; i += BB_THREADS) {
+      int row = none;
+      if (i < offsets) {
+        row = axis_index(a, lut, unclipped(a, AXES == 2 ? i % a.span : i));
+        if (AXES == 2) row += axis_index(a, lut, unclipped(a, i / a.span)) * a.per_axis;
+      }
+      rows[i] = (uint16_t)row;
+    }
+  }
   for (int i = threadIdx.x; i < BB_HEADS * a.rows; i += BB_THREADS) {
     acc[i] = 0.f;
     bins[i] = 0;
   }
   __syncthreads();
-  const int64_t per = (a.NM + BB_TILE - 1) / BB_TILE, total = per * a.B;
+  const int64_t per = (a.NM + TILE - 1) / TILE, total = per * a.B;
   for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-    const int b = (int)(t / per);
-    const int64_t nm = (t - b * per) * BB_TILE + threadIdx.x * BB_VEC;
-    const bool in = nm < a.NM;
-    int row[BB_VEC];
-#pragma unroll
-    for (int j = 0; j < BB_VEC; ++j) row[j] = BB_NO_ROW;
-    if (in) pair_rows<P, VEC>(a, lut, b, nm, row);
-    float g[BB_HEADS][BB_VEC];
+    const int b = total < (1ll << 31) ? (int)((uint32_t)t / (uint32_t)per) : (int)(t / per);
+    const int64_t nm = (t - b * per) * TILE + threadIdx.x * PAIRS;
+    float g[BB_HEADS][PER];
 #pragma unroll
     for (int h = 0; h < BB_HEADS; ++h) {
+      const T* p = dout + ((int64_t)b * a.H + h0 + h) * a.NM + nm;
 #pragma unroll
-      for (int j = 0; j < BB_VEC; ++j) g[h][j] = 0.f;
-      if (in && h < nh) {
-        const T* p = dout + ((int64_t)b * a.H + h0 + h) * a.NM + nm;
-        if constexpr (VEC) {
-          ld8(p, g[h]);
+      for (int u = 0; u < BB_STEPS; ++u) {
+        const bool in = h < nh && nm + u * STEP < a.NM;
+        if constexpr (PAIRS == 2 && sizeof(T) == 2) {
+          const uint32_t w = in ? __ldg(reinterpret_cast<const uint32_t*>(p + u * STEP)) : 0u;
+          g[h][2 * u] = ldf(reinterpret_cast<const T*>(&w));
+          g[h][2 * u + 1] = ldf(reinterpret_cast<const T*>(&w) + 1);
+        } else if constexpr (PAIRS == 2) {
+          const float2 w = in ? __ldg(reinterpret_cast<const float2*>(p + u * STEP)) : make_float2(0.f, 0.f);
+          g[h][2 * u] = w.x;
+          g[h][2 * u + 1] = w.y;
         } else {
-#pragma unroll
-          for (int j = 0; j < BB_VEC; ++j)
-            if (nm + j < a.NM) g[h][j] = ldf(p + j);
+          g[h][u] = in ? ldf(p + u * STEP) : 0.f;
         }
       }
+    }
+    int row[PER];
+#pragma unroll
+    for (int u = 0; u < BB_STEPS; ++u)
+      pair_entries<P, AXES, PAIRS, BY_OFFSET>(a, lut, b, nm + u * STEP, BY_OFFSET ? offsets : none, row + u * PAIRS);
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (BY_OFFSET) row[j] = rows[row[j]];
+#pragma unroll
+    for (int h = 0; h < BB_HEADS; ++h) {
       float top = 0.f;
 #pragma unroll
-      for (int j = 0; j < BB_VEC; ++j)
-        if (row[j] != BB_NO_ROW) top = bb_max_nan(top, fabsf(g[h][j]));
+      for (int j = 0; j < PER; ++j)
+        if (row[j] != none) top = bb_max_nan(top, fabsf(g[h][j]));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = bb_max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
       if (lane == 0) wmax[h][warp] = top;
@@ -237,8 +341,8 @@ __global__ void __launch_bounds__(BB_THREADS) bucket_bwd_kernel(const __grid_con
         down[h] = __int_as_float((127 - t1) << 23);
         rest[h] = __int_as_float((127 - t + t1) << 23);
 #pragma unroll
-        for (int j = 0; j < BB_VEC; ++j)
-          if (row[j] != BB_NO_ROW) atomicAdd(bins + h * a.rows + row[j], __float2int_rn(g[h][j] * up * up2));
+        for (int j = 0; j < PER; ++j)
+          if (row[j] != none) atomicAdd(bins + h * a.rows + row[j], __float2int_rn(g[h][j] * up * up2));
       }
     }
     __syncthreads();
@@ -262,13 +366,13 @@ __global__ void __launch_bounds__(BB_THREADS) bucket_bwd_kernel(const __grid_con
         if (!isfinite(top)) {
           __syncthreads();
 #pragma unroll
-          for (int j = 0; j < BB_VEC; ++j) {
-            raw[threadIdx.x * BB_VEC + j] = g[h][j];
-            raw_row[threadIdx.x * BB_VEC + j] = (uint16_t)row[j];
+          for (int j = 0; j < PER; ++j) {
+            raw[threadIdx.x * PER + j] = g[h][j];
+            raw_row[threadIdx.x * PER + j] = (uint16_t)row[j];
           }
           __syncthreads();
           for (int i = threadIdx.x; i < a.rows; i += BB_THREADS)
-            for (int j = 0; j < BB_TILE; ++j)
+            for (int j = 0; j < TILE; ++j)
               if (raw_row[j] == i) acc[h * a.rows + i] += raw[j];
         }
       }
@@ -279,30 +383,34 @@ __global__ void __launch_bounds__(BB_THREADS) bucket_bwd_kernel(const __grid_con
   for (int i = threadIdx.x; i < nh * a.rows; i += BB_THREADS) o[i] = acc[i];
 }
 
-// dtable[row, h] = sum over blocks of part[block][h][row], in block order.
+// dtable[row, h] = sum over blocks of part[block][h][row], in a fixed order:
+// 32 elements x 32 lanes of blocks.
 template <typename TB>
-__global__ void __launch_bounds__(256) bucket_table_kernel(const float* __restrict__ part, int64_t blocks, int rows,
-                                                           int H, TB* __restrict__ dtable) {
-  __shared__ float red[8][33];
+__global__ void __launch_bounds__(1024) bucket_table_kernel(const float* __restrict__ part, int64_t blocks, int rows,
+                                                            int H, TB* __restrict__ dtable) {
+  __shared__ float red[32][33];
   const int x = threadIdx.x & 31, l = threadIdx.x >> 5;
   const int64_t n = (int64_t)rows * H, i = (int64_t)blockIdx.x * 32 + x;
   float v = 0.f;
   if (i < n) {
-#pragma unroll 4
-    for (int64_t b = l; b < blocks; b += 8) v += part[b * n + i];
+#pragma unroll 8
+    for (int64_t b = l; b < blocks; b += 32) v += __ldg(part + b * n + i);
   }
   red[l][x] = v;
   __syncthreads();
-  if (l == 0 && i < n) {
-    v = 0.f;
-    for (int k = 0; k < 8; ++k) v += red[k][x];
-    const int64_t h = i / rows, r = i - h * rows;
+  v = warp_sum(red[x][l]);  // lane x holds lane-sum x of element l
+  const int64_t j = (int64_t)blockIdx.x * 32 + l;
+  if (x == 0 && j < n) {
+    const int64_t h = j / rows, r = j - h * rows;
     stf(dtable + r * H + h, v);
   }
 }
 
+// Blocks of the backward along x: sized for the narrower tile, so that it does
+// not depend on alignment.
 static int64_t bucket_bwd_blocks(int64_t B, int64_t H, int64_t NM) {
-  const int64_t tiles = (NM + BB_TILE - 1) / BB_TILE * B, groups = (H + BB_HEADS - 1) / BB_HEADS;
+  const int64_t tile = BB_THREADS * BB_STEPS;
+  const int64_t tiles = (NM + tile - 1) / tile * B, groups = (H + BB_HEADS - 1) / BB_HEADS;
   const int64_t want = ((int64_t)sm_count() * BB_BLOCKS_PER_SM + groups - 1) / groups;
   return tiles < want ? tiles : want;
 }
@@ -337,12 +445,32 @@ static int bucket_args(const int32_t* edges, int n_edges, int one_sided, const v
   a->Nk = Nk;
   a->M = M;
   a->NM = Nq * M;
+  const int64_t last = edges[n_edges - 1];
+  a->span = a->lut ? (int)(one_sided ? last + 1 : 2 * last + 1) : 0;
+  a->div_shift = 32;
+  if (M >= 1 && a->NM < (1ll << 31)) {
+    uint32_t l = 0;
+    while ((1ll << l) < M) ++l;
+    a->div_shift = l;
+    a->div_mul = (uint32_t)(((1ull << 32) * ((1ull << l) - (uint64_t)M)) / (uint64_t)M + 1);
+  }
   if (B * a->NM > 0) AFFB_REQUIRE(q_pos && k_pos, "bucket_bias: null positions");
+  const uintptr_t pair = pos_type == AFFB_POS_I64 ? 16 : 8;
+  AFFB_REQUIRE(axes == 1 || (((uintptr_t)q_pos | (uintptr_t)k_pos) & (pair - 1)) == 0,
+               "bucket_bias: positions of two axes must be aligned to a pair of coordinates");
   return AFFB_OK;
 }
 
-static bool bb_vec(const BucketArgs& a, const void* t) {
-  return a.M % BB_VEC == 0 && ((uintptr_t)t & 15) == 0 && ((uintptr_t)a.member & 15) == 0;
+// Two pairs a lane: both of one query, and 4- or 8-byte accesses aligned.
+static bool bb_two(const BucketArgs& a, const void* t, int64_t size) {
+  return a.M % 2 == 0 && ((uintptr_t)t & (2 * size - 1)) == 0 && ((uintptr_t)a.member & 7) == 0;
+}
+// Entries of a table by offset, or 0 where it is not worth expanding: it has
+// to fit, and a block has to read it oftener than it writes it.
+static int64_t bb_offsets(const BucketArgs& a, int64_t entry_bytes, int64_t most_bytes, int64_t blocks) {
+  if (!a.span) return 0;
+  const int64_t n = a.axes == 2 ? (int64_t)a.span * a.span : a.span;
+  return n * entry_bytes <= most_bytes && n * blocks <= a.NM * a.B ? n : 0;
 }
 
 #define BB_POS(pos_type, P, ...)                                   \
@@ -352,30 +480,35 @@ static bool bb_vec(const BucketArgs& a, const void* t) {
     default: { using P = int64_t; __VA_ARGS__; break; }            \
   }
 
-constexpr int BB_TABLE_SMEM = 96 * 1024;  // larger tables are read through L1 instead
-
-template <typename T, typename TB, typename P, bool VEC>
+template <typename T, typename TB, typename P, int AXES, int PAIRS>
 static cudaError_t bucket_fwd_launch(const BucketArgs& a, const void* table, void* out, cudaStream_t st) {
-  const int64_t bytes = (int64_t)a.rows * a.H * 4;
-  const int in_smem = bytes <= BB_TABLE_SMEM;
-  const int smem = BB_LUT + (in_smem ? (int)bytes : 0);
-  auto* k = bucket_fwd_kernel<T, TB, P, VEC>;
+  const int64_t v = sizeof(typename Heads4<T>::type);
+  const int64_t tiles = (a.NM + BB_THREADS * PAIRS * BB_STEPS - 1) / (BB_THREADS * PAIRS * BB_STEPS) * a.B;
+  const int64_t blocks = imin64(tiles, (int64_t)sm_count() * 4);
+  const int64_t all = (a.H + BB_HEADS - 1) / BB_HEADS;
+  const int64_t offsets = bb_offsets(a, v, BB_TABLE_SMEM, blocks);
+  const int64_t entries = (offsets ? offsets : a.rows) + 1;
+  const int64_t fit = BB_TABLE_SMEM / (entries * v);
+  const int groups = (int)(fit < 1 ? 1 : fit < all ? fit : all);
+  const int smem = (int)(groups * entries * v) + a.lut;
+  auto* k = offsets ? bucket_fwd_kernel<T, TB, P, AXES, PAIRS, true> : bucket_fwd_kernel<T, TB, P, AXES, PAIRS, false>;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, BB_LUT + BB_TABLE_SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
-  const int64_t threads = (a.NM + BB_VEC - 1) / BB_VEC * a.B;
-  const unsigned blocks = (unsigned)imin64((threads + BB_THREADS - 1) / BB_THREADS, (int64_t)sm_count() * 8);
-  k<<<blocks, BB_THREADS, smem, st>>>(a, (const TB*)table, in_smem, (T*)out);
+  const dim3 grid((unsigned)blocks, (unsigned)((all + groups - 1) / groups));
+  k<<<grid, BB_THREADS, smem, st>>>(a, (const TB*)table, groups, (T*)out);
   return cudaGetLastError();
 }
 
-template <typename T, typename P, bool VEC>
+template <typename T, typename P, int AXES, int PAIRS>
 static cudaError_t bucket_bwd_launch(const BucketArgs& a, const void* dout, float* part, int64_t blocks,
                                      cudaStream_t st) {
-  const int smem = BB_LUT + 2 * BB_HEADS * a.rows * 4;
-  auto* k = bucket_bwd_kernel<T, P, VEC>;
-  if (smem > 32 * 1024) {
+  const int64_t offsets = bb_offsets(a, 2, 16 * 1024, blocks);
+  const int tile = BB_THREADS * PAIRS * BB_STEPS;
+  const int smem = 2 * BB_HEADS * a.rows * 4 + tile * 6 + (offsets ? (int)((offsets + 2) & ~1) * 2 : 0) + a.lut;
+  auto* k = offsets ? bucket_bwd_kernel<T, P, AXES, PAIRS, true> : bucket_bwd_kernel<T, P, AXES, PAIRS, false>;
+  if (smem > 47 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
@@ -405,14 +538,16 @@ extern "C" int affb_bucket_bias_fwd(const void* table, int table_dtype, const in
                "bucket_bias: the output must be fp32, fp16 or bf16");
   if (B * a.NM == 0) return AFFB_OK;
   AFFB_REQUIRE(table && out, "bucket_bias: null pointer");
-  const bool vec = bb_vec(a, out);
+  const bool two = bb_two(a, out, out_dtype == AFFB_F32 ? 4 : 2);
   cudaStream_t st = as_stream(stream);
   cudaError_t e = cudaSuccess;
   AFFB_DISPATCH(table_dtype, TB, {
     AFFB_DISPATCH(out_dtype, T, {
       BB_POS(pos_type, P, {
-        if (vec) e = bucket_fwd_launch<T, TB, P, true>(a, table, out, st);
-        else e = bucket_fwd_launch<T, TB, P, false>(a, table, out, st);
+        if (axes == 1) e = two ? bucket_fwd_launch<T, TB, P, 1, 2>(a, table, out, st)
+                               : bucket_fwd_launch<T, TB, P, 1, 1>(a, table, out, st);
+        else e = two ? bucket_fwd_launch<T, TB, P, 2, 2>(a, table, out, st)
+                     : bucket_fwd_launch<T, TB, P, 2, 1>(a, table, out, st);
       })
     })
   });
@@ -444,18 +579,21 @@ extern "C" int affb_bucket_bias_bwd(const void* dout, int dout_dtype, const int3
     AFFB_REQUIRE(dout, "bucket_bias: null pointer");
     blocks = bucket_bwd_blocks(B, H, a.NM);
     AFFB_REQUIRE(workspace && workspace_bytes >= blocks * n * 4, "bucket_bias: workspace too small");
-    const bool vec = bb_vec(a, dout);
+    const bool two = bb_two(a, dout, dout_dtype == AFFB_F32 ? 4 : 2);
     cudaError_t e = cudaSuccess;
     AFFB_DISPATCH(dout_dtype, T, {
       BB_POS(pos_type, P, {
-        if (vec) e = bucket_bwd_launch<T, P, true>(a, dout, (float*)workspace, blocks, st);
-        else e = bucket_bwd_launch<T, P, false>(a, dout, (float*)workspace, blocks, st);
+        float* part = (float*)workspace;
+        if (axes == 1) e = two ? bucket_bwd_launch<T, P, 1, 2>(a, dout, part, blocks, st)
+                               : bucket_bwd_launch<T, P, 1, 1>(a, dout, part, blocks, st);
+        else e = two ? bucket_bwd_launch<T, P, 2, 2>(a, dout, part, blocks, st)
+                     : bucket_bwd_launch<T, P, 2, 1>(a, dout, part, blocks, st);
       })
     });
     if ((rc = bb_status(e))) return rc;
   }
   AFFB_DISPATCH(table_dtype, TB,
-                bucket_table_kernel<TB><<<(unsigned)((n + 31) / 32), 256, 0, st>>>((const float*)workspace, blocks,
+                bucket_table_kernel<TB><<<(unsigned)((n + 31) / 32), 1024, 0, st>>>((const float*)workspace, blocks,
                                                                                    a.rows, (int)H, (TB*)dtable));
   AFFB_LAUNCH_CHECK("affb_bucket_bias_bwd");
   return AFFB_OK;

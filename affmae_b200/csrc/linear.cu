@@ -414,6 +414,19 @@ static const void* kernel_of(int act) {
   }
 }
 
+// The kernel's shared-memory limit, raised once per device (idempotent, so a
+// race between threads is harmless).
+static cudaError_t allow_smem(const void* k, int slot) {
+  static bool done[64][12];
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev < 64 && done[dev][slot]) return cudaSuccess;
+  err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+  if (err == cudaSuccess && dev < 64) done[dev][slot] = true;
+  return err;
+}
+
 static bool tma_rows(const void* p, int dtype, int64_t N) {
   return aligned_to(p, 16) && N * dtype_size(dtype) % 16 == 0;
 }
@@ -472,7 +485,7 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
   const void* k = e.out_dtype == AFFB_F32    ? kernel_of<float>(e.act)
                   : e.out_dtype == AFFB_BF16 ? kernel_of<__nv_bfloat16>(e.act)
                                              : kernel_of<__half>(e.act);
-  cudaError_t err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+  cudaError_t err = allow_smem(k, (e.out_dtype == AFFB_F32 ? 0 : e.out_dtype == AFFB_BF16 ? 4 : 8) + e.act);
   if (err == cudaSuccess) {
     const int64_t units = (int64_t)s.mt * s.nt * s.splits;
     void* args[] = {&ma, &mb, &mo, &mz, &p};

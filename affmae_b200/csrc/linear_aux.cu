@@ -67,7 +67,7 @@ constexpr int DZ_MIN_ROWS = 64;
 
 int64_t linear_dz_strips(int64_t R, int64_t C) {
   const int64_t cols = (C + DZ_COLS - 1) / DZ_COLS;
-  const int64_t want = ((int64_t)sm_count() * 8 + cols - 1) / cols;
+  const int64_t want = ((int64_t)sm_count() * 6 + cols - 1) / cols;
   const int64_t most = (R + DZ_MIN_ROWS - 1) / DZ_MIN_ROWS;
   return want < most ? want : (most > 0 ? most : 1);
 }
@@ -204,27 +204,27 @@ __device__ __forceinline__ float activate_code(int act, float z) {
   }
 }
 
-// Block: 32 consecutive elements x 8 lanes of parts, summed in a fixed order.
-__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ part, int64_t S, int64_t M, int64_t N,
-                                                        int64_t ld, LinearEpilogue e) {
-  __shared__ float red[8][33];
+// Block: 32 consecutive elements x 32 lanes of parts, summed in a fixed order.
+__global__ void __launch_bounds__(1024) sum_parts_kernel(const float* __restrict__ part, int64_t S, int64_t M,
+                                                         int64_t N, int64_t ld, LinearEpilogue e) {
+  __shared__ float red[32][33];
   const int x = threadIdx.x & 31, l = threadIdx.x >> 5;
   const int64_t n = M * N, plane = M * ld;
   for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < n; i0 += (int64_t)gridDim.x * 32) {
-    const int64_t i = i0 + x;
-    const int64_t m = i < n ? i / N : 0, c = i < n ? i - m * N : 0;
-    const float* p = part + m * ld + c;
+    int64_t i = i0 + x;
     float s = 0.f;
     if (i < n) {
-#pragma unroll 4
-      for (int64_t k = l; k < S; k += 8) s += __ldg(p + k * plane);
+      const int64_t m = i / N;
+      const float* p = part + m * ld + (i - m * N);
+#pragma unroll 8
+      for (int64_t k = l; k < S; k += 32) s += __ldg(p + k * plane);
     }
     red[l][x] = s;
     __syncthreads();
-    if (l == 0 && i < n) {
-      float v = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v += red[k][x];
+    float v = warp_sum(red[x][l]);
+    i = i0 + l;
+    if (x == 0 && i < n) {
+      const int64_t m = i / N, c = i - m * N;
       if (e.row_scale) v *= e.row_scale[m];
       if (e.col_scale) v *= e.col_scale[c];
       if (e.bias) v += load_as(e.bias, e.bias_dtype, c);
@@ -240,8 +240,8 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict_
 int linear_sum(const float* part, int64_t S, int64_t M, int64_t N, int64_t ld, const LinearEpilogue& e,
                cudaStream_t st) {
   if (M * N == 0) return AFFB_OK;
-  const unsigned blocks = (unsigned)imin64((M * N + 31) / 32, (int64_t)sm_count() * 16);
-  sum_parts_kernel<<<blocks, 256, 0, st>>>(part, S, M, N, ld, e);
+  const unsigned blocks = (unsigned)imin64((M * N + 31) / 32, (int64_t)sm_count() * 4);
+  sum_parts_kernel<<<blocks, 1024, 0, st>>>(part, S, M, N, ld, e);
   AFFB_LAUNCH_CHECK("linear: sum of partial products");
   return AFFB_OK;
 }

@@ -7,11 +7,13 @@
 //   dx = ds + rstd (g - s rstd^2 mean(g s)),  ddelta = f dx,
 //   dw = sum over rows of dy s rstd.
 //
-// Bound by HBM: every tensor is read and written once.  A row of up to
-// 32 * 8 * 4 channels is held by one warp in registers, a longer one by a
-// block of eight warps (up to 8192 channels in registers, beyond that the row
-// is read again for the second pass).  dw is summed per block in row order and
-// then over blocks in order, so it does not depend on timing.
+// Bound by HBM: every tensor is read and written once.  A row is shared by
+// TPR threads that hold it in registers, NV chunks of VEC channels each; TPR
+// is the smallest of 8, 16, 32 and a whole block whose chunks cover the row
+// with few idle lanes (96 channels: 16 threads of one chunk; 384: 16 of
+// three).  Rows beyond 4 chunks a thread of a block are read again for the
+// second pass.  dw is summed per block in row order and then over blocks in
+// order, so it does not depend on timing.
 #include "common.cuh"
 
 #include <cuda_fp8.h>
@@ -23,6 +25,7 @@ constexpr float E4M3_MAX = 448.f;
 struct RmsArgs {
   const void* x;
   const void* delta;       // or null
+  int delta_dtype;
   const float* row_scale;  // [R / rows_per_scale] or null
   int64_t rows_per_scale;
   const float* w;          // null: rows are quantised as they are, without the norm
@@ -92,43 +95,51 @@ __device__ __forceinline__ float rms_max_nan(float a, float b) {
 struct AddOp { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
 struct MaxOp { __device__ __forceinline__ float operator()(float a, float b) const { return rms_max_nan(a, b); } };
 
-// Reduction over the THREADS / 32 warps that share a row (all lanes get it).
-template <int WARPS, typename Op>
+// Reduction over the TPR threads that share a row (all of them get it).  A
+// block-wide one writes to `red`, which the reduction before must not use.
+template <int TPR, typename Op>
 __device__ __forceinline__ float row_reduce(float v, float* red, Op op) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if constexpr (WARPS > 1) {
-    const int warp = threadIdx.x >> 5;
-    __syncthreads();  // red may still be read by the reduction before
-    if ((threadIdx.x & 31) == 0) red[warp] = v;
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if constexpr (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int i = 1; i < WARPS; ++i) v = op(v, red[i]);
+    for (int i = 1; i < TPR / 32; ++i) v = op(v, red[i]);
   }
   return v;
 }
 
-// W warps share a row; NV chunks of VEC channels a lane are kept in registers
-// (NV == 0: none, the row is read again).
-template <typename TX, typename TD, int W, int NV, int VEC>
+__device__ __forceinline__ float group_scale(const float* row_scale, int64_t r, int64_t rows_per_scale) {
+  // 32-bit division where it fits: a 64-bit one costs as much as a narrow row
+  const int64_t g = (r | rows_per_scale) >> 31 ? r / rows_per_scale : (int64_t)((uint32_t)r / (uint32_t)rows_per_scale);
+  return row_scale[g];
+}
+
+// NV == 0: the row is read again instead of kept.
+template <typename TX, int TPR, int NV, int VEC>
 __global__ void __launch_bounds__(256) rms_fwd_kernel(RmsArgs a) {
-  __shared__ float red[8];
-  constexpr int ROWS = 8 / W;
+  __shared__ float red[3][8];  // sums of squares (two rows in turn), maxima
+  constexpr int ROWS = 256 / TPR;
   constexpr int KEEP = NV > 0 ? NV : 1;
-  const int t = threadIdx.x % (W * 32);
+  const int t = threadIdx.x % TPR;
   const int C = a.C;
-  const int steps = NV > 0 ? NV : (C + W * 32 * VEC - 1) / (W * 32 * VEC);
-  for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / (W * 32); r < a.R; r += (int64_t)gridDim.x * ROWS) {
-    const float f = a.row_scale ? a.row_scale[r / a.rows_per_scale] : 1.f;
+  const float inv_c = 1.f / (float)C;
+  int flip = 0;
+  const int steps = NV > 0 ? NV : (C + TPR * VEC - 1) / (TPR * VEC);
+  // the threads of a warp stay together (shuffles): rows past the end are computed on nothing
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.R; r0 += (int64_t)gridDim.x * ROWS) {
+    const int64_t r = r0 + threadIdx.x / TPR;
+    const bool in = r < a.R;
+    const float f = a.row_scale && in ? group_scale(a.row_scale, r, a.rows_per_scale) : 1.f;
     const TX* x = (const TX*)a.x + r * C;
-    const TD* d = (const TD*)a.delta + r * C;
     float v[KEEP][VEC];
     auto row_chunk = [&](int c, float* o) {
       rms_load<TX, VEC>(x + c, o);
       if (a.delta) {
         float dd[VEC];
-        rms_load<TD, VEC>(d + c, dd);
+        rms_load_as<VEC>(a.delta, a.delta_dtype, r * C + c, dd);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o[k] = a.row_scale ? fmaf(f, dd[k], o[k]) : o[k] + dd[k];
       }
@@ -136,51 +147,66 @@ __global__ void __launch_bounds__(256) rms_fwd_kernel(RmsArgs a) {
     float sq = 0.f;
 #pragma unroll
     for (int i = 0; i < steps; ++i) {
-      const int c = (i * W * 32 + t) * VEC;
+      const int c = (i * TPR + t) * VEC;
       float* o = v[NV > 0 ? i : 0];
 #pragma unroll
       for (int k = 0; k < VEC; ++k) o[k] = 0.f;
-      if (c < C) {
+      if (in && c < C) {
         row_chunk(c, o);
         if (a.s) rms_store<TX, VEC>((TX*)a.s + r * C + c, o);
       }
 #pragma unroll
       for (int k = 0; k < VEC; ++k) sq = fmaf(o[k], o[k], sq);
     }
-    const float rstd = a.w ? 1.f / sqrtf(row_reduce<W>(sq, red, AddOp()) / (float)C + a.eps) : 1.f;
-    if (a.rstd && t == 0) a.rstd[r] = rstd;
-    float top = 0.f;
+    float rstd = 1.f;
+    if (a.w) {
+      rstd = rsqrtf(row_reduce<TPR>(sq, red[flip], AddOp()) * inv_c + a.eps);
+      flip ^= 1;
+      if (a.rstd && in && t == 0) a.rstd[r] = rstd;
+    }
+    // y: kept in place of the row
+    auto normed = [&](int c, float* o) {
+      if (a.w) {
+        float wv[VEC];
+        rms_load<float, VEC>(a.w + c, wv);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) o[k] = o[k] * rstd * wv[k];
+      }
+    };
+    float top = 0.f, inv = 1.f;
     if (a.q) {
 #pragma unroll
       for (int i = 0; i < steps; ++i) {
-        const int c = (i * W * 32 + t) * VEC;
-        if (c < C) {
+        const int c = (i * TPR + t) * VEC;
+        if (in && c < C) {
           float* o = v[NV > 0 ? i : 0];
           if (NV == 0) row_chunk(c, o);
+          normed(c, o);
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) top = rms_max_nan(top, fabsf(a.w ? o[k] * rstd * a.w[c + k] : o[k]));
+          for (int k = 0; k < VEC; ++k) top = rms_max_nan(top, fabsf(o[k]));
         }
       }
-      top = row_reduce<W>(top, red, MaxOp());
+      top = row_reduce<TPR>(top, red[2], MaxOp());
+      const float scale = top == 0.f ? 1.f : top * (1.f / E4M3_MAX);
+      inv = 1.f / scale;
+      if (in && t == 0) a.scale[r] = scale;
+      // a row too small for the reciprocal of its scale (below 2^-126 * 448) is divided
+      if (isinf(inv)) inv = 0.f;
+      if (inv == 0.f) top = scale;
     }
-    const float scale = top == 0.f ? 1.f : top / E4M3_MAX;
-    if (a.q && t == 0) a.scale[r] = scale;
 #pragma unroll
     for (int i = 0; i < steps; ++i) {
-      const int c = (i * W * 32 + t) * VEC;
-      if (c < C) {
+      const int c = (i * TPR + t) * VEC;
+      if (in && c < C) {
         float* o = v[NV > 0 ? i : 0];
         if (NV == 0) row_chunk(c, o);
-        float y[VEC], wv[VEC];
-        if (a.w) rms_load<float, VEC>(a.w + c, wv);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) y[k] = a.w ? o[k] * rstd * wv[k] : o[k];
+        if (NV == 0 || !a.q) normed(c, o);
         if (a.q) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) y[k] = y[k] / scale;
-          store_e4m3<VEC>(a.q + r * C + c, y);
+          for (int k = 0; k < VEC; ++k) o[k] = inv != 0.f ? o[k] * inv : o[k] / top;
+          store_e4m3<VEC>(a.q + r * C + c, o);
         } else {
-          rms_store_as<VEC>(a.y, a.y_dtype, r * C + c, y);
+          rms_store_as<VEC>(a.y, a.y_dtype, r * C + c, o);
         }
       }
     }
@@ -199,71 +225,74 @@ struct RmsBwdArgs {
   int64_t R;
   int C;
   void* dx;                // x's dtype, or null
-  void* ddelta;            // TD, or null
+  void* ddelta;            // or null
+  int delta_dtype;
   float* part;             // [blocks][C] sums of dy s rstd, or null
 };
 
-template <typename TX, typename TD, int W, int NV, int VEC>
+template <typename TX, int TPR, int NV, int VEC>
 __global__ void __launch_bounds__(256) rms_bwd_kernel(RmsBwdArgs a) {
   extern __shared__ float dws[];  // [ROWS][C]: sums of each row slot of the block
-  __shared__ float red[8];
-  constexpr int ROWS = 8 / W;
+  __shared__ float red[2][8];
+  constexpr int ROWS = 256 / TPR;
   constexpr int KEEP = NV > 0 ? NV : 1;
-  const int t = threadIdx.x % (W * 32), slot = threadIdx.x / (W * 32);
+  const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
   const int C = a.C;
-  const int steps = NV > 0 ? NV : (C + W * 32 * VEC - 1) / (W * 32 * VEC);
-  // the sums of a long row stay in the block's own row of `part`
-  float* sums = NV > 0 ? dws + slot * C : (a.part ? a.part + (int64_t)blockIdx.x * C : nullptr);
-  if (a.part)
-    for (int i = 0; i < steps; ++i) {
-      const int c = (i * W * 32 + t) * VEC;
-      if (c < C)
+  const float inv_c = 1.f / (float)C;
+  const int steps = NV > 0 ? NV : (C + TPR * VEC - 1) / (TPR * VEC);
+  float sums[KEEP][VEC], wv[KEEP][VEC];
+  // the sums of a row too long for registers stay in the block's own row of `part`
+  float* far = NV == 0 && a.part ? a.part + (int64_t)blockIdx.x * C : nullptr;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) sums[c + k] = 0.f;
+  for (int i = 0; i < steps; ++i) {
+    const int c = (i * TPR + t) * VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      sums[NV > 0 ? i : 0][k] = 0.f;
+      if (far && c < C) far[c + k] = 0.f;
     }
-  for (int64_t r = (int64_t)blockIdx.x * ROWS + slot; r < a.R; r += (int64_t)gridDim.x * ROWS) {
-    const float rstd = a.rstd[r];
+    if (NV > 0 && c < C) rms_load<float, VEC>(a.w + c, wv[NV > 0 ? i : 0]);
+  }
+  int flip = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.R; r0 += (int64_t)gridDim.x * ROWS) {
+    const int64_t r = r0 + slot;
+    const bool in = r < a.R;
+    const float rstd = in ? a.rstd[r] : 0.f;
     float sv[KEEP][VEC], gv[KEEP][VEC];
     auto chunk = [&](int c, float* s, float* g) {
       rms_load<TX, VEC>((const TX*)a.s + r * C + c, s);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) g[k] = 0.f;
       if (a.dy) rms_load_as<VEC>(a.dy, a.y_dtype, r * C + c, g);
+      if (NV == 0) rms_load<float, VEC>(a.w + c, wv[0]);
     };
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < steps; ++i) {
-      const int c = (i * W * 32 + t) * VEC;
-      float *s = sv[NV > 0 ? i : 0], *g = gv[NV > 0 ? i : 0];
-      if (c < C) {
-        chunk(c, s, g);
-        float wv[VEC];
-        rms_load<float, VEC>(a.w + c, wv);
+      const int c = (i * TPR + t) * VEC, n = NV > 0 ? i : 0;
+      if (in && c < C) {
+        chunk(c, sv[n], gv[n]);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          if (a.part) sums[c + k] += g[k] * s[k] * rstd;
-          g[k] *= wv[k];
-          dot = fmaf(g[k], s[k], dot);
+          const float gs = gv[n][k] * sv[n][k];
+          if (far) far[c + k] += gs * rstd;
+          else sums[n][k] = fmaf(gs, rstd, sums[n][k]);
+          dot = fmaf(gs, wv[n][k], dot);
         }
       }
     }
     if (!a.dx && !a.ddelta) continue;
-    const float coef = row_reduce<W>(dot, red, AddOp()) / (float)C * rstd * rstd;
-    const float f = a.row_scale ? a.row_scale[r / a.rows_per_scale] : 1.f;
+    const float coef = row_reduce<TPR>(dot, red[flip], AddOp()) * inv_c * rstd * rstd;
+    flip ^= 1;
+    const float f = a.row_scale && in ? group_scale(a.row_scale, r, a.rows_per_scale) : 1.f;
 #pragma unroll
     for (int i = 0; i < steps; ++i) {
-      const int c = (i * W * 32 + t) * VEC;
-      if (c < C) {
-        float *s = sv[NV > 0 ? i : 0], *g = gv[NV > 0 ? i : 0], o[VEC];
-        if (NV == 0) {
-          chunk(c, s, g);
-          float wv[VEC];
-          rms_load<float, VEC>(a.w + c, wv);
+      const int c = (i * TPR + t) * VEC, n = NV > 0 ? i : 0;
+      if (in && c < C) {
+        float o[VEC];
+        if (NV == 0) chunk(c, sv[0], gv[0]);
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) g[k] *= wv[k];
-        }
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) o[k] = rstd * (g[k] - s[k] * coef);
+        for (int k = 0; k < VEC; ++k) o[k] = rstd * (gv[n][k] * wv[n][k] - sv[n][k] * coef);
         if (a.ds) {
           float d[VEC];
           rms_load<TX, VEC>((const TX*)a.ds + r * C + c, d);
@@ -274,12 +303,19 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(RmsBwdArgs a) {
         if (a.ddelta) {
 #pragma unroll
           for (int k = 0; k < VEC; ++k) o[k] *= f;
-          rms_store<TD, VEC>((TD*)a.ddelta + r * C + c, o);
+          rms_store_as<VEC>(a.ddelta, a.delta_dtype, r * C + c, o);
         }
       }
     }
   }
   if (a.part && NV > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (c < C)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) dws[slot * C + c + k] = sums[i][k];
+    }
     __syncthreads();
     for (int c = threadIdx.x; c < C; c += 256) {
       float v = 0.f;
@@ -289,64 +325,80 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(RmsBwdArgs a) {
   }
 }
 
-// dw[c] = sum over blocks of part[block][c], in block order.
-__global__ void __launch_bounds__(256) rms_dw_kernel(const float* __restrict__ part, int64_t blocks, int C,
-                                                     float* __restrict__ dw) {
-  __shared__ float red[8][33];
+// dw[c] = sum over blocks of part[block][c], in a fixed order: 32 channels x
+// 32 lanes of blocks.
+__global__ void __launch_bounds__(1024) rms_dw_kernel(const float* __restrict__ part, int64_t blocks, int C,
+                                                      float* __restrict__ dw) {
+  __shared__ float red[32][33];
   const int x = threadIdx.x & 31, l = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + x;
   float v = 0.f;
   if (c < C) {
-#pragma unroll 4
-    for (int64_t b = l; b < blocks; b += 8) v += part[b * C + c];
+#pragma unroll 8
+    for (int64_t b = l; b < blocks; b += 32) v += __ldg(part + b * C + c);
   }
   red[l][x] = v;
   __syncthreads();
-  if (l == 0 && c < C) {
-    v = 0.f;
-    for (int k = 0; k < 8; ++k) v += red[k][x];
-    dw[c] = v;
+  v = warp_sum(red[x][l]);
+  if (x == 0 && blockIdx.x * 32 + l < C) dw[blockIdx.x * 32 + l] = v;
+}
+
+// Threads that share a row, and chunks each holds (0: more than fit).
+struct RowLayout {
+  int tpr, nv;
+};
+static RowLayout rms_layout(int64_t C, int vec) {
+  const int64_t n = (C + vec - 1) / vec;  // chunks of a row
+  if (vec == 8) {
+    if (n <= 8) return {8, 1};
+    if (n <= 16) return {16, 1};
+    if (n <= 32) return {32, 1};
+    if (n <= 48) return {16, 3};
+    if (n <= 64) return {32, 2};
+    if (n <= 128) return {32, 4};
+  } else {
+    if (n <= 32) return {32, 1};
+    if (n <= 128) return {32, 4};
   }
+  return {256, n <= 256 ? 1 : n <= 512 ? 2 : n <= 1024 ? 4 : 0};
 }
 
 constexpr int RMS_BWD_BLOCKS_PER_SM = 4;
-static int64_t rms_bwd_blocks(int64_t R, int rows) {
+static int64_t rms_bwd_blocks(int64_t R, int64_t rows) {
   return imin64((R + rows - 1) / rows, (int64_t)sm_count() * RMS_BWD_BLOCKS_PER_SM);
 }
-// Rows a block takes side by side (the kernels' ROWS).
-static int rms_rows(int C, bool vec) { return C <= 32 * (vec ? 8 : 1) * 4 ? 8 : 1; }
 
-template <typename TX, typename TD, int VEC>
+#define RMS_LAYOUTS(VEC, L, GO)                      \
+  if (VEC == 8 && L.tpr == 8) GO(8, 1)               \
+  else if (VEC == 8 && L.tpr == 16 && L.nv == 1) GO(16, 1) \
+  else if (VEC == 8 && L.tpr == 16) GO(16, 3)        \
+  else if (L.tpr == 32 && L.nv == 1) GO(32, 1)       \
+  else if (VEC == 8 && L.tpr == 32 && L.nv == 2) GO(32, 2) \
+  else if (L.tpr == 32) GO(32, 4)                    \
+  else if (L.nv == 1) GO(256, 1)                     \
+  else if (L.nv == 2) GO(256, 2)                     \
+  else if (L.nv == 4) GO(256, 4)                     \
+  else GO(256, 0)
+
+template <typename TX, int VEC>
 static void rms_fwd_launch(const RmsArgs& a, cudaStream_t st) {
-  const int64_t sms = sm_count();
-  const int C = a.C;
-#define RMS_FWD(W, NV)                                                                                \
-  rms_fwd_kernel<TX, TD, W, NV, VEC>                                                                  \
-      <<<(unsigned)imin64((a.R + 8 / W - 1) / (8 / W), sms * 8), 256, 0, st>>>(a)
-  if (C <= 32 * VEC) RMS_FWD(1, 1);
-  else if (C <= 64 * VEC) RMS_FWD(1, 2);
-  else if (C <= 128 * VEC) RMS_FWD(1, 4);
-  else if (C <= 256 * VEC) RMS_FWD(8, 1);
-  else if (C <= 512 * VEC) RMS_FWD(8, 2);
-  else if (C <= 1024 * VEC) RMS_FWD(8, 4);
-  else RMS_FWD(8, 0);
-#undef RMS_FWD
+  const RowLayout l = rms_layout(a.C, VEC);
+  const int64_t rows = 256 / l.tpr;
+  const unsigned blocks = (unsigned)imin64((a.R + rows - 1) / rows, (int64_t)sm_count() * 8);
+#define RMS_GO(TPR, NV) rms_fwd_kernel<TX, TPR, NV, VEC><<<blocks, 256, 0, st>>>(a);
+  RMS_LAYOUTS(VEC, l, RMS_GO)
+#undef RMS_GO
 }
 
-template <typename TX, typename TD, int VEC>
+template <typename TX, int VEC>
 static void rms_bwd_launch(const RmsBwdArgs& a, cudaStream_t st) {
-  const int C = a.C;
-#define RMS_BWD(W, NV)                                                                                        \
-  rms_bwd_kernel<TX, TD, W, NV, VEC><<<(unsigned)rms_bwd_blocks(a.R, 8 / W), 256,                             \
-                                       a.part && NV > 0 ? (size_t)(8 / W) * C * 4 : 0, st>>>(a)
-  if (C <= 32 * VEC) RMS_BWD(1, 1);
-  else if (C <= 64 * VEC) RMS_BWD(1, 2);
-  else if (C <= 128 * VEC) RMS_BWD(1, 4);
-  else if (C <= 256 * VEC) RMS_BWD(8, 1);
-  else if (C <= 512 * VEC) RMS_BWD(8, 2);
-  else if (C <= 1024 * VEC) RMS_BWD(8, 4);
-  else RMS_BWD(8, 0);
-#undef RMS_BWD
+  const RowLayout l = rms_layout(a.C, VEC);
+  const int64_t rows = 256 / l.tpr;
+  const unsigned blocks = (unsigned)rms_bwd_blocks(a.R, rows);
+  const size_t smem = a.part && l.nv > 0 ? (size_t)rows * a.C * 4 : 0;  // at most 32 KB
+#define RMS_GO(TPR, NV) rms_bwd_kernel<TX, TPR, NV, VEC><<<blocks, 256, smem, st>>>(a);
+  RMS_LAYOUTS(VEC, l, RMS_GO)
+#undef RMS_GO
 }
 
 static bool rms_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -360,15 +412,6 @@ static int rms_check(int x_dtype, int delta_dtype, bool has_delta, int64_t R, in
                "rms_norm: row_scale needs delta and a group count that divides the rows");
   return AFFB_OK;
 }
-
-#define RMS_DISPATCH(xd, dd, TX, TD, ...)                                       \
-  AFFB_DISPATCH(xd, TX, {                                                       \
-    switch (dd) {                                                               \
-      case AFFB_F32: { using TD = float; __VA_ARGS__; break; }                  \
-      case AFFB_F16: { using TD = __half; __VA_ARGS__; break; }                 \
-      default: { using TD = __nv_bfloat16; __VA_ARGS__; break; }                \
-    }                                                                           \
-  })
 
 }  // namespace affb
 
@@ -387,15 +430,14 @@ extern "C" int affb_rms_norm_fwd(const void* x, int x_dtype, const void* delta, 
   AFFB_REQUIRE(!s || delta, "rms_norm: the sum is written only with delta");
   if (R == 0) return AFFB_OK;
   AFFB_REQUIRE(x && weight, "rms_norm: null pointer");
-  RmsArgs a{x, delta, row_scale, row_scale ? R / groups : 1, weight, eps, R, (int)C, s, rstd, y, y_dtype,
+  RmsArgs a{x, delta, delta_dtype, row_scale, row_scale ? R / groups : 1, weight, eps, R, (int)C, s, rstd, y, y_dtype,
             (uint8_t*)q, q_scale};
   const bool vec = C % 8 == 0 && rms_aligned(x) && rms_aligned(delta) && rms_aligned(weight) && rms_aligned(s) &&
                    rms_aligned(y) && ((uintptr_t)q & 7) == 0;
   cudaStream_t st = as_stream(stream);
-  const int dd = delta ? delta_dtype : x_dtype;
-  RMS_DISPATCH(x_dtype, dd, TX, TD, {
-    if (vec) rms_fwd_launch<TX, TD, 8>(a, st);
-    else rms_fwd_launch<TX, TD, 1>(a, st);
+  AFFB_DISPATCH(x_dtype, TX, {
+    if (vec) rms_fwd_launch<TX, 8>(a, st);
+    else rms_fwd_launch<TX, 1>(a, st);
   });
   AFFB_LAUNCH_CHECK("affb_rms_norm_fwd");
   return AFFB_OK;
@@ -407,12 +449,12 @@ extern "C" int affb_quantize_e4m3(const void* x, int dtype, int64_t R, int64_t C
   if (rc) return rc;
   if (R == 0) return AFFB_OK;
   AFFB_REQUIRE(x && q && q_scale, "quantize_e4m3: null pointer");
-  RmsArgs a{x, nullptr, nullptr, 1, nullptr, 0.f, R, (int)C, nullptr, nullptr, nullptr, AFFB_F32, (uint8_t*)q, q_scale};
+  RmsArgs a{x, nullptr, AFFB_F32, nullptr, 1, nullptr, 0.f, R, (int)C, nullptr, nullptr, nullptr, AFFB_F32, (uint8_t*)q, q_scale};
   const bool vec = C % 8 == 0 && rms_aligned(x) && ((uintptr_t)q & 7) == 0;
   cudaStream_t st = as_stream(stream);
   AFFB_DISPATCH(dtype, TX, {
-    if (vec) rms_fwd_launch<TX, TX, 8>(a, st);
-    else rms_fwd_launch<TX, TX, 1>(a, st);
+    if (vec) rms_fwd_launch<TX, 8>(a, st);
+    else rms_fwd_launch<TX, 1>(a, st);
   });
   AFFB_LAUNCH_CHECK("affb_quantize_e4m3");
   return AFFB_OK;
@@ -443,16 +485,15 @@ extern "C" int affb_rms_norm_bwd(const void* dy, int y_dtype, const void* ds, co
   AFFB_REQUIRE(s && rstd && weight, "rms_norm: null pointer");
   const bool vec = C % 8 == 0 && rms_aligned(dy) && rms_aligned(ds) && rms_aligned(s) && rms_aligned(weight) &&
                    rms_aligned(dx) && rms_aligned(ddelta);
-  const int64_t blocks = rms_bwd_blocks(R, rms_rows((int)C, vec));
+  const int64_t blocks = rms_bwd_blocks(R, 256 / rms_layout(C, vec ? 8 : 1).tpr);
   AFFB_REQUIRE(!dweight || (workspace && workspace_bytes >= blocks * C * 4), "rms_norm: workspace too small");
-  RmsBwdArgs a{dy, y_dtype, ds, s, rstd, weight, row_scale, row_scale ? R / groups : 1, R, (int)C, dx, ddelta,
+  RmsBwdArgs a{dy, y_dtype, ds, s, rstd, weight, row_scale, row_scale ? R / groups : 1, R, (int)C, dx, ddelta, delta_dtype,
                dweight ? (float*)workspace : nullptr};
-  const int dd = ddelta ? delta_dtype : x_dtype;
-  RMS_DISPATCH(x_dtype, dd, TX, TD, {
-    if (vec) rms_bwd_launch<TX, TD, 8>(a, st);
-    else rms_bwd_launch<TX, TD, 1>(a, st);
+  AFFB_DISPATCH(x_dtype, TX, {
+    if (vec) rms_bwd_launch<TX, 8>(a, st);
+    else rms_bwd_launch<TX, 1>(a, st);
   });
-  if (dweight) rms_dw_kernel<<<(unsigned)((C + 31) / 32), 256, 0, st>>>((const float*)workspace, blocks, (int)C, dweight);
+  if (dweight) rms_dw_kernel<<<(unsigned)((C + 31) / 32), 1024, 0, st>>>((const float*)workspace, blocks, (int)C, dweight);
   AFFB_LAUNCH_CHECK("affb_rms_norm_bwd");
   return AFFB_OK;
 }

@@ -17,6 +17,7 @@ as ``index(y) * n + index(x)`` of ``n = bucket_count(edges, 1, one_sided)``.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 import torch.nn as nn
@@ -47,11 +48,20 @@ def bucket_count(edges, axes: int = 1, one_sided: bool = False) -> int:
 
 
 def _check_edges(edges) -> tuple[int, ...]:
-    edges = tuple(edges)
+    return _checked(tuple(edges))
+
+
+@functools.lru_cache(maxsize=256)
+def _checked(edges) -> tuple[int, ...]:
     if not 1 <= len(edges) <= 64 or any(int(e) != e or not 1 <= e <= 1 << 30 for e in edges) \
             or any(a >= b for a, b in zip(edges, edges[1:])):
         raise RuntimeError("bucket_bias: edges must be 1 to 64 ascending integers in [1, 2^30]")
     return tuple(int(e) for e in edges)
+
+
+@functools.lru_cache(maxsize=256)
+def _edge_array(edges):
+    return (ctypes.c_int32 * len(edges))(*edges)
 
 
 def _check(table, edges, q_pos, k_pos, member_idx, one_sided, dtype) -> tuple[int, ...]:
@@ -91,7 +101,7 @@ def _members(member_idx):
 
 def bucket_bias_fwd(table, edges, q_pos, k_pos, member_idx, one_sided, dtype):
     """bias [B,H,Nq,M]; dense inputs, int32 members."""
-    arr = (ctypes.c_int32 * len(edges))(*edges)
+    arr = _edge_array(edges)
     B, Nq, axes = q_pos.shape
     Nk, H = k_pos.shape[1], table.shape[1]
     M = member_idx.shape[2] if member_idx is not None else Nk
@@ -99,13 +109,13 @@ def bucket_bias_fwd(table, edges, q_pos, k_pos, member_idx, one_sided, dtype):
     out = torch.empty((B, H, Nq, M), device=dev, dtype=dtype)
     nat.call_on(dev, "affb_bucket_bias_fwd", nat.ptr(table), nat.dcode(table), ctypes.addressof(arr), len(edges),
                 int(one_sided), nat.ptr(q_pos), nat.ptr(k_pos), _POS[q_pos.dtype], axes, nat.ptr(member_idx), B, H, Nq,
-                Nk, M, nat.ptr(out), nat.dcode(out), nat.stream(dev))
+                Nk, M, nat.ptr(out), nat.dcode(out))
     return out
 
 
 def bucket_bias_bwd(dout, edges, q_pos, k_pos, member_idx, one_sided, dtype):
     """The table's gradient in `dtype`; dense inputs, int32 members."""
-    arr = (ctypes.c_int32 * len(edges))(*edges)
+    arr = _edge_array(edges)
     B, Nq, axes = q_pos.shape
     _, H, _, M = dout.shape
     dev = dout.device
@@ -113,15 +123,14 @@ def bucket_bias_bwd(dout, edges, q_pos, k_pos, member_idx, one_sided, dtype):
     ws = nat.workspace("affb_bucket_bias_bwd_workspace_bytes", dev, len(edges), int(one_sided), axes, B, H, Nq, M)
     nat.call_on(dev, "affb_bucket_bias_bwd", nat.ptr(dout), nat.dcode(dout), ctypes.addressof(arr), len(edges),
                 int(one_sided), nat.ptr(q_pos), nat.ptr(k_pos), _POS[q_pos.dtype], axes, nat.ptr(member_idx), B, H, Nq,
-                k_pos.shape[1], M, nat.ptr(dtable), nat.dcode(dtable), nat.ptr(ws), ws.numel() if ws is not None else 0,
-                nat.stream(dev))
+                k_pos.shape[1], M, nat.ptr(dtable), nat.dcode(dtable), nat.ptr(ws), ws.numel() if ws is not None else 0)
     return dtable
 
 
 class BucketBiasFunction(Function):
     @staticmethod
     def forward(ctx, table, edges, q_pos, k_pos, member_idx, one_sided, dtype):
-        qp, kp, mem = q_pos.contiguous(), k_pos.contiguous(), _members(member_idx)
+        qp, kp, mem = nat.dense(q_pos), nat.dense(k_pos), _members(member_idx)
         out = bucket_bias_fwd(table.contiguous(), edges, qp, kp, mem, one_sided, dtype)
         ctx.save_for_backward(qp, kp, mem)
         ctx.meta = (edges, bool(one_sided), table.dtype)
@@ -148,6 +157,9 @@ def bucket_bias(table: torch.Tensor, edges, q_pos: torch.Tensor, k_pos: torch.Te
     Differentiable once in the table."""
     dtype = table.dtype if dtype is None else dtype
     edges = _check(table, edges, q_pos, k_pos, member_idx, one_sided, dtype)
+    if not (torch.is_grad_enabled() and table.requires_grad):
+        return bucket_bias_fwd(table.contiguous(), edges, nat.dense(q_pos), nat.dense(k_pos), _members(member_idx),
+                               one_sided, dtype)
     return BucketBiasFunction.apply(table, edges, q_pos, k_pos, member_idx, one_sided, dtype)
 
 

@@ -71,8 +71,7 @@ def linear_fwd(x, weight, bias, residual, act: int, save: bool):
     ws = nat.workspace("affb_linear_fwd_workspace_bytes", dev, dt, M, N, K)
     nat.call_on(dev, "affb_linear_fwd", nat.ptr(x), nat.ptr(weight), nat.ptr(bc),
                 nat.dcode(bc) if bc is not None else 0, nat.ptr(rc), nat.dcode(rc) if rc is not None else 0, act, dt,
-                M, N, K, nat.ptr(out), nat.dcode(out), nat.ptr(z), nat.ptr(ws), ws.numel() if ws is not None else 0,
-                nat.stream(dev))
+                M, N, K, nat.ptr(out), nat.dcode(out), nat.ptr(z), nat.ptr(ws), ws.numel() if ws is not None else 0)
     return out, z
 
 
@@ -97,7 +96,7 @@ def linear_bwd(dout, z, x, weight, act: int, need_x: bool, need_w: bool, bias_dt
         ws = nat.workspace("affb_linear_bwd_workspace_bytes", dev, dt, M, N, K)
         nat.call_on(dev, "affb_linear_bwd", nat.ptr(dout), nat.dcode(dout), nat.ptr(z), nat.ptr(x), nat.ptr(weight), act,
                     dt, M, N, K, nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.dcode(db) if db is not None else 0,
-                    nat.ptr(ws), ws.numel() if ws is not None else 0, nat.stream(dev))
+                    nat.ptr(ws), ws.numel() if ws is not None else 0)
     return dx, dw, db
 
 
@@ -134,6 +133,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     "silu".  Differentiable once in x, weight, bias and residual."""
     code = _act_code(act)
     _check_operands(x, weight, bias, residual)
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))):
+        return linear_fwd(nat.dense(x), nat.dense(weight), bias, residual, code, False)[0]
     return FusedLinearFunction.apply(x, weight, bias, residual, code)
 
 
@@ -171,7 +172,7 @@ def quantize_e4m3(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
     scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
     nat.call_on(x.device, "affb_quantize_e4m3", nat.ptr(xc), nat.dcode(xc), xc.numel() // C, C, nat.ptr(q),
-                nat.ptr(scale), nat.stream(x.device))
+                nat.ptr(scale))
     return q, scale
 
 
@@ -203,7 +204,7 @@ def linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     ws = nat.workspace("affb_linear_e4m3_workspace_bytes", dev, M, N, K)
     nat.call_on(dev, "affb_linear_e4m3", nat.ptr(xc), nat.ptr(xs), nat.ptr(wc), nat.ptr(wsc), nat.ptr(bc), nat.ptr(rc),
                 nat.dcode(rc) if rc is not None else 0, code, M, N, K, nat.ptr(out), nat.dcode(out), nat.ptr(ws),
-                ws.numel() if ws is not None else 0, nat.stream(dev))
+                ws.numel() if ws is not None else 0)
     return out
 
 

@@ -53,7 +53,7 @@ def _launch(x, delta, row_scale, weight, eps, out_dtype, keep):
     xc = nat.dense(x)
     dc = nat.dense(delta) if delta is not None else None
     rs = row_scale.float().contiguous() if row_scale is not None else None
-    w = nat.dense(weight.detach().float())
+    w = nat.dense(weight.detach().float() if weight.requires_grad or weight.dtype != torch.float32 else weight)
     s = torch.empty(x.shape, device=dev, dtype=x.dtype) if dc is not None else None
     rstd = torch.empty(R, device=dev, dtype=torch.float32) if keep else None
     y = q = scale = None
@@ -65,7 +65,7 @@ def _launch(x, delta, row_scale, weight, eps, out_dtype, keep):
     nat.call_on(dev, "affb_rms_norm_fwd", nat.ptr(xc), nat.dcode(xc), nat.ptr(dc),
                 nat.dcode(dc) if dc is not None else 0, nat.ptr(rs), rs.numel() if rs is not None else 0, nat.ptr(w),
                 float(eps), R, C, nat.ptr(s), nat.ptr(rstd), nat.ptr(y), nat.dcode(y) if y is not None else 0,
-                nat.ptr(q), nat.ptr(scale), nat.stream(dev))
+                nat.ptr(q), nat.ptr(scale))
     return xc, rs, w, s, rstd, y, q, scale
 
 
@@ -82,8 +82,7 @@ def rms_norm_bwd(dy, ds, s, rstd, weight, row_scale, need_x: bool, need_w: bool,
     nat.call_on(dev, "affb_rms_norm_bwd", nat.ptr(dy), nat.dcode(dy) if dy is not None else 0, nat.ptr(ds), nat.ptr(s),
                 nat.dcode(s), nat.ptr(rstd), nat.ptr(weight), nat.ptr(row_scale),
                 row_scale.numel() if row_scale is not None else 0, R, C, nat.ptr(dx), nat.ptr(dd),
-                nat.dcode(dd) if dd is not None else 0, nat.ptr(dw), nat.ptr(ws), ws.numel() if ws is not None else 0,
-                nat.stream(dev))
+                nat.dcode(dd) if dd is not None else 0, nat.ptr(dw), nat.ptr(ws), ws.numel() if ws is not None else 0)
     return dx, dw, dd
 
 
@@ -123,10 +122,12 @@ def fused_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, del
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in _FLOATS:
         raise RuntimeError(f"rms_norm: unsupported output dtype {out_dtype}")
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, delta))):
+        _, _, _, s, _, y, _, _ = _launch(x, delta, row_scale, weight, eps, out_dtype, False)
+        return y if s is None else (s, y)
     return FusedRMSNormFunction.apply(x, weight, delta, row_scale, eps, out_dtype)
 
 
-@torch.no_grad()
 def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, delta: torch.Tensor | None = None,
                   row_scale: torch.Tensor | None = None):
     """(q, scale), or (s, q, scale) when ``delta`` is given: the norm with its

@@ -313,7 +313,7 @@ def _(x, weight, eps, delta, row_scale):
 def bucket_bias_fwd(table: Tensor, edges: list[int], q_pos: Tensor, k_pos: Tensor, member_idx: Optional[Tensor],
                     one_sided: bool, dtype: torch.dtype) -> Tensor:
     edges = _bb._check(table, edges, q_pos, k_pos, member_idx, one_sided, dtype)
-    return _bb.bucket_bias_fwd(table.contiguous(), edges, q_pos.contiguous(), k_pos.contiguous(),
+    return _bb.bucket_bias_fwd(table.contiguous(), edges, _nat.dense(q_pos), _nat.dense(k_pos),
                                _bb._members(member_idx), one_sided, dtype)
 
 
@@ -326,7 +326,7 @@ def _(table, edges, q_pos, k_pos, member_idx, one_sided, dtype):
 @custom_op("affb200::bucket_bias_bwd", mutates_args=())
 def bucket_bias_bwd(dout: Tensor, edges: list[int], q_pos: Tensor, k_pos: Tensor, member_idx: Optional[Tensor],
                     one_sided: bool, dtype: torch.dtype) -> Tensor:
-    return _bb.bucket_bias_bwd(_nat.dense(dout), tuple(edges), q_pos.contiguous(), k_pos.contiguous(),
+    return _bb.bucket_bias_bwd(_nat.dense(dout), tuple(edges), _nat.dense(q_pos), _nat.dense(k_pos),
                                _bb._members(member_idx), one_sided, dtype)
 
 

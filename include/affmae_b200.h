@@ -425,7 +425,8 @@ int affb_rms_norm_bwd(const void* dy, int y_dtype, const void* ds, const void* s
  * n_edges + sign(d) c(|d|), or one sided c(max(-d, 0)); two axes (x, y)
  * combine as index(y) * n + index(x), n = 2 n_edges + 1 (n_edges + 1).
  * edges: host array, ascending in [1, 2^30], at most 64 (32 with two axes);
- * table [n^axes, H]; q_pos [B,Nq,axes], k_pos [B,Nk,axes] of pos_type;
+ * table [n^axes, H]; q_pos [B,Nq,axes], k_pos [B,Nk,axes] of pos_type, aligned
+ * to a pair of coordinates where axes = 2;
  * member_idx [B,Nq,M] int32 key indices, or NULL: all keys (M = Nk); an index
  * outside [0, Nk) gives bias 0.  out [B,H,Nq,M].                            */
 enum { AFFB_POS_F32 = 0, AFFB_POS_I32 = 1, AFFB_POS_I64 = 2 };
