@@ -63,10 +63,38 @@ struct GemmArgs {
 __device__ __forceinline__ int part_a(int i) { return (0x010120 >> (4 * i)) & 15; }
 __device__ __forceinline__ int part_b(int i) { return (0x001102 >> (4 * i)) & 15; }
 
-template <typename T> struct code_of;
-template <> struct code_of<float> { static constexpr int value = AFFB_F32; };
-template <> struct code_of<__half> { static constexpr int value = AFFB_F16; };
-template <> struct code_of<__nv_bfloat16> { static constexpr int value = AFFB_BF16; };
+// The units of work of a block: (split, row tile, column tile), column tiles
+// fastest, every gridDim.x-th.  Divides once, then steps by additions.
+struct Units {
+  int s, mi, ni, step_m, step_n;
+  __device__ __forceinline__ explicit Units(const GemmArgs& p) {
+    const int tiles = p.mt * p.nt, t = blockIdx.x % tiles;
+    s = blockIdx.x / tiles;
+    mi = t / p.nt;
+    ni = t - mi * p.nt;
+    step_m = gridDim.x / p.nt;
+    step_n = gridDim.x - step_m * p.nt;
+  }
+  __device__ __forceinline__ bool more(const GemmArgs& p) const { return s < p.splits; }
+  __device__ __forceinline__ void next(const GemmArgs& p) {
+    mi += step_m;
+    ni += step_n;
+    if (ni >= p.nt) {
+      ni -= p.nt;
+      ++mi;
+    }
+    while (mi >= p.mt) {
+      mi -= p.mt;
+      ++s;
+    }
+  }
+  __device__ __forceinline__ int first_k(int total_k, const GemmArgs& p) const {
+    return p.splits == 1 ? 0 : (int)((int64_t)total_k * s / p.splits);
+  }
+  __device__ __forceinline__ int last_k(int total_k, const GemmArgs& p) const {
+    return p.splits == 1 ? total_k : (int)((int64_t)total_k * (s + 1) / p.splits);
+  }
+};
 
 // 32 columns of one row into a warp's staging buffer, in the swizzle that the
 // TMA store undoes (64-byte rows: 64B swizzle, 128-byte rows: 128B).
@@ -145,24 +173,25 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
   fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
-  const int units = p.mt * p.nt * p.splits;
   const int total_k = p.kblocks * p.parts;
-  const int ke = p.f8 ? 128 : 64;  // elements of one k block
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0;
+      const int ke = p.f8 ? 128 : 64;  // elements of one k block
+      int st = 0, count = 0;
+      uint32_t phase = 1;
       bool ok = true;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        const int tile = u % (p.mt * p.nt), s = u / (p.mt * p.nt);
-        const int m0 = tile / p.nt * TILE_M, n0 = tile % p.nt * p.bn;
-        const int kb0 = (int)((int64_t)total_k * s / p.splits), kb1 = (int)((int64_t)total_k * (s + 1) / p.splits);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int st = it % p.stages;
-          if (!(ok = bar_wait(empty + 8 * st, ((it / p.stages) & 1) ^ 1, failed))) break;
-          const int part = kb / p.kblocks, k0 = (kb - part * p.kblocks) * ke;
+      const uint32_t base = smem_addr(smem);
+      for (Units u(p); u.more(p) && ok; u.next(p)) {
+        const int m0 = u.mi * TILE_M, n0 = u.ni * p.bn;
+        const int kb0 = u.first_k(total_k, p), kb1 = u.last_k(total_k, p);
+        int part = p.parts > 1 ? kb0 / p.kblocks : 0;
+        int kk = kb0 - part * p.kblocks;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!(ok = bar_wait(empty + 8 * st, phase, failed))) break;
+          const int k0 = kk * ke;
           const int za = p.parts > 1 ? part_a(part) : 0, zb = p.parts > 1 ? part_b(part) : 0;
-          const uint32_t bar = full + 8 * st, a = smem_addr(smem + st * stage_bytes), b = a + A_BYTES;
+          const uint32_t bar = full + 8 * st, a = base + st * stage_bytes, b = a + A_BYTES;
           bar_expect(bar, stage_bytes);
           if (p.a_mn) {
             tma_load(a, &map_a, m0, k0, za, bar);
@@ -175,42 +204,58 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
           } else {
             tma_load(b, &map_b, k0, n0, zb, bar);
           }
+          ++count;
+          if (++kk == p.kblocks) {
+            kk = 0;
+            ++part;
+          }
+          if (++st == p.stages) {
+            st = 0;
+            phase ^= 1;
+          }
         }
       }
       if (!ok)  // loads still in flight must land before the block's memory is given back
-        for (int i = it > p.stages ? it - p.stages : 0; i < it; ++i)
+        for (int i = count > p.stages ? count - p.stages : 0; i < count; ++i)
           bar_drain(full + 8 * (i % p.stages), (i / p.stages) & 1);
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      int it = 0, acc_it = 0;
+      int st = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 1;
       bool ok = true;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++acc_it) {
-        const int s = u / (p.mt * p.nt);
-        const int kb0 = (int)((int64_t)total_k * s / p.splits), kb1 = (int)((int64_t)total_k * (s + 1) / p.splits);
-        const int acc = acc_it & 1;
-        if (!(ok = bar_wait(acc_empty + 8 * acc, ((acc_it >> 1) & 1) ^ 1, failed))) break;
+      // advance of 32 bytes along k (K-major) or of 16 k rows (MN-major)
+      const uint64_t sa = p.a_mn ? 2048 >> 4 : 32 >> 4, sb = p.b_mn ? 2048 >> 4 : 32 >> 4;
+      const uint32_t base = smem_addr(smem);
+      const uint64_t da0 = smem_desc(base, p.a_mn ? 8192 : 0, 1024);
+      const uint64_t db0 = smem_desc(base + A_BYTES, p.b_mn ? 8192 : 0, 1024);
+      for (Units u(p); u.more(p) && ok; u.next(p)) {
+        const int n_k = u.last_k(total_k, p) - u.first_k(total_k, p);
+        if (!(ok = bar_wait(acc_empty + 8 * acc, acc_phase, failed))) break;
         fence_after();
         const uint32_t d = tmem + acc * 256;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int st = it % p.stages;
-          if (!(ok = bar_wait(full + 8 * st, (it / p.stages) & 1, failed))) break;
+        for (int kb = 0; kb < n_k; ++kb) {
+          if (!(ok = bar_wait(full + 8 * st, phase, failed))) break;
           fence_after();
-          const uint32_t a = smem_addr(smem + st * stage_bytes), b = a + A_BYTES;
-          // advance of 32 bytes along k (K-major) or of 16 k rows (MN-major)
-          const uint64_t da = smem_desc(a, p.a_mn ? 8192 : 0, 1024), db = smem_desc(b, p.b_mn ? 8192 : 0, 1024);
-          const uint64_t sa = p.a_mn ? 2048 >> 4 : 32 >> 4, sb = p.b_mn ? 2048 >> 4 : 32 >> 4;
+          const uint64_t off = (uint64_t)((uint32_t)(st * stage_bytes) >> 4);
+          const uint64_t da = da0 + off, db = db0 + off;
           if (p.f8) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma_f8(d, da + k * sa, db + k * sb, p.idesc, kb > kb0 || k > 0);
+            for (int k = 0; k < 4; ++k) mma_f8(d, da + k * sa, db + k * sb, p.idesc, kb > 0 || k > 0);
           } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma_f16(d, da + k * sa, db + k * sb, p.idesc, kb > kb0 || k > 0);
+            for (int k = 0; k < 4; ++k) mma_f16(d, da + k * sa, db + k * sb, p.idesc, kb > 0 || k > 0);
           }
           mma_commit(empty + 8 * st);
+          if (++st == p.stages) {
+            st = 0;
+            phase ^= 1;
+          }
         }
         if (ok) mma_commit(acc_full + 8 * acc);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
       }
       if (!ok) {
         mma_commit(drain);
@@ -222,12 +267,11 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
     const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
     unsigned char* my = staging + ew * p.bufs * p.buf_bytes;
     float* bias = cols + ew * 2 * CHUNK;
-    int acc_it = 0, buf = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x, ++acc_it) {
-      const int tile = u % (p.mt * p.nt), s = u / (p.mt * p.nt);
-      const int m0 = tile / p.nt * TILE_M, n0 = tile % p.nt * p.bn;
+    int acc = 0, buf = 0;
+    uint32_t acc_phase = 0;
+    for (Units u(p); u.more(p); u.next(p)) {
+      const int s = u.s, m0 = u.mi * TILE_M, n0 = u.ni * p.bn;
       const int ncols = min(p.bn, p.N - n0);
-      const int acc = acc_it & 1;
       const int m = m0 + quad * 32 + lane;
       // the next chunk's bias and column scale of this lane's column
       float nb = 0.f, ns = 1.f;
@@ -245,15 +289,24 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
       if (per_col) fetch(half * CHUNK);
       const float rs = (p.e.row_scale && m < p.M) ? p.e.row_scale[m] : 1.f;
       // all lanes of the warp leave together
-      if (__any_sync(0xffffffffu, !bar_wait(acc_full + 8 * acc, (acc_it >> 1) & 1, failed))) break;
+      if (__any_sync(0xffffffffu, !bar_wait(acc_full + 8 * acc, acc_phase, failed))) break;
       fence_after();
+      // the accumulator's next chunk is on its way while one is worked on
+      uint32_t r[32];
+      const uint32_t lanes = tmem + acc * 256 + ((uint32_t)(quad * 32) << 16);
+      if (half * CHUNK < ncols) tmem_load32(lanes + half * CHUNK, r);
       for (int c = half * CHUNK; c < ncols; c += 2 * CHUNK) {
-        uint32_t r[32];
-        tmem_load32(tmem + acc * 256 + c + ((uint32_t)(quad * 32) << 16), r);
         tmem_wait_load();
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        if (c + 2 * CHUNK < ncols) {
+          tmem_load32(lanes + c + 2 * CHUNK, r);
+        } else {  // all of it has been read
+          fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(acc_empty + 8 * acc);
+        }
         if (per_col) {
           __syncwarp();  // the chunk before has been read
           bias[lane] = nb;
@@ -311,9 +364,13 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
           if (p.bufs == 2) buf ^= 1;
         }
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(acc_empty + 8 * acc);
+      if (half * CHUNK >= ncols) {  // a warp without a chunk in a narrow tile
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(acc_empty + 8 * acc);
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
     }
     if (lane == 0) store_wait_all();
     __syncwarp();

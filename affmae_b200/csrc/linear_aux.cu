@@ -237,11 +237,39 @@ __global__ void __launch_bounds__(1024) sum_parts_kernel(const float* __restrict
   }
 }
 
+// Few parts: a thread sums one element's in order.
+__global__ void __launch_bounds__(256) sum_few_parts_kernel(const float* __restrict__ part, int S, int64_t M, int64_t N,
+                                                            int64_t ld, LinearEpilogue e) {
+  const int64_t n = M * N, plane = M * ld;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t m = i / N, c = i - m * N;
+    const float* p = part + m * ld + c;
+    float v = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < S; ++k) v += __ldg(p + k * plane);
+    if (e.row_scale) v *= e.row_scale[m];
+    if (e.col_scale) v *= e.col_scale[c];
+    if (e.bias) v += load_as(e.bias, e.bias_dtype, c);
+    if (e.z) store_as(e.z, e.z_dtype, i, v);
+    v = activate_code(e.act, v);
+    if (e.residual) v += load_as(e.residual, e.residual_dtype, i);
+    store_as(e.out, e.out_dtype, i, v);
+  }
+}
+
 int linear_sum(const float* part, int64_t S, int64_t M, int64_t N, int64_t ld, const LinearEpilogue& e,
                cudaStream_t st) {
   if (M * N == 0) return AFFB_OK;
-  const unsigned blocks = (unsigned)imin64((M * N + 31) / 32, (int64_t)sm_count() * 4);
-  sum_parts_kernel<<<blocks, 1024, 0, st>>>(part, S, M, N, ld, e);
+  // Lanes over the parts only where elements are few (1184 parts of 192: 24 us
+  // with a thread an element, 9 with lanes); otherwise a thread an element
+  // streams them at full width (12 parts of 768 x 384: 7 against 107 us).
+  if (M * N >= (int64_t)sm_count() * 64) {
+    const unsigned blocks = (unsigned)imin64((M * N + 255) / 256, (int64_t)sm_count() * 8);
+    sum_few_parts_kernel<<<blocks, 256, 0, st>>>(part, (int)S, M, N, ld, e);
+  } else {
+    const unsigned blocks = (unsigned)imin64((M * N + 31) / 32, (int64_t)sm_count() * 4);
+    sum_parts_kernel<<<blocks, 1024, 0, st>>>(part, S, M, N, ld, e);
+  }
   AFFB_LAUNCH_CHECK("linear: sum of partial products");
   return AFFB_OK;
 }

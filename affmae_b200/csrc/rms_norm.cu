@@ -267,6 +267,14 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(RmsBwdArgs a) {
       if (NV == 0) rms_load<float, VEC>(a.w + c, wv[0]);
     };
     float dot = 0.f;
+    float dv[KEEP][VEC];  // ds, requested with the rest of the row
+    if (NV > 0 && a.ds && in) {
+#pragma unroll
+      for (int i = 0; i < steps; ++i) {
+        const int c = (i * TPR + t) * VEC;
+        if (c < C) rms_load<TX, VEC>((const TX*)a.ds + r * C + c, dv[NV > 0 ? i : 0]);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < steps; ++i) {
       const int c = (i * TPR + t) * VEC, n = NV > 0 ? i : 0;
@@ -294,10 +302,9 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(RmsBwdArgs a) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o[k] = rstd * (gv[n][k] * wv[n][k] - sv[n][k] * coef);
         if (a.ds) {
-          float d[VEC];
-          rms_load<TX, VEC>((const TX*)a.ds + r * C + c, d);
+          if (NV == 0) rms_load<TX, VEC>((const TX*)a.ds + r * C + c, dv[0]);
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) o[k] += d[k];
+          for (int k = 0; k < VEC; ++k) o[k] += dv[n][k];
         }
         if (a.dx) rms_store<TX, VEC>((TX*)a.dx + r * C + c, o);
         if (a.ddelta) {

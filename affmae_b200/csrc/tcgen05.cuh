@@ -46,12 +46,16 @@ __device__ __forceinline__ bool bar_poll(uint32_t bar, uint32_t parity) {
 }
 // True once the barrier's phase of this parity has completed; false when the
 // block has failed or the wait ran out (which marks the block as failed).
+// The timer is read only by a wait that has already polled long: one read
+// takes longer than a stage of the pipeline does.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
-  if (bar_poll(bar, parity)) return true;
+#pragma unroll 1
+  for (int i = 0; i < 4096; ++i)
+    if (bar_poll(bar, parity)) return true;
   const unsigned long long t0 = now_ns();
   for (;;) {
 #pragma unroll 1
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 256; ++i)
       if (bar_poll(bar, parity)) return true;
     if (*failed) return false;
     if (now_ns() - t0 > WAIT_NS) break;
