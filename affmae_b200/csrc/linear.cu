@@ -7,10 +7,15 @@
 // are brought in by TMA as 128-byte-swizzled tiles, K-major (rows of k) or
 // MN-major (rows of m or n, for the two products of the backward, which
 // contract over the other index of the stored matrices), and multiplied by
-// tcgen05.mma with the 128 x BN accumulator in tensor memory.  A block is
-// persistent and split by role: one warp issues the loads, one the products,
-// eight take the finished accumulator (two are in flight) through the
-// epilogue into shared memory, from where TMA stores write it.
+// tcgen05.mma with the accumulator in tensor memory.  A block is persistent
+// and split by role: one warp issues the loads, one the products, twelve take
+// the finished accumulator (two are in flight) through the epilogue into
+// shared memory, from where TMA stores write it.
+//
+// An SM takes in about 50 bytes a cycle, so a block that multiplies 128 x 256
+// tiles waits for its 48 KB of operands twice as long as the products take.
+// Two blocks of a cluster therefore share a 256 x 256 tile (cta_group::2):
+// each loads half of either operand, 32 KB, and keeps half of the rows.
 //
 // fp32 operands are split into three bf16 parts (8 mantissa bits each) and
 // the six leading products of parts are summed into the same accumulator,
@@ -30,9 +35,10 @@ namespace affb {
 using namespace tc5;
 
 constexpr int TILE_M = 128;
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 12;
+constexpr int EPI_GROUPS = EPI_WARPS / 4;   // warps that share the 32 rows of a quarter of tensor memory
 constexpr int LIN_THREADS = 64 + EPI_WARPS * 32;
-constexpr int A_BYTES = TILE_M * 128;
+constexpr int A_BYTES = TILE_M * 128;   // a block's rows of a tile
 constexpr int SMEM_MAX = 232448;     // 227 KB of a block
 constexpr int MAX_STAGES = 8;
 constexpr int STAGE_ROWS = 32;       // rows x columns of one warp's staging buffer
@@ -49,7 +55,8 @@ struct GemmArgs {
   int parts;         // pairs of operand parts summed (1, or 6 for fp32)
   int stages;
   int a_mn, b_mn, f8;
-  int b_bytes;
+  int a_blocks, b_blocks;  // MN-major: one load of that many 64-column blocks (0: a load each)
+  int b_bytes;       // a block's part of B
   uint32_t idesc;
   int direct;        // outputs not addressable by TMA: plain stores
   int bufs;          // staging buffers of a warp (2, or 1 where fp32 outputs make them large)
@@ -63,17 +70,17 @@ struct GemmArgs {
 __device__ __forceinline__ int part_a(int i) { return (0x010120 >> (4 * i)) & 15; }
 __device__ __forceinline__ int part_b(int i) { return (0x001102 >> (4 * i)) & 15; }
 
-// The units of work of a block: (split, row tile, column tile), column tiles
-// fastest, every gridDim.x-th.  Divides once, then steps by additions.
+// The units of work of a block or pair: (split, row tile, column tile), column
+// tiles fastest, every step-th.  Divides once, then steps by additions.
 struct Units {
   int s, mi, ni, step_m, step_n;
-  __device__ __forceinline__ explicit Units(const GemmArgs& p) {
-    const int tiles = p.mt * p.nt, t = blockIdx.x % tiles;
-    s = blockIdx.x / tiles;
+  __device__ __forceinline__ Units(const GemmArgs& p, int first, int step) {
+    const int tiles = p.mt * p.nt, t = first % tiles;
+    s = first / tiles;
     mi = t / p.nt;
     ni = t - mi * p.nt;
-    step_m = gridDim.x / p.nt;
-    step_n = gridDim.x - step_m * p.nt;
+    step_m = step / p.nt;
+    step_n = step - step_m * p.nt;
   }
   __device__ __forceinline__ bool more(const GemmArgs& p) const { return s < p.splits; }
   __device__ __forceinline__ void next(const GemmArgs& p) {
@@ -135,7 +142,16 @@ __device__ __forceinline__ void add_row(const T* p, int n, float* v) {
   }
 }
 
-template <typename TO, int ACT>
+// One k block: four products of 32 bytes along k.
+template <int CG, bool F8>
+__device__ __forceinline__ void mma_block(uint32_t d, uint64_t a, uint64_t b, uint64_t sa, uint64_t sb, uint32_t idesc,
+                                          bool accumulate) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) mma<CG, F8>(d, a + k * sa, b + k * sb, idesc, accumulate || k > 0);
+}
+
+// CG: blocks that share a tile of CG * 128 rows.
+template <typename TO, int ACT, int CG>
 __global__ void __launch_bounds__(LIN_THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_z,
@@ -151,7 +167,8 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
   volatile int* failed = reinterpret_cast<volatile int*>(bars + 200);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 208);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
       bar_init(full + 8 * i, 1);
@@ -159,7 +176,7 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(acc_full + 8 * i, 1);
-      bar_init(acc_empty + 8 * i, EPI_WARPS);
+      bar_init(acc_empty + 8 * i, EPI_WARPS * CG);
     }
     bar_init(drain, 1);
     bar_init_fence();
@@ -167,61 +184,74 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
     tma_prefetch(&map_a);
     tma_prefetch(&map_b);
   }
-  if (warp == 1) tmem_alloc<512>(smem_addr(tmem_slot));
+  if (warp == 1) tmem_alloc<CG>(smem_addr(tmem_slot));
   fence_before();
   __syncthreads();
+  if (CG == 2) cluster_sync();
   fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
   const int total_k = p.kblocks * p.parts;
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
 
   if (warp == 0) {
-    if (lane == 0) {
-      const int ke = p.f8 ? 128 : 64;  // elements of one k block
-      int st = 0, count = 0;
-      uint32_t phase = 1;
-      bool ok = true;
-      const uint32_t base = smem_addr(smem);
-      for (Units u(p); u.more(p) && ok; u.next(p)) {
-        const int m0 = u.mi * TILE_M, n0 = u.ni * p.bn;
-        const int kb0 = u.first_k(total_k, p), kb1 = u.last_k(total_k, p);
-        int part = p.parts > 1 ? kb0 / p.kblocks : 0;
-        int kk = kb0 - part * p.kblocks;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = bar_wait(empty + 8 * st, phase, failed))) break;
-          const int k0 = kk * ke;
-          const int za = p.parts > 1 ? part_a(part) : 0, zb = p.parts > 1 ? part_b(part) : 0;
-          const uint32_t bar = full + 8 * st, a = base + st * stage_bytes, b = a + A_BYTES;
-          bar_expect(bar, stage_bytes);
-          if (p.a_mn) {
-            tma_load(a, &map_a, m0, k0, za, bar);
-            tma_load(a + 8192, &map_a, m0 + 64, k0, za, bar);
+    const bool leads = elect_one();
+    const int ke = p.f8 ? 128 : 64;  // elements of one k block
+    int st = 0, count = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    const uint32_t base = smem_addr(smem);
+    // both blocks' loads complete on the first block's barrier, where the products are issued
+    const uint32_t full_at = CG == 2 ? peer_addr(full, 0) : full;
+    for (Units u(p, first, step); u.more(p) && ok; u.next(p)) {
+      const int m0 = (u.mi * CG + (int)rank) * TILE_M, n0 = u.ni * p.bn + (int)rank * (p.bn / CG);
+      const int kb0 = u.first_k(total_k, p), kb1 = u.last_k(total_k, p);
+      int part = p.parts > 1 ? kb0 / p.kblocks : 0;
+      int kk = kb0 - part * p.kblocks;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!(ok = warp_wait(empty + 8 * st, phase, failed))) break;
+        const int k0 = kk * ke;
+        const int za = p.parts > 1 ? part_a(part) : 0, zb = p.parts > 1 ? part_b(part) : 0;
+        const uint32_t bar = full_at + 8 * st, a = base + st * stage_bytes, b = a + A_BYTES;
+        if (leads) {
+          if (rank == 0) bar_expect(full + 8 * st, stage_bytes * CG);
+          if (p.a_blocks) {
+            tma_load4<CG>(a, &map_a, 0, k0, m0 >> 6, za, bar);
+          } else if (p.a_mn) {
+            tma_load<CG>(a, &map_a, m0, k0, za, bar);
+            tma_load<CG>(a + 8192, &map_a, m0 + 64, k0, za, bar);
           } else {
-            tma_load(a, &map_a, k0, m0, za, bar);
+            tma_load<CG>(a, &map_a, k0, m0, za, bar);
           }
-          if (p.b_mn) {
-            for (int j = 0; j * 8192 < p.b_bytes; ++j) tma_load(b + j * 8192, &map_b, n0 + 64 * j, k0, zb, bar);
+          if (p.b_blocks) {
+            tma_load4<CG>(b, &map_b, 0, k0, n0 >> 6, zb, bar);
+          } else if (p.b_mn) {
+            for (int j = 0; j * 8192 < p.b_bytes; ++j) tma_load<CG>(b + j * 8192, &map_b, n0 + 64 * j, k0, zb, bar);
           } else {
-            tma_load(b, &map_b, k0, n0, zb, bar);
-          }
-          ++count;
-          if (++kk == p.kblocks) {
-            kk = 0;
-            ++part;
-          }
-          if (++st == p.stages) {
-            st = 0;
-            phase ^= 1;
+            tma_load<CG>(b, &map_b, k0, n0, zb, bar);
           }
         }
+        ++count;
+        if (++kk == p.kblocks) {
+          kk = 0;
+          ++part;
+        }
+        if (++st == p.stages) {
+          st = 0;
+          phase ^= 1;
+        }
       }
-      if (!ok)  // loads still in flight must land before the block's memory is given back
+    }
+    if (!ok) {  // loads still in flight must land before the block's memory is given back
+      if (CG == 2) settle();
+      else
         for (int i = count > p.stages ? count - p.stages : 0; i < count; ++i)
           bar_drain(full + 8 * (i % p.stages), (i / p.stages) & 1);
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (rank == 0) {
+      const bool leads = elect_one();
       int st = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 1;
       bool ok = true;
@@ -230,47 +260,52 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
       const uint32_t base = smem_addr(smem);
       const uint64_t da0 = smem_desc(base, p.a_mn ? 8192 : 0, 1024);
       const uint64_t db0 = smem_desc(base + A_BYTES, p.b_mn ? 8192 : 0, 1024);
-      for (Units u(p); u.more(p) && ok; u.next(p)) {
+      for (Units u(p, first, step); u.more(p) && ok; u.next(p)) {
         const int n_k = u.last_k(total_k, p) - u.first_k(total_k, p);
-        if (!(ok = bar_wait(acc_empty + 8 * acc, acc_phase, failed))) break;
+        if (!(ok = warp_wait(acc_empty + 8 * acc, acc_phase, failed))) break;
         fence_after();
         const uint32_t d = tmem + acc * 256;
         for (int kb = 0; kb < n_k; ++kb) {
-          if (!(ok = bar_wait(full + 8 * st, phase, failed))) break;
+          if (!(ok = warp_wait(full + 8 * st, phase, failed))) break;
           fence_after();
           const uint64_t off = (uint64_t)((uint32_t)(st * stage_bytes) >> 4);
-          const uint64_t da = da0 + off, db = db0 + off;
-          if (p.f8) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma_f8(d, da + k * sa, db + k * sb, p.idesc, kb > 0 || k > 0);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma_f16(d, da + k * sa, db + k * sb, p.idesc, kb > 0 || k > 0);
+          if (leads) {
+            if (p.f8) mma_block<CG, true>(d, da0 + off, db0 + off, sa, sb, p.idesc, kb > 0);
+            else mma_block<CG, false>(d, da0 + off, db0 + off, sa, sb, p.idesc, kb > 0);
+            mma_commit<CG>(empty + 8 * st);
           }
-          mma_commit(empty + 8 * st);
           if (++st == p.stages) {
             st = 0;
             phase ^= 1;
           }
         }
-        if (ok) mma_commit(acc_full + 8 * acc);
+        if (ok && leads) mma_commit<CG>(acc_full + 8 * acc);
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
       if (!ok) {
-        mma_commit(drain);
+        if (leads) mma_commit<CG>(drain);
         bar_drain(drain, 0);
       }
     }
     __syncwarp();
   } else {
-    const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+    const int ew = warp - 2, quad = warp & 3, group = ew >> 2;
+    const uint32_t done_at = CG == 2 ? peer_addr(acc_empty, 0) : acc_empty;  // where the products wait
+    const auto read_all = [&](int acc) {  // this warp has read its part of the accumulator
+      fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 2) bar_arrive_cluster(done_at + 8 * acc);
+        else bar_arrive(done_at + 8 * acc);
+      }
+    };
     unsigned char* my = staging + ew * p.bufs * p.buf_bytes;
     float* bias = cols + ew * 2 * CHUNK;
     int acc = 0, buf = 0;
     uint32_t acc_phase = 0;
-    for (Units u(p); u.more(p); u.next(p)) {
-      const int s = u.s, m0 = u.mi * TILE_M, n0 = u.ni * p.bn;
+    for (Units u(p, first, step); u.more(p); u.next(p)) {
+      const int s = u.s, m0 = (u.mi * CG + (int)rank) * TILE_M, n0 = u.ni * p.bn;
       const int ncols = min(p.bn, p.N - n0);
       const int m = m0 + quad * 32 + lane;
       // the next chunk's bias and column scale of this lane's column
@@ -286,7 +321,7 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
         if (p.e.col_scale) ns = p.e.col_scale[n];
       };
       const bool per_col = p.e.bias || p.e.col_scale;
-      if (per_col) fetch(half * CHUNK);
+      if (per_col) fetch(group * CHUNK);
       const float rs = (p.e.row_scale && m < p.M) ? p.e.row_scale[m] : 1.f;
       // all lanes of the warp leave together
       if (__any_sync(0xffffffffu, !bar_wait(acc_full + 8 * acc, acc_phase, failed))) break;
@@ -294,25 +329,22 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
       // the accumulator's next chunk is on its way while one is worked on
       uint32_t r[32];
       const uint32_t lanes = tmem + acc * 256 + ((uint32_t)(quad * 32) << 16);
-      if (half * CHUNK < ncols) tmem_load32(lanes + half * CHUNK, r);
-      for (int c = half * CHUNK; c < ncols; c += 2 * CHUNK) {
+      constexpr int NEXT = EPI_GROUPS * CHUNK;
+      if (group * CHUNK < ncols) tmem_load32(lanes + group * CHUNK, r);
+      else read_all(acc);  // no chunk for this warp in a narrow tile
+      for (int c = group * CHUNK; c < ncols; c += NEXT) {
         tmem_wait_load();
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        if (c + 2 * CHUNK < ncols) {
-          tmem_load32(lanes + c + 2 * CHUNK, r);
-        } else {  // all of it has been read
-          fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(acc_empty + 8 * acc);
-        }
+        if (c + NEXT < ncols) tmem_load32(lanes + c + NEXT, r);
+        else read_all(acc);
         if (per_col) {
           __syncwarp();  // the chunk before has been read
           bias[lane] = nb;
           bias[CHUNK + lane] = ns;
           __syncwarp();
-          fetch(c + 2 * CHUNK);
+          fetch(c + NEXT);
           if (p.e.col_scale) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] *= rs * bias[CHUNK + i];
@@ -364,11 +396,6 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
           if (p.bufs == 2) buf ^= 1;
         }
       }
-      if (half * CHUNK >= ncols) {  // a warp without a chunk in a narrow tile
-        fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(acc_empty + 8 * acc);
-      }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
@@ -377,9 +404,10 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
   }
   fence_before();
   __syncthreads();
+  if (CG == 2) cluster_sync();  // nothing of the other block's is on its way here any more
   if (warp == 1) {
     fence_after();
-    tmem_free<512>(tmem);
+    tmem_free<CG>(tmem);
   }
   if (threadIdx.x == 0 && *failed) atomicExch(&g_linear_failed, 1);
 }
@@ -401,20 +429,31 @@ static EncodeFn encode_fn() {
   return fn;
 }
 
-// A [planes][rows][cols] array with row pitch `ld` (elements).
+// A [planes][rows][cols] array with row pitch `ld` (elements); `blocks`: seen
+// as [planes][cols / 64][rows][64], boxes of that many blocks of 64 columns.
 static int make_map(CUtensorMap* map, int dtype, const void* base, int64_t cols, int64_t rows, int64_t planes,
-                    int64_t ld, int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
+                    int64_t ld, int box_cols, int box_rows, CUtensorMapSwizzle swizzle, int blocks = 0) {
   const CUtensorMapDataType t = dtype == AFFB_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                 : dtype == AFFB_F16  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                 : dtype == AFFB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                      : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
-  const cuuint64_t strides[2] = {(cuuint64_t)(ld * dtype_size(dtype)), (cuuint64_t)(rows * ld * dtype_size(dtype))};
-  const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, es[3] = {1, 1, 1};
+  const int64_t es = dtype_size(dtype);
+  cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes, 1};
+  cuuint64_t strides[3] = {(cuuint64_t)(ld * es), (cuuint64_t)(rows * ld * es), 0};
+  cuuint32_t box[4] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  if (blocks) {
+    dims[0] = 64;
+    dims[2] = (cuuint64_t)(cols / 64);
+    dims[3] = (cuuint64_t)planes;
+    strides[1] = (cuuint64_t)(64 * es);
+    strides[2] = (cuuint64_t)(rows * ld * es);
+    box[2] = (cuuint32_t)blocks;
+  }
   EncodeFn fn = encode_fn();
   AFFB_REQUIRE(fn, "linear: the driver has no tensor-map encoder");
-  const CUresult rc = fn(map, t, 3, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult rc = fn(map, t, blocks ? 4 : 3, const_cast<void*>(base), dims, strides, box, step,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   AFFB_REQUIRE(rc == CUDA_SUCCESS, "linear: tensor map refused (code %d)", (int)rc);
   return AFFB_OK;
 }
@@ -428,24 +467,32 @@ struct Operand {
 };
 
 struct Shape {
-  int bn, nt, mt, splits;
+  int cg, bn, nt, mt, splits;
 };
 
-// Tile width and split of the contraction.  Few, wide tiles feed the tensor
-// cores best; with fewer tiles than SMs narrower tiles (down to 64 columns)
-// and then a split contraction (at least 4 k blocks a part) fill the GPU.
+// Tile and split of the contraction.
+// Pairs of blocks (256-row tiles up to 256 columns wide) where there are
+// enough tiles, or enough k blocks to split, for all of them; else single
+// blocks, whose tiles are narrowed (down to 64 columns) and whose contraction
+// is split (at least 4 k blocks a part) until they fill the GPU.
 static Shape choose_shape(int64_t M, int64_t N, int64_t total_k) {
   const int64_t sms = sm_count();
   Shape s;
-  s.mt = (int)((M + TILE_M - 1) / TILE_M);
-  s.nt = (int)((N + 255) / 256);
-  while ((int64_t)s.mt * s.nt * 2 <= sms && (N + s.nt * 2 - 1) / (s.nt * 2) >= 64) s.nt *= 2;
+  const int64_t wide = (N + 255) / 256;
+  const int64_t pair_tiles = (M + 255) / 256 * wide;
+  const int64_t most_splits = total_k >= 8 ? total_k / 4 : 1;
+  s.cg = M > TILE_M && pair_tiles * most_splits >= sms / 2 ? 2 : 1;
+  const int64_t teams = sms / s.cg;
+  s.mt = (int)((M + TILE_M * s.cg - 1) / (TILE_M * s.cg));
+  s.nt = (int)wide;
+  if (s.cg == 1)
+    while ((int64_t)s.mt * s.nt * 2 <= sms && (N + s.nt * 2 - 1) / (s.nt * 2) >= 64) s.nt *= 2;
   const int64_t per = (N + s.nt - 1) / s.nt;
-  s.bn = (int)(s.nt == 1 ? round_up(per, 16) : round_up(per, 32));
+  s.bn = (int)round_up(per, s.nt == 1 && s.cg == 1 ? 16 : 32);
   s.nt = (int)((N + s.bn - 1) / s.bn);
   const int64_t tiles = (int64_t)s.mt * s.nt;
-  int64_t sp = sms / tiles;
-  if (sp > total_k / 4) sp = total_k / 4;
+  int64_t sp = teams / tiles;
+  if (sp > most_splits) sp = most_splits;
   s.splits = (int)(sp < 2 ? 1 : sp);
   return s;
 }
@@ -461,20 +508,26 @@ static int64_t k_blocks(int dtype, int64_t K) {
   return (K + ke - 1) / ke * (dtype == AFFB_F32 ? 6 : 1);
 }
 
-template <typename TO>
+template <typename TO, int CG>
 static const void* kernel_of(int act) {
   switch (act) {
-    case AFFB_ACT_RELU: return (const void*)gemm_kernel<TO, AFFB_ACT_RELU>;
-    case AFFB_ACT_GELU: return (const void*)gemm_kernel<TO, AFFB_ACT_GELU>;
-    case AFFB_ACT_SILU: return (const void*)gemm_kernel<TO, AFFB_ACT_SILU>;
-    default: return (const void*)gemm_kernel<TO, AFFB_ACT_NONE>;
+    case AFFB_ACT_RELU: return (const void*)gemm_kernel<TO, AFFB_ACT_RELU, CG>;
+    case AFFB_ACT_GELU: return (const void*)gemm_kernel<TO, AFFB_ACT_GELU, CG>;
+    case AFFB_ACT_SILU: return (const void*)gemm_kernel<TO, AFFB_ACT_SILU, CG>;
+    default: return (const void*)gemm_kernel<TO, AFFB_ACT_NONE, CG>;
   }
+}
+template <int CG>
+static const void* kernel_of(int out_dtype, int act) {
+  return out_dtype == AFFB_F32    ? kernel_of<float, CG>(act)
+         : out_dtype == AFFB_BF16 ? kernel_of<__nv_bfloat16, CG>(act)
+                                  : kernel_of<__half, CG>(act);
 }
 
 // The kernel's shared-memory limit, raised once per device (idempotent, so a
 // race between threads is harmless).
 static cudaError_t allow_smem(const void* k, int slot) {
-  static bool done[64][12];
+  static bool done[64][24];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
@@ -503,8 +556,12 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
   p.parts = dtype == AFFB_F32 ? 6 : 1;
   p.kblocks = (int)(total_k / p.parts);
   p.a_mn = a.mn; p.b_mn = b.mn; p.f8 = dtype == AFFB_E4M3;
-  p.b_bytes = b.mn ? (int)round_up(s.bn, 64) * 128 : s.bn * 128;
-  p.idesc = instr_desc(et == AFFB_BF16 ? 1 : 0, a.mn, b.mn, (uint32_t)s.bn);
+  const int half_n = s.bn / s.cg;  // a block's columns of B
+  p.b_bytes = b.mn ? (int)round_up(half_n, 64) * 128 : half_n * 128;
+  // blocks of 64 columns in one load where no block runs past its row, and the tiles begin at a block
+  p.a_blocks = a.mn && a.cols % 64 == 0 ? TILE_M / 64 : 0;
+  p.b_blocks = b.mn && b.cols % 64 == 0 && half_n % 64 == 0 ? half_n / 64 : 0;
+  p.idesc = instr_desc(et == AFFB_BF16 ? 1 : 0, a.mn, b.mn, (uint32_t)(TILE_M * s.cg), (uint32_t)s.bn);
   LinearEpilogue full = e;
   if (s.splits > 1) {
     e = LinearEpilogue{};
@@ -518,7 +575,7 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
   p.z_off = (int)dtype_size(e.out_dtype) * STAGE_ROWS * CHUNK;
   p.buf_bytes = p.z_off + (e.z ? (int)dtype_size(e.z_dtype) * STAGE_ROWS * CHUNK : 0);
   const int stage = A_BYTES + p.b_bytes;
-  p.bufs = p.buf_bytes > 4096 ? 1 : 2;
+  p.bufs = p.buf_bytes > 2048 ? 1 : 2;
   const int fixed = 1024 + EPI_WARPS * p.bufs * p.buf_bytes + COLS_BYTES + BAR_BYTES;
   p.stages = (SMEM_MAX - fixed) / stage;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
@@ -529,24 +586,34 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
   const int ke = p.f8 ? 128 : 64;
   int rc;
   if ((rc = make_map(&ma, et, a.p, a.cols, a.rows, planes, a.ld, a.mn ? 64 : ke, a.mn ? 64 : TILE_M,
-                     CU_TENSOR_MAP_SWIZZLE_128B)))
+                     CU_TENSOR_MAP_SWIZZLE_128B, p.a_blocks)))
     return rc;
-  if ((rc = make_map(&mb, et, b.p, b.cols, b.rows, planes, b.ld, b.mn ? 64 : ke, b.mn ? 64 : s.bn,
-                     CU_TENSOR_MAP_SWIZZLE_128B)))
+  if ((rc = make_map(&mb, et, b.p, b.cols, b.rows, planes, b.ld, b.mn ? 64 : ke, b.mn ? 64 : half_n,
+                     CU_TENSOR_MAP_SWIZZLE_128B, p.b_blocks)))
     return rc;
   if (!p.direct) {
     const auto sw = [](int t) { return t == AFFB_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B; };
     if ((rc = make_map(&mo, e.out_dtype, e.out, p.N, M, s.splits, p.N, CHUNK, STAGE_ROWS, sw(e.out_dtype)))) return rc;
     if (e.z && (rc = make_map(&mz, e.z_dtype, e.z, p.N, M, 1, p.N, CHUNK, STAGE_ROWS, sw(e.z_dtype)))) return rc;
   }
-  const void* k = e.out_dtype == AFFB_F32    ? kernel_of<float>(e.act)
-                  : e.out_dtype == AFFB_BF16 ? kernel_of<__nv_bfloat16>(e.act)
-                                             : kernel_of<__half>(e.act);
-  cudaError_t err = allow_smem(k, (e.out_dtype == AFFB_F32 ? 0 : e.out_dtype == AFFB_BF16 ? 4 : 8) + e.act);
+  const void* k = s.cg == 2 ? kernel_of<2>(e.out_dtype, e.act) : kernel_of<1>(e.out_dtype, e.act);
+  const int slot = (s.cg - 1) * 12 + (e.out_dtype == AFFB_F32 ? 0 : e.out_dtype == AFFB_BF16 ? 4 : 8) + e.act;
+  cudaError_t err = allow_smem(k, slot);
   if (err == cudaSuccess) {
     const int64_t units = (int64_t)s.mt * s.nt * s.splits;
     void* args[] = {&ma, &mb, &mo, &mz, &p};
-    err = cudaLaunchKernel(k, dim3((unsigned)imin64(units, sm_count())), dim3(LIN_THREADS), args, (size_t)smem, st);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(imin64(units, sm_count() / s.cg) * s.cg));
+    cfg.blockDim = dim3(LIN_THREADS);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)s.cg;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = s.cg == 2 ? 1 : 0;
+    err = cudaLaunchKernelExC(&cfg, k, args);
   }
   if (err != cudaSuccess) {
     cudaGetLastError();
