@@ -42,6 +42,34 @@ __device__ __forceinline__ float normal_tail(float a) {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// Two fp32 values in one register pair: the additions, products and FMAs of
+// sm_100 on pairs issue once for both.
+using pair_t = unsigned long long;
+__device__ __forceinline__ pair_t pack2(float a, float b) {
+  pair_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(pair_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
+  pair_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+  pair_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) {
+  pair_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ pair_t both(float v) { return pack2(v, v); }
+
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == AFFB_ACT_RELU) {
@@ -54,6 +82,30 @@ __device__ __forceinline__ float activate(float z) {
     return __fdividef(z, 1.f + exp2_approx(-LOG2E * z));
   } else {
     return z;
+  }
+}
+
+// activate() of two values, the polynomial of GELU on pairs.
+template <int ACT>
+__device__ __forceinline__ void activate_pair(float& x, float& y) {
+  if constexpr (ACT == AFFB_ACT_GELU) {
+    const float ax = min_nan(fabsf(x), 64.f), ay = min_nan(fabsf(y), 64.f);
+    const pair_t a = pack2(ax, ay);
+    pair_t p = both(-1.41679106e-06f);
+    p = fma2(p, a, both(5.36095686e-05f));
+    p = fma2(p, a, both(-0.000875660044f));
+    p = fma2(p, a, both(0.00834226329f));
+    p = fma2(p, a, both(-0.0537395962f));
+    p = fma2(p, a, both(-0.458566278f));
+    p = fma2(p, a, both(-1.15125847f));
+    p = fma2(p, a, both(-0.999988079f));
+    float px, py;
+    unpack2(p, px, py);
+    x = fmaf(-ax, exp2_approx(px), fmaxf(x, 0.f));
+    y = fmaf(-ay, exp2_approx(py), fmaxf(y, 0.f));
+  } else {
+    x = activate<ACT>(x);
+    y = activate<ACT>(y);
   }
 }
 

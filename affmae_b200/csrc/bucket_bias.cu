@@ -24,6 +24,8 @@
 // the tile's sums to fp32 bins.  The blocks' bins are summed in block order.
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace affb {
 
 constexpr int BB_THREADS = 256;
@@ -48,22 +50,21 @@ struct BucketArgs {
   const void* k_pos;    // [B,Nk,axes]
   const int* member;    // [B,Nq,M] or null (M = Nk)
   int B, H;
-  int64_t Nq, Nk, M, NM;
-  uint32_t div_mul, div_shift;  // n / M for n < 2^31 (div_shift 32: not usable)
+  int Nk, M;
+  int NM;               // pairs of one batch element in this launch (a multiple of M, below 2^31)
+  int64_t batch_pairs;  // pairs of a whole batch element: stride of lists, biases and gradients
+  int64_t q_batch;      // queries of a whole batch element
+  uint32_t div_mul, div_shift;  // n / M for n < 2^31
 };
 
-// n / M by a multiplication (n < 2^31) where M allows it.
-__device__ __forceinline__ int64_t query_of(const BucketArgs& a, int64_t nm) {
-  if (a.div_shift < 32) {
-    const uint32_t n = (uint32_t)nm;
-    return (__umulhi(a.div_mul, n) + n) >> a.div_shift;
-  }
-  return nm / a.M;
+// n / M by a multiplication.
+__device__ __forceinline__ int query_of(const BucketArgs& a, int nm) {
+  return (int)((__umulhi(a.div_mul, (uint32_t)nm) + (uint32_t)nm) >> a.div_shift);
 }
 
+// A NaN counts as the farthest key before the query.
 __device__ __forceinline__ int offset_of(float k, float q) {
-  const int d = __float2int_rn(k - q);  // saturates; NaN counts as 0
-  return max(-(1 << 30), min(1 << 30, d));
+  return __float2int_rn(fminf(fmaxf(k - q, -1073741824.f), 1073741824.f));
 }
 __device__ __forceinline__ int offset_of(int k, int q) {
   const int64_t d = (int64_t)k - q;
@@ -97,68 +98,108 @@ __device__ __forceinline__ int axis_index(const BucketArgs& a, const uint8_t* lu
   const int c = a.lut ? lut[min(n, a.lut - 1)] : search_edges(a, n);
   return a.one_sided ? c : d < 0 ? a.k - c : a.k + c;
 }
-// Index of an offset cut off at the last edge: [0, span).
-__device__ __forceinline__ int clipped(const BucketArgs& a, int d) {
-  const int last = a.lut - 1;
-  return a.one_sided ? min(max(-d, 0), last) : max(-last, min(last, d)) + last;
-}
-// The offset that `clipped` index i stands for.
+// The offset that index i of [0, span) stands for where offsets are cut off at
+// the last edge.
 __device__ __forceinline__ int unclipped(const BucketArgs& a, int i) { return a.one_sided ? -i : i - (a.lut - 1); }
 
-// Entry of a pair in the table in shared memory: its row, or (BY_OFFSET) the
-// combined clipped offset.
-template <typename P, bool BY_OFFSET>
-__device__ __forceinline__ int entry1(const BucketArgs& a, const uint8_t* lut, P q, P k) {
-  const int d = offset_of(k, q);
-  return BY_OFFSET ? clipped(a, d) : axis_index(a, lut, d);
-}
-template <typename P, bool BY_OFFSET>
-__device__ __forceinline__ int entry2(const BucketArgs& a, const uint8_t* lut, P qx, P qy, P kx, P ky) {
-  const int dx = offset_of(kx, qx), dy = offset_of(ky, qy);
-  return BY_OFFSET ? clipped(a, dy) * a.span + clipped(a, dx)
-                   : axis_index(a, lut, dy) * a.per_axis + axis_index(a, lut, dx);
-}
+// Index of a pair's offset along each axis, combined.  BY_OFFSET: of the
+// offset cut off at the last edge, else of its bucket.
+template <typename P, int AXES, bool BY_OFFSET>
+struct EntryOf {
+  const BucketArgs& a;
+  const uint8_t* lut;
+  int last, high, my, add;
+
+  __device__ __forceinline__ EntryOf(const BucketArgs& args, const uint8_t* l) : a(args), lut(l) {
+    last = a.lut - 1;
+    high = a.one_sided ? 0 : last;
+    my = a.one_sided ? -a.span : a.span;
+    add = a.one_sided ? 0 : last * (AXES == 2 ? a.span + 1 : 1);
+  }
+  // the cut-off offset
+  __device__ __forceinline__ int cut(P k, P q) const {
+    if constexpr (std::is_same<P, float>::value) {
+      // adding 1.5 * 2^23 rounds to an integer (ties to even) in the low mantissa bits
+      const float t = fminf(fmaxf(k - q, (float)-last), (float)high) + 12582912.f;
+      return __float_as_int(t) - 0x4B400000;
+    } else {
+      return max(-last, min(high, offset_of(k, q)));
+    }
+  }
+  __device__ __forceinline__ int one(P k, P q) const {
+    if constexpr (BY_OFFSET) return (a.one_sided ? -cut(k, q) : cut(k, q)) + add;
+    return axis_index(a, lut, offset_of(k, q));
+  }
+  __device__ __forceinline__ int two(P kx, P ky, P qx, P qy) const {
+    if constexpr (BY_OFFSET) {
+      const int x = cut(kx, qx), y = cut(ky, qy);
+      return my * y + (a.one_sided ? -x : x) + add;
+    }
+    return axis_index(a, lut, offset_of(ky, qy)) * a.per_axis + axis_index(a, lut, offset_of(kx, qx));
+  }
+};
 
 template <typename P> struct alignas(2 * sizeof(P)) Pos2 { P x, y; };
 
-// Entries of the pairs nm .. nm + PAIRS - 1 of batch element b (`none` where
-// there is no such pair or the list names no key).  PAIRS == 2: nm and M even.
+// Entries of the pairs nm + u * STEP + j of batch element b (`none` where there
+// is no such pair or the list names no key).  PAIRS == 2: nm and M even.
+// Free of branches, so that the loads of all steps are in flight together.
 template <typename P, int AXES, int PAIRS, bool BY_OFFSET>
-__device__ __forceinline__ void pair_entries(const BucketArgs& a, const uint8_t* lut, int b, int64_t nm, int none,
-                                             int* e) {
-#pragma unroll
-  for (int j = 0; j < PAIRS; ++j) e[j] = none;
-  if (nm >= a.NM) return;
-  const int64_t i = query_of(a, nm), m = nm - i * a.M;
-  int64_t id[PAIRS];
-  if (a.member) {
-    const int* mp = a.member + (int64_t)b * a.NM + nm;
-    if constexpr (PAIRS == 2) {
-      const int2 u = __ldg(reinterpret_cast<const int2*>(mp));
-      id[0] = u.x;
-      id[1] = u.y;
-    } else {
-      id[0] = __ldg(mp);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < PAIRS; ++j) id[j] = m + j;
-  }
-  const P* qb = (const P*)a.q_pos + ((int64_t)b * a.Nq + i) * AXES;
+__device__ __forceinline__ void tile_entries(const BucketArgs& a, const EntryOf<P, AXES, BY_OFFSET>& entry, int b, int nm,
+                                             int none, int (*e)[PAIRS]) {
+  constexpr int STEP = BB_THREADS * PAIRS;
+  const P* qb = (const P*)a.q_pos + (int64_t)b * a.q_batch * AXES;
   const P* kb = (const P*)a.k_pos + (int64_t)b * a.Nk * AXES;
-  if constexpr (AXES == 1) {
-    const P q = __ldg(qb);
+  int id[BB_STEPS][PAIRS], query[BB_STEPS];
 #pragma unroll
-    for (int j = 0; j < PAIRS; ++j)
-      if (id[j] >= 0 && id[j] < a.Nk) e[j] = entry1<P, BY_OFFSET>(a, lut, q, __ldg(kb + id[j]));
-  } else {
-    const Pos2<P> q = *reinterpret_cast<const Pos2<P>*>(qb);
-#pragma unroll
-    for (int j = 0; j < PAIRS; ++j)
-      if (id[j] >= 0 && id[j] < a.Nk) {
-        const Pos2<P> k = *reinterpret_cast<const Pos2<P>*>(kb + 2 * id[j]);
-        e[j] = entry2<P, BY_OFFSET>(a, lut, q.x, q.y, k.x, k.y);
+  for (int u = 0; u < BB_STEPS; ++u) {
+    const int n = nm + u * STEP < a.NM ? nm + u * STEP : 0;
+    query[u] = query_of(a, n);
+    if (a.member) {
+      const int* mp = a.member + (int64_t)b * a.batch_pairs + n;
+      if constexpr (PAIRS == 2) {
+        const int2 w = __ldg(reinterpret_cast<const int2*>(mp));
+        id[u][0] = w.x;
+        id[u][1] = w.y;
+      } else {
+        id[u][0] = __ldg(mp);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j) id[u][j] = n - query[u] * a.M + j;
+    }
+  }
+  if constexpr (AXES == 1) {
+    P q[BB_STEPS], k[BB_STEPS][PAIRS];
+#pragma unroll
+    for (int u = 0; u < BB_STEPS; ++u) {
+      const P* qp = qb + query[u];
+      q[u] = __ldg(qp);
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j) k[u][j] = __ldg((unsigned)id[u][j] < (unsigned)a.Nk ? kb + id[u][j] : qp);
+    }
+#pragma unroll
+    for (int u = 0; u < BB_STEPS; ++u)
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j)
+        e[u][j] = (unsigned)id[u][j] < (unsigned)a.Nk && nm + u * STEP < a.NM ? entry.one(k[u][j], q[u]) : none;
+  } else {
+    Pos2<P> q[BB_STEPS], k[BB_STEPS][PAIRS];
+#pragma unroll
+    for (int u = 0; u < BB_STEPS; ++u) {
+      const Pos2<P>* qp = reinterpret_cast<const Pos2<P>*>(qb) + query[u];
+      q[u] = *qp;
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j)
+        k[u][j] = *((unsigned)id[u][j] < (unsigned)a.Nk ? reinterpret_cast<const Pos2<P>*>(kb) + id[u][j] : qp);
+    }
+#pragma unroll
+    for (int u = 0; u < BB_STEPS; ++u)
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j)
+        e[u][j] = (unsigned)id[u][j] < (unsigned)a.Nk && nm + u * STEP < a.NM
+                      ? entry.two(k[u][j].x, k[u][j].y, q[u].x, q[u].y)
+                      : none;
   }
 }
 
@@ -199,17 +240,17 @@ __global__ void __launch_bounds__(BB_THREADS, 4)
   }
   __syncthreads();
   constexpr int STEP = BB_THREADS * PAIRS, TILE = STEP * BB_STEPS;
-  const int64_t per = (a.NM + TILE - 1) / TILE, total = per * a.B;
+  const EntryOf<P, AXES, BY_OFFSET> entry(a, lut);
+  const uint32_t per = ((uint32_t)a.NM + TILE - 1) / TILE;
+  const int64_t total = (int64_t)per * a.B;
   for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-    const int b = total < (1ll << 31) ? (int)((uint32_t)t / (uint32_t)per) : (int)(t / per);
-    const int64_t nm = (t - b * per) * TILE + threadIdx.x * PAIRS;
+    const int b = total < (1ll << 31) ? (int)((uint32_t)t / per) : (int)(t / per);
+    const int nm = (int)(t - (int64_t)b * per) * TILE + threadIdx.x * PAIRS;
     int e[BB_STEPS][PAIRS];
-#pragma unroll
-    for (int u = 0; u < BB_STEPS; ++u)
-      pair_entries<P, AXES, PAIRS, BY_OFFSET>(a, lut, b, nm + u * STEP, entries, e[u]);
+    tile_entries<P, AXES, PAIRS, BY_OFFSET>(a, entry, b, nm, entries, e);
     for (int g = 0; g < groups; ++g) {
       const V* tg = tab + g * (entries + 1);
-      T* o = out + ((int64_t)b * a.H + h0 + g * BB_HEADS) * a.NM + nm;
+      T* o = out + ((int64_t)b * a.H + h0 + g * BB_HEADS) * a.batch_pairs + nm;
       V v[BB_STEPS][PAIRS];
 #pragma unroll
       for (int u = 0; u < BB_STEPS; ++u)
@@ -221,7 +262,7 @@ __global__ void __launch_bounds__(BB_THREADS, 4)
 #pragma unroll
         for (int u = 0; u < BB_STEPS; ++u) {
           if (nm + u * STEP >= a.NM) break;
-          T* p = o + h * a.NM + u * STEP;
+          T* p = o + h * a.batch_pairs + u * STEP;
           if constexpr (sizeof(T) == 2) {
             if constexpr (PAIRS == 2)
               *reinterpret_cast<uint32_t*>(p) = head_bits(v[u][0], h) | (head_bits(v[u][1], h) << 16);
@@ -248,7 +289,8 @@ __device__ __forceinline__ float bb_max_nan(float a, float b) {
 // Block (x: tiles taken in turn, y: group of BB_HEADS heads).
 template <typename T, typename P, int AXES, int PAIRS, bool BY_OFFSET>
 __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
-    bucket_bwd_kernel(const __grid_constant__ BucketArgs a, const T* __restrict__ dout, float* __restrict__ part) {
+    bucket_bwd_kernel(const __grid_constant__ BucketArgs a, const T* __restrict__ dout, float* __restrict__ part,
+                      int resume) {
   constexpr int STEP = BB_THREADS * PAIRS, TILE = STEP * BB_STEPS, PER = BB_STEPS * PAIRS;
   extern __shared__ unsigned char sm[];
   __shared__ float wmax[BB_HEADS][BB_THREADS / 32];
@@ -275,19 +317,22 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
       rows[i] = (uint16_t)row;
     }
   }
+  float* mine = part + ((int64_t)blockIdx.x * a.H + h0) * a.rows;
   for (int i = threadIdx.x; i < BB_HEADS * a.rows; i += BB_THREADS) {
-    acc[i] = 0.f;
+    acc[i] = resume && i < nh * a.rows ? mine[i] : 0.f;  // of the launch before (more than 2^31 pairs)
     bins[i] = 0;
   }
   __syncthreads();
-  const int64_t per = (a.NM + TILE - 1) / TILE, total = per * a.B;
+  const EntryOf<P, AXES, BY_OFFSET> entry(a, lut);
+  const uint32_t per = ((uint32_t)a.NM + TILE - 1) / TILE;
+  const int64_t total = (int64_t)per * a.B;
   for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-    const int b = total < (1ll << 31) ? (int)((uint32_t)t / (uint32_t)per) : (int)(t / per);
-    const int64_t nm = (t - b * per) * TILE + threadIdx.x * PAIRS;
+    const int b = total < (1ll << 31) ? (int)((uint32_t)t / per) : (int)(t / per);
+    const int nm = (int)(t - (int64_t)b * per) * TILE + threadIdx.x * PAIRS;
     float g[BB_HEADS][PER];
 #pragma unroll
     for (int h = 0; h < BB_HEADS; ++h) {
-      const T* p = dout + ((int64_t)b * a.H + h0 + h) * a.NM + nm;
+      const T* p = dout + ((int64_t)b * a.H + h0 + h) * a.batch_pairs + nm;
 #pragma unroll
       for (int u = 0; u < BB_STEPS; ++u) {
         const bool in = h < nh && nm + u * STEP < a.NM;
@@ -305,18 +350,18 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
       }
     }
     int row[PER];
+    tile_entries<P, AXES, PAIRS, BY_OFFSET>(a, entry, b, nm, BY_OFFSET ? offsets : none,
+                                            reinterpret_cast<int(*)[PAIRS]>(row));
+    if (BY_OFFSET) {
 #pragma unroll
-    for (int u = 0; u < BB_STEPS; ++u)
-      pair_entries<P, AXES, PAIRS, BY_OFFSET>(a, lut, b, nm + u * STEP, BY_OFFSET ? offsets : none, row + u * PAIRS);
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (BY_OFFSET) row[j] = rows[row[j]];
+      for (int j = 0; j < PER; ++j) row[j] = rows[row[j]];
+    }
 #pragma unroll
     for (int h = 0; h < BB_HEADS; ++h) {
+      if (h >= nh) break;
       float top = 0.f;
 #pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (row[j] != none) top = bb_max_nan(top, fabsf(g[h][j]));
+      for (int j = 0; j < PER; ++j) top = bb_max_nan(top, row[j] != none ? fabsf(g[h][j]) : 0.f);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = bb_max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
       if (lane == 0) wmax[h][warp] = top;
@@ -327,10 +372,11 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
     bool odd = false;      // an infinity or NaN among the tile's gradients
 #pragma unroll
     for (int h = 0; h < BB_HEADS; ++h) {
+      down[h] = 0.f;
+      if (h >= nh) continue;
       float top = 0.f;
 #pragma unroll
       for (int w = 0; w < BB_THREADS / 32; ++w) top = bb_max_nan(top, wmax[h][w]);
-      down[h] = 0.f;
       if (!isfinite(top)) {
         odd = true;
       } else if (top > 0.f) {
@@ -341,8 +387,11 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
         down[h] = __int_as_float((127 - t1) << 23);
         rest[h] = __int_as_float((127 - t + t1) << 23);
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-          if (row[j] != none) atomicAdd(bins + h * a.rows + row[j], __float2int_rn(g[h][j] * up * up2));
+        for (int j = 0; j < PER; ++j) {
+          // rounded to an integer by adding 1.5 * 2^23
+          const int q = __float_as_int(fmaf(g[h][j] * up, up2, 12582912.f)) - 0x4B400000;
+          if (row[j] != none) atomicAdd(bins + h * a.rows + row[j], q);
+        }
       }
     }
     __syncthreads();
@@ -362,7 +411,7 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
 #pragma unroll
       for (int h = 0; h < BB_HEADS; ++h) {
         float top = 0.f;
-        for (int w = 0; w < BB_THREADS / 32; ++w) top = bb_max_nan(top, wmax[h][w]);
+        for (int w = 0; w < BB_THREADS / 32 && h < nh; ++w) top = bb_max_nan(top, wmax[h][w]);
         if (!isfinite(top)) {
           __syncthreads();
 #pragma unroll
@@ -379,8 +428,7 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
     }
     __syncthreads();
   }
-  float* o = part + ((int64_t)blockIdx.x * a.H + h0) * a.rows;
-  for (int i = threadIdx.x; i < nh * a.rows; i += BB_THREADS) o[i] = acc[i];
+  for (int i = threadIdx.x; i < nh * a.rows; i += BB_THREADS) mine[i] = acc[i];
 }
 
 // dtable[row, h] = sum over blocks of part[block][h][row], in a fixed order:
@@ -429,7 +477,8 @@ static int bucket_args(const int32_t* edges, int n_edges, int one_sided, const v
   AFFB_REQUIRE(pos_type >= AFFB_POS_F32 && pos_type <= AFFB_POS_I64, "bucket_bias: unknown position type");
   AFFB_REQUIRE(B >= 0 && H >= 1 && Nq >= 0 && Nk >= 0 && M >= 0, "bucket_bias: negative size or no head");
   AFFB_REQUIRE(member || M == Nk || B * Nq * M == 0, "bucket_bias: without member_idx every key is taken (M = Nk)");
-  AFFB_REQUIRE(B < (1ll << 31) && H < (1 << 18) && Nq < (1ll << 40) && Nk < (1ll << 40), "bucket_bias: size too large");
+  AFFB_REQUIRE(B < (1ll << 31) && H < (1 << 18) && Nq < (1ll << 40) && Nk < (1ll << 30) && M < (1ll << 30),
+               "bucket_bias: size too large");
   a->k = n_edges;
   a->lut = edges[n_edges - 1] < BB_LUT ? edges[n_edges - 1] + 1 : 0;
   a->one_sided = one_sided != 0;
@@ -441,24 +490,37 @@ static int bucket_args(const int32_t* edges, int n_edges, int one_sided, const v
   a->member = member;
   a->B = (int)B;
   a->H = (int)H;
-  a->Nq = Nq;
-  a->Nk = Nk;
-  a->M = M;
-  a->NM = Nq * M;
+  a->Nk = (int)Nk;
+  a->M = (int)M;
+  a->batch_pairs = Nq * M;
+  a->q_batch = Nq;
   const int64_t last = edges[n_edges - 1];
   a->span = a->lut ? (int)(one_sided ? last + 1 : 2 * last + 1) : 0;
-  a->div_shift = 32;
-  if (M >= 1 && a->NM < (1ll << 31)) {
-    uint32_t l = 0;
-    while ((1ll << l) < M) ++l;
-    a->div_shift = l;
-    a->div_mul = (uint32_t)(((1ull << 32) * ((1ull << l) - (uint64_t)M)) / (uint64_t)M + 1);
-  }
-  if (B * a->NM > 0) AFFB_REQUIRE(q_pos && k_pos, "bucket_bias: null positions");
+  uint32_t l = 0;
+  while ((1ll << l) < M) ++l;
+  a->div_shift = l;
+  if (M >= 1) a->div_mul = (uint32_t)(((1ull << 32) * ((1ull << l) - (uint64_t)M)) / (uint64_t)M + 1);
+  if (B * a->batch_pairs > 0) AFFB_REQUIRE(q_pos && k_pos, "bucket_bias: null positions");
   const uintptr_t pair = pos_type == AFFB_POS_I64 ? 16 : 8;
   AFFB_REQUIRE(axes == 1 || (((uintptr_t)q_pos | (uintptr_t)k_pos) & (pair - 1)) == 0,
                "bucket_bias: positions of two axes must be aligned to a pair of coordinates");
   return AFFB_OK;
+}
+
+// The launches that cover all queries, each with fewer than 2^31 pairs a batch
+// element: f(arguments, first pair).
+template <typename F>
+static cudaError_t bb_chunks(const BucketArgs& all, int64_t pos_size, F f) {
+  const int64_t most = ((1ll << 31) - 65536) / all.M;  // queries of a launch
+  for (int64_t q = 0; q < all.q_batch; q += most) {
+    BucketArgs a = all;
+    a.NM = (int)(imin64(most, all.q_batch - q) * all.M);
+    a.q_pos = (const char*)all.q_pos + q * all.axes * pos_size;
+    if (a.member) a.member += q * all.M;
+    const cudaError_t e = f(a, q * all.M);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 // Two pairs a lane: both of one query, and 4- or 8-byte accesses aligned.
@@ -470,7 +532,7 @@ static bool bb_two(const BucketArgs& a, const void* t, int64_t size) {
 static int64_t bb_offsets(const BucketArgs& a, int64_t entry_bytes, int64_t most_bytes, int64_t blocks) {
   if (!a.span) return 0;
   const int64_t n = a.axes == 2 ? (int64_t)a.span * a.span : a.span;
-  return n * entry_bytes <= most_bytes && n * blocks <= a.NM * a.B ? n : 0;
+  return n * entry_bytes <= most_bytes && n * blocks <= (int64_t)a.NM * a.B ? n : 0;
 }
 
 #define BB_POS(pos_type, P, ...)                                   \
@@ -483,7 +545,7 @@ static int64_t bb_offsets(const BucketArgs& a, int64_t entry_bytes, int64_t most
 template <typename T, typename TB, typename P, int AXES, int PAIRS>
 static cudaError_t bucket_fwd_launch(const BucketArgs& a, const void* table, void* out, cudaStream_t st) {
   const int64_t v = sizeof(typename Heads4<T>::type);
-  const int64_t tiles = (a.NM + BB_THREADS * PAIRS * BB_STEPS - 1) / (BB_THREADS * PAIRS * BB_STEPS) * a.B;
+  const int64_t tiles = ((int64_t)a.NM + BB_THREADS * PAIRS * BB_STEPS - 1) / (BB_THREADS * PAIRS * BB_STEPS) * a.B;
   const int64_t blocks = imin64(tiles, (int64_t)sm_count() * 4);
   const int64_t all = (a.H + BB_HEADS - 1) / BB_HEADS;
   const int64_t offsets = bb_offsets(a, v, BB_TABLE_SMEM, blocks);
@@ -502,7 +564,7 @@ static cudaError_t bucket_fwd_launch(const BucketArgs& a, const void* table, voi
 }
 
 template <typename T, typename P, int AXES, int PAIRS>
-static cudaError_t bucket_bwd_launch(const BucketArgs& a, const void* dout, float* part, int64_t blocks,
+static cudaError_t bucket_bwd_launch(const BucketArgs& a, const void* dout, float* part, int64_t blocks, bool resume,
                                      cudaStream_t st) {
   const int64_t offsets = bb_offsets(a, 2, 16 * 1024, blocks);
   const int tile = BB_THREADS * PAIRS * BB_STEPS;
@@ -513,7 +575,7 @@ static cudaError_t bucket_bwd_launch(const BucketArgs& a, const void* dout, floa
     if (e != cudaSuccess) return e;
   }
   const dim3 grid((unsigned)blocks, (unsigned)((a.H + BB_HEADS - 1) / BB_HEADS));
-  k<<<grid, BB_THREADS, smem, st>>>(a, (const T*)dout, part);
+  k<<<grid, BB_THREADS, smem, st>>>(a, (const T*)dout, part, resume);
   return cudaGetLastError();
 }
 
@@ -536,7 +598,7 @@ extern "C" int affb_bucket_bias_fwd(const void* table, int table_dtype, const in
   if (rc) return rc;
   AFFB_REQUIRE(out_dtype == AFFB_F32 || out_dtype == AFFB_F16 || out_dtype == AFFB_BF16,
                "bucket_bias: the output must be fp32, fp16 or bf16");
-  if (B * a.NM == 0) return AFFB_OK;
+  if (B * a.batch_pairs == 0) return AFFB_OK;
   AFFB_REQUIRE(table && out, "bucket_bias: null pointer");
   const bool two = bb_two(a, out, out_dtype == AFFB_F32 ? 4 : 2);
   cudaStream_t st = as_stream(stream);
@@ -544,10 +606,13 @@ extern "C" int affb_bucket_bias_fwd(const void* table, int table_dtype, const in
   AFFB_DISPATCH(table_dtype, TB, {
     AFFB_DISPATCH(out_dtype, T, {
       BB_POS(pos_type, P, {
-        if (axes == 1) e = two ? bucket_fwd_launch<T, TB, P, 1, 2>(a, table, out, st)
-                               : bucket_fwd_launch<T, TB, P, 1, 1>(a, table, out, st);
-        else e = two ? bucket_fwd_launch<T, TB, P, 2, 2>(a, table, out, st)
-                     : bucket_fwd_launch<T, TB, P, 2, 1>(a, table, out, st);
+        e = bb_chunks(a, sizeof(P), [&](const BucketArgs& c, int64_t first) {
+          T* o = (T*)out + first;
+          if (axes == 1) return two ? bucket_fwd_launch<T, TB, P, 1, 2>(c, table, o, st)
+                                    : bucket_fwd_launch<T, TB, P, 1, 1>(c, table, o, st);
+          return two ? bucket_fwd_launch<T, TB, P, 2, 2>(c, table, o, st)
+                     : bucket_fwd_launch<T, TB, P, 2, 1>(c, table, o, st);
+        });
       })
     })
   });
@@ -575,19 +640,23 @@ extern "C" int affb_bucket_bias_bwd(const void* dout, int dout_dtype, const int3
   cudaStream_t st = as_stream(stream);
   const int64_t n = (int64_t)a.rows * H;
   int64_t blocks = 0;
-  if (B * a.NM > 0) {
+  if (B * a.batch_pairs > 0) {
     AFFB_REQUIRE(dout, "bucket_bias: null pointer");
-    blocks = bucket_bwd_blocks(B, H, a.NM);
+    blocks = bucket_bwd_blocks(B, H, a.batch_pairs);
     AFFB_REQUIRE(workspace && workspace_bytes >= blocks * n * 4, "bucket_bias: workspace too small");
     const bool two = bb_two(a, dout, dout_dtype == AFFB_F32 ? 4 : 2);
     cudaError_t e = cudaSuccess;
     AFFB_DISPATCH(dout_dtype, T, {
       BB_POS(pos_type, P, {
         float* part = (float*)workspace;
-        if (axes == 1) e = two ? bucket_bwd_launch<T, P, 1, 2>(a, dout, part, blocks, st)
-                               : bucket_bwd_launch<T, P, 1, 1>(a, dout, part, blocks, st);
-        else e = two ? bucket_bwd_launch<T, P, 2, 2>(a, dout, part, blocks, st)
-                     : bucket_bwd_launch<T, P, 2, 1>(a, dout, part, blocks, st);
+        e = bb_chunks(a, sizeof(P), [&](const BucketArgs& c, int64_t first) {
+          const T* g = (const T*)dout + first;
+          const bool more = first > 0;
+          if (axes == 1) return two ? bucket_bwd_launch<T, P, 1, 2>(c, g, part, blocks, more, st)
+                                    : bucket_bwd_launch<T, P, 1, 1>(c, g, part, blocks, more, st);
+          return two ? bucket_bwd_launch<T, P, 2, 2>(c, g, part, blocks, more, st)
+                     : bucket_bwd_launch<T, P, 2, 1>(c, g, part, blocks, more, st);
+        });
       })
     });
     if ((rc = bb_status(e))) return rc;

@@ -8,7 +8,7 @@
 // MN-major (rows of m or n, for the two products of the backward, which
 // contract over the other index of the stored matrices), and multiplied by
 // tcgen05.mma with the accumulator in tensor memory.  A block is persistent
-// and split by role: one warp issues the loads, one the products, twelve take
+// and split by role: one warp issues the loads, one the products, sixteen take
 // the finished accumulator (two are in flight) through the epilogue into
 // shared memory, from where TMA stores write it.
 //
@@ -35,16 +35,17 @@ namespace affb {
 using namespace tc5;
 
 constexpr int TILE_M = 128;
-constexpr int EPI_WARPS = 12;
-constexpr int EPI_GROUPS = EPI_WARPS / 4;   // warps that share the 32 rows of a quarter of tensor memory
+constexpr int EPI_WARPS = 16;
 constexpr int LIN_THREADS = 64 + EPI_WARPS * 32;
 constexpr int A_BYTES = TILE_M * 128;   // a block's rows of a tile
 constexpr int SMEM_MAX = 232448;     // 227 KB of a block
 constexpr int MAX_STAGES = 8;
-constexpr int STAGE_ROWS = 32;       // rows x columns of one warp's staging buffer
-constexpr int CHUNK = 32;
+constexpr int WARP_ROWS = 32;        // a warp's part of a tile: 32 rows x 64 columns
+constexpr int WARP_COLS = 64;
+constexpr int CHUNK = 32;            // worked on at a time
+constexpr int BUF_BYTES = WARP_ROWS * 128;  // staged rows of 128 bytes: 64 columns of 16 bits or 32 of fp32
 constexpr int BAR_BYTES = 256;
-constexpr int COLS_BYTES = EPI_WARPS * 2 * CHUNK * 4;  // each epilogue warp's bias and column scales of a chunk
+constexpr int COLS_BYTES = EPI_WARPS * 2 * WARP_COLS * 4;  // each epilogue warp's bias and column scales
 
 // Set when a block's waits ran out; read by affb_linear_status.
 __device__ int g_linear_failed;
@@ -59,9 +60,7 @@ struct GemmArgs {
   int b_bytes;       // a block's part of B
   uint32_t idesc;
   int direct;        // outputs not addressable by TMA: plain stores
-  int bufs;          // staging buffers of a warp (2, or 1 where fp32 outputs make them large)
-  int buf_bytes;     // one of them: out chunk, then z chunk
-  int z_off;
+  int bufs;          // staging buffers of a warp: out, and z where it is wanted
   LinearEpilogue e;
 };
 
@@ -103,10 +102,11 @@ struct Units {
   }
 };
 
-// 32 columns of one row into a warp's staging buffer, in the swizzle that the
-// TMA store undoes (64-byte rows: 64B swizzle, 128-byte rows: 128B).
+// 32 columns of one row into a warp's staging buffer, in the 128-byte swizzle
+// that the TMA store undoes: half 0 or 1 of a row of 16-bit values, or all of
+// a row of fp32.
 template <typename T>
-__device__ __forceinline__ void stage_row(unsigned char* buf, int lane, const float* v) {
+__device__ __forceinline__ void stage_row(unsigned char* buf, int lane, int half, const float* v) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -115,7 +115,7 @@ __device__ __forceinline__ void stage_row(unsigned char* buf, int lane, const fl
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      st8(reinterpret_cast<T*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)), v + 8 * j);
+      st8(reinterpret_cast<T*>(buf + lane * 128 + (((4 * half + j) ^ (lane & 7)) << 4)), v + 8 * j);
   }
 }
 template <typename T>
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
   unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const int stage_bytes = A_BYTES + p.b_bytes;
   unsigned char* staging = smem + p.stages * stage_bytes;
-  float* cols = reinterpret_cast<float*>(staging + EPI_WARPS * p.bufs * p.buf_bytes);
+  float* cols = reinterpret_cast<float*>(staging + EPI_WARPS * p.bufs * BUF_BYTES);
   unsigned char* bars = reinterpret_cast<unsigned char*>(cols) + COLS_BYTES;
   const uint32_t full = smem_addr(bars), empty = full + 8 * MAX_STAGES;
   const uint32_t acc_full = empty + 8 * MAX_STAGES, acc_empty = acc_full + 16, drain = acc_empty + 16;
@@ -300,66 +300,72 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
         else bar_arrive(done_at + 8 * acc);
       }
     };
-    unsigned char* my = staging + ew * p.bufs * p.buf_bytes;
-    float* bias = cols + ew * 2 * CHUNK;
-    int acc = 0, buf = 0;
+    unsigned char* buf = staging + ew * p.bufs * BUF_BYTES;
+    unsigned char* zbuf = buf + BUF_BYTES;
+    float* bias = cols + ew * 2 * WARP_COLS;
+    const bool per_col = p.e.bias || p.e.col_scale;
+    const int z_bytes = p.e.z_dtype == AFFB_F32 ? 4 : 2;
+    int acc = 0;
     uint32_t acc_phase = 0;
     for (Units u(p, first, step); u.more(p); u.next(p)) {
-      const int s = u.s, m0 = (u.mi * CG + (int)rank) * TILE_M, n0 = u.ni * p.bn;
-      const int ncols = min(p.bn, p.N - n0);
-      const int m = m0 + quad * 32 + lane;
-      // the next chunk's bias and column scale of this lane's column
-      float nb = 0.f, ns = 1.f;
-      const auto fetch = [&](int c) {
-        if (c + lane >= ncols) return;
-        const int n = n0 + c + lane;
-        if (p.e.bias) {
-          if (p.e.bias_dtype == AFFB_F32) nb = ((const float*)p.e.bias)[n];
-          else if (p.e.bias_dtype == AFFB_BF16) nb = __bfloat162float(((const __nv_bfloat16*)p.e.bias)[n]);
-          else nb = __half2float(((const __half*)p.e.bias)[n]);
+      const int s = u.s, m0 = (u.mi * CG + (int)rank) * TILE_M + quad * WARP_ROWS;
+      const int c0 = group * WARP_COLS, n0 = u.ni * p.bn + c0;
+      const int ncols = min(min(p.bn - c0, p.N - n0), WARP_COLS);  // <= 0: nothing for this warp in a narrow tile
+      const int m = m0 + lane;
+      if (per_col) {
+        __syncwarp();  // the tile before has been read
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int c = h * CHUNK + lane, n = n0 + c;
+          if (c < ncols) {
+            float b = 0.f;
+            if (p.e.bias) {
+              if (p.e.bias_dtype == AFFB_F32) b = ((const float*)p.e.bias)[n];
+              else if (p.e.bias_dtype == AFFB_BF16) b = __bfloat162float(((const __nv_bfloat16*)p.e.bias)[n]);
+              else b = __half2float(((const __half*)p.e.bias)[n]);
+            }
+            bias[c] = b;
+            if (p.e.col_scale) bias[WARP_COLS + c] = p.e.col_scale[n];
+          }
         }
-        if (p.e.col_scale) ns = p.e.col_scale[n];
-      };
-      const bool per_col = p.e.bias || p.e.col_scale;
-      if (per_col) fetch(group * CHUNK);
+        __syncwarp();
+      }
       const float rs = (p.e.row_scale && m < p.M) ? p.e.row_scale[m] : 1.f;
       // all lanes of the warp leave together
-      if (__any_sync(0xffffffffu, !bar_wait(acc_full + 8 * acc, acc_phase, failed))) break;
+      if (!warp_wait(acc_full + 8 * acc, acc_phase, failed)) break;
       fence_after();
-      // the accumulator's next chunk is on its way while one is worked on
-      uint32_t r[32];
-      const uint32_t lanes = tmem + acc * 256 + ((uint32_t)(quad * 32) << 16);
-      constexpr int NEXT = EPI_GROUPS * CHUNK;
-      if (group * CHUNK < ncols) tmem_load32(lanes + group * CHUNK, r);
-      else read_all(acc);  // no chunk for this warp in a narrow tile
-      for (int c = group * CHUNK; c < ncols; c += NEXT) {
+      if (ncols <= 0) read_all(acc);
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        const int c = h * CHUNK;
+        if (c >= ncols) break;
+        uint32_t r[32];
+        tmem_load32(tmem + acc * 256 + c0 + c + ((uint32_t)(quad * 32) << 16), r);
         tmem_wait_load();
+        if (c + CHUNK >= ncols) read_all(acc);
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        if (c + NEXT < ncols) tmem_load32(lanes + c + NEXT, r);
-        else read_all(acc);
-        if (per_col) {
-          __syncwarp();  // the chunk before has been read
-          bias[lane] = nb;
-          bias[CHUNK + lane] = ns;
-          __syncwarp();
-          fetch(c + NEXT);
-          if (p.e.col_scale) {
+        if (p.e.col_scale) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= rs * bias[CHUNK + i];
+          for (int i = 0; i < 32; i += 2) {
+            const float2 w = *reinterpret_cast<const float2*>(bias + WARP_COLS + c + i);
+            unpack2(mul2(pack2(v[i], v[i + 1]), mul2(both(rs), pack2(w.x, w.y))), v[i], v[i + 1]);
           }
+        }
+        if (per_col) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] += bias[i];
+          for (int i = 0; i < 32; i += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(bias + c + i);
+            unpack2(add2(pack2(v[i], v[i + 1]), pack2(w.x, w.y)), v[i], v[i + 1]);
+            unpack2(add2(pack2(v[i + 2], v[i + 3]), pack2(w.z, w.w)), v[i + 2], v[i + 3]);
+          }
         }
         const int n = min(CHUNK, ncols - c);
         const int64_t off = ((int64_t)s * p.M + m) * p.N + n0 + c;
-        unsigned char* ob = my + buf * p.buf_bytes;
-        if (!p.direct) {  // the buffer's last store has been read
-          if (lane == 0) {
-            if (p.bufs == 2) store_wait_read<1>();
-            else store_wait_read<0>();
-          }
+        // the buffers' last stores have been read (those of the tile before, or of fp32's first half)
+        if (!p.direct && (h == 0 || sizeof(TO) == 4 || (p.e.z && z_bytes == 4))) {
+          if (lane == 0) store_wait_read<0>();
           __syncwarp();
         }
         if (p.e.z) {
@@ -370,13 +376,13 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
               else store_row((__half*)p.e.z + off, n, v);
             }
           } else {
-            if (p.e.z_dtype == AFFB_F32) stage_row<float>(ob + p.z_off, lane, v);
-            else if (p.e.z_dtype == AFFB_BF16) stage_row<__nv_bfloat16>(ob + p.z_off, lane, v);
-            else stage_row<__half>(ob + p.z_off, lane, v);
+            if (p.e.z_dtype == AFFB_F32) stage_row<float>(zbuf, lane, h, v);
+            else if (p.e.z_dtype == AFFB_BF16) stage_row<__nv_bfloat16>(zbuf, lane, h, v);
+            else stage_row<__half>(zbuf, lane, h, v);
           }
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = activate<ACT>(v[i]);
+        for (int i = 0; i < 32; i += 2) activate_pair<ACT>(v[i], v[i + 1]);
         if (p.e.residual && m < p.M) {
           if (p.e.residual_dtype == AFFB_F32) add_row((const float*)p.e.residual + off, n, v);
           else if (p.e.residual_dtype == AFFB_BF16) add_row((const __nv_bfloat16*)p.e.residual + off, n, v);
@@ -385,15 +391,18 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
         if (p.direct) {
           if (m < p.M) store_row((TO*)p.e.out + off, n, v);
         } else {
-          stage_row<TO>(ob, lane, v);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store(&map_out, smem_addr(ob), n0 + c, m0 + quad * 32, s);
-            if (p.e.z) tma_store(&map_z, smem_addr(ob + p.z_off), n0 + c, m0 + quad * 32, s);
-            store_commit();
+          stage_row<TO>(buf, lane, h, v);
+          const bool last = c + CHUNK >= ncols;
+          const bool out_now = sizeof(TO) == 4 || last, z_now = p.e.z && (z_bytes == 4 || last);
+          if (out_now || z_now) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (out_now) tma_store(&map_out, smem_addr(buf), n0 + (sizeof(TO) == 4 ? c : 0), m0, s);
+              if (z_now) tma_store(&map_z, smem_addr(zbuf), n0 + (z_bytes == 4 ? c : 0), m0, s);
+              store_commit();
+            }
           }
-          if (p.bufs == 2) buf ^= 1;
         }
       }
       acc ^= 1;
@@ -466,14 +475,19 @@ struct Operand {
   bool mn;
 };
 
+constexpr int PAIR_K = 6;
+
 struct Shape {
   int cg, bn, nt, mt, splits;
 };
 
 // Tile and split of the contraction.
 // Pairs of blocks (256-row tiles up to 256 columns wide) where there are
-// enough tiles, or enough k blocks to split, for all of them; else single
-// blocks, whose tiles are narrowed (down to 64 columns) and whose contraction
+// enough tiles, or enough k blocks to split, for all of them, and a tile's
+// contraction is long enough to be worth the pair's handshakes (524288 x 96 ->
+// 192, two k blocks: 87 us by pairs, 57 by single blocks; 524288 x 384 -> 768,
+// six: 292 against 329; 8192 x 4096 -> 8192 e4m3, 32: 190 against 215); else
+// single blocks, whose tiles are narrowed (down to 64 columns) and whose contraction
 // is split (at least 4 k blocks a part) until they fill the GPU.
 static Shape choose_shape(int64_t M, int64_t N, int64_t total_k) {
   const int64_t sms = sm_count();
@@ -481,14 +495,14 @@ static Shape choose_shape(int64_t M, int64_t N, int64_t total_k) {
   const int64_t wide = (N + 255) / 256;
   const int64_t pair_tiles = (M + 255) / 256 * wide;
   const int64_t most_splits = total_k >= 8 ? total_k / 4 : 1;
-  s.cg = M > TILE_M && pair_tiles * most_splits >= sms / 2 ? 2 : 1;
+  s.cg = M > TILE_M && total_k >= PAIR_K && pair_tiles * most_splits >= sms / 2 ? 2 : 1;
   const int64_t teams = sms / s.cg;
   s.mt = (int)((M + TILE_M * s.cg - 1) / (TILE_M * s.cg));
   s.nt = (int)wide;
   if (s.cg == 1)
     while ((int64_t)s.mt * s.nt * 2 <= sms && (N + s.nt * 2 - 1) / (s.nt * 2) >= 64) s.nt *= 2;
   const int64_t per = (N + s.nt - 1) / s.nt;
-  s.bn = (int)round_up(per, s.nt == 1 && s.cg == 1 ? 16 : 32);
+  s.bn = (int)round_up(per, s.nt > 1 ? 64 : s.cg == 1 ? 16 : 32);  // stores are 64 columns wide
   s.nt = (int)((N + s.bn - 1) / s.bn);
   const int64_t tiles = (int64_t)s.mt * s.nt;
   int64_t sp = teams / tiles;
@@ -572,11 +586,9 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
   p.e = e;
   p.direct = s.splits > 1 ? 0
                           : !(tma_rows(e.out, e.out_dtype, N) && (!e.z || tma_rows(e.z, e.z_dtype, N)));
-  p.z_off = (int)dtype_size(e.out_dtype) * STAGE_ROWS * CHUNK;
-  p.buf_bytes = p.z_off + (e.z ? (int)dtype_size(e.z_dtype) * STAGE_ROWS * CHUNK : 0);
+  p.bufs = e.z ? 2 : 1;
   const int stage = A_BYTES + p.b_bytes;
-  p.bufs = p.buf_bytes > 2048 ? 1 : 2;
-  const int fixed = 1024 + EPI_WARPS * p.bufs * p.buf_bytes + COLS_BYTES + BAR_BYTES;
+  const int fixed = 1024 + EPI_WARPS * p.bufs * BUF_BYTES + COLS_BYTES + BAR_BYTES;
   p.stages = (SMEM_MAX - fixed) / stage;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   AFFB_REQUIRE(p.stages >= 2, "linear: no room for two stages");
@@ -592,9 +604,13 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
                      CU_TENSOR_MAP_SWIZZLE_128B, p.b_blocks)))
     return rc;
   if (!p.direct) {
-    const auto sw = [](int t) { return t == AFFB_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B; };
-    if ((rc = make_map(&mo, e.out_dtype, e.out, p.N, M, s.splits, p.N, CHUNK, STAGE_ROWS, sw(e.out_dtype)))) return rc;
-    if (e.z && (rc = make_map(&mz, e.z_dtype, e.z, p.N, M, 1, p.N, CHUNK, STAGE_ROWS, sw(e.z_dtype)))) return rc;
+    const auto cols = [](int t) { return t == AFFB_F32 ? 32 : 64; };  // of a staged row of 128 bytes
+    if ((rc = make_map(&mo, e.out_dtype, e.out, p.N, M, s.splits, p.N, cols(e.out_dtype), WARP_ROWS,
+                       CU_TENSOR_MAP_SWIZZLE_128B)))
+      return rc;
+    if (e.z && (rc = make_map(&mz, e.z_dtype, e.z, p.N, M, 1, p.N, cols(e.z_dtype), WARP_ROWS,
+                              CU_TENSOR_MAP_SWIZZLE_128B)))
+      return rc;
   }
   const void* k = s.cg == 2 ? kernel_of<2>(e.out_dtype, e.act) : kernel_of<1>(e.out_dtype, e.act);
   const int slot = (s.cg - 1) * 12 + (e.out_dtype == AFFB_F32 ? 0 : e.out_dtype == AFFB_BF16 ? 4 : 8) + e.act;
