@@ -152,7 +152,7 @@ def call(name: str, *args) -> None:
     """Call an entry point; raise RuntimeError carrying the library's message."""
     global CALLS
     CALLS += 1
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != 0:
         msg = lib().affb_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed (code {rc}): {msg}")
@@ -160,7 +160,8 @@ def call(name: str, *args) -> None:
 
 def dense(t: torch.Tensor) -> torch.Tensor:
     """`t` contiguous and 16-byte aligned (itself where it already is)."""
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -182,9 +183,13 @@ def stream(device=None) -> int:
 def call_on(device: torch.device, name: str, *args) -> None:
     """``call`` with `device` current (kernels launch on the current device)
     and that device's current stream as the last argument."""
+    global CALLS
     index = device.index
     if index == _current_device():
-        call(name, *args, _raw_stream(index))
+        CALLS += 1
+        rc = getattr(_lib or lib(), name)(*args, _raw_stream(index))
+        if rc != 0:
+            raise RuntimeError(f"{name} failed (code {rc}): {lib().affb_last_error().decode(errors='replace')}")
     else:
         with torch.cuda.device(device):
             call(name, *args, _raw_stream(torch.cuda.current_device()))
@@ -205,7 +210,7 @@ def workspace(name: str, device, *args):
     """Uninitialised device memory of the size the library's function `name`
     asks for (None where it needs none), from the current stream's pool."""
     n = _size(name, *args)
-    return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 def require_cuda(*tensors) -> None:

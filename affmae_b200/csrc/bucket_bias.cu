@@ -227,16 +227,23 @@ __global__ void __launch_bounds__(BB_THREADS, 4)
   const int h0 = blockIdx.y * groups * BB_HEADS, nh = min(groups * BB_HEADS, a.H - h0);
   fill_lut(a, lut);
   __syncthreads();
-  for (int i = threadIdx.x; i <= entries; i += BB_THREADS) {  // the last entry is zero
-    int row = i;
-    if (BY_OFFSET && i < entries) {
-      row = axis_index(a, lut, unclipped(a, AXES == 2 ? i % a.span : i));
-      if (AXES == 2) row += axis_index(a, lut, unclipped(a, i / a.span)) * a.per_axis;
+  const auto fill = [&](int i, int row) {  // entry i: the heads of a table row (row < 0: zero)
+    for (int g = 0; g < groups; ++g) {
+      T* t = reinterpret_cast<T*>(tab + g * (entries + 1) + i);
+#pragma unroll
+      for (int h = 0; h < BB_HEADS; ++h)
+        stf(t + h, row >= 0 && g * BB_HEADS + h < nh ? ldf(table + row * a.H + h0 + g * BB_HEADS + h) : 0.f);
     }
-    for (int h = 0; h < groups * BB_HEADS; ++h) {
-      const float v = i < entries && h < nh ? ldf(table + (int64_t)row * a.H + h0 + h) : 0.f;
-      stf(reinterpret_cast<T*>(tab + (h / BB_HEADS) * (entries + 1) + i) + h % BB_HEADS, v);
+  };
+  if (threadIdx.x == 0) fill(entries, -1);
+  if (BY_OFFSET && AXES == 2) {
+    // a warp takes whole rows of offsets along y
+    for (int y = threadIdx.x >> 5; y < a.span; y += BB_THREADS / 32) {
+      const int ry = axis_index(a, lut, unclipped(a, y)) * a.per_axis;
+      for (int x = threadIdx.x & 31; x < a.span; x += 32) fill(y * a.span + x, ry + axis_index(a, lut, unclipped(a, x)));
     }
+  } else {
+    for (int i = threadIdx.x; i < entries; i += BB_THREADS) fill(i, BY_OFFSET ? axis_index(a, lut, unclipped(a, i)) : i);
   }
   __syncthreads();
   constexpr int STEP = BB_THREADS * PAIRS, TILE = STEP * BB_STEPS;
@@ -308,13 +315,15 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
   fill_lut(a, lut);
   __syncthreads();
   if (BY_OFFSET) {
-    for (int i = threadIdx.x; i <= offsets; i += BB_THREADS) {
-      int row = none;
-      if (i < offsets) {
-        row = axis_index(a, lut, unclipped(a, AXES == 2 ? i % a.span : i));
-        if (AXES == 2) row += axis_index(a, lut, unclipped(a, i / a.span)) * a.per_axis;
+    if (threadIdx.x == 0) rows[offsets] = (uint16_t)none;
+    if (AXES == 2) {
+      for (int y = threadIdx.x >> 5; y < a.span; y += BB_THREADS / 32) {
+        const int ry = axis_index(a, lut, unclipped(a, y)) * a.per_axis;
+        for (int x = threadIdx.x & 31; x < a.span; x += 32)
+          rows[y * a.span + x] = (uint16_t)(ry + axis_index(a, lut, unclipped(a, x)));
       }
-      rows[i] = (uint16_t)row;
+    } else {
+      for (int i = threadIdx.x; i < offsets; i += BB_THREADS) rows[i] = (uint16_t)axis_index(a, lut, unclipped(a, i));
     }
   }
   float* mine = part + ((int64_t)blockIdx.x * a.H + h0) * a.rows;

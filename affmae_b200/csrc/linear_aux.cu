@@ -204,27 +204,28 @@ __device__ __forceinline__ float activate_code(int act, float z) {
   }
 }
 
-// Block: 32 consecutive elements x 32 lanes of parts, summed in a fixed order.
-__global__ void __launch_bounds__(1024) sum_parts_kernel(const float* __restrict__ part, int64_t S, int64_t M,
-                                                         int64_t N, int64_t ld, LinearEpilogue e) {
-  __shared__ float red[32][33];
+// Block: 32 consecutive elements x L lanes of parts, summed in a fixed order.
+template <int L>
+__global__ void __launch_bounds__(32 * L) sum_parts_kernel(const float* __restrict__ part, int S, int64_t M, int64_t N,
+                                                           int64_t ld, LinearEpilogue e) {
+  __shared__ float red[L][33];
   const int x = threadIdx.x & 31, l = threadIdx.x >> 5;
   const int64_t n = M * N, plane = M * ld;
   for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < n; i0 += (int64_t)gridDim.x * 32) {
-    int64_t i = i0 + x;
+    const int64_t i = i0 + x;
+    const int64_t m = i < n ? i / N : 0, c = i < n ? i - m * N : 0;
     float s = 0.f;
     if (i < n) {
-      const int64_t m = i / N;
-      const float* p = part + m * ld + (i - m * N);
+      const float* p = part + m * ld + c;
 #pragma unroll 8
-      for (int64_t k = l; k < S; k += 32) s += __ldg(p + k * plane);
+      for (int k = l; k < S; k += L) s += __ldg(p + k * plane);
     }
     red[l][x] = s;
     __syncthreads();
-    float v = warp_sum(red[x][l]);
-    i = i0 + l;
-    if (x == 0 && i < n) {
-      const int64_t m = i / N, c = i - m * N;
+    if (l == 0 && i < n) {
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < L; ++k) v += red[k][x];
       if (e.row_scale) v *= e.row_scale[m];
       if (e.col_scale) v *= e.col_scale[c];
       if (e.bias) v += load_as(e.bias, e.bias_dtype, c);
@@ -260,16 +261,19 @@ __global__ void __launch_bounds__(256) sum_few_parts_kernel(const float* __restr
 int linear_sum(const float* part, int64_t S, int64_t M, int64_t N, int64_t ld, const LinearEpilogue& e,
                cudaStream_t st) {
   if (M * N == 0) return AFFB_OK;
-  // Lanes over the parts only where elements are few (1184 parts of 192: 24 us
-  // with a thread an element, 9 with lanes); otherwise a thread an element
-  // streams them at full width (12 parts of 768 x 384: 7 against 107 us).
-  if (M * N >= (int64_t)sm_count() * 64) {
-    const unsigned blocks = (unsigned)imin64((M * N + 255) / 256, (int64_t)sm_count() * 8);
-    sum_few_parts_kernel<<<blocks, 256, 0, st>>>(part, (int)S, M, N, ld, e);
-  } else {
-    const unsigned blocks = (unsigned)imin64((M * N + 31) / 32, (int64_t)sm_count() * 4);
-    sum_parts_kernel<<<blocks, 1024, 0, st>>>(part, S, M, N, ld, e);
-  }
+  // Lanes over the parts until the threads fill the GPU: a thread an element
+  // streams 12 parts of 768 x 384 in 7 us (with 32 lanes 107), eight lanes sum
+  // 74 parts of 192 x 96 in 5.5 us (23 without), 32 lanes 888 parts of 192 in
+  // 9 us (24 with eight).
+  const int64_t n = M * N, fill = (int64_t)sm_count() * 1024;
+  const unsigned blocks = (unsigned)imin64((n + 31) / 32, (int64_t)sm_count() * 32);
+  if (n >= fill || S < 8)
+    sum_few_parts_kernel<<<(unsigned)imin64((n + 255) / 256, (int64_t)sm_count() * 8), 256, 0, st>>>(part, (int)S, M, N,
+                                                                                                     ld, e);
+  else if (n * 8 >= fill / 2 || S < 32)
+    sum_parts_kernel<8><<<blocks, 256, 0, st>>>(part, (int)S, M, N, ld, e);
+  else
+    sum_parts_kernel<32><<<blocks, 1024, 0, st>>>(part, (int)S, M, N, ld, e);
   AFFB_LAUNCH_CHECK("linear: sum of partial products");
   return AFFB_OK;
 }

@@ -66,6 +66,13 @@ def _edge_array(edges):
 
 def _check(table, edges, q_pos, k_pos, member_idx, one_sided, dtype) -> tuple[int, ...]:
     edges = _check_edges(edges)
+    qs, ks, dev, pt = q_pos.shape, k_pos.shape, table.device, q_pos.dtype
+    # the common case in a few comparisons; whatever else is looked at in order below
+    if dev.type == "cuda" and q_pos.device == dev and k_pos.device == dev and len(qs) == 3 and len(ks) == 3 \
+            and (qs[2] == 1 or (qs[2] == 2 and len(edges) <= 32)) and qs[2] == ks[2] and qs[0] == ks[0] and pt in _POS \
+            and k_pos.dtype == pt and len(table.shape) == 2 and table.shape[0] == bucket_count(edges, qs[2], one_sided) \
+            and table.dtype in _FLOATS and dtype in _FLOATS and member_idx is None:
+        return edges
     nat.require_cuda(table, q_pos, k_pos, member_idx)
     if q_pos.dim() != 3 or k_pos.dim() != 3 or q_pos.shape[2] not in (1, 2) or q_pos.shape[2] != k_pos.shape[2] \
             or q_pos.shape[0] != k_pos.shape[0]:
@@ -106,7 +113,7 @@ def bucket_bias_fwd(table, edges, q_pos, k_pos, member_idx, one_sided, dtype):
     Nk, H = k_pos.shape[1], table.shape[1]
     M = member_idx.shape[2] if member_idx is not None else Nk
     dev = table.device
-    out = torch.empty((B, H, Nq, M), device=dev, dtype=dtype)
+    out = table.new_empty((B, H, Nq, M), dtype=dtype)
     nat.call_on(dev, "affb_bucket_bias_fwd", nat.ptr(table), nat.dcode(table), ctypes.addressof(arr), len(edges),
                 int(one_sided), nat.ptr(q_pos), nat.ptr(k_pos), _POS[q_pos.dtype], axes, nat.ptr(member_idx), B, H, Nq,
                 Nk, M, nat.ptr(out), nat.dcode(out))

@@ -24,6 +24,7 @@ from .. import _native as nat
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_CODE = nat._DTYPE_CODE
 
 
 def _act_code(act: str) -> int:
@@ -34,6 +35,15 @@ def _act_code(act: str) -> int:
 
 
 def _check(x, weight, bias, residual):
+    """Shapes, devices and the bias's type (refuses in the order a caller would
+    want to know).  The accepted case is decided by a few comparisons: a
+    one-token call takes as long as its checks."""
+    xs, ws, dev = x.shape, weight.shape, x.device
+    if dev.type == "cuda" and len(ws) == 2 and xs and xs[-1] == ws[1] and ws[0] and ws[1] and weight.device == dev \
+            and (bias is None or (bias.shape == ws[:1] and bias.dtype in _FLOATS and bias.device == dev)) \
+            and (residual is None or (residual.shape[:-1] == xs[:-1] and len(residual.shape) == len(xs)
+                                      and residual.shape[-1] == ws[0] and residual.device == dev)):
+        return
     nat.require_cuda(x, weight, bias, residual)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise RuntimeError(f"linear: input {tuple(x.shape)} does not match weight {tuple(weight.shape)} [out, in]")
@@ -42,16 +52,15 @@ def _check(x, weight, bias, residual):
     out_shape = (*x.shape[:-1], weight.shape[0])
     if residual is not None and tuple(residual.shape) != out_shape:
         raise RuntimeError(f"linear: residual {tuple(residual.shape)} does not have the output's shape {out_shape}")
-    for t in (weight, bias, residual):
-        if t is not None and t.device != x.device:
-            raise RuntimeError("linear: tensors are on different devices")
+    raise RuntimeError("linear: tensors are on different devices")
 
 
 def _check_operands(x, weight, bias, residual):
     _check(x, weight, bias, residual)
-    if x.dtype not in _FLOATS or weight.dtype != x.dtype:
+    dt = x.dtype
+    if dt not in _FLOATS or weight.dtype != dt:
         raise RuntimeError(f"linear: input ({x.dtype}) and weight ({weight.dtype}) must share one of fp32, fp16, bf16")
-    if residual is not None and residual.dtype not in (x.dtype, torch.float32):
+    if residual is not None and residual.dtype != dt and residual.dtype != torch.float32:
         raise RuntimeError(f"linear: residual must be {x.dtype} or float32, got {residual.dtype}")
 
 
@@ -62,16 +71,25 @@ def linear_fwd(x, weight, bias, residual, act: int, save: bool):
     N, K = weight.shape
     M = x.numel() // K
     dev = x.device
-    out_shape = (*x.shape[:-1], N)
-    bc = bias.contiguous() if bias is not None else None
-    rc = residual.contiguous() if residual is not None else None
-    out = torch.empty(out_shape, device=dev, dtype=x.dtype if rc is None else rc.dtype)
-    z = torch.empty(out_shape, device=dev, dtype=x.dtype) if save and linear_saves(act, rc) else None
-    dt = nat.dcode(x)
+    dt = _CODE[x.dtype]
+    bptr = bdt = rptr = zptr = wptr = None
+    if bias is not None:
+        bias = bias if bias.is_contiguous() else bias.contiguous()
+        bptr, bdt = bias.data_ptr(), _CODE[bias.dtype]
+    if residual is None:
+        out, rdt = x.new_empty((*x.shape[:-1], N)), dt
+    else:
+        residual = residual if residual.is_contiguous() else residual.contiguous()
+        out, rptr, rdt = torch.empty_like(residual), residual.data_ptr(), _CODE[residual.dtype]
+    z = None
+    if save and linear_saves(act, residual):
+        z = x.new_empty(out.shape)
+        zptr = z.data_ptr()
     ws = nat.workspace("affb_linear_fwd_workspace_bytes", dev, dt, M, N, K)
-    nat.call_on(dev, "affb_linear_fwd", nat.ptr(x), nat.ptr(weight), nat.ptr(bc),
-                nat.dcode(bc) if bc is not None else 0, nat.ptr(rc), nat.dcode(rc) if rc is not None else 0, act, dt,
-                M, N, K, nat.ptr(out), nat.dcode(out), nat.ptr(z), nat.ptr(ws), ws.numel() if ws is not None else 0)
+    if ws is not None:
+        wptr = ws.data_ptr()
+    nat.call_on(dev, "affb_linear_fwd", x.data_ptr(), weight.data_ptr(), bptr, bdt or 0, rptr, rdt, act, dt, M, N, K,
+                out.data_ptr(), rdt, zptr, wptr, ws.numel() if wptr else 0)
     return out, z
 
 
@@ -133,7 +151,9 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     "silu".  Differentiable once in x, weight, bias and residual."""
     code = _act_code(act)
     _check_operands(x, weight, bias, residual)
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))):
+    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                         or (bias is not None and bias.requires_grad)
+                                         or (residual is not None and residual.requires_grad))):
         return linear_fwd(nat.dense(x), nat.dense(weight), bias, residual, code, False)[0]
     return FusedLinearFunction.apply(x, weight, bias, residual, code)
 
@@ -189,23 +209,34 @@ def linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     if out_dtype not in _FLOATS or (residual is not None and residual.dtype not in _FLOATS):
         raise RuntimeError("linear_e4m3: output and residual must be fp32, fp16 or bf16")
     N, K = weight.shape
-    if tuple(x_scale.shape) != tuple(x.shape[:-1]) or tuple(weight_scale.shape) != (N,):
-        raise RuntimeError("linear_e4m3: scales must have one value per row")
-    nat.require_cuda(x_scale, weight_scale)
     dev = x.device
+    if x_scale.shape != x.shape[:-1] or weight_scale.shape != weight.shape[:1]:
+        raise RuntimeError("linear_e4m3: scales must have one value per row")
     if x_scale.device != dev or weight_scale.device != dev:
-        raise RuntimeError("linear_e4m3: tensors are on different devices")
+        raise RuntimeError("linear_e4m3: scales must be on the operands' device")
     M = x.numel() // K
-    xc, wc = nat.dense(x), nat.dense(weight)
-    xs, wsc = x_scale.to(torch.float32).contiguous(), weight_scale.to(torch.float32).contiguous()
-    bc = bias.to(torch.float32).contiguous() if bias is not None else None
-    rc = residual.contiguous() if residual is not None else None
-    out = torch.empty((*x.shape[:-1], N), device=dev, dtype=out_dtype)
+    x, weight = nat.dense(x), nat.dense(weight)
+    x_scale, weight_scale = _f32(x_scale), _f32(weight_scale)
+    bptr = rptr = wptr = None
+    rdt = 0
+    if bias is not None:
+        bias = _f32(bias)
+        bptr = bias.data_ptr()
+    if residual is not None:
+        residual = residual if residual.is_contiguous() else residual.contiguous()
+        rptr, rdt = residual.data_ptr(), _CODE[residual.dtype]
+    out = x.new_empty((*x.shape[:-1], N), dtype=out_dtype)
     ws = nat.workspace("affb_linear_e4m3_workspace_bytes", dev, M, N, K)
-    nat.call_on(dev, "affb_linear_e4m3", nat.ptr(xc), nat.ptr(xs), nat.ptr(wc), nat.ptr(wsc), nat.ptr(bc), nat.ptr(rc),
-                nat.dcode(rc) if rc is not None else 0, code, M, N, K, nat.ptr(out), nat.dcode(out), nat.ptr(ws),
-                ws.numel() if ws is not None else 0)
+    if ws is not None:
+        wptr = ws.data_ptr()
+    nat.call_on(dev, "affb_linear_e4m3", x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(),
+                bptr, rptr, rdt, code, M, N, K, out.data_ptr(), _CODE[out_dtype], wptr, ws.numel() if wptr else 0)
     return out
+
+
+def _f32(t):
+    """`t` as a dense fp32 vector (itself where it is one)."""
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
 class LinearE4M3(nn.Module):

@@ -21,9 +21,16 @@ from torch.autograd.function import once_differentiable
 from .. import _native as nat
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_CODE = nat._DTYPE_CODE
 
 
 def _check(x, weight, delta, row_scale):
+    xs, dev = x.shape, x.device
+    # the common case in a few comparisons; whatever else is looked at in order below
+    if dev.type == "cuda" and xs and xs[-1] and weight.shape == xs[-1:] and weight.device == dev and row_scale is None \
+            and x.dtype in _FLOATS and weight.dtype in _FLOATS \
+            and (delta is None or (delta.shape == xs and delta.dtype in _FLOATS and delta.device == dev)):
+        return
     nat.require_cuda(x, weight, delta, row_scale)
     if x.dim() < 1 or tuple(weight.shape) != (x.shape[-1],) or x.shape[-1] < 1:
         raise RuntimeError(f"rms_norm: weight {tuple(weight.shape)} does not match the rows of {tuple(x.shape)}")
@@ -51,21 +58,29 @@ def _launch(x, delta, row_scale, weight, eps, out_dtype, keep):
     R = x.numel() // C
     dev = x.device
     xc = nat.dense(x)
-    dc = nat.dense(delta) if delta is not None else None
-    rs = row_scale.float().contiguous() if row_scale is not None else None
     w = nat.dense(weight.detach().float() if weight.requires_grad or weight.dtype != torch.float32 else weight)
-    s = torch.empty(x.shape, device=dev, dtype=x.dtype) if dc is not None else None
-    rstd = torch.empty(R, device=dev, dtype=torch.float32) if keep else None
-    y = q = scale = None
+    s = rs = rstd = y = q = scale = None
+    dptr = sptr = rptr = kptr = yptr = qptr = cptr = None
+    ddt = ydt = groups = 0
+    if delta is not None:
+        delta = nat.dense(delta)
+        s = torch.empty_like(xc)
+        dptr, ddt, sptr = delta.data_ptr(), _CODE[delta.dtype], s.data_ptr()
+    if row_scale is not None:
+        rs = row_scale.float().contiguous()
+        rptr, groups = rs.data_ptr(), rs.numel()
+    if keep:
+        rstd = xc.new_empty(R, dtype=torch.float32)
+        kptr = rstd.data_ptr()
     if out_dtype is None:
-        q = torch.empty(x.shape, device=dev, dtype=torch.float8_e4m3fn)
-        scale = torch.empty(x.shape[:-1], device=dev, dtype=torch.float32)
+        q = torch.empty_like(xc, dtype=torch.float8_e4m3fn)
+        scale = xc.new_empty(x.shape[:-1], dtype=torch.float32)
+        qptr, cptr = q.data_ptr(), scale.data_ptr()
     else:
-        y = torch.empty(x.shape, device=dev, dtype=out_dtype)
-    nat.call_on(dev, "affb_rms_norm_fwd", nat.ptr(xc), nat.dcode(xc), nat.ptr(dc),
-                nat.dcode(dc) if dc is not None else 0, nat.ptr(rs), rs.numel() if rs is not None else 0, nat.ptr(w),
-                float(eps), R, C, nat.ptr(s), nat.ptr(rstd), nat.ptr(y), nat.dcode(y) if y is not None else 0,
-                nat.ptr(q), nat.ptr(scale))
+        y = torch.empty_like(xc, dtype=out_dtype)
+        yptr, ydt = y.data_ptr(), _CODE[out_dtype]
+    nat.call_on(dev, "affb_rms_norm_fwd", xc.data_ptr(), _CODE[xc.dtype], dptr, ddt, rptr, groups, w.data_ptr(),
+                float(eps), R, C, sptr, kptr, yptr, ydt, qptr, cptr)
     return xc, rs, w, s, rstd, y, q, scale
 
 
@@ -122,7 +137,8 @@ def fused_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, del
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in _FLOATS:
         raise RuntimeError(f"rms_norm: unsupported output dtype {out_dtype}")
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, delta))):
+    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                         or (delta is not None and delta.requires_grad))):
         _, _, _, s, _, y, _, _ = _launch(x, delta, row_scale, weight, eps, out_dtype, False)
         return y if s is None else (s, y)
     return FusedRMSNormFunction.apply(x, weight, delta, row_scale, eps, out_dtype)
