@@ -108,33 +108,33 @@ template <typename P, int AXES, bool BY_OFFSET>
 struct EntryOf {
   const BucketArgs& a;
   const uint8_t* lut;
-  int last, high, my, add;
+  int last, high;       // offsets are cut off to [-last, high]
+  int mx, my, add;      // entry = mx x + my y + add
 
   __device__ __forceinline__ EntryOf(const BucketArgs& args, const uint8_t* l) : a(args), lut(l) {
     last = a.lut - 1;
     high = a.one_sided ? 0 : last;
-    my = a.one_sided ? -a.span : a.span;
+    mx = a.one_sided ? -1 : 1;
+    my = AXES == 2 ? mx * a.span : 0;
     add = a.one_sided ? 0 : last * (AXES == 2 ? a.span + 1 : 1);
+    if (std::is_same<P, float>::value) add = (int)((uint32_t)add - 0x4B400000u * (uint32_t)(mx + my));
   }
-  // the cut-off offset
-  __device__ __forceinline__ int cut(P k, P q) const {
-    if constexpr (std::is_same<P, float>::value) {
-      // adding 1.5 * 2^23 rounds to an integer (ties to even) in the low mantissa bits
-      const float t = fminf(fmaxf(k - q, (float)-last), (float)high) + 12582912.f;
-      return __float_as_int(t) - 0x4B400000;
-    } else {
-      return max(-last, min(high, offset_of(k, q)));
-    }
+  // The cut-off offset; of fp32 positions plus 0x4B400000, which `add` takes
+  // out again: adding 1.5 * 2^23 rounds to an integer (ties to even) in the
+  // low mantissa bits.
+  __device__ __forceinline__ uint32_t cut(P k, P q) const {
+    if constexpr (std::is_same<P, float>::value)
+      return __float_as_uint(fminf(fmaxf(k - q, (float)-last), (float)high) + 12582912.f);
+    else
+      return (uint32_t)max(-last, min(high, offset_of(k, q)));
   }
   __device__ __forceinline__ int one(P k, P q) const {
-    if constexpr (BY_OFFSET) return (a.one_sided ? -cut(k, q) : cut(k, q)) + add;
+    if constexpr (BY_OFFSET) return (int)((uint32_t)mx * cut(k, q) + (uint32_t)add);
     return axis_index(a, lut, offset_of(k, q));
   }
   __device__ __forceinline__ int two(P kx, P ky, P qx, P qy) const {
-    if constexpr (BY_OFFSET) {
-      const int x = cut(kx, qx), y = cut(ky, qy);
-      return my * y + (a.one_sided ? -x : x) + add;
-    }
+    if constexpr (BY_OFFSET)
+      return (int)((uint32_t)my * cut(ky, qy) + ((uint32_t)mx * cut(kx, qx) + (uint32_t)add));
     return axis_index(a, lut, offset_of(ky, qy)) * a.per_axis + axis_index(a, lut, offset_of(kx, qx));
   }
 };
@@ -142,65 +142,56 @@ struct EntryOf {
 template <typename P> struct alignas(2 * sizeof(P)) Pos2 { P x, y; };
 
 // Entries of the pairs nm + u * STEP + j of batch element b (`none` where there
-// is no such pair or the list names no key).  PAIRS == 2: nm and M even.
-// Free of branches, so that the loads of all steps are in flight together.
+// is no such pair or the list names no key; Nk >= 1).  PAIRS == 2: nm and M
+// even.  Free of branches, so that the loads of all steps are in flight
+// together.
 template <typename P, int AXES, int PAIRS, bool BY_OFFSET>
 __device__ __forceinline__ void tile_entries(const BucketArgs& a, const EntryOf<P, AXES, BY_OFFSET>& entry, int b, int nm,
                                              int none, int (*e)[PAIRS]) {
   constexpr int STEP = BB_THREADS * PAIRS;
-  const P* qb = (const P*)a.q_pos + (int64_t)b * a.q_batch * AXES;
-  const P* kb = (const P*)a.k_pos + (int64_t)b * a.Nk * AXES;
-  int id[BB_STEPS][PAIRS], query[BB_STEPS];
+  using K = typename std::conditional<AXES == 2, Pos2<P>, P>::type;
+  const K* qb = (const K*)a.q_pos + (int64_t)b * a.q_batch;
+  const K* kb = (const K*)a.k_pos + (int64_t)b * a.Nk;
+  uint32_t id[BB_STEPS][PAIRS];
+  K q[BB_STEPS], k[BB_STEPS][PAIRS];
 #pragma unroll
   for (int u = 0; u < BB_STEPS; ++u) {
-    const int n = nm + u * STEP < a.NM ? nm + u * STEP : 0;
-    query[u] = query_of(a, n);
+    const bool in = nm + u * STEP < a.NM;
+    const int n = in ? nm + u * STEP : 0;
+    const int query = query_of(a, n);
     if (a.member) {
       const int* mp = a.member + (int64_t)b * a.batch_pairs + n;
       if constexpr (PAIRS == 2) {
-        const int2 w = __ldg(reinterpret_cast<const int2*>(mp));
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(mp));
         id[u][0] = w.x;
         id[u][1] = w.y;
       } else {
-        id[u][0] = __ldg(mp);
+        id[u][0] = (uint32_t)__ldg(mp);
+      }
+      if (!in) {
+#pragma unroll
+        for (int j = 0; j < PAIRS; ++j) id[u][j] = ~0u;
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < PAIRS; ++j) id[u][j] = n - query[u] * a.M + j;
+      for (int j = 0; j < PAIRS; ++j) id[u][j] = in ? (uint32_t)(n - query * a.M + j) : ~0u;
     }
+    q[u] = qb[query];
   }
-  if constexpr (AXES == 1) {
-    P q[BB_STEPS], k[BB_STEPS][PAIRS];
+  const uint32_t top = (uint32_t)a.Nk - 1;
 #pragma unroll
-    for (int u = 0; u < BB_STEPS; ++u) {
-      const P* qp = qb + query[u];
-      q[u] = __ldg(qp);
+  for (int u = 0; u < BB_STEPS; ++u)
 #pragma unroll
-      for (int j = 0; j < PAIRS; ++j) k[u][j] = __ldg((unsigned)id[u][j] < (unsigned)a.Nk ? kb + id[u][j] : qp);
+    for (int j = 0; j < PAIRS; ++j) k[u][j] = kb[min(id[u][j], top)];
+#pragma unroll
+  for (int u = 0; u < BB_STEPS; ++u)
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) {
+      int v;
+      if constexpr (AXES == 2) v = entry.two(k[u][j].x, k[u][j].y, q[u].x, q[u].y);
+      else v = entry.one(k[u][j], q[u]);
+      e[u][j] = id[u][j] <= top ? v : none;
     }
-#pragma unroll
-    for (int u = 0; u < BB_STEPS; ++u)
-#pragma unroll
-      for (int j = 0; j < PAIRS; ++j)
-        e[u][j] = (unsigned)id[u][j] < (unsigned)a.Nk && nm + u * STEP < a.NM ? entry.one(k[u][j], q[u]) : none;
-  } else {
-    Pos2<P> q[BB_STEPS], k[BB_STEPS][PAIRS];
-#pragma unroll
-    for (int u = 0; u < BB_STEPS; ++u) {
-      const Pos2<P>* qp = reinterpret_cast<const Pos2<P>*>(qb) + query[u];
-      q[u] = *qp;
-#pragma unroll
-      for (int j = 0; j < PAIRS; ++j)
-        k[u][j] = *((unsigned)id[u][j] < (unsigned)a.Nk ? reinterpret_cast<const Pos2<P>*>(kb) + id[u][j] : qp);
-    }
-#pragma unroll
-    for (int u = 0; u < BB_STEPS; ++u)
-#pragma unroll
-      for (int j = 0; j < PAIRS; ++j)
-        e[u][j] = (unsigned)id[u][j] < (unsigned)a.Nk && nm + u * STEP < a.NM
-                      ? entry.two(k[u][j].x, k[u][j].y, q[u].x, q[u].y)
-                      : none;
-  }
 }
 
 // Four heads of one table entry, in the output's type.
@@ -302,9 +293,10 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
   extern __shared__ unsigned char sm[];
   __shared__ float wmax[BB_HEADS][BB_THREADS / 32];
   const int none = a.rows;
-  float* acc = reinterpret_cast<float*>(sm);                            // [BB_HEADS][rows]
-  int* bins = reinterpret_cast<int*>(acc + BB_HEADS * a.rows);          // [BB_HEADS][rows]
-  float* raw = reinterpret_cast<float*>(bins + BB_HEADS * a.rows);      // [TILE] values, only of an odd tile
+  const int stride = a.rows + 1;  // a bin more for pairs that have no row
+  float* acc = reinterpret_cast<float*>(sm);                            // [BB_HEADS][stride]
+  int* bins = reinterpret_cast<int*>(acc + BB_HEADS * stride);          // [BB_HEADS][stride]
+  float* raw = reinterpret_cast<float*>(bins + BB_HEADS * stride);      // [TILE] values, only of an odd tile
   uint16_t* raw_row = reinterpret_cast<uint16_t*>(raw + TILE);          // [TILE]
   // BY_OFFSET: the row of every combined clipped offset, and `none` last
   const int offsets = AXES == 2 ? a.span * a.span : a.span;
@@ -327,10 +319,12 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
     }
   }
   float* mine = part + ((int64_t)blockIdx.x * a.H + h0) * a.rows;
-  for (int i = threadIdx.x; i < BB_HEADS * a.rows; i += BB_THREADS) {
-    acc[i] = resume && i < nh * a.rows ? mine[i] : 0.f;  // of the launch before (more than 2^31 pairs)
-    bins[i] = 0;
-  }
+  for (int h = 0; h < BB_HEADS; ++h)
+    for (int i = threadIdx.x; i < stride; i += BB_THREADS) {
+      // what the launch before (of more than 2^31 pairs) has summed
+      acc[h * stride + i] = resume && h < nh && i < a.rows ? mine[h * a.rows + i] : 0.f;
+      bins[h * stride + i] = 0;
+    }
   __syncthreads();
   const EntryOf<P, AXES, BY_OFFSET> entry(a, lut);
   const uint32_t per = ((uint32_t)a.NM + TILE - 1) / TILE;
@@ -339,12 +333,15 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
     const int b = total < (1ll << 31) ? (int)((uint32_t)t / per) : (int)(t / per);
     const int nm = (int)(t - (int64_t)b * per) * TILE + threadIdx.x * PAIRS;
     float g[BB_HEADS][PER];
+    const T* p0 = dout + ((int64_t)b * a.H + h0) * a.batch_pairs + nm;
 #pragma unroll
     for (int h = 0; h < BB_HEADS; ++h) {
-      const T* p = dout + ((int64_t)b * a.H + h0 + h) * a.batch_pairs + nm;
+      if (h >= nh) break;
+      const T* p = p0 + h * a.batch_pairs;
+      float top = 0.f;
 #pragma unroll
       for (int u = 0; u < BB_STEPS; ++u) {
-        const bool in = h < nh && nm + u * STEP < a.NM;
+        const bool in = nm + u * STEP < a.NM;
         if constexpr (PAIRS == 2 && sizeof(T) == 2) {
           const uint32_t w = in ? __ldg(reinterpret_cast<const uint32_t*>(p + u * STEP)) : 0u;
           g[h][2 * u] = ldf(reinterpret_cast<const T*>(&w));
@@ -357,6 +354,11 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
           g[h][u] = in ? ldf(p + u * STEP) : 0.f;
         }
       }
+#pragma unroll
+      for (int j = 0; j < PER; ++j) top = bb_max_nan(top, fabsf(g[h][j]));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = bb_max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (lane == 0) wmax[h][warp] = top;
     }
     int row[PER];
     tile_entries<P, AXES, PAIRS, BY_OFFSET>(a, entry, b, nm, BY_OFFSET ? offsets : none,
@@ -364,16 +366,6 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
     if (BY_OFFSET) {
 #pragma unroll
       for (int j = 0; j < PER; ++j) row[j] = rows[row[j]];
-    }
-#pragma unroll
-    for (int h = 0; h < BB_HEADS; ++h) {
-      if (h >= nh) break;
-      float top = 0.f;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) top = bb_max_nan(top, row[j] != none ? fabsf(g[h][j]) : 0.f);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = bb_max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (lane == 0) wmax[h][warp] = top;
     }
     __syncthreads();
     float down[BB_HEADS];  // 2^-(t / 2) of the scale 2^t, 0: nothing to add
@@ -389,30 +381,34 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
       if (!isfinite(top)) {
         odd = true;
       } else if (top > 0.f) {
-        // top < 2^e: values times 2^(BITS - e) stay below 2^BITS.  The power is
-        // applied in two halves, as it may itself pass the range of fp32.
+        // top < 2^e: values times 2^t = 2^(BITS - e) stay below 2^BITS, and are
+        // rounded to integers by adding 1.5 * 2^23.  The power is taken in two
+        // halves where it may itself pass the range of fp32.
         const int t = BB_BITS - (((__float_as_int(top) >> 23) & 255) - 126), t1 = t / 2;
         const float up = __int_as_float((127 + t1) << 23), up2 = __int_as_float((127 + t - t1) << 23);
         down[h] = __int_as_float((127 - t1) << 23);
         rest[h] = __int_as_float((127 - t + t1) << 23);
+        int* bin = bins + h * stride;
+        if (t > -120 && t < 120) {
+          const float whole = up * up2;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          // rounded to an integer by adding 1.5 * 2^23
-          const int q = __float_as_int(fmaf(g[h][j] * up, up2, 12582912.f)) - 0x4B400000;
-          if (row[j] != none) atomicAdd(bins + h * a.rows + row[j], q);
+          for (int j = 0; j < PER; ++j)
+            atomicAdd(bin + row[j], __float_as_int(fmaf(g[h][j], whole, 12582912.f)) - 0x4B400000);
+        } else {
+#pragma unroll
+          for (int j = 0; j < PER; ++j)
+            atomicAdd(bin + row[j], __float_as_int(fmaf(g[h][j] * up, up2, 12582912.f)) - 0x4B400000);
         }
       }
     }
     __syncthreads();
+    for (int i = threadIdx.x; i <= a.rows; i += BB_THREADS) {
 #pragma unroll
-    for (int h = 0; h < BB_HEADS; ++h) {
-      if (down[h] != 0.f) {
-        for (int i = threadIdx.x; i < a.rows; i += BB_THREADS) {
-          const int s = bins[h * a.rows + i];
-          if (s != 0) {
-            acc[h * a.rows + i] += (float)s * down[h] * rest[h];
-            bins[h * a.rows + i] = 0;
-          }
+      for (int h = 0; h < BB_HEADS; ++h) {
+        if (down[h] != 0.f) {
+          const int v = bins[h * stride + i];
+          bins[h * stride + i] = 0;
+          acc[h * stride + i] += (float)v * down[h] * rest[h];
         }
       }
     }
@@ -431,13 +427,14 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
           __syncthreads();
           for (int i = threadIdx.x; i < a.rows; i += BB_THREADS)
             for (int j = 0; j < TILE; ++j)
-              if (raw_row[j] == i) acc[h * a.rows + i] += raw[j];
+              if (raw_row[j] == i) acc[h * stride + i] += raw[j];
         }
       }
     }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < nh * a.rows; i += BB_THREADS) mine[i] = acc[i];
+  for (int h = 0; h < nh; ++h)
+    for (int i = threadIdx.x; i < a.rows; i += BB_THREADS) mine[h * a.rows + i] = acc[h * stride + i];
 }
 
 // dtable[row, h] = sum over blocks of part[block][h][row], in a fixed order:
@@ -509,7 +506,7 @@ static int bucket_args(const int32_t* edges, int n_edges, int one_sided, const v
   while ((1ll << l) < M) ++l;
   a->div_shift = l;
   if (M >= 1) a->div_mul = (uint32_t)(((1ull << 32) * ((1ull << l) - (uint64_t)M)) / (uint64_t)M + 1);
-  if (B * a->batch_pairs > 0) AFFB_REQUIRE(q_pos && k_pos, "bucket_bias: null positions");
+  if (B * a->batch_pairs > 0 && Nk > 0) AFFB_REQUIRE(q_pos && k_pos, "bucket_bias: null positions");
   const uintptr_t pair = pos_type == AFFB_POS_I64 ? 16 : 8;
   AFFB_REQUIRE(axes == 1 || (((uintptr_t)q_pos | (uintptr_t)k_pos) & (pair - 1)) == 0,
                "bucket_bias: positions of two axes must be aligned to a pair of coordinates");
@@ -577,7 +574,7 @@ static cudaError_t bucket_bwd_launch(const BucketArgs& a, const void* dout, floa
                                      cudaStream_t st) {
   const int64_t offsets = bb_offsets(a, 2, 16 * 1024, blocks);
   const int tile = BB_THREADS * PAIRS * BB_STEPS;
-  const int smem = 2 * BB_HEADS * a.rows * 4 + tile * 6 + (offsets ? (int)((offsets + 2) & ~1) * 2 : 0) + a.lut;
+  const int smem = 2 * BB_HEADS * (a.rows + 1) * 4 + tile * 6 + (offsets ? (int)((offsets + 2) & ~1) * 2 : 0) + a.lut;
   auto* k = offsets ? bucket_bwd_kernel<T, P, AXES, PAIRS, true> : bucket_bwd_kernel<T, P, AXES, PAIRS, false>;
   if (smem > 47 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -611,6 +608,8 @@ extern "C" int affb_bucket_bias_fwd(const void* table, int table_dtype, const in
   AFFB_REQUIRE(table && out, "bucket_bias: null pointer");
   const bool two = bb_two(a, out, out_dtype == AFFB_F32 ? 4 : 2);
   cudaStream_t st = as_stream(stream);
+  if (Nk == 0)  // lists that can only name keys that are not there
+    return bb_status(cudaMemsetAsync(out, 0, (size_t)(B * H * a.batch_pairs * (out_dtype == AFFB_F32 ? 4 : 2)), st));
   cudaError_t e = cudaSuccess;
   AFFB_DISPATCH(table_dtype, TB, {
     AFFB_DISPATCH(out_dtype, T, {
@@ -649,7 +648,7 @@ extern "C" int affb_bucket_bias_bwd(const void* dout, int dout_dtype, const int3
   cudaStream_t st = as_stream(stream);
   const int64_t n = (int64_t)a.rows * H;
   int64_t blocks = 0;
-  if (B * a.batch_pairs > 0) {
+  if (B * a.batch_pairs > 0 && Nk > 0) {
     AFFB_REQUIRE(dout, "bucket_bias: null pointer");
     blocks = bucket_bwd_blocks(B, H, a.batch_pairs);
     AFFB_REQUIRE(workspace && workspace_bytes >= blocks * n * 4, "bucket_bias: workspace too small");

@@ -634,3 +634,25 @@ def test_refusals_of_shapes_and_types(cuda):
     (g,) = torch.autograd.grad(fused_linear(xg, w, act="gelu").sum(), xg, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_bucket_bias_nan_positions_and_no_keys(cuda):
+    """A NaN position counts as the farthest key before the query, by either way of finding buckets; lists without
+    any key give a bias of zero and no gradient."""
+    edges = (1, 2, 5)
+    pos = torch.arange(16, device=cuda).float().view(1, 16, 1).clone()
+    kp = pos.clone()
+    kp[0, 3] = float("nan")
+    for one in (False, True):
+        rows = bucket_count(edges, 1, one)
+        table = rnd(cuda, 95, rows, 2)
+        far = rows - 1 if one else 0
+        small = bucket_bias(table, edges, pos, kp, None, one)                       # few pairs: buckets looked up
+        many = bucket_bias(table, edges, pos.expand(64, -1, -1), kp.expand(64, -1, -1), None, one)  # by offset
+        assert torch.equal(small[0, :, 5, 3], table[far]) and torch.equal(many[9], small[0])
+    member = torch.randint(-1, 3, (1, 16, 8), device=cuda)
+    table = rnd(cuda, 96, 7, 2).requires_grad_(True)
+    bias = bucket_bias(table, edges, pos, pos[:, :0], member)
+    assert not bias.any()
+    assert not torch.autograd.grad(bias.sum(), table)[0].any()
