@@ -58,8 +58,9 @@ struct GemmArgs {
   int a_mn, b_mn, f8;
   int a_blocks, b_blocks;  // MN-major: one load of that many 64-column blocks (0: a load each)
   int b_bytes;       // a block's part of B
-  uint32_t idesc;
+  uint32_t idesc;    // without the width
   int direct;        // outputs not addressable by TMA: plain stores
+  int res_rows;      // rows of the residual are 16-byte aligned
   int bufs;          // staging buffers of a warp: out, and z where it is wanted
   LinearEpilogue e;
 };
@@ -80,6 +81,12 @@ struct Units {
     ni = t - mi * p.nt;
     step_m = step / p.nt;
     step_n = step - step_m * p.nt;
+  }
+  // Columns multiplied: the last tile's are rounded up to 32 (unless B comes in
+  // blocks of 64, which a narrower tile would not begin at).
+  __device__ __forceinline__ int width(const GemmArgs& p) const {
+    const int left = (p.N - ni * p.bn + 31) & ~31;
+    return p.b_blocks || left > p.bn ? p.bn : left;
   }
   __device__ __forceinline__ bool more(const GemmArgs& p) const { return s < p.splits; }
   __device__ __forceinline__ void next(const GemmArgs& p) {
@@ -118,27 +125,54 @@ __device__ __forceinline__ void stage_row(unsigned char* buf, int lane, int half
       st8(reinterpret_cast<T*>(buf + lane * 128 + (((4 * half + j) ^ (lane & 7)) << 4)), v + 8 * j);
   }
 }
+// Plain accesses where TMA cannot address the rows (their pitch or start is
+// not a multiple of 16 bytes): the warp goes through a staging buffer, so that
+// its lanes write or read neighbouring columns of one row after the other.
 template <typename T>
-__device__ __forceinline__ void store_row(T* p, int n, const float* v) {
-#pragma unroll
-  for (int i = 0; i < CHUNK; ++i)
-    if (i < n) stf(p + i, v[i]);
+__device__ __forceinline__ void store_rows(unsigned char* buf, int lane, const float* v, T* p, int64_t ld, int rows,
+                                           int n) {
+  stage_row<T>(buf, lane, 0, v);
+  __syncwarp();
+  constexpr int PER = 16 / sizeof(T);
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r)
+    if (lane < n)
+      p[r * ld + lane] = *reinterpret_cast<const T*>(buf + r * 128 + (((lane / PER) ^ (r & 7)) << 4) +
+                                                     (lane % PER) * sizeof(T));
+  __syncwarp();
 }
-// 32 columns of a row of the residual added to v (n valid).
+__device__ __forceinline__ float load_float(const void* p, int dtype, int64_t i) {
+  if (dtype == AFFB_F32) return ((const float*)p)[i];
+  if (dtype == AFFB_BF16) return __bfloat162float(((const __nv_bfloat16*)p)[i]);
+  return __half2float(((const __half*)p)[i]);
+}
+__device__ __forceinline__ void add_rows(unsigned char* buf, int lane, float* v, const void* p, int dtype, int64_t first,
+                                         int64_t ld, int rows, int n) {
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r)
+    if (lane < n)
+      *reinterpret_cast<float*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) =
+          load_float(p, dtype, first + r * ld + lane);
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float4 w = *reinterpret_cast<const float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4));
+    v[4 * j] += w.x;
+    v[4 * j + 1] += w.y;
+    v[4 * j + 2] += w.z;
+    v[4 * j + 3] += w.w;
+  }
+  __syncwarp();
+}
+// 32 columns of a row of the residual added to v, 16-byte aligned.
 template <typename T>
-__device__ __forceinline__ void add_row(const T* p, int n, float* v) {
-  if (n == CHUNK && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+__device__ __forceinline__ void add_row(const T* p, float* v) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float r[8];
-      ld8(p + 8 * j, r);
+  for (int j = 0; j < 4; ++j) {
+    float r[8];
+    ld8(p + 8 * j, r);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[8 * j + i] += r[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < CHUNK; ++i)
-      if (i < n) v[i] += ldf(p + i);
+    for (int i = 0; i < 8; ++i) v[8 * j + i] += r[i];
   }
 }
 
@@ -204,7 +238,7 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
     // both blocks' loads complete on the first block's barrier, where the products are issued
     const uint32_t full_at = CG == 2 ? peer_addr(full, 0) : full;
     for (Units u(p, first, step); u.more(p) && ok; u.next(p)) {
-      const int m0 = (u.mi * CG + (int)rank) * TILE_M, n0 = u.ni * p.bn + (int)rank * (p.bn / CG);
+      const int m0 = (u.mi * CG + (int)rank) * TILE_M, n0 = u.ni * p.bn + (int)rank * (u.width(p) / CG);
       const int kb0 = u.first_k(total_k, p), kb1 = u.last_k(total_k, p);
       int part = p.parts > 1 ? kb0 / p.kblocks : 0;
       int kk = kb0 - part * p.kblocks;
@@ -262,6 +296,7 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
       const uint64_t db0 = smem_desc(base + A_BYTES, p.b_mn ? 8192 : 0, 1024);
       for (Units u(p, first, step); u.more(p) && ok; u.next(p)) {
         const int n_k = u.last_k(total_k, p) - u.first_k(total_k, p);
+        const uint32_t idesc = p.idesc | ((uint32_t)u.width(p) >> 3 << 17);
         if (!(ok = warp_wait(acc_empty + 8 * acc, acc_phase, failed))) break;
         fence_after();
         const uint32_t d = tmem + acc * 256;
@@ -270,8 +305,8 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
           fence_after();
           const uint64_t off = (uint64_t)((uint32_t)(st * stage_bytes) >> 4);
           if (leads) {
-            if (p.f8) mma_block<CG, true>(d, da0 + off, db0 + off, sa, sb, p.idesc, kb > 0);
-            else mma_block<CG, false>(d, da0 + off, db0 + off, sa, sb, p.idesc, kb > 0);
+            if (p.f8) mma_block<CG, true>(d, da0 + off, db0 + off, sa, sb, idesc, kb > 0);
+            else mma_block<CG, false>(d, da0 + off, db0 + off, sa, sb, idesc, kb > 0);
             mma_commit<CG>(empty + 8 * st);
           }
           if (++st == p.stages) {
@@ -362,7 +397,9 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
           }
         }
         const int n = min(CHUNK, ncols - c);
-        const int64_t off = ((int64_t)s * p.M + m) * p.N + n0 + c;
+        // first element of the warp's rows, and how many there are
+        const int64_t off = ((int64_t)s * p.M + m0) * p.N + n0 + c;
+        const int rows = min(WARP_ROWS, p.M - m0);
         // the buffers' last stores have been read (those of the tile before, or of fp32's first half)
         if (!p.direct && (h == 0 || sizeof(TO) == 4 || (p.e.z && z_bytes == 4))) {
           if (lane == 0) store_wait_read<0>();
@@ -370,11 +407,9 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
         }
         if (p.e.z) {
           if (p.direct) {
-            if (m < p.M) {
-              if (p.e.z_dtype == AFFB_F32) store_row((float*)p.e.z + off, n, v);
-              else if (p.e.z_dtype == AFFB_BF16) store_row((__nv_bfloat16*)p.e.z + off, n, v);
-              else store_row((__half*)p.e.z + off, n, v);
-            }
+            if (p.e.z_dtype == AFFB_F32) store_rows(buf, lane, v, (float*)p.e.z + off, p.N, rows, n);
+            else if (p.e.z_dtype == AFFB_BF16) store_rows(buf, lane, v, (__nv_bfloat16*)p.e.z + off, p.N, rows, n);
+            else store_rows(buf, lane, v, (__half*)p.e.z + off, p.N, rows, n);
           } else {
             if (p.e.z_dtype == AFFB_F32) stage_row<float>(zbuf, lane, h, v);
             else if (p.e.z_dtype == AFFB_BF16) stage_row<__nv_bfloat16>(zbuf, lane, h, v);
@@ -383,13 +418,24 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 2) activate_pair<ACT>(v[i], v[i + 1]);
-        if (p.e.residual && m < p.M) {
-          if (p.e.residual_dtype == AFFB_F32) add_row((const float*)p.e.residual + off, n, v);
-          else if (p.e.residual_dtype == AFFB_BF16) add_row((const __nv_bfloat16*)p.e.residual + off, n, v);
-          else add_row((const __half*)p.e.residual + off, n, v);
+        if (p.e.residual) {
+          if (p.direct || !p.res_rows || n < CHUNK) {
+            if (p.direct) {
+              add_rows(buf, lane, v, p.e.residual, p.e.residual_dtype, off, p.N, rows, n);
+            } else if (m < p.M) {
+#pragma unroll
+              for (int i = 0; i < CHUNK; ++i)
+                if (i < n) v[i] += load_float(p.e.residual, p.e.residual_dtype, off + (int64_t)lane * p.N + i);
+            }
+          } else if (m < p.M) {
+            const int64_t o = off + (int64_t)lane * p.N;
+            if (p.e.residual_dtype == AFFB_F32) add_row((const float*)p.e.residual + o, v);
+            else if (p.e.residual_dtype == AFFB_BF16) add_row((const __nv_bfloat16*)p.e.residual + o, v);
+            else add_row((const __half*)p.e.residual + o, v);
+          }
         }
         if (p.direct) {
-          if (m < p.M) store_row((TO*)p.e.out + off, n, v);
+          store_rows(buf, lane, v, (TO*)p.e.out + off, p.N, rows, n);
         } else {
           stage_row<TO>(buf, lane, h, v);
           const bool last = c + CHUNK >= ncols;
@@ -575,7 +621,7 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
   // blocks of 64 columns in one load where no block runs past its row, and the tiles begin at a block
   p.a_blocks = a.mn && a.cols % 64 == 0 ? TILE_M / 64 : 0;
   p.b_blocks = b.mn && b.cols % 64 == 0 && half_n % 64 == 0 ? half_n / 64 : 0;
-  p.idesc = instr_desc(et == AFFB_BF16 ? 1 : 0, a.mn, b.mn, (uint32_t)(TILE_M * s.cg), (uint32_t)s.bn);
+  p.idesc = instr_desc(et == AFFB_BF16 ? 1 : 0, a.mn, b.mn, (uint32_t)(TILE_M * s.cg), 0);  // n: each tile's own
   LinearEpilogue full = e;
   if (s.splits > 1) {
     e = LinearEpilogue{};
@@ -586,6 +632,7 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
   p.e = e;
   p.direct = s.splits > 1 ? 0
                           : !(tma_rows(e.out, e.out_dtype, N) && (!e.z || tma_rows(e.z, e.z_dtype, N)));
+  p.res_rows = e.residual && tma_rows(e.residual, e.residual_dtype, p.N);
   p.bufs = e.z ? 2 : 1;
   const int stage = A_BYTES + p.b_bytes;
   const int fixed = 1024 + EPI_WARPS * p.bufs * BUF_BYTES + COLS_BYTES + BAR_BYTES;

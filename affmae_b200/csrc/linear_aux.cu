@@ -9,19 +9,19 @@
 namespace affb {
 
 // ------------------------------------------------------------------ pack --
+// A warp a row, lanes over its columns.
 template <typename U>
 __global__ void __launch_bounds__(256) pack_rows_kernel(const U* __restrict__ src, int64_t R, int64_t C,
                                                         U* __restrict__ dst, int64_t ld) {
-  const int64_t n = R * C;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / C;
-    dst[r * ld + (i - r * C)] = src[i];
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < R; r += (int64_t)gridDim.x * 8) {
+#pragma unroll 4
+    for (int64_t c = threadIdx.x & 31; c < C; c += 32) dst[r * ld + c] = src[r * C + c];
   }
 }
 
 int linear_pack(const void* src, int64_t elem, int64_t R, int64_t C, void* dst, int64_t ld, cudaStream_t st) {
   if (R * C == 0) return AFFB_OK;
-  const unsigned blocks = (unsigned)imin64((R * C + 255) / 256, (int64_t)sm_count() * 16);
+  const unsigned blocks = (unsigned)imin64((R + 7) / 8, (int64_t)sm_count() * 16);
   if (elem == 1) pack_rows_kernel<uint8_t><<<blocks, 256, 0, st>>>((const uint8_t*)src, R, C, (uint8_t*)dst, ld);
   else pack_rows_kernel<uint16_t><<<blocks, 256, 0, st>>>((const uint16_t*)src, R, C, (uint16_t*)dst, ld);
   AFFB_LAUNCH_CHECK("linear: pack");
@@ -40,21 +40,28 @@ __device__ __forceinline__ void split3(float v, __nv_bfloat16* o) {
   o[2] = __float2bfloat16_rn(isfinite(r1) ? r1 - __bfloat162float(o[1]) : 0.f);
 }
 
+// A warp a row; a lane takes two columns, so that the parts are written in
+// words (rows of the parts are 16-byte aligned).
 __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, int64_t R, int64_t C,
                                                          __nv_bfloat16* __restrict__ dst, int64_t ld) {
-  const int64_t n = R * C, part = R * ld;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / C, o = r * ld + (i - r * C);
-    __nv_bfloat16 p[3];
-    split3(src[i], p);
+  const int64_t part = R * ld;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < R; r += (int64_t)gridDim.x * 8) {
+    const float* s = src + r * C;
+    __nv_bfloat16* d = dst + r * ld;
+#pragma unroll 4
+    for (int64_t c = (threadIdx.x & 31) * 2; c < C; c += 64) {
+      __nv_bfloat16 a[3], b[3];
+      split3(s[c], a);
+      split3(c + 1 < C ? s[c + 1] : 0.f, b);
 #pragma unroll
-    for (int k = 0; k < 3; ++k) dst[o + k * part] = p[k];
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<__nv_bfloat162*>(d + c + k * part) = __nv_bfloat162(a[k], b[k]);
+    }
   }
 }
 
 int linear_split(const float* src, int64_t R, int64_t C, void* dst, int64_t ld, cudaStream_t st) {
   if (R * C == 0) return AFFB_OK;
-  const unsigned blocks = (unsigned)imin64((R * C + 255) / 256, (int64_t)sm_count() * 16);
+  const unsigned blocks = (unsigned)imin64((R + 7) / 8, (int64_t)sm_count() * 16);
   split_rows_kernel<<<blocks, 256, 0, st>>>(src, R, C, (__nv_bfloat16*)dst, ld);
   AFFB_LAUNCH_CHECK("linear: split");
   return AFFB_OK;
