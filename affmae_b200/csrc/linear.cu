@@ -44,7 +44,7 @@ constexpr int WARP_ROWS = 32;        // a warp's part of a tile: 32 rows x 64 co
 constexpr int WARP_COLS = 64;
 constexpr int CHUNK = 32;            // worked on at a time
 constexpr int BUF_BYTES = WARP_ROWS * 128;  // staged rows of 128 bytes: 64 columns of 16 bits or 32 of fp32
-constexpr int BAR_BYTES = 256;
+constexpr int BAR_BYTES = 512;
 constexpr int COLS_BYTES = EPI_WARPS * 2 * WARP_COLS * 4;  // each epilogue warp's bias and column scales
 
 // Set when a block's waits ran out; read by affb_linear_status.
@@ -61,6 +61,7 @@ struct GemmArgs {
   uint32_t idesc;    // without the width
   int direct;        // outputs not addressable by TMA: plain stores
   int res_rows;      // rows of the residual are 16-byte aligned
+  int res_tma;       // the residual is brought into the second staging buffer while the products run
   int bufs;          // staging buffers of a warp: out, and z where it is wanted
   LinearEpilogue e;
 };
@@ -164,6 +165,28 @@ __device__ __forceinline__ void add_rows(unsigned char* buf, int lane, float* v,
   }
   __syncwarp();
 }
+// stage_row's counterpart: 32 columns of a staged row added to v.
+template <typename T>
+__device__ __forceinline__ void add_staged(const unsigned char* buf, int lane, int half, float* v) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float4 w = *reinterpret_cast<const float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4));
+      v[4 * j] += w.x;
+      v[4 * j + 1] += w.y;
+      v[4 * j + 2] += w.z;
+      v[4 * j + 3] += w.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float w[8];
+      ld8_shared(reinterpret_cast<const T*>(buf + lane * 128 + (((4 * half + j) ^ (lane & 7)) << 4)), w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[8 * j + i] += w[i];
+    }
+  }
+}
 // 32 columns of a row of the residual added to v, 16-byte aligned.
 template <typename T>
 __device__ __forceinline__ void add_row(const T* p, float* v) {
@@ -188,8 +211,8 @@ __device__ __forceinline__ void mma_block(uint32_t d, uint64_t a, uint64_t b, ui
 template <typename TO, int ACT, int CG>
 __global__ void __launch_bounds__(LIN_THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_z,
-                const __grid_constant__ GemmArgs p) {
+                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_2,
+                const __grid_constant__ GemmArgs p) {  // map_2: z, or the residual
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const int stage_bytes = A_BYTES + p.b_bytes;
@@ -213,6 +236,7 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
       bar_init(acc_empty + 8 * i, EPI_WARPS * CG);
     }
     bar_init(drain, 1);
+    for (int i = 0; i < EPI_WARPS; ++i) bar_init(full + 256 + 8 * i, 1);
     bar_init_fence();
     *failed = 0;
     tma_prefetch(&map_a);
@@ -337,6 +361,14 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
     };
     unsigned char* buf = staging + ew * p.bufs * BUF_BYTES;
     unsigned char* zbuf = buf + BUF_BYTES;
+    const uint32_t res_bar = full + 256 + 8 * ew;
+    uint32_t res_phase = 0;
+    const auto fetch_residual = [&](int n, int m) {  // one box: 32 rows of 128 bytes
+      if (lane == 0) {
+        bar_expect(res_bar, BUF_BYTES);
+        tma_load<1>(smem_addr(zbuf), &map_2, n, m, 0, res_bar);
+      }
+    };
     float* bias = cols + ew * 2 * WARP_COLS;
     const bool per_col = p.e.bias || p.e.col_scale;
     const int z_bytes = p.e.z_dtype == AFFB_F32 ? 4 : 2;
@@ -365,6 +397,7 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
         }
         __syncwarp();
       }
+      if (p.res_tma && ncols > 0) fetch_residual(n0, m0);
       const float rs = (p.e.row_scale && m < p.M) ? p.e.row_scale[m] : 1.f;
       // all lanes of the warp leave together
       if (!warp_wait(acc_full + 8 * acc, acc_phase, failed)) break;
@@ -418,7 +451,23 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 2) activate_pair<ACT>(v[i], v[i + 1]);
-        if (p.e.residual) {
+        if (p.res_tma) {
+          const bool wide = p.e.residual_dtype == AFFB_F32;
+          if (h == 0 || wide) {
+            if (!warp_wait(res_bar, res_phase, failed)) break;
+            res_phase ^= 1;
+          }
+          if (wide) {
+            add_staged<float>(zbuf, lane, h, v);
+            __syncwarp();
+            if (h == 0 && CHUNK < ncols) fetch_residual(n0 + CHUNK, m0);
+          } else if (p.e.residual_dtype == AFFB_BF16) {
+            add_staged<__nv_bfloat16>(zbuf, lane, h, v);
+          } else {
+            add_staged<__half>(zbuf, lane, h, v);
+          }
+          if (!wide) __syncwarp();
+        } else if (p.e.residual) {
           if (p.direct || !p.res_rows || n < CHUNK) {
             if (p.direct) {
               add_rows(buf, lane, v, p.e.residual, p.e.residual_dtype, off, p.N, rows, n);
@@ -445,7 +494,7 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
             __syncwarp();
             if (lane == 0) {
               if (out_now) tma_store(&map_out, smem_addr(buf), n0 + (sizeof(TO) == 4 ? c : 0), m0, s);
-              if (z_now) tma_store(&map_z, smem_addr(zbuf), n0 + (z_bytes == 4 ? c : 0), m0, s);
+              if (z_now) tma_store(&map_2, smem_addr(zbuf), n0 + (z_bytes == 4 ? c : 0), m0, s);
               store_commit();
             }
           }
@@ -455,6 +504,7 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
       if (acc == 0) acc_phase ^= 1;
     }
     if (lane == 0) store_wait_all();
+    if (p.res_tma && *failed) settle();  // a residual on its way
     __syncwarp();
   }
   fence_before();
@@ -633,7 +683,8 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
   p.direct = s.splits > 1 ? 0
                           : !(tma_rows(e.out, e.out_dtype, N) && (!e.z || tma_rows(e.z, e.z_dtype, N)));
   p.res_rows = e.residual && tma_rows(e.residual, e.residual_dtype, p.N);
-  p.bufs = e.z ? 2 : 1;
+  p.res_tma = p.res_rows && !e.z && !p.direct;
+  p.bufs = e.z || p.res_tma ? 2 : 1;
   const int stage = A_BYTES + p.b_bytes;
   const int fixed = 1024 + EPI_WARPS * p.bufs * BUF_BYTES + COLS_BYTES + BAR_BYTES;
   p.stages = (SMEM_MAX - fixed) / stage;
@@ -657,6 +708,9 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
       return rc;
     if (e.z && (rc = make_map(&mz, e.z_dtype, e.z, p.N, M, 1, p.N, cols(e.z_dtype), WARP_ROWS,
                               CU_TENSOR_MAP_SWIZZLE_128B)))
+      return rc;
+    if (p.res_tma && (rc = make_map(&mz, e.residual_dtype, e.residual, p.N, M, 1, p.N, cols(e.residual_dtype), WARP_ROWS,
+                                    CU_TENSOR_MAP_SWIZZLE_128B)))
       return rc;
   }
   const void* k = s.cg == 2 ? kernel_of<2>(e.out_dtype, e.act) : kernel_of<1>(e.out_dtype, e.act);
@@ -731,7 +785,7 @@ static int check_sizes(int64_t M, int64_t N, int64_t K) {
 
 static int forward(const void* x, const void* w, int dtype, int64_t M, int64_t N, int64_t K, const LinearEpilogue& e,
                    void* workspace, int64_t workspace_bytes, cudaStream_t st) {
-  if (M <= SMALL_ROWS) return linear_small(x, w, dtype, M, N, K, e, st);
+  if (M <= small_rows(dtype)) return linear_small(x, w, dtype, M, N, K, e, st);
   Arena ws{(unsigned char*)workspace, 0, workspace ? workspace_bytes : 0};
   Operand a, b;
   int rc;
@@ -758,7 +812,7 @@ extern "C" int affb_linear_status(int* failed) {
 }
 
 extern "C" int64_t affb_linear_fwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
-  if (M <= SMALL_ROWS || N < 1 || K < 1) return 0;
+  if (M <= small_rows(dtype) || N < 1 || K < 1) return 0;
   return copy_bytes(dtype, M, K, false) + copy_bytes(dtype, N, K, false) + partial_bytes(M, N, k_blocks(dtype, K));
 }
 

@@ -29,8 +29,11 @@ struct LinearEpilogue {
   int z_dtype;
 };
 
-// linear_small.cu: out = epilogue(x w^T) for M <= SMALL_ROWS rows, one launch.
-constexpr int SMALL_ROWS = 8;
+// linear_small.cu: out = epilogue(x w^T) for M <= small_rows(dtype) <= 8 rows,
+// one launch.  K = 4096, N = 8192 against the tensor-core product: bf16 4 rows
+// 22 us (28), 8 rows 37 (28); e4m3 2 rows 11.5 (16), 4 rows 17.6 (16); fp32
+// (K = 1024, N = 4096) 8 rows 15 (35, six products of parts).
+inline int64_t small_rows(int dtype) { return dtype == AFFB_F32 ? 8 : dtype == AFFB_E4M3 ? 3 : 4; }
 int linear_small(const void* x, const void* w, int dtype, int64_t M, int64_t N, int64_t K, const LinearEpilogue& e,
                  cudaStream_t st);
 
