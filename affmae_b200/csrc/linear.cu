@@ -556,9 +556,13 @@ static int make_map(CUtensorMap* map, int dtype, const void* base, int64_t cols,
   }
   EncodeFn fn = encode_fn();
   AFFB_REQUIRE(fn, "linear: the driver has no tensor-map encoder");
-  const CUresult rc = fn(map, t, blocks ? 4 : 3, const_cast<void*>(base), dims, strides, box, step,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const auto encode = [&] {
+    return fn(map, t, blocks ? 4 : 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult rc = encode();
+  // a thread that has made no runtime call yet (autograd's, say) has no context; this call gives it one
+  if (rc == CUDA_ERROR_INVALID_CONTEXT && cudaFree(nullptr) == cudaSuccess) rc = encode();
   AFFB_REQUIRE(rc == CUDA_SUCCESS, "linear: tensor map refused (code %d)", (int)rc);
   return AFFB_OK;
 }

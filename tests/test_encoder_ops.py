@@ -98,6 +98,29 @@ def test_linear_forward_and_gradients(cuda, dtype, shape, act):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("shape", [(5000, 256, 192), (20011, 640, 448), (2000, 1024, 96), (900, 1032, 64),
+                                   (600, 384, 520)])
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+def test_linear_gradients_of_larger_layers(cuda, dtype, shape, act):
+    """Several tiles a block, blocks in pairs, and columns that do not fill the last tile."""
+    M, N, K = shape
+    x, w, b = rnd(cuda, 1, M, K, dtype=dtype), rnd(cuda, 2, N, K, std=K ** -0.5, dtype=dtype), rnd(cuda, 3, N, dtype=dtype)
+    dout = rnd(cuda, 4, M, N, dtype=dtype)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = fused_linear(*leaves, act=act)
+    grads = torch.autograd.grad(y, leaves, dout)
+    out, out_tol, dx, dx_tol, dw, dw_tol, db, db_tol = linear_ref(x, w, b, act, None, dout)
+    within(y, out, out_tol, "y")
+    within(grads[0], dx, dx_tol, "dx")
+    within(grads[1], dw, dw_tol, "dw")
+    within(grads[2], db, db_tol, "db")
+    again = torch.autograd.grad(fused_linear(*leaves, act=act), leaves, dout)
+    assert all(torch.equal(p, q) for p, q in zip(grads, again))
+    assert linear_status()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(4, 48, 32), (131, 200, 64), (140, 77, 33)])
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
 @pytest.mark.parametrize("types", [(BF16, BF16, BF16), (BF16, FP32, FP32), (FP16, FP32, FP16), (FP32, FP32, FP32),
@@ -218,6 +241,20 @@ def test_linear_on_a_side_stream_and_repeatable(cuda):
     torch.cuda.current_stream().wait_stream(s)
     for a, b_ in zip(got, want):
         assert torch.equal(a, b_)
+
+
+@pytest.mark.gpu
+def test_linear_as_a_threads_first_call(cuda):
+    """A thread that has made no CUDA call of its own yet (as autograd's have not) may begin with a product."""
+    import threading
+    x, w = rnd(cuda, 33, 256, 64, dtype=BF16), rnd(cuda, 34, 64, 64, dtype=BF16)
+    with torch.no_grad():
+        want = fused_linear(x, w)
+        got = []
+        t = threading.Thread(target=lambda: got.append(fused_linear(x, w)))
+        t.start()
+        t.join()
+    assert got and torch.equal(got[0], want)
 
 
 @pytest.mark.gpu
