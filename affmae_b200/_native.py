@@ -180,19 +180,17 @@ def stream(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """``call`` with `device` current (kernels launch on the current device)
-    and that device's current stream as the last argument."""
+def call_on(index: int, name: str, *args) -> None:
+    """``call`` with CUDA device `index` current (kernels launch on the current
+    device) and that device's current stream as the last argument."""
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return call_on(index, name, *args)
     global CALLS
-    index = device.index
-    if index == _current_device():
-        CALLS += 1
-        rc = getattr(_lib or lib(), name)(*args, _raw_stream(index))
-        if rc != 0:
-            raise RuntimeError(f"{name} failed (code {rc}): {lib().affb_last_error().decode(errors='replace')}")
-    else:
-        with torch.cuda.device(device):
-            call(name, *args, _raw_stream(torch.cuda.current_device()))
+    CALLS += 1
+    rc = getattr(_lib or lib(), name)(*args, _raw_stream(index))
+    if rc != 0:
+        raise RuntimeError(f"{name} failed (code {rc}): {lib().affb_last_error().decode(errors='replace')}")
 
 
 # the interpreter-level queries behind torch.cuda.current_device() / current_stream(), without their wrappers
@@ -202,15 +200,17 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", stream)
 
 
 @functools.lru_cache(maxsize=4096)
-def _size(name: str, *args) -> int:
-    return getattr(lib(), name)(*args)
+def _size(index: int, name: str, *args) -> int:
+    with torch.cuda.device(index):
+        return getattr(lib(), name)(*args)
 
 
-def workspace(name: str, device, *args):
-    """Uninitialised device memory of the size the library's function `name`
-    asks for (None where it needs none), from the current stream's pool."""
-    n = _size(name, *args)
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+def workspace(index: int, name: str, like, *args):
+    """Uninitialised memory on `like`'s device `index`, of the size the
+    library's function `name` asks for (None where it needs none), from the
+    current stream's pool."""
+    n = _size(index, name, *args)
+    return like.new_empty(n, dtype=torch.uint8) if n else None
 
 
 def require_cuda(*tensors) -> None:

@@ -66,9 +66,9 @@ def _edge_array(edges):
 
 def _check(table, edges, q_pos, k_pos, member_idx, one_sided, dtype) -> tuple[int, ...]:
     edges = _check_edges(edges)
-    qs, ks, dev, pt = q_pos.shape, k_pos.shape, table.device, q_pos.dtype
+    qs, ks, d, pt = q_pos.shape, k_pos.shape, table.get_device(), q_pos.dtype
     # the common case in a few comparisons; whatever else is looked at in order below
-    if dev.type == "cuda" and q_pos.device == dev and k_pos.device == dev and len(qs) == 3 and len(ks) == 3 \
+    if d >= 0 and q_pos.get_device() == d and k_pos.get_device() == d and len(qs) == 3 and len(ks) == 3 \
             and (qs[2] == 1 or (qs[2] == 2 and len(edges) <= 32)) and qs[2] == ks[2] and qs[0] == ks[0] and pt in _POS \
             and k_pos.dtype == pt and len(table.shape) == 2 and table.shape[0] == bucket_count(edges, qs[2], one_sided) \
             and table.dtype in _FLOATS and dtype in _FLOATS and member_idx is None:
@@ -112,9 +112,8 @@ def bucket_bias_fwd(table, edges, q_pos, k_pos, member_idx, one_sided, dtype):
     B, Nq, axes = q_pos.shape
     Nk, H = k_pos.shape[1], table.shape[1]
     M = member_idx.shape[2] if member_idx is not None else Nk
-    dev = table.device
     out = table.new_empty((B, H, Nq, M), dtype=dtype)
-    nat.call_on(dev, "affb_bucket_bias_fwd", nat.ptr(table), nat.dcode(table), ctypes.addressof(arr), len(edges),
+    nat.call_on(table.get_device(), "affb_bucket_bias_fwd", nat.ptr(table), nat.dcode(table), ctypes.addressof(arr), len(edges),
                 int(one_sided), nat.ptr(q_pos), nat.ptr(k_pos), _POS[q_pos.dtype], axes, nat.ptr(member_idx), B, H, Nq,
                 Nk, M, nat.ptr(out), nat.dcode(out))
     return out
@@ -125,10 +124,10 @@ def bucket_bias_bwd(dout, edges, q_pos, k_pos, member_idx, one_sided, dtype):
     arr = _edge_array(edges)
     B, Nq, axes = q_pos.shape
     _, H, _, M = dout.shape
-    dev = dout.device
-    dtable = torch.empty((bucket_count(edges, axes, one_sided), H), device=dev, dtype=dtype)
-    ws = nat.workspace("affb_bucket_bias_bwd_workspace_bytes", dev, len(edges), int(one_sided), axes, B, H, Nq, M)
-    nat.call_on(dev, "affb_bucket_bias_bwd", nat.ptr(dout), nat.dcode(dout), ctypes.addressof(arr), len(edges),
+    index = dout.get_device()
+    dtable = dout.new_empty((bucket_count(edges, axes, one_sided), H), dtype=dtype)
+    ws = nat.workspace(index, "affb_bucket_bias_bwd_workspace_bytes", dout, len(edges), int(one_sided), axes, B, H, Nq, M)
+    nat.call_on(index, "affb_bucket_bias_bwd", nat.ptr(dout), nat.dcode(dout), ctypes.addressof(arr), len(edges),
                 int(one_sided), nat.ptr(q_pos), nat.ptr(k_pos), _POS[q_pos.dtype], axes, nat.ptr(member_idx), B, H, Nq,
                 k_pos.shape[1], M, nat.ptr(dtable), nat.dcode(dtable), nat.ptr(ws), ws.numel() if ws is not None else 0)
     return dtable

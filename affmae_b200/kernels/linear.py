@@ -38,11 +38,12 @@ def _check(x, weight, bias, residual):
     """Shapes, devices and the bias's type (refuses in the order a caller would
     want to know).  The accepted case is decided by a few comparisons: a
     one-token call takes as long as its checks."""
-    xs, ws, dev = x.shape, weight.shape, x.device
-    if dev.type == "cuda" and len(ws) == 2 and xs and xs[-1] == ws[1] and ws[0] and ws[1] and weight.device == dev \
-            and (bias is None or (bias.shape == ws[:1] and bias.dtype in _FLOATS and bias.device == dev)) \
-            and (residual is None or (residual.shape[:-1] == xs[:-1] and len(residual.shape) == len(xs)
-                                      and residual.shape[-1] == ws[0] and residual.device == dev)):
+    xs, ws, d = x.shape, weight.shape, x.get_device()
+    if d >= 0 and len(ws) == 2 and xs and xs[-1] == ws[1] and ws[0] and ws[1] and weight.get_device() == d \
+            and (bias is None or (bias.get_device() == d and bias.dim() == 1 and bias.shape[0] == ws[0]
+                                  and bias.dtype in _FLOATS)) \
+            and (residual is None or (residual.get_device() == d and residual.dim() == len(xs)
+                                      and residual.shape[-1] == ws[0] and residual.shape[:-1] == xs[:-1])):
         return
     nat.require_cuda(x, weight, bias, residual)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
@@ -70,26 +71,29 @@ def linear_fwd(x, weight, bias, residual, act: int, save: bool):
     x and weight dense."""
     N, K = weight.shape
     M = x.numel() // K
-    dev = x.device
+    index = x.get_device()
     dt = _CODE[x.dtype]
-    bptr = bdt = rptr = zptr = wptr = None
+    bptr = rptr = zptr = wptr = None
+    bdt = wbytes = 0
     if bias is not None:
-        bias = bias if bias.is_contiguous() else bias.contiguous()
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
         bptr, bdt = bias.data_ptr(), _CODE[bias.dtype]
     if residual is None:
         out, rdt = x.new_empty((*x.shape[:-1], N)), dt
     else:
-        residual = residual if residual.is_contiguous() else residual.contiguous()
+        if not residual.is_contiguous():
+            residual = residual.contiguous()
         out, rptr, rdt = torch.empty_like(residual), residual.data_ptr(), _CODE[residual.dtype]
     z = None
     if save and linear_saves(act, residual):
         z = x.new_empty(out.shape)
         zptr = z.data_ptr()
-    ws = nat.workspace("affb_linear_fwd_workspace_bytes", dev, dt, M, N, K)
+    ws = nat.workspace(index, "affb_linear_fwd_workspace_bytes", x, dt, M, N, K)
     if ws is not None:
-        wptr = ws.data_ptr()
-    nat.call_on(dev, "affb_linear_fwd", x.data_ptr(), weight.data_ptr(), bptr, bdt or 0, rptr, rdt, act, dt, M, N, K,
-                out.data_ptr(), rdt, zptr, wptr, ws.numel() if wptr else 0)
+        wptr, wbytes = ws.data_ptr(), ws.numel()
+    nat.call_on(index, "affb_linear_fwd", x.data_ptr(), weight.data_ptr(), bptr, bdt, rptr, rdt, act, dt, M, N, K,
+                out.data_ptr(), rdt, zptr, wptr, wbytes)
     return out, z
 
 
@@ -105,14 +109,14 @@ def linear_bwd(dout, z, x, weight, act: int, need_x: bool, need_w: bool, bias_dt
     residual)."""
     N, K = weight.shape
     M = x.numel() // K
-    dev = x.device
+    index = x.get_device()
     dx = torch.empty_like(x) if need_x else None
     dw = torch.empty_like(weight) if need_w else None
-    db = torch.empty(N, device=dev, dtype=bias_dtype) if bias_dtype is not None else None
+    db = x.new_empty(N, dtype=bias_dtype) if bias_dtype is not None else None
     if need_x or need_w or db is not None:
         dt = nat.dcode(x)
-        ws = nat.workspace("affb_linear_bwd_workspace_bytes", dev, dt, M, N, K)
-        nat.call_on(dev, "affb_linear_bwd", nat.ptr(dout), nat.dcode(dout), nat.ptr(z), nat.ptr(x), nat.ptr(weight), act,
+        ws = nat.workspace(index, "affb_linear_bwd_workspace_bytes", x, dt, M, N, K)
+        nat.call_on(index, "affb_linear_bwd", nat.ptr(dout), nat.dcode(dout), nat.ptr(z), nat.ptr(x), nat.ptr(weight), act,
                     dt, M, N, K, nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.dcode(db) if db is not None else 0,
                     nat.ptr(ws), ws.numel() if ws is not None else 0)
     return dx, dw, db
@@ -149,7 +153,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     of these; residual [..., N] in x's dtype or fp32.  The output has the
     residual's dtype, else x's.  act: "none", "relu", "gelu" (exact) or
     "silu".  Differentiable once in x, weight, bias and residual."""
-    code = _act_code(act)
+    code = ACTIVATIONS[act] if act in ACTIVATIONS else _act_code(act)
     _check_operands(x, weight, bias, residual)
     if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                          or (bias is not None and bias.requires_grad)
@@ -191,7 +195,7 @@ def quantize_e4m3(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     C = x.shape[-1]
     q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
     scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
-    nat.call_on(x.device, "affb_quantize_e4m3", nat.ptr(xc), nat.dcode(xc), xc.numel() // C, C, nat.ptr(q),
+    nat.call_on(x.get_device(), "affb_quantize_e4m3", nat.ptr(xc), nat.dcode(xc), xc.numel() // C, C, nat.ptr(q),
                 nat.ptr(scale))
     return q, scale
 
@@ -209,16 +213,16 @@ def linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     if out_dtype not in _FLOATS or (residual is not None and residual.dtype not in _FLOATS):
         raise RuntimeError("linear_e4m3: output and residual must be fp32, fp16 or bf16")
     N, K = weight.shape
-    dev = x.device
+    index = x.get_device()
     if x_scale.shape != x.shape[:-1] or weight_scale.shape != weight.shape[:1]:
         raise RuntimeError("linear_e4m3: scales must have one value per row")
-    if x_scale.device != dev or weight_scale.device != dev:
+    if x_scale.get_device() != index or weight_scale.get_device() != index:
         raise RuntimeError("linear_e4m3: scales must be on the operands' device")
     M = x.numel() // K
     x, weight = nat.dense(x), nat.dense(weight)
     x_scale, weight_scale = _f32(x_scale), _f32(weight_scale)
     bptr = rptr = wptr = None
-    rdt = 0
+    rdt = wbytes = 0
     if bias is not None:
         bias = _f32(bias)
         bptr = bias.data_ptr()
@@ -226,11 +230,11 @@ def linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
         residual = residual if residual.is_contiguous() else residual.contiguous()
         rptr, rdt = residual.data_ptr(), _CODE[residual.dtype]
     out = x.new_empty((*x.shape[:-1], N), dtype=out_dtype)
-    ws = nat.workspace("affb_linear_e4m3_workspace_bytes", dev, M, N, K)
+    ws = nat.workspace(index, "affb_linear_e4m3_workspace_bytes", x, M, N, K)
     if ws is not None:
-        wptr = ws.data_ptr()
-    nat.call_on(dev, "affb_linear_e4m3", x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(),
-                bptr, rptr, rdt, code, M, N, K, out.data_ptr(), _CODE[out_dtype], wptr, ws.numel() if wptr else 0)
+        wptr, wbytes = ws.data_ptr(), ws.numel()
+    nat.call_on(index, "affb_linear_e4m3", x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(),
+                bptr, rptr, rdt, code, M, N, K, out.data_ptr(), _CODE[out_dtype], wptr, wbytes)
     return out
 
 

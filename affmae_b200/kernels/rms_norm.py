@@ -25,11 +25,11 @@ _CODE = nat._DTYPE_CODE
 
 
 def _check(x, weight, delta, row_scale):
-    xs, dev = x.shape, x.device
+    xs, d = x.shape, x.get_device()
     # the common case in a few comparisons; whatever else is looked at in order below
-    if dev.type == "cuda" and xs and xs[-1] and weight.shape == xs[-1:] and weight.device == dev and row_scale is None \
-            and x.dtype in _FLOATS and weight.dtype in _FLOATS \
-            and (delta is None or (delta.shape == xs and delta.dtype in _FLOATS and delta.device == dev)):
+    if d >= 0 and row_scale is None and xs and xs[-1] and weight.dim() == 1 and weight.shape[0] == xs[-1] \
+            and weight.get_device() == d and x.dtype in _FLOATS and weight.dtype in _FLOATS \
+            and (delta is None or (delta.get_device() == d and delta.dtype in _FLOATS and delta.shape == xs)):
         return
     nat.require_cuda(x, weight, delta, row_scale)
     if x.dim() < 1 or tuple(weight.shape) != (x.shape[-1],) or x.shape[-1] < 1:
@@ -56,7 +56,6 @@ def _launch(x, delta, row_scale, weight, eps, out_dtype, keep):
     `keep`, s only with delta."""
     C = x.shape[-1]
     R = x.numel() // C
-    dev = x.device
     xc = nat.dense(x)
     w = nat.dense(weight.detach().float() if weight.requires_grad or weight.dtype != torch.float32 else weight)
     s = rs = rstd = y = q = scale = None
@@ -79,7 +78,7 @@ def _launch(x, delta, row_scale, weight, eps, out_dtype, keep):
     else:
         y = torch.empty_like(xc, dtype=out_dtype)
         yptr, ydt = y.data_ptr(), _CODE[out_dtype]
-    nat.call_on(dev, "affb_rms_norm_fwd", xc.data_ptr(), _CODE[xc.dtype], dptr, ddt, rptr, groups, w.data_ptr(),
+    nat.call_on(x.get_device(), "affb_rms_norm_fwd", xc.data_ptr(), _CODE[xc.dtype], dptr, ddt, rptr, groups, w.data_ptr(),
                 float(eps), R, C, sptr, kptr, yptr, ydt, qptr, cptr)
     return xc, rs, w, s, rstd, y, q, scale
 
@@ -89,12 +88,12 @@ def rms_norm_bwd(dy, ds, s, rstd, weight, row_scale, need_x: bool, need_w: bool,
     ddelta); weight, row_scale, dw fp32; dy or ds may be None."""
     C = s.shape[-1]
     R = s.numel() // C
-    dev = s.device
+    index = s.get_device()
     dx = torch.empty_like(s) if need_x else None
-    dd = torch.empty(s.shape, device=dev, dtype=delta_dtype) if delta_dtype is not None else None
-    dw = torch.empty(C, device=dev, dtype=torch.float32) if need_w else None
-    ws = nat.workspace("affb_rms_norm_bwd_workspace_bytes", dev, R, C) if need_w else None
-    nat.call_on(dev, "affb_rms_norm_bwd", nat.ptr(dy), nat.dcode(dy) if dy is not None else 0, nat.ptr(ds), nat.ptr(s),
+    dd = torch.empty_like(s, dtype=delta_dtype) if delta_dtype is not None else None
+    dw = s.new_empty(C, dtype=torch.float32) if need_w else None
+    ws = nat.workspace(index, "affb_rms_norm_bwd_workspace_bytes", s, R, C) if need_w else None
+    nat.call_on(index, "affb_rms_norm_bwd", nat.ptr(dy), nat.dcode(dy) if dy is not None else 0, nat.ptr(ds), nat.ptr(s),
                 nat.dcode(s), nat.ptr(rstd), nat.ptr(weight), nat.ptr(row_scale),
                 row_scale.numel() if row_scale is not None else 0, R, C, nat.ptr(dx), nat.ptr(dd),
                 nat.dcode(dd) if dd is not None else 0, nat.ptr(dw), nat.ptr(ws), ws.numel() if ws is not None else 0)
