@@ -40,7 +40,8 @@ constexpr int BB_TABLE_SMEM = 64 * 1024;   // of one block's heads
 struct BucketArgs {
   int edges[BB_MAX_EDGES];
   int k;                // number of edges
-  int lut;              // entries of the byte table (last edge + 1), or 0: search the edges
+  int lut;              // distances up to the last edge, last + 1 (0: more than BB_LUT)
+  int use_lut;          // a byte table of them is filled, else the edges are searched
   int one_sided;
   int axes;
   int per_axis;         // index values of one axis
@@ -80,22 +81,34 @@ __device__ __forceinline__ int offset_of(int64_t k, int64_t q) {
   return (int)(d < -(1 << 30) ? -(1 << 30) : d > (1 << 30) ? (1 << 30) : d);
 }
 
-// c(n) by binary search of the edges.
-__device__ __forceinline__ int search_edges(const BucketArgs& a, int n) {
-  int lo = 0, hi = a.k;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (a.edges[mid] <= n) lo = mid + 1;
-    else hi = mid;
+// Where a kernel finds buckets: a byte table of distances, or (null) the edges.
+struct Buckets {
+  const uint8_t* lut;
+  const int* edges;
+};
+// c(n) by binary search of the edges (in shared memory).
+__device__ __forceinline__ int search_edges(const int* edges, int k, int n) {
+  int c = 0;
+#pragma unroll
+  for (int s = BB_MAX_EDGES; s > 0; s >>= 1)
+    if (c + s <= k && edges[c + s - 1] <= n) c += s;
+  return c;
+}
+// Fills the edges (BB_MAX_EDGES ints at `sm`) and, after them, the byte table
+// where one is wanted; ends with a barrier.
+__device__ __forceinline__ Buckets fill_buckets(const BucketArgs& a, int* sm) {
+  for (int i = threadIdx.x; i < a.k; i += BB_THREADS) sm[i] = a.edges[i];
+  __syncthreads();
+  uint8_t* lut = reinterpret_cast<uint8_t*>(sm + BB_MAX_EDGES);
+  if (a.use_lut) {
+    for (int i = threadIdx.x; i < a.lut; i += BB_THREADS) lut[i] = (uint8_t)search_edges(sm, a.k, i);
+    __syncthreads();
   }
-  return lo;
+  return {a.use_lut ? lut : nullptr, sm};
 }
-__device__ __forceinline__ void fill_lut(const BucketArgs& a, uint8_t* lut) {
-  for (int i = threadIdx.x; i < a.lut; i += BB_THREADS) lut[i] = (uint8_t)search_edges(a, i);
-}
-__device__ __forceinline__ int axis_index(const BucketArgs& a, const uint8_t* lut, int d) {
+__device__ __forceinline__ int axis_index(const BucketArgs& a, const Buckets& f, int d) {
   const int n = a.one_sided ? max(-d, 0) : abs(d);
-  const int c = a.lut ? lut[min(n, a.lut - 1)] : search_edges(a, n);
+  const int c = f.lut ? f.lut[min(n, a.lut - 1)] : search_edges(f.edges, a.k, n);
   return a.one_sided ? c : d < 0 ? a.k - c : a.k + c;
 }
 // The offset that index i of [0, span) stands for where offsets are cut off at
@@ -107,11 +120,11 @@ __device__ __forceinline__ int unclipped(const BucketArgs& a, int i) { return a.
 template <typename P, int AXES, bool BY_OFFSET>
 struct EntryOf {
   const BucketArgs& a;
-  const uint8_t* lut;
+  const Buckets find;
   int last, high;       // offsets are cut off to [-last, high]
   int mx, my, add;      // entry = mx x + my y + add
 
-  __device__ __forceinline__ EntryOf(const BucketArgs& args, const uint8_t* l) : a(args), lut(l) {
+  __device__ __forceinline__ EntryOf(const BucketArgs& args, const Buckets& f) : a(args), find(f) {
     last = a.lut - 1;
     high = a.one_sided ? 0 : last;
     mx = a.one_sided ? -1 : 1;
@@ -130,12 +143,12 @@ struct EntryOf {
   }
   __device__ __forceinline__ int one(P k, P q) const {
     if constexpr (BY_OFFSET) return (int)((uint32_t)mx * cut(k, q) + (uint32_t)add);
-    return axis_index(a, lut, offset_of(k, q));
+    return axis_index(a, find, offset_of(k, q));
   }
   __device__ __forceinline__ int two(P kx, P ky, P qx, P qy) const {
     if constexpr (BY_OFFSET)
       return (int)((uint32_t)my * cut(ky, qy) + ((uint32_t)mx * cut(kx, qx) + (uint32_t)add));
-    return axis_index(a, lut, offset_of(ky, qy)) * a.per_axis + axis_index(a, lut, offset_of(kx, qx));
+    return axis_index(a, find, offset_of(ky, qy)) * a.per_axis + axis_index(a, find, offset_of(kx, qx));
   }
 };
 
@@ -214,10 +227,8 @@ __global__ void __launch_bounds__(BB_THREADS, 4)
   extern __shared__ unsigned char sm[];
   const int entries = BY_OFFSET ? (AXES == 2 ? a.span * a.span : a.span) : a.rows;
   V* tab = reinterpret_cast<V*>(sm);                                        // [groups][entries + 1]
-  uint8_t* lut = sm + (size_t)groups * (entries + 1) * sizeof(V);
   const int h0 = blockIdx.y * groups * BB_HEADS, nh = min(groups * BB_HEADS, a.H - h0);
-  fill_lut(a, lut);
-  __syncthreads();
+  const Buckets find = fill_buckets(a, reinterpret_cast<int*>(sm + (size_t)groups * (entries + 1) * sizeof(V)));
   const auto fill = [&](int i, int row) {  // entry i: the heads of a table row (row < 0: zero)
     for (int g = 0; g < groups; ++g) {
       T* t = reinterpret_cast<T*>(tab + g * (entries + 1) + i);
@@ -230,15 +241,15 @@ __global__ void __launch_bounds__(BB_THREADS, 4)
   if (BY_OFFSET && AXES == 2) {
     // a warp takes whole rows of offsets along y
     for (int y = threadIdx.x >> 5; y < a.span; y += BB_THREADS / 32) {
-      const int ry = axis_index(a, lut, unclipped(a, y)) * a.per_axis;
-      for (int x = threadIdx.x & 31; x < a.span; x += 32) fill(y * a.span + x, ry + axis_index(a, lut, unclipped(a, x)));
+      const int ry = axis_index(a, find, unclipped(a, y)) * a.per_axis;
+      for (int x = threadIdx.x & 31; x < a.span; x += 32) fill(y * a.span + x, ry + axis_index(a, find, unclipped(a, x)));
     }
   } else {
-    for (int i = threadIdx.x; i < entries; i += BB_THREADS) fill(i, BY_OFFSET ? axis_index(a, lut, unclipped(a, i)) : i);
+    for (int i = threadIdx.x; i < entries; i += BB_THREADS) fill(i, BY_OFFSET ? axis_index(a, find, unclipped(a, i)) : i);
   }
   __syncthreads();
   constexpr int STEP = BB_THREADS * PAIRS, TILE = STEP * BB_STEPS;
-  const EntryOf<P, AXES, BY_OFFSET> entry(a, lut);
+  const EntryOf<P, AXES, BY_OFFSET> entry(a, find);
   const uint32_t per = ((uint32_t)a.NM + TILE - 1) / TILE;
   const int64_t total = (int64_t)per * a.B;
   for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
@@ -301,21 +312,19 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
   // BY_OFFSET: the row of every combined clipped offset, and `none` last
   const int offsets = AXES == 2 ? a.span * a.span : a.span;
   uint16_t* rows = raw_row + TILE;
-  uint8_t* lut = reinterpret_cast<uint8_t*>(rows + (BY_OFFSET ? (offsets + 2) & ~1 : 0));
   const int h0 = blockIdx.y * BB_HEADS, nh = min(BB_HEADS, a.H - h0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  fill_lut(a, lut);
-  __syncthreads();
+  const Buckets find = fill_buckets(a, reinterpret_cast<int*>(rows + (BY_OFFSET ? (offsets + 2) & ~1 : 0)));
   if (BY_OFFSET) {
     if (threadIdx.x == 0) rows[offsets] = (uint16_t)none;
     if (AXES == 2) {
       for (int y = threadIdx.x >> 5; y < a.span; y += BB_THREADS / 32) {
-        const int ry = axis_index(a, lut, unclipped(a, y)) * a.per_axis;
+        const int ry = axis_index(a, find, unclipped(a, y)) * a.per_axis;
         for (int x = threadIdx.x & 31; x < a.span; x += 32)
-          rows[y * a.span + x] = (uint16_t)(ry + axis_index(a, lut, unclipped(a, x)));
+          rows[y * a.span + x] = (uint16_t)(ry + axis_index(a, find, unclipped(a, x)));
       }
     } else {
-      for (int i = threadIdx.x; i < offsets; i += BB_THREADS) rows[i] = (uint16_t)axis_index(a, lut, unclipped(a, i));
+      for (int i = threadIdx.x; i < offsets; i += BB_THREADS) rows[i] = (uint16_t)axis_index(a, find, unclipped(a, i));
     }
   }
   float* mine = part + ((int64_t)blockIdx.x * a.H + h0) * a.rows;
@@ -326,7 +335,7 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
       bins[h * stride + i] = 0;
     }
   __syncthreads();
-  const EntryOf<P, AXES, BY_OFFSET> entry(a, lut);
+  const EntryOf<P, AXES, BY_OFFSET> entry(a, find);
   const uint32_t per = ((uint32_t)a.NM + TILE - 1) / TILE;
   const int64_t total = (int64_t)per * a.B;
   for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
@@ -541,6 +550,13 @@ static int64_t bb_offsets(const BucketArgs& a, int64_t entry_bytes, int64_t most
   return n * entry_bytes <= most_bytes && n * blocks <= (int64_t)a.NM * a.B ? n : 0;
 }
 
+// A byte table of distances is filled where a block looks up more of them than
+// that (an expanded table asks for `span` of them, or one axis's worth).
+static int bb_use_lut(const BucketArgs& a, int64_t offsets, int64_t blocks) {
+  if (!a.lut) return 0;
+  return offsets > 0 || (int64_t)a.lut * blocks <= (int64_t)a.NM * a.B * a.axes;
+}
+
 #define BB_POS(pos_type, P, ...)                                   \
   switch (pos_type) {                                              \
     case AFFB_POS_F32: { using P = float; __VA_ARGS__; break; }    \
@@ -558,14 +574,16 @@ static cudaError_t bucket_fwd_launch(const BucketArgs& a, const void* table, voi
   const int64_t entries = (offsets ? offsets : a.rows) + 1;
   const int64_t fit = BB_TABLE_SMEM / (entries * v);
   const int groups = (int)(fit < 1 ? 1 : fit < all ? fit : all);
-  const int smem = (int)(groups * entries * v) + a.lut;
+  BucketArgs c = a;
+  c.use_lut = bb_use_lut(a, offsets, blocks);
+  const int smem = (int)(groups * entries * v) + BB_MAX_EDGES * 4 + (c.use_lut ? a.lut : 0);
   auto* k = offsets ? bucket_fwd_kernel<T, TB, P, AXES, PAIRS, true> : bucket_fwd_kernel<T, TB, P, AXES, PAIRS, false>;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
   const dim3 grid((unsigned)blocks, (unsigned)((all + groups - 1) / groups));
-  k<<<grid, BB_THREADS, smem, st>>>(a, (const TB*)table, groups, (T*)out);
+  k<<<grid, BB_THREADS, smem, st>>>(c, (const TB*)table, groups, (T*)out);
   return cudaGetLastError();
 }
 
@@ -574,14 +592,17 @@ static cudaError_t bucket_bwd_launch(const BucketArgs& a, const void* dout, floa
                                      cudaStream_t st) {
   const int64_t offsets = bb_offsets(a, 2, 16 * 1024, blocks);
   const int tile = BB_THREADS * PAIRS * BB_STEPS;
-  const int smem = 2 * BB_HEADS * (a.rows + 1) * 4 + tile * 6 + (offsets ? (int)((offsets + 2) & ~1) * 2 : 0) + a.lut;
+  BucketArgs c = a;
+  c.use_lut = bb_use_lut(a, offsets, blocks);
+  const int smem = 2 * BB_HEADS * (a.rows + 1) * 4 + tile * 6 + (offsets ? (int)((offsets + 2) & ~1) * 2 : 0) +
+                   BB_MAX_EDGES * 4 + (c.use_lut ? a.lut : 0);
   auto* k = offsets ? bucket_bwd_kernel<T, P, AXES, PAIRS, true> : bucket_bwd_kernel<T, P, AXES, PAIRS, false>;
   if (smem > 47 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
   const dim3 grid((unsigned)blocks, (unsigned)((a.H + BB_HEADS - 1) / BB_HEADS));
-  k<<<grid, BB_THREADS, smem, st>>>(a, (const T*)dout, part, resume);
+  k<<<grid, BB_THREADS, smem, st>>>(c, (const T*)dout, part, resume);
   return cudaGetLastError();
 }
 

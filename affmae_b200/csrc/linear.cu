@@ -581,15 +581,24 @@ struct Shape {
   int cg, bn, nt, mt, splits;
 };
 
-// Tile and split of the contraction.
+// Tile and split of the contraction; `step`: multiple that the width of tiles
+// beside one another has to be (what one store covers).
+//
 // Pairs of blocks (256-row tiles up to 256 columns wide) where there are
 // enough tiles, or enough k blocks to split, for all of them, and a tile's
 // contraction is long enough to be worth the pair's handshakes (524288 x 96 ->
 // 192, two k blocks: 87 us by pairs, 57 by single blocks; 524288 x 384 -> 768,
 // six: 292 against 329; 8192 x 4096 -> 8192 e4m3, 32: 190 against 215); else
-// single blocks, whose tiles are narrowed (down to 64 columns) and whose contraction
-// is split (at least 4 k blocks a part) until they fill the GPU.
-static Shape choose_shape(int64_t M, int64_t N, int64_t total_k) {
+// single blocks.
+// Tiles that leave SMs idle are split along the contraction, at least 4 k
+// blocks a part.  The width is the one that costs least, a k block of a tile
+// taken as its columns and 64 more for what does not depend on them, and a
+// split as SPLIT_COST for the launch that sums the parts (13107 x 771 in fp32:
+// three rounds of 208 columns instead of 256, 95 -> 91 us; 5243 x 384: 63
+// pairs of 128 columns instead of 42 of 192, 11.8 -> 10.9 us).
+constexpr int64_t SPLIT_COST = 2000;  // about 3 us
+
+static Shape choose_shape(int64_t M, int64_t N, int64_t total_k, int step) {
   const int64_t sms = sm_count();
   Shape s;
   const int64_t wide = (N + 255) / 256;
@@ -598,22 +607,40 @@ static Shape choose_shape(int64_t M, int64_t N, int64_t total_k) {
   s.cg = M > TILE_M && total_k >= PAIR_K && pair_tiles * most_splits >= sms / 2 ? 2 : 1;
   const int64_t teams = sms / s.cg;
   s.mt = (int)((M + TILE_M * s.cg - 1) / (TILE_M * s.cg));
-  s.nt = (int)wide;
-  if (s.cg == 1)
-    while ((int64_t)s.mt * s.nt * 2 <= sms && (N + s.nt * 2 - 1) / (s.nt * 2) >= 64) s.nt *= 2;
-  const int64_t per = (N + s.nt - 1) / s.nt;
-  s.bn = (int)round_up(per, s.nt > 1 ? 64 : s.cg == 1 ? 16 : 32);  // stores are 64 columns wide
-  s.nt = (int)((N + s.bn - 1) / s.bn);
-  const int64_t tiles = (int64_t)s.mt * s.nt;
-  int64_t sp = teams / tiles;
-  if (sp > most_splits) sp = most_splits;
-  s.splits = (int)(sp < 2 ? 1 : sp);
+  int64_t best = 0;
+  for (int64_t nt = wide; nt <= 4 * wide + 3; ++nt) {
+    const int64_t per = (N + nt - 1) / nt;
+    const int64_t bn = round_up(per, nt > 1 ? step : s.cg == 1 ? 16 : 32);
+    if (bn > 256 || (nt > wide && bn < 64)) continue;
+    const int64_t tiles = s.mt * ((N + bn - 1) / bn);
+    int64_t sp = teams / tiles < most_splits ? teams / tiles : most_splits;
+    if (sp < 2) sp = 1;
+    for (int64_t splits = 1; splits <= sp; splits += sp > 1 ? sp - 1 : 1) {  // none, or as many as fit
+      const int64_t cost = (tiles * splits + teams - 1) / teams * ((total_k + splits - 1) / splits) * (bn + 64) +
+                           (splits > 1 ? SPLIT_COST : 0);
+      if (best == 0 || cost < best) {
+        best = cost;
+        s.bn = (int)bn;
+        s.nt = (int)((N + bn - 1) / bn);
+        s.splits = (int)splits;
+      }
+    }
+  }
   return s;
 }
+// Columns that one store of the epilogue covers: 128 bytes by TMA.
+static int store_step(bool direct, int out_dtype) { return direct || out_dtype == AFFB_F32 ? 32 : 64; }
 
 static int64_t partial_bytes(int64_t M, int64_t N, int64_t total_k) {
-  const Shape s = choose_shape(M, N, total_k);
-  return s.splits > 1 ? round_up((int64_t)s.splits * M * round_up(N, 4) * 4, 256) : 0;
+  int64_t most = 0;
+  for (int step = 32; step <= 64; step += 32) {
+    const Shape s = choose_shape(M, N, total_k, step);
+    if (s.splits > 1) {
+      const int64_t b = round_up((int64_t)s.splits * M * round_up(N, 4) * 4, 256);
+      if (b > most) most = b;
+    }
+  }
+  return most;
 }
 
 // K blocks of a contraction of length K (all part pairs).
@@ -661,7 +688,8 @@ static bool tma_rows(const void* p, int dtype, int64_t N) {
 static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K, LinearEpilogue e,
                 unsigned char* ws, cudaStream_t st) {
   const int64_t total_k = k_blocks(dtype, K);
-  const Shape s = choose_shape(M, N, total_k);
+  const bool plain = !(tma_rows(e.out, e.out_dtype, N) && (!e.z || tma_rows(e.z, e.z_dtype, N)));
+  const Shape s = choose_shape(M, N, total_k, store_step(plain, e.out_dtype == AFFB_F32 && e.z ? e.z_dtype : e.out_dtype));
   const int et = dtype == AFFB_F32 ? AFFB_BF16 : dtype;  // element type in memory
   const int64_t planes = dtype == AFFB_F32 ? 3 : 1;
   GemmArgs p{};
@@ -684,8 +712,7 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
     p.N = (int)round_up(N, 4);  // pitch of the partial products (columns past N hold zeros)
   }
   p.e = e;
-  p.direct = s.splits > 1 ? 0
-                          : !(tma_rows(e.out, e.out_dtype, N) && (!e.z || tma_rows(e.z, e.z_dtype, N)));
+  p.direct = s.splits > 1 ? 0 : plain;
   p.res_rows = e.residual && tma_rows(e.residual, e.residual_dtype, p.N);
   p.res_tma = p.res_rows && !e.z && !p.direct;
   p.bufs = e.z || p.res_tma ? 2 : 1;
@@ -789,7 +816,7 @@ static int check_sizes(int64_t M, int64_t N, int64_t K) {
 
 static int forward(const void* x, const void* w, int dtype, int64_t M, int64_t N, int64_t K, const LinearEpilogue& e,
                    void* workspace, int64_t workspace_bytes, cudaStream_t st) {
-  if (M <= small_rows(dtype)) return linear_small(x, w, dtype, M, N, K, e, st);
+  if (few_rows(dtype, M, N, K)) return linear_small(x, w, dtype, M, N, K, e, st);
   Arena ws{(unsigned char*)workspace, 0, workspace ? workspace_bytes : 0};
   Operand a, b;
   int rc;
@@ -816,7 +843,7 @@ extern "C" int affb_linear_status(int* failed) {
 }
 
 extern "C" int64_t affb_linear_fwd_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
-  if (M <= small_rows(dtype) || N < 1 || K < 1) return 0;
+  if (N < 1 || K < 1 || few_rows(dtype, M, N, K)) return 0;
   return copy_bytes(dtype, M, K, false) + copy_bytes(dtype, N, K, false) + partial_bytes(M, N, k_blocks(dtype, K));
 }
 

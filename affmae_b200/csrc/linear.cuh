@@ -29,11 +29,14 @@ struct LinearEpilogue {
   int z_dtype;
 };
 
-// linear_small.cu: out = epilogue(x w^T) for M <= small_rows(dtype) <= 8 rows,
-// one launch.  K = 4096, N = 8192 against the tensor-core product: bf16 4 rows
-// 22 us (28), 8 rows 37 (28); e4m3 2 rows 11.5 (16), 4 rows 17.6 (16); fp32
-// (K = 1024, N = 4096) 8 rows 15 (35, six products of parts).
-inline int64_t small_rows(int dtype) { return dtype == AFFB_F32 ? 8 : dtype == AFFB_E4M3 ? 3 : 4; }
+// linear_small.cu: out = epilogue(x w^T) for few rows (at most 8), one launch.
+// Against the tensor-core product, with w [8192,4096]: bf16 2 rows 14.6 us (17),
+// 3 rows 18.4 (17); e4m3 2 rows 11.5 (16.6), 4 rows 17.5 (16.6); with w
+// [4096,1024]: bf16 4 rows 7.0 (8.3), fp32 (six products of parts) 8 rows 15 (28).
+inline bool few_rows(int dtype, int64_t M, int64_t N, int64_t K) {
+  if (dtype == AFFB_F32) return M <= 8;
+  return M <= 2 || (M <= 4 && M * N * K <= (64ll << 20));
+}
 int linear_small(const void* x, const void* w, int dtype, int64_t M, int64_t N, int64_t K, const LinearEpilogue& e,
                  cudaStream_t st);
 
