@@ -834,7 +834,10 @@ using namespace affb;
 
 extern "C" int affb_linear_status(int* failed) {
   AFFB_REQUIRE(failed, "affb_linear_status: null pointer");
-  const cudaError_t e = cudaMemcpyFromSymbol(failed, g_linear_failed, sizeof(int));
+  int norms = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(failed, g_linear_failed, sizeof(int));
+  if (e == cudaSuccess) e = rms_failed(&norms);
+  *failed |= norms;
   if (e != cudaSuccess) {
     set_error("affb_linear_status: %s", cudaGetErrorString(e));
     return AFFB_ERR_CUDA;

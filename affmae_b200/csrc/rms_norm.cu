@@ -12,11 +12,15 @@
 // is the smallest of 8, 16, 32 and a whole block whose chunks cover the row
 // with few idle lanes (96 channels: 16 threads of one chunk; 384: 16 of
 // three).  Rows beyond 4 chunks a thread of a block are read again for the
-// second pass.  dw is summed per block in row order and then over blocks in
+// second pass.  Where there are several rounds of rows a block brings them in
+// by bulk copies, two to four rounds ahead (the rows of a round are
+// contiguous): registers alone keep too few bytes on the way.  dw is summed per block in row order and then over blocks in
 // order, so it does not depend on timing.
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 #include <cuda_fp8.h>
+
+#include <type_traits>
 
 namespace affb {
 
@@ -111,15 +115,130 @@ __device__ __forceinline__ float row_reduce(float v, float* red, Op op) {
   return v;
 }
 
+// Set when a wait on a copy ran out; read by rms_failed().
+__device__ int g_rms_failed;
+
+// Rounds of rows on their way into shared memory: up to three arrays with the
+// same rows, stage after stage.
+struct RowPipe {
+  const void* src[3];
+  int row_bytes[3];   // 0: no such array
+  int rows;           // of a round
+  int stages;
+  int stage_bytes;
+};
+constexpr int PIPE_HEAD = 128;  // barriers and the failure flag, before the stages
+
+template <int ROWS>
+struct PipeReader {
+  const RowPipe& p;
+  unsigned char* base;
+  uint32_t bars;
+  volatile int* failed;
+  int64_t R;
+  int stage;
+  uint32_t phase;
+
+  __device__ __forceinline__ PipeReader(const RowPipe& pipe, unsigned char* smem, int64_t rows) : p(pipe), R(rows) {
+    base = smem + PIPE_HEAD;
+    bars = tc5::smem_addr(smem);
+    failed = reinterpret_cast<volatile int*>(smem + 64);
+    stage = 0;
+    phase = 0;
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < p.stages; ++i) tc5::bar_init(bars + 8 * i, 1);
+      tc5::bar_init_fence();
+      *failed = 0;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+      for (int i = 0; i < p.stages; ++i) issue(i, i);
+  }
+  // One thread: the copies of this block's round `it` into stage `st`.
+  __device__ __forceinline__ void issue(int64_t it, int st) {
+    const int64_t r0 = ((int64_t)blockIdx.x + it * gridDim.x) * ROWS;
+    if (r0 >= R) return;
+    const int n = (int)imin64(ROWS, R - r0);
+    tc5::bar_expect(bars + 8 * st, (uint32_t)(n * (p.row_bytes[0] + p.row_bytes[1] + p.row_bytes[2])));
+    uint32_t to = tc5::smem_addr(base + st * p.stage_bytes);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      if (p.row_bytes[i]) {
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
+                     "l"((const unsigned char*)p.src[i] + r0 * p.row_bytes[i]), "r"(n * p.row_bytes[i]),
+                     "r"(bars + 8 * st)
+                     : "memory");
+        to += ROWS * p.row_bytes[i];
+      }
+    }
+  }
+  // All threads: the round has landed; false (for all) when a wait ran out.
+  __device__ __forceinline__ bool wait() {
+    return !__syncthreads_or(!tc5::bar_wait(bars + 8 * stage, phase, failed));
+  }
+  // Row `slot` of array i of the current round.
+  __device__ __forceinline__ const unsigned char* row(int i, int slot) const {
+    const unsigned char* q = base + stage * p.stage_bytes;
+    for (int j = 0; j < i; ++j) q += ROWS * p.row_bytes[j];
+    return q + slot * p.row_bytes[i];
+  }
+  // All threads are done with the round `it`: its stage takes round it + stages.
+  __device__ __forceinline__ void next(int64_t it) {
+    __syncthreads();
+    if (threadIdx.x == 0) issue(it + p.stages, stage);
+    if (++stage == p.stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+  // After a wait that ran out: what is still on its way has to land.
+  __device__ __forceinline__ void give_up(int64_t it) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < p.stages; ++i) {
+        const int st = (stage + i) % p.stages;
+        if (((int64_t)blockIdx.x + (it + i) * gridDim.x) * ROWS < R)
+          tc5::bar_drain(bars + 8 * st, stage + i >= p.stages ? phase ^ 1 : phase);
+      }
+      atomicExch(&g_rms_failed, 1);
+    }
+  }
+};
+
+template <bool PIPE, typename T, int VEC>
+__device__ __forceinline__ void row_load(const T* global, const unsigned char* staged, int c, float* o) {
+  if constexpr (PIPE) ld8_shared(reinterpret_cast<const T*>(staged) + c, o);
+  else rms_load<T, VEC>(global + c, o);
+}
+template <bool PIPE, int VEC>
+__device__ __forceinline__ void row_load_as(const void* global, int dtype, int64_t i, const unsigned char* staged, int c,
+                                            float* o) {
+  if constexpr (PIPE) {
+    if (dtype == AFFB_F32) ld8_shared(reinterpret_cast<const float*>(staged) + c, o);
+    else if (dtype == AFFB_BF16) ld8_shared(reinterpret_cast<const __nv_bfloat16*>(staged) + c, o);
+    else ld8_shared(reinterpret_cast<const __half*>(staged) + c, o);
+  } else {
+    rms_load_as<VEC>(global, dtype, i + c, o);
+  }
+}
+
+template <bool PIPE, int ROWS>
+__device__ __forceinline__ auto make_reader(const RowPipe& p, unsigned char* smem, int64_t R) {
+  if constexpr (PIPE) return PipeReader<ROWS>(p, smem, R);
+  else return char(0);
+}
+
 __device__ __forceinline__ float group_scale(const float* row_scale, int64_t r, int64_t rows_per_scale) {
   // 32-bit division where it fits: a 64-bit one costs as much as a narrow row
   const int64_t g = (r | rows_per_scale) >> 31 ? r / rows_per_scale : (int64_t)((uint32_t)r / (uint32_t)rows_per_scale);
   return row_scale[g];
 }
 
-// NV == 0: the row is read again instead of kept.
-template <typename TX, int TPR, int NV, int VEC>
-__global__ void __launch_bounds__(256) rms_fwd_kernel(RmsArgs a) {
+// NV == 0: the row is read again instead of kept.  PIPE: rows come through
+// shared memory (x, delta).
+template <typename TX, int TPR, int NV, int VEC, bool PIPE>
+__global__ void __launch_bounds__(256) rms_fwd_kernel(const __grid_constant__ RmsArgs a,
+                                                      const __grid_constant__ RowPipe pipe) {
+  extern __shared__ __align__(128) unsigned char staged[];
   __shared__ float red[3][8];  // sums of squares (two rows in turn), maxima
   constexpr int ROWS = 256 / TPR;
   constexpr int KEEP = NV > 0 ? NV : 1;
@@ -128,18 +247,29 @@ __global__ void __launch_bounds__(256) rms_fwd_kernel(RmsArgs a) {
   const float inv_c = 1.f / (float)C;
   int flip = 0;
   const int steps = NV > 0 ? NV : (C + TPR * VEC - 1) / (TPR * VEC);
+  const int slot = threadIdx.x / TPR;
+  PipeReader<ROWS>* reader = nullptr;
+  typename std::conditional<PIPE, PipeReader<ROWS>, char>::type store = make_reader<PIPE, ROWS>(pipe, staged, a.R);
+  if constexpr (PIPE) reader = &store;
+  int64_t it = 0;
   // the threads of a warp stay together (shuffles): rows past the end are computed on nothing
-  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.R; r0 += (int64_t)gridDim.x * ROWS) {
-    const int64_t r = r0 + threadIdx.x / TPR;
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.R; r0 += (int64_t)gridDim.x * ROWS, ++it) {
+    if constexpr (PIPE) {
+      if (!reader->wait()) {
+        reader->give_up(it);
+        break;
+      }
+    }
+    const int64_t r = r0 + slot;
     const bool in = r < a.R;
     const float f = a.row_scale && in ? group_scale(a.row_scale, r, a.rows_per_scale) : 1.f;
     const TX* x = (const TX*)a.x + r * C;
     float v[KEEP][VEC];
     auto row_chunk = [&](int c, float* o) {
-      rms_load<TX, VEC>(x + c, o);
+      row_load<PIPE, TX, VEC>(x, PIPE ? reader->row(0, slot) : nullptr, c, o);
       if (a.delta) {
         float dd[VEC];
-        rms_load_as<VEC>(a.delta, a.delta_dtype, r * C + c, dd);
+        row_load_as<PIPE, VEC>(a.delta, a.delta_dtype, r * C, PIPE ? reader->row(1, slot) : nullptr, c, dd);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o[k] = a.row_scale ? fmaf(f, dd[k], o[k]) : o[k] + dd[k];
       }
@@ -202,14 +332,19 @@ __global__ void __launch_bounds__(256) rms_fwd_kernel(RmsArgs a) {
         if (NV == 0) row_chunk(c, o);
         if (NV == 0 || !a.q) normed(c, o);
         if (a.q) {
+          if (inv != 0.f) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) o[k] = inv != 0.f ? o[k] * inv : o[k] / top;
+            for (int k = 0; k < VEC; ++k) o[k] *= inv;
+          } else {
+            for (int k = 0; k < VEC; ++k) o[k] /= top;
+          }
           store_e4m3<VEC>(a.q + r * C + c, o);
         } else {
           rms_store_as<VEC>(a.y, a.y_dtype, r * C + c, o);
         }
       }
     }
+    if constexpr (PIPE) reader->next(it);
   }
 }
 
@@ -230,9 +365,12 @@ struct RmsBwdArgs {
   float* part;             // [blocks][C] sums of dy s rstd, or null
 };
 
-template <typename TX, int TPR, int NV, int VEC>
-__global__ void __launch_bounds__(256) rms_bwd_kernel(RmsBwdArgs a) {
-  extern __shared__ float dws[];  // [ROWS][C]: sums of each row slot of the block
+// PIPE: rows come through shared memory (s, dy, ds).
+template <typename TX, int TPR, int NV, int VEC, bool PIPE>
+__global__ void __launch_bounds__(256) rms_bwd_kernel(const __grid_constant__ RmsBwdArgs a,
+                                                      const __grid_constant__ RowPipe pipe) {
+  extern __shared__ __align__(128) unsigned char staged[];
+  float* dws = reinterpret_cast<float*>(staged);  // at the end: [ROWS][C], sums of each row slot of the block
   __shared__ float red[2][8];
   constexpr int ROWS = 256 / TPR;
   constexpr int KEEP = NV > 0 ? NV : 1;
@@ -254,21 +392,31 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(RmsBwdArgs a) {
     if (NV > 0 && c < C) rms_load<float, VEC>(a.w + c, wv[NV > 0 ? i : 0]);
   }
   int flip = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.R; r0 += (int64_t)gridDim.x * ROWS) {
+  PipeReader<ROWS>* reader = nullptr;
+  typename std::conditional<PIPE, PipeReader<ROWS>, char>::type store = make_reader<PIPE, ROWS>(pipe, staged, a.R);
+  if constexpr (PIPE) reader = &store;
+  int64_t it = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.R; r0 += (int64_t)gridDim.x * ROWS, ++it) {
     const int64_t r = r0 + slot;
     const bool in = r < a.R;
+    if constexpr (PIPE) {
+      if (!reader->wait()) {
+        reader->give_up(it);
+        break;
+      }
+    }
     const float rstd = in ? a.rstd[r] : 0.f;
     float sv[KEEP][VEC], gv[KEEP][VEC];
     auto chunk = [&](int c, float* s, float* g) {
-      rms_load<TX, VEC>((const TX*)a.s + r * C + c, s);
+      row_load<PIPE, TX, VEC>((const TX*)a.s + r * C, PIPE ? reader->row(0, slot) : nullptr, c, s);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) g[k] = 0.f;
-      if (a.dy) rms_load_as<VEC>(a.dy, a.y_dtype, r * C + c, g);
+      if (a.dy) row_load_as<PIPE, VEC>(a.dy, a.y_dtype, r * C, PIPE ? reader->row(1, slot) : nullptr, c, g);
       if (NV == 0) rms_load<float, VEC>(a.w + c, wv[0]);
     };
     float dot = 0.f;
     float dv[KEEP][VEC];  // ds, requested with the rest of the row
-    if (NV > 0 && a.ds && in) {
+    if (NV > 0 && !PIPE && a.ds && in) {
 #pragma unroll
       for (int i = 0; i < steps; ++i) {
         const int c = (i * TPR + t) * VEC;
@@ -289,7 +437,10 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(RmsBwdArgs a) {
         }
       }
     }
-    if (!a.dx && !a.ddelta) continue;
+    if (!a.dx && !a.ddelta) {
+      if constexpr (PIPE) reader->next(it);
+      continue;
+    }
     const float coef = row_reduce<TPR>(dot, red[flip], AddOp()) * inv_c * rstd * rstd;
     flip ^= 1;
     const float f = a.row_scale && in ? group_scale(a.row_scale, r, a.rows_per_scale) : 1.f;
@@ -302,7 +453,8 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(RmsBwdArgs a) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o[k] = rstd * (gv[n][k] * wv[n][k] - sv[n][k] * coef);
         if (a.ds) {
-          if (NV == 0) rms_load<TX, VEC>((const TX*)a.ds + r * C + c, dv[0]);
+          if (NV == 0 || PIPE)
+            row_load<PIPE, TX, VEC>((const TX*)a.ds + r * C, PIPE ? reader->row(2, slot) : nullptr, c, dv[n]);
 #pragma unroll
           for (int k = 0; k < VEC; ++k) o[k] += dv[n][k];
         }
@@ -314,8 +466,10 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(RmsBwdArgs a) {
         }
       }
     }
+    if constexpr (PIPE) reader->next(it);
   }
   if (a.part && NV > 0) {
+    if constexpr (PIPE) __syncthreads();  // the stages' memory is used again
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * VEC;
@@ -350,17 +504,23 @@ __global__ void __launch_bounds__(1024) rms_dw_kernel(const float* __restrict__ 
   if (x == 0 && blockIdx.x * 32 + l < C) dw[blockIdx.x * 32 + l] = v;
 }
 
+constexpr int PIPE_BYTES = 54 * 1024;  // of a block: four on an SM
+constexpr int PIPE_MOST = 112 * 1024;  // two on an SM
+
 // Threads that share a row, and chunks each holds (0: more than fit).
+// `row_bytes`: of the rows that come through shared memory; where two rounds of
+// sixteen rows would not fit there, a row of 33 to 48 chunks is shared by 32
+// threads instead of 16 (backward of 83888 x 384 fp32: 138 -> 115 us).
 struct RowLayout {
   int tpr, nv;
 };
-static RowLayout rms_layout(int64_t C, int vec) {
+static RowLayout rms_layout(int64_t C, int vec, int64_t row_bytes) {
   const int64_t n = (C + vec - 1) / vec;  // chunks of a row
   if (vec == 8) {
     if (n <= 8) return {8, 1};
     if (n <= 16) return {16, 1};
     if (n <= 32) return {32, 1};
-    if (n <= 48) return {16, 3};
+    if (n <= 48 && 32 * row_bytes <= PIPE_MOST) return {16, 3};
     if (n <= 64) return {32, 2};
     if (n <= 128) return {32, 4};
   } else {
@@ -387,26 +547,83 @@ static int64_t rms_bwd_blocks(int64_t R, int64_t rows) {
   else if (L.nv == 4) GO(256, 4)                     \
   else GO(256, 0)
 
+// The pipe of a kernel whose blocks of `rows` rows a round take `blocks`
+// blocks: stages 0 where a block has fewer than three rounds (nothing to
+// prefetch), or two stages do not fit beside a second block.
+static RowPipe rms_pipe(const RowLayout& l, int64_t R, int64_t blocks, const void* a, int64_t a_bytes, const void* b,
+                        int64_t b_bytes, const void* c, int64_t c_bytes) {
+  RowPipe p{{a, b, c}, {(int)a_bytes, b ? (int)b_bytes : 0, c ? (int)c_bytes : 0}, 256 / l.tpr, 0, 0};
+  if (l.nv == 0 || R < 3 * blocks * p.rows) return p;
+  p.stage_bytes = p.rows * (p.row_bytes[0] + p.row_bytes[1] + p.row_bytes[2]);
+  p.stage_bytes = (p.stage_bytes + 127) / 128 * 128;
+  p.stages = PIPE_BYTES / p.stage_bytes;
+  if (p.stages > 4) p.stages = 4;
+  if (p.stages < 2) p.stages = 2 * p.stage_bytes <= PIPE_MOST ? 2 : 0;
+  return p;
+}
+static int rms_pipe_smem(const RowPipe& p) { return PIPE_HEAD + p.stages * p.stage_bytes; }
+// Blocks of it that an SM holds (228 KB, 1 KB of its own and some statics a block).
+static int64_t rms_pipe_blocks(const RowPipe& p) { return imin64(4, 228 * 1024 / (rms_pipe_smem(p) + 1536)); }
+
+template <typename K, typename A>
+static cudaError_t rms_go(K kernel, unsigned blocks, int smem, const A& a, const RowPipe& p, cudaStream_t st) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
+  kernel<<<blocks, 256, smem, st>>>(a, p);
+  return cudaGetLastError();
+}
+
 template <typename TX, int VEC>
-static void rms_fwd_launch(const RmsArgs& a, cudaStream_t st) {
-  const RowLayout l = rms_layout(a.C, VEC);
-  const int64_t rows = 256 / l.tpr;
-  const unsigned blocks = (unsigned)imin64((a.R + rows - 1) / rows, (int64_t)sm_count() * 8);
-#define RMS_GO(TPR, NV) rms_fwd_kernel<TX, TPR, NV, VEC><<<blocks, 256, 0, st>>>(a);
+static cudaError_t rms_fwd_launch(const RmsArgs& a, cudaStream_t st) {
+  const int64_t row_bytes = a.C * (int64_t)sizeof(TX) + (a.delta ? a.C * (a.delta_dtype == AFFB_F32 ? 4 : 2) : 0);
+  const RowLayout l = rms_layout(a.C, VEC, sizeof(TX) == 2 ? row_bytes : 0);
+  const int64_t rows = 256 / l.tpr, rounds = (a.R + rows - 1) / rows;
+  // fp32 rows keep enough bytes on the way without the pipe (16384 x 4096: 129 us, 146 with it; bf16: 121 and 90)
+  RowPipe p{};
+  if (VEC == 8 && sizeof(TX) == 2)
+    p = rms_pipe(l, a.R, (int64_t)sm_count() * 4, a.x, a.C * (int64_t)sizeof(TX), a.delta,
+                 a.C * (a.delta_dtype == AFFB_F32 ? 4 : 2), nullptr, 0);
+  const unsigned blocks = (unsigned)imin64(rounds, (int64_t)sm_count() * (p.stages ? rms_pipe_blocks(p) : 8));
+#define RMS_GO(TPR, NV)                                                                                          \
+  {                                                                                                              \
+    if constexpr (VEC == 8 && NV > 0)                                                                            \
+      if (p.stages) return rms_go(rms_fwd_kernel<TX, TPR, NV, VEC, true>, blocks, rms_pipe_smem(p), a, p, st);   \
+    return rms_go(rms_fwd_kernel<TX, TPR, NV, VEC, false>, blocks, 0, a, p, st);                                 \
+  }
   RMS_LAYOUTS(VEC, l, RMS_GO)
 #undef RMS_GO
 }
 
 template <typename TX, int VEC>
-static void rms_bwd_launch(const RmsBwdArgs& a, cudaStream_t st) {
-  const RowLayout l = rms_layout(a.C, VEC);
+static cudaError_t rms_bwd_launch(const RmsBwdArgs& a, int64_t* part_rows, cudaStream_t st) {
+  const int64_t sx = a.C * (int64_t)sizeof(TX), sy = a.C * (a.y_dtype == AFFB_F32 ? 4 : 2);
+  const RowLayout l = rms_layout(a.C, VEC, sx + (a.dy ? sy : 0) + (a.ds ? sx : 0));
   const int64_t rows = 256 / l.tpr;
-  const unsigned blocks = (unsigned)rms_bwd_blocks(a.R, rows);
-  const size_t smem = a.part && l.nv > 0 ? (size_t)rows * a.C * 4 : 0;  // at most 32 KB
-#define RMS_GO(TPR, NV) rms_bwd_kernel<TX, TPR, NV, VEC><<<blocks, 256, smem, st>>>(a);
+  int64_t blocks = rms_bwd_blocks(a.R, rows);
+  const int sums = a.part && l.nv > 0 ? (int)(rows * a.C * 4) : 0;  // at most 32 KB
+  RowPipe p{};
+  if (VEC == 8) p = rms_pipe(l, a.R, blocks, a.s, sx, a.dy, sy, a.ds, sx);
+  if (p.stages) blocks = imin64(blocks, sm_count() * rms_pipe_blocks(p));
+  *part_rows = blocks;
+#define RMS_GO(TPR, NV)                                                                                         \
+  {                                                                                                             \
+    if constexpr (VEC == 8 && NV > 0)                                                                           \
+      if (p.stages)                                                                                             \
+        return rms_go(rms_bwd_kernel<TX, TPR, NV, VEC, true>, (unsigned)blocks,                                 \
+                      rms_pipe_smem(p) > sums ? rms_pipe_smem(p) : sums, a, p, st);                             \
+    return rms_go(rms_bwd_kernel<TX, TPR, NV, VEC, false>, (unsigned)blocks, sums, a, p, st);                   \
+  }
   RMS_LAYOUTS(VEC, l, RMS_GO)
 #undef RMS_GO
 }
+static int rms_status(cudaError_t e) {
+  if (e == cudaSuccess) return AFFB_OK;
+  set_error("rms_norm: launch failed: %s", cudaGetErrorString(e));
+  return AFFB_ERR_CUDA;
+}
+cudaError_t rms_failed(int* failed) { return cudaMemcpyFromSymbol(failed, g_rms_failed, sizeof(int)); }
 
 static bool rms_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -442,12 +659,7 @@ extern "C" int affb_rms_norm_fwd(const void* x, int x_dtype, const void* delta, 
   const bool vec = C % 8 == 0 && rms_aligned(x) && rms_aligned(delta) && rms_aligned(weight) && rms_aligned(s) &&
                    rms_aligned(y) && ((uintptr_t)q & 7) == 0;
   cudaStream_t st = as_stream(stream);
-  AFFB_DISPATCH(x_dtype, TX, {
-    if (vec) rms_fwd_launch<TX, 8>(a, st);
-    else rms_fwd_launch<TX, 1>(a, st);
-  });
-  AFFB_LAUNCH_CHECK("affb_rms_norm_fwd");
-  return AFFB_OK;
+  AFFB_DISPATCH(x_dtype, TX, return rms_status(vec ? rms_fwd_launch<TX, 8>(a, st) : rms_fwd_launch<TX, 1>(a, st)));
 }
 
 extern "C" int affb_quantize_e4m3(const void* x, int dtype, int64_t R, int64_t C, void* q, float* q_scale,
@@ -459,12 +671,7 @@ extern "C" int affb_quantize_e4m3(const void* x, int dtype, int64_t R, int64_t C
   RmsArgs a{x, nullptr, AFFB_F32, nullptr, 1, nullptr, 0.f, R, (int)C, nullptr, nullptr, nullptr, AFFB_F32, (uint8_t*)q, q_scale};
   const bool vec = C % 8 == 0 && rms_aligned(x) && ((uintptr_t)q & 7) == 0;
   cudaStream_t st = as_stream(stream);
-  AFFB_DISPATCH(dtype, TX, {
-    if (vec) rms_fwd_launch<TX, 8>(a, st);
-    else rms_fwd_launch<TX, 1>(a, st);
-  });
-  AFFB_LAUNCH_CHECK("affb_quantize_e4m3");
-  return AFFB_OK;
+  AFFB_DISPATCH(dtype, TX, return rms_status(vec ? rms_fwd_launch<TX, 8>(a, st) : rms_fwd_launch<TX, 1>(a, st)));
 }
 
 extern "C" int64_t affb_rms_norm_bwd_workspace_bytes(int64_t R, int64_t C) {
@@ -492,14 +699,14 @@ extern "C" int affb_rms_norm_bwd(const void* dy, int y_dtype, const void* ds, co
   AFFB_REQUIRE(s && rstd && weight, "rms_norm: null pointer");
   const bool vec = C % 8 == 0 && rms_aligned(dy) && rms_aligned(ds) && rms_aligned(s) && rms_aligned(weight) &&
                    rms_aligned(dx) && rms_aligned(ddelta);
-  const int64_t blocks = rms_bwd_blocks(R, 256 / rms_layout(C, vec ? 8 : 1).tpr);
-  AFFB_REQUIRE(!dweight || (workspace && workspace_bytes >= blocks * C * 4), "rms_norm: workspace too small");
+  AFFB_REQUIRE(!dweight || (workspace && workspace_bytes >= affb_rms_norm_bwd_workspace_bytes(R, C)),
+               "rms_norm: workspace too small");
+  int64_t blocks = 0;
   RmsBwdArgs a{dy, y_dtype, ds, s, rstd, weight, row_scale, row_scale ? R / groups : 1, R, (int)C, dx, ddelta, delta_dtype,
                dweight ? (float*)workspace : nullptr};
-  AFFB_DISPATCH(x_dtype, TX, {
-    if (vec) rms_bwd_launch<TX, 8>(a, st);
-    else rms_bwd_launch<TX, 1>(a, st);
-  });
+  AFFB_DISPATCH(x_dtype, TX,
+                if ((rc = rms_status(vec ? rms_bwd_launch<TX, 8>(a, &blocks, st) : rms_bwd_launch<TX, 1>(a, &blocks, st))))
+                  return rc);
   if (dweight) rms_dw_kernel<<<(unsigned)((C + 31) / 32), 1024, 0, st>>>((const float*)workspace, blocks, (int)C, dweight);
   AFFB_LAUNCH_CHECK("affb_rms_norm_bwd");
   return AFFB_OK;

@@ -265,7 +265,7 @@ class LinearE4M3(nn.Module):
 
 
 def linear_status() -> bool:
-    """True unless a product on the current device gave up a bounded wait
+    """True unless a product or norm on the current device gave up a bounded wait
     (which leaves its output incomplete).  Synchronises."""
     import ctypes
     failed = ctypes.c_int(0)

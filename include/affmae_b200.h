@@ -391,8 +391,8 @@ int64_t affb_linear_e4m3_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int affb_linear_e4m3(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
                      const float* bias, const void* residual, int residual_dtype, int act, int64_t M, int64_t N,
                      int64_t K, void* out, int out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
-/* 1 in *failed if a product on this device ever gave up one of its bounded
- * waits (its output is then incomplete), else 0.  Synchronises.             */
+/* 1 in *failed if a product or norm on this device ever gave up one of its
+ * bounded waits (its output is then incomplete), else 0.  Synchronises.     */
 int affb_linear_status(int* failed);
 
 /* ------------------------------------------- root-mean-square norm --
