@@ -120,8 +120,9 @@ __device__ __forceinline__ float activate_grad(float z) {
     const float pdf = 0.3989422804014327f * exp2_approx(-0.5f * LOG2E * a * a);
     return fmaf(copysignf(a, z), pdf, z > 0.f ? 1.f - t : t);
   } else if constexpr (ACT == AFFB_ACT_SILU) {
-    const float s = __fdividef(1.f, 1.f + exp2_approx(-LOG2E * z));
-    return s > 0.f ? s * fmaf(z, 1.f - s, 1.f) : s;
+    const float c = max_nan(min_nan(z, 64.f), -64.f);  // keeps inf * 0 out
+    const float s = __fdividef(1.f, 1.f + exp2_approx(-LOG2E * c));
+    return s * fmaf(c, 1.f - s, 1.f);
   } else {
     return 1.f;
   }

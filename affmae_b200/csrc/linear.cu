@@ -873,7 +873,7 @@ extern "C" int affb_linear_fwd(const void* x, const void* weight, const void* bi
   if (M == 0) return AFFB_OK;
   AFFB_REQUIRE(x && weight && out, "linear: null pointer");
   AFFB_REQUIRE(workspace || affb_linear_fwd_workspace_bytes(dtype, M, N, K) == 0, "linear: workspace missing");
-  LinearEpilogue e{nullptr, nullptr, bias, bias_dtype, residual, residual_dtype, act, out, out_dtype, z, dtype};
+  LinearEpilogue e{nullptr, nullptr, bias, bias_dtype, residual, residual_dtype, act, out, out_dtype, z, z_type(dtype, act)};
   return forward(x, weight, dtype, M, N, K, e, workspace, workspace_bytes, as_stream(stream));
 }
 

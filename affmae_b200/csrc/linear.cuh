@@ -13,6 +13,14 @@ inline bool is_float_dtype(int dtype) { return dtype == AFFB_F32 || dtype == AFF
 inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 inline bool aligned_to(const void* p, int64_t a) { return ((uintptr_t)p & (uintptr_t)(a - 1)) == 0; }
 
+// Type of the pre-activation sums kept for the backward: fp16 in place of bf16
+// where the activation is smooth (its gradient wants absolute accuracy: with
+// bf16 sums the GELU layer's dx is off by 1.45 times its own rounding, with
+// fp16 ones by 1.35), the operands' own for the sign that ReLU needs.
+inline int z_type(int dtype, int act) {
+  return dtype == AFFB_BF16 && (act == AFFB_ACT_GELU || act == AFFB_ACT_SILU) ? AFFB_F16 : dtype;
+}
+
 // What follows the sums x . w of an output: scales (e4m3 operands), bias,
 // activation, residual, and where they go.
 struct LinearEpilogue {

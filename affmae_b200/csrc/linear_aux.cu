@@ -92,8 +92,8 @@ __device__ __forceinline__ void ldn(const T* p, float* o) {
 // Block: DZ_COLS columns x one strip of rows.  A thread keeps VEC columns and
 // walks down the strip; the threads of a column group are summed in order, so
 // the sums do not depend on timing.
-template <typename TO, typename T, int ACT, int VEC>
-__global__ void __launch_bounds__(DZ_THREADS) dz_kernel(const TO* __restrict__ dout, const T* __restrict__ z, int64_t R,
+template <typename TO, typename T, typename TZ, int ACT, int VEC>
+__global__ void __launch_bounds__(DZ_THREADS) dz_kernel(const TO* __restrict__ dout, const TZ* __restrict__ z, int64_t R,
                                                         int64_t C, void* __restrict__ dz, int64_t ld, int64_t strip,
                                                         float* __restrict__ part) {
   constexpr bool SPLIT = std::is_same<T, float>::value;
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(DZ_THREADS) dz_kernel(const TO* __restrict__ d
       ldn<TO, VEC>(dout + r * C + c, d);
       if constexpr (ACT != AFFB_ACT_NONE) {
         float zz[VEC];
-        ldn<T, VEC>(z + r * C + c, zz);
+        ldn<TZ, VEC>(z + r * C + c, zz);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) d[k] *= activate_grad<ACT>(zz[k]);
       }
@@ -162,10 +162,14 @@ static int dz_launch(const void* dout, const void* z, int64_t R, int64_t C, void
   const int64_t strip = (R + strips - 1) / strips;
   const dim3 grid((unsigned)((C + DZ_COLS - 1) / DZ_COLS), (unsigned)strips);
   const bool vec = C % 8 == 0 && aligned_to(dout, 16) && aligned_to(z, 16) && aligned_to(dz, 16) && ld % 8 == 0;
+  // the type that z_type() names
+  using TZ = typename std::conditional<std::is_same<T, __nv_bfloat16>::value &&
+                                           (ACT == AFFB_ACT_GELU || ACT == AFFB_ACT_SILU),
+                                       __half, T>::type;
   if (vec)
-    dz_kernel<TO, T, ACT, 8><<<grid, DZ_THREADS, 0, st>>>((const TO*)dout, (const T*)z, R, C, dz, ld, strip, part);
+    dz_kernel<TO, T, TZ, ACT, 8><<<grid, DZ_THREADS, 0, st>>>((const TO*)dout, (const TZ*)z, R, C, dz, ld, strip, part);
   else
-    dz_kernel<TO, T, ACT, 1><<<grid, DZ_THREADS, 0, st>>>((const TO*)dout, (const T*)z, R, C, dz, ld, strip, part);
+    dz_kernel<TO, T, TZ, ACT, 1><<<grid, DZ_THREADS, 0, st>>>((const TO*)dout, (const TZ*)z, R, C, dz, ld, strip, part);
   AFFB_LAUNCH_CHECK("linear: activation gradient");
   return AFFB_OK;
 }

@@ -118,11 +118,11 @@ __device__ __forceinline__ float row_reduce(float v, float* red, Op op) {
 // Set when a wait on a copy ran out; read by rms_failed().
 __device__ int g_rms_failed;
 
-// Rounds of rows on their way into shared memory: up to three arrays with the
+// Rounds of rows on their way into shared memory: up to four arrays with the
 // same rows, stage after stage.
 struct RowPipe {
-  const void* src[3];
-  int row_bytes[3];   // 0: no such array
+  const void* src[4];
+  int row_bytes[4];   // 0: no such array
   int rows;           // of a round
   int stages;
   int stage_bytes;
@@ -159,10 +159,10 @@ struct PipeReader {
     const int64_t r0 = ((int64_t)blockIdx.x + it * gridDim.x) * ROWS;
     if (r0 >= R) return;
     const int n = (int)imin64(ROWS, R - r0);
-    tc5::bar_expect(bars + 8 * st, (uint32_t)(n * (p.row_bytes[0] + p.row_bytes[1] + p.row_bytes[2])));
+    tc5::bar_expect(bars + 8 * st, (uint32_t)(n * (p.row_bytes[0] + p.row_bytes[1] + p.row_bytes[2] + p.row_bytes[3])));
     uint32_t to = tc5::smem_addr(base + st * p.stage_bytes);
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 0; i < 4; ++i) {
       if (p.row_bytes[i]) {
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
                      "l"((const unsigned char*)p.src[i] + r0 * p.row_bytes[i]), "r"(n * p.row_bytes[i]),
@@ -352,7 +352,8 @@ struct RmsBwdArgs {
   const void* dy;          // y_dtype, or null
   int y_dtype;
   const void* ds;          // x's dtype, or null
-  const void* s;           // x's dtype: the saved sum (x itself without delta)
+  const void* s;           // x's dtype: the saved sum, or x where delta is given
+  const void* delta;       // delta_dtype: the sum is x + f delta again (a 16-bit sum is not what was normed), or null
   const float* rstd;
   const float* w;
   const float* row_scale;
@@ -365,7 +366,7 @@ struct RmsBwdArgs {
   float* part;             // [blocks][C] sums of dy s rstd, or null
 };
 
-// PIPE: rows come through shared memory (s, dy, ds).
+// PIPE: rows come through shared memory (s, dy, ds, delta).
 template <typename TX, int TPR, int NV, int VEC, bool PIPE>
 __global__ void __launch_bounds__(256) rms_bwd_kernel(const __grid_constant__ RmsBwdArgs a,
                                                       const __grid_constant__ RowPipe pipe) {
@@ -406,9 +407,16 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(const __grid_constant__ Rm
       }
     }
     const float rstd = in ? a.rstd[r] : 0.f;
+    const float f = a.row_scale && in ? group_scale(a.row_scale, r, a.rows_per_scale) : 1.f;
     float sv[KEEP][VEC], gv[KEEP][VEC];
     auto chunk = [&](int c, float* s, float* g) {
       row_load<PIPE, TX, VEC>((const TX*)a.s + r * C, PIPE ? reader->row(0, slot) : nullptr, c, s);
+      if (a.delta) {
+        float dd[VEC];
+        row_load_as<PIPE, VEC>(a.delta, a.delta_dtype, r * C, PIPE ? reader->row(3, slot) : nullptr, c, dd);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s[k] = a.row_scale ? fmaf(f, dd[k], s[k]) : s[k] + dd[k];
+      }
 #pragma unroll
       for (int k = 0; k < VEC; ++k) g[k] = 0.f;
       if (a.dy) row_load_as<PIPE, VEC>(a.dy, a.y_dtype, r * C, PIPE ? reader->row(1, slot) : nullptr, c, g);
@@ -443,7 +451,6 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(const __grid_constant__ Rm
     }
     const float coef = row_reduce<TPR>(dot, red[flip], AddOp()) * inv_c * rstd * rstd;
     flip ^= 1;
-    const float f = a.row_scale && in ? group_scale(a.row_scale, r, a.rows_per_scale) : 1.f;
 #pragma unroll
     for (int i = 0; i < steps; ++i) {
       const int c = (i * TPR + t) * VEC, n = NV > 0 ? i : 0;
@@ -551,10 +558,15 @@ static int64_t rms_bwd_blocks(int64_t R, int64_t rows) {
 // blocks: stages 0 where a block has fewer than three rounds (nothing to
 // prefetch), or two stages do not fit beside a second block.
 static RowPipe rms_pipe(const RowLayout& l, int64_t R, int64_t blocks, const void* a, int64_t a_bytes, const void* b,
-                        int64_t b_bytes, const void* c, int64_t c_bytes) {
-  RowPipe p{{a, b, c}, {(int)a_bytes, b ? (int)b_bytes : 0, c ? (int)c_bytes : 0}, 256 / l.tpr, 0, 0};
+                        int64_t b_bytes, const void* c = nullptr, int64_t c_bytes = 0, const void* d = nullptr,
+                        int64_t d_bytes = 0) {
+  RowPipe p{{a, b, c, d},
+            {(int)a_bytes, b ? (int)b_bytes : 0, c ? (int)c_bytes : 0, d ? (int)d_bytes : 0},
+            256 / l.tpr,
+            0,
+            0};
   if (l.nv == 0 || R < 3 * blocks * p.rows) return p;
-  p.stage_bytes = p.rows * (p.row_bytes[0] + p.row_bytes[1] + p.row_bytes[2]);
+  p.stage_bytes = p.rows * (p.row_bytes[0] + p.row_bytes[1] + p.row_bytes[2] + p.row_bytes[3]);
   p.stage_bytes = (p.stage_bytes + 127) / 128 * 128;
   p.stages = PIPE_BYTES / p.stage_bytes;
   if (p.stages > 4) p.stages = 4;
@@ -584,7 +596,7 @@ static cudaError_t rms_fwd_launch(const RmsArgs& a, cudaStream_t st) {
   RowPipe p{};
   if (VEC == 8 && sizeof(TX) == 2)
     p = rms_pipe(l, a.R, (int64_t)sm_count() * 4, a.x, a.C * (int64_t)sizeof(TX), a.delta,
-                 a.C * (a.delta_dtype == AFFB_F32 ? 4 : 2), nullptr, 0);
+                 a.C * (a.delta_dtype == AFFB_F32 ? 4 : 2));
   const unsigned blocks = (unsigned)imin64(rounds, (int64_t)sm_count() * (p.stages ? rms_pipe_blocks(p) : 8));
 #define RMS_GO(TPR, NV)                                                                                          \
   {                                                                                                              \
@@ -599,12 +611,13 @@ static cudaError_t rms_fwd_launch(const RmsArgs& a, cudaStream_t st) {
 template <typename TX, int VEC>
 static cudaError_t rms_bwd_launch(const RmsBwdArgs& a, int64_t* part_rows, cudaStream_t st) {
   const int64_t sx = a.C * (int64_t)sizeof(TX), sy = a.C * (a.y_dtype == AFFB_F32 ? 4 : 2);
-  const RowLayout l = rms_layout(a.C, VEC, sx + (a.dy ? sy : 0) + (a.ds ? sx : 0));
+  const int64_t sd = a.C * (a.delta_dtype == AFFB_F32 ? 4 : 2);
+  const RowLayout l = rms_layout(a.C, VEC, sx + (a.dy ? sy : 0) + (a.ds ? sx : 0) + (a.delta ? sd : 0));
   const int64_t rows = 256 / l.tpr;
   int64_t blocks = rms_bwd_blocks(a.R, rows);
   const int sums = a.part && l.nv > 0 ? (int)(rows * a.C * 4) : 0;  // at most 32 KB
   RowPipe p{};
-  if (VEC == 8) p = rms_pipe(l, a.R, blocks, a.s, sx, a.dy, sy, a.ds, sx);
+  if (VEC == 8) p = rms_pipe(l, a.R, blocks, a.s, sx, a.dy, sy, a.ds, sx, a.delta, sd);
   if (p.stages) blocks = imin64(blocks, sm_count() * rms_pipe_blocks(p));
   *part_rows = blocks;
 #define RMS_GO(TPR, NV)                                                                                         \
@@ -681,10 +694,10 @@ extern "C" int64_t affb_rms_norm_bwd_workspace_bytes(int64_t R, int64_t C) {
 }
 
 extern "C" int affb_rms_norm_bwd(const void* dy, int y_dtype, const void* ds, const void* s, int x_dtype,
-                                 const float* rstd, const float* weight, const float* row_scale, int64_t groups,
+                                 const void* delta, const float* rstd, const float* weight, const float* row_scale, int64_t groups,
                                  int64_t R, int64_t C, void* dx, void* ddelta, int delta_dtype, float* dweight,
                                  void* workspace, int64_t workspace_bytes, void* stream) {
-  int rc = rms_check(x_dtype, delta_dtype, ddelta != nullptr, R, C, ddelta ? row_scale : nullptr, groups);
+  int rc = rms_check(x_dtype, delta_dtype, ddelta || delta, R, C, ddelta || delta ? row_scale : nullptr, groups);
   if (rc) return rc;
   AFFB_REQUIRE(!dy || y_dtype == AFFB_F32 || y_dtype == AFFB_F16 || y_dtype == AFFB_BF16,
                "rms_norm: dy must be fp32, fp16 or bf16");
@@ -698,11 +711,11 @@ extern "C" int affb_rms_norm_bwd(const void* dy, int y_dtype, const void* ds, co
   }
   AFFB_REQUIRE(s && rstd && weight, "rms_norm: null pointer");
   const bool vec = C % 8 == 0 && rms_aligned(dy) && rms_aligned(ds) && rms_aligned(s) && rms_aligned(weight) &&
-                   rms_aligned(dx) && rms_aligned(ddelta);
+                   rms_aligned(dx) && rms_aligned(ddelta) && rms_aligned(delta);
   AFFB_REQUIRE(!dweight || (workspace && workspace_bytes >= affb_rms_norm_bwd_workspace_bytes(R, C)),
                "rms_norm: workspace too small");
   int64_t blocks = 0;
-  RmsBwdArgs a{dy, y_dtype, ds, s, rstd, weight, row_scale, row_scale ? R / groups : 1, R, (int)C, dx, ddelta, delta_dtype,
+  RmsBwdArgs a{dy, y_dtype, ds, s, delta, rstd, weight, row_scale, row_scale ? R / groups : 1, R, (int)C, dx, ddelta, delta_dtype,
                dweight ? (float*)workspace : nullptr};
   AFFB_DISPATCH(x_dtype, TX,
                 if ((rc = rms_status(vec ? rms_bwd_launch<TX, 8>(a, &blocks, st) : rms_bwd_launch<TX, 1>(a, &blocks, st))))

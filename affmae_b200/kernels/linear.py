@@ -87,7 +87,7 @@ def linear_fwd(x, weight, bias, residual, act: int, save: bool):
         out, rptr, rdt = torch.empty_like(residual), residual.data_ptr(), _CODE[residual.dtype]
     z = None
     if save and linear_saves(act, residual):
-        z = x.new_empty(out.shape)
+        z = x.new_empty(out.shape, dtype=z_dtype(x.dtype, act))
         zptr = z.data_ptr()
     ws = nat.workspace(index, "affb_linear_fwd_workspace_bytes", x, dt, M, N, K)
     if ws is not None:
@@ -101,6 +101,12 @@ def linear_saves(act: int, residual) -> bool:
     """Whether the backward needs the pre-activation sums: not without an
     activation, and the sign of ReLU's output serves as well as theirs."""
     return act != 0 and not (act == ACTIVATIONS["relu"] and residual is None)
+
+
+def z_dtype(dtype: torch.dtype, act: int) -> torch.dtype:
+    """Type of the pre-activation sums kept for the backward: fp16 instead of
+    bf16 for GELU and SiLU, whose gradients want their absolute accuracy."""
+    return torch.float16 if dtype == torch.bfloat16 and act >= ACTIVATIONS["gelu"] else dtype
 
 
 def linear_bwd(dout, z, x, weight, act: int, need_x: bool, need_w: bool, bias_dtype):

@@ -9,7 +9,8 @@
 * ``FusedRMSNorm``: the module.
 
 Statistics are fp32, taken of the sum before it is rounded to x's dtype; the
-backward reads the rounded sum.
+backward forms a 16-bit stream's sum again from x and delta (in fp32 it reads
+the sum).
 """
 from __future__ import annotations
 
@@ -83,9 +84,10 @@ def _launch(x, delta, row_scale, weight, eps, out_dtype, keep):
     return xc, rs, w, s, rstd, y, q, scale
 
 
-def rms_norm_bwd(dy, ds, s, rstd, weight, row_scale, need_x: bool, need_w: bool, delta_dtype):
+def rms_norm_bwd(dy, ds, s, rstd, weight, row_scale, need_x: bool, need_w: bool, delta_dtype, delta=None):
     """(dx, dw, ddelta), None where not needed (`delta_dtype` None: no
-    ddelta); weight, row_scale, dw fp32; dy or ds may be None."""
+    ddelta); weight, row_scale, dw fp32; dy or ds may be None.  With `delta`,
+    s is x and the sum is formed again."""
     C = s.shape[-1]
     R = s.numel() // C
     index = s.get_device()
@@ -94,9 +96,10 @@ def rms_norm_bwd(dy, ds, s, rstd, weight, row_scale, need_x: bool, need_w: bool,
     dw = s.new_empty(C, dtype=torch.float32) if need_w else None
     ws = nat.workspace(index, "affb_rms_norm_bwd_workspace_bytes", s, R, C) if need_w else None
     nat.call_on(index, "affb_rms_norm_bwd", nat.ptr(dy), nat.dcode(dy) if dy is not None else 0, nat.ptr(ds), nat.ptr(s),
-                nat.dcode(s), nat.ptr(rstd), nat.ptr(weight), nat.ptr(row_scale),
+                nat.dcode(s), nat.ptr(delta), nat.ptr(rstd), nat.ptr(weight), nat.ptr(row_scale),
                 row_scale.numel() if row_scale is not None else 0, R, C, nat.ptr(dx), nat.ptr(dd),
-                nat.dcode(dd) if dd is not None else 0, nat.ptr(dw), nat.ptr(ws), ws.numel() if ws is not None else 0)
+                nat.dcode(dd if dd is not None else delta) if dd is not None or delta is not None else 0, nat.ptr(dw),
+                nat.ptr(ws), ws.numel() if ws is not None else 0)
     return dx, dw, dd
 
 
@@ -107,19 +110,20 @@ class FusedRMSNormFunction(Function):
         keep = any(ctx.needs_input_grad[:3])
         xc, rs, w, s, rstd, y, _, _ = _launch(x, delta, row_scale, weight, eps, out_dtype, keep)
         if keep:
-            ctx.save_for_backward(xc if s is None else s, rstd, w, rs)
+            again = s is not None and x.dtype != torch.float32
+            ctx.save_for_backward(xc if s is None or again else s, rstd, w, rs, nat.dense(delta) if again else None)
             ctx.meta = (weight.dtype, delta.dtype if delta is not None else None)
         return y if s is None else (s, y)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        s, rstd, w, rs = ctx.saved_tensors
+        s, rstd, w, rs, delta = ctx.saved_tensors
         wdt, ddt = ctx.meta
         ds, dy = grads if ddt is not None else (None, grads[0])
         need_x, need_w, need_d = ctx.needs_input_grad[:3]
         dx, dw, dd = rms_norm_bwd(nat.dense(dy) if dy is not None else None, nat.dense(ds) if ds is not None else None,
-                                  s, rstd, w, rs, need_x, need_w, ddt if need_d else None)
+                                  s, rstd, w, rs, need_x, need_w, ddt if need_d else None, delta)
         return dx, dw.to(wdt) if need_w else None, dd, None, None, None
 
 

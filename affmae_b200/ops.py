@@ -200,7 +200,8 @@ def _(x, weight, bias, act, residual):
     shape = (*x.shape[:-1], weight.shape[0])
     saves = _li.linear_saves(_li._act_code(act), residual)
     return (x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype),
-            x.new_empty(shape if saves else _EMPTY))
+            x.new_empty(shape if saves else _EMPTY,
+                        dtype=_li.z_dtype(x.dtype, _li._act_code(act)) if saves else x.dtype))
 
 
 @custom_op("affb200::linear_bwd", mutates_args=())
@@ -264,11 +265,13 @@ def _(x, weight, eps, delta, row_scale, out_dtype):
 @custom_op("affb200::rms_norm_bwd", mutates_args=())
 def rms_norm_bwd(dy: Optional[Tensor], ds: Optional[Tensor], s: Tensor, rstd: Tensor, weight: Tensor,
                  row_scale: Optional[Tensor], delta: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
+    """s: the forward's sum in fp32; x itself in 16 bits or without delta."""
     dx, dw, dd = _rn.rms_norm_bwd(_nat.dense(dy) if dy is not None else None,
                                   _nat.dense(ds) if ds is not None else None, _nat.dense(s), rstd,
                                   _nat.dense(weight.float()),
                                   row_scale.float().contiguous() if row_scale is not None else None, True, True,
-                                  delta.dtype if delta is not None else None)
+                                  delta.dtype if delta is not None else None,
+                                  _nat.dense(delta) if delta is not None and s.dtype != torch.float32 else None)
     return dx, dw.to(weight.dtype), (dd if dd is not None else s.new_empty(_EMPTY))
 
 
@@ -281,7 +284,7 @@ def _(dy, ds, s, rstd, weight, row_scale, delta):
 def _rms_setup(ctx, inputs, output):
     x, weight, eps, delta, row_scale, out_dtype = inputs
     s, y, rstd = output
-    ctx.save_for_backward(x if delta is None else s, rstd, weight, row_scale, delta)
+    ctx.save_for_backward(s if delta is not None and x.dtype == torch.float32 else x, rstd, weight, row_scale, delta)
     ctx.set_materialize_grads(False)
 
 

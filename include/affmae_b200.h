@@ -365,8 +365,11 @@ int affb_cast_f32(const float* src, void* dst, int dtype, int64_t n, void* strea
  * ---------------------------------------------------- matrix product --
  * z = x w^T + bias, out = act(z) + residual.  x [M,K] T, weight [N,K] T,
  * bias [N] bias_dtype or NULL, residual [M,N] residual_dtype or NULL,
- * out [M,N] out_dtype (T or fp32), z [M,N] T or NULL: the pre-activation
- * sums for the backward.  N, K >= 1, M >= 0.  x and weight 16-byte aligned.
+ * out [M,N] out_dtype (T or fp32), z [M,N] or NULL: the pre-activation sums
+ * for the backward, in T, or fp16 where T is bf16 and the activation smooth
+ * (GELU, SiLU): its gradient needs them to an absolute accuracy, and the three
+ * bits more keep their rounding out of the gradients; past 65504 they are
+ * infinite, where the gradient is constant.  N, K >= 1, M >= 0.  x and weight 16-byte aligned.
  * Sums are fp32; fp32 operands are multiplied as three bf16 parts each
  * (error of the order of 2^-24; an infinite operand gives NaN).
  * workspace: affb_linear_fwd_workspace_bytes(...) bytes, 256-byte aligned, no
@@ -409,13 +412,15 @@ int affb_rms_norm_fwd(const void* x, int x_dtype, const void* delta, int delta_d
 /* Rows of x [R,C] as e4m3 values q [R,C] with q_scale [R]: the scale above,
  * of the rows themselves (weights and inputs of affb_linear_e4m3).          */
 int affb_quantize_e4m3(const void* x, int dtype, int64_t R, int64_t C, void* q, float* q_scale, void* stream);
-/* dy [R,C] y_dtype or NULL, ds [R,C] x_dtype or NULL: gradients of y and s;
- * s [R,C] x_dtype: the forward's sum (x itself without delta).  dx [R,C]
- * x_dtype, ddelta [R,C] delta_dtype, dweight [C] fp32, each written unless
- * NULL.  workspace: affb_rms_norm_bwd_workspace_bytes(R, C) bytes.          */
+/* dy [R,C] y_dtype or NULL, ds [R,C] x_dtype or NULL: gradients of y and s.
+ * s [R,C] x_dtype: the forward's sum (x itself without delta); with delta
+ * [R,C] delta_dtype not NULL, s is x and the sum is formed again (a sum that
+ * was rounded to 16 bits is not the one that was normed).  dx [R,C] x_dtype,
+ * ddelta [R,C] delta_dtype, dweight [C] fp32, each written unless NULL.
+ * workspace: affb_rms_norm_bwd_workspace_bytes(R, C) bytes.                 */
 int64_t affb_rms_norm_bwd_workspace_bytes(int64_t R, int64_t C);
-int affb_rms_norm_bwd(const void* dy, int y_dtype, const void* ds, const void* s, int x_dtype, const float* rstd,
-                      const float* weight, const float* row_scale, int64_t groups, int64_t R, int64_t C, void* dx,
+int affb_rms_norm_bwd(const void* dy, int y_dtype, const void* ds, const void* s, int x_dtype, const void* delta,
+                      const float* rstd, const float* weight, const float* row_scale, int64_t groups, int64_t R, int64_t C, void* dx,
                       void* ddelta, int delta_dtype, float* dweight, void* workspace, int64_t workspace_bytes,
                       void* stream);
 

@@ -200,6 +200,21 @@ def test_linear_nonfinite_rows_stay_in_their_rows(cuda):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_linear_gradients_of_huge_sums(cuda, act):
+    """Sums beyond fp16's range (in which bf16 layers keep them): the slope is 1 above and 0 below."""
+    x = torch.full((64, 32), 300.0, device=cuda, dtype=BF16).requires_grad_(True)
+    w = torch.full((16, 32), 50.0, device=cuda, dtype=BF16)
+    w[::2] *= -1
+    dout = rnd(cuda, 35, 64, 16, dtype=BF16)
+    y = fused_linear(x, w, None, act)
+    (dx,) = torch.autograd.grad(y, x, dout)
+    assert (y[:, 1::2] == torch.tensor(32 * 300 * 50.0, device=cuda).to(BF16)).all() and not y[:, ::2].any()
+    want = dout.double()[:, 1::2].sum(1, keepdim=True) * 50
+    within(dx, want.expand(-1, 32), 8 * E * 50 * dout.double().abs().sum(1, keepdim=True) + U[BF16] * want.abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["gelu", "silu"])
 def test_linear_gradients_against_differences(cuda, act):
     """Directional differences of the fp32 forward: the central difference's own error is h^2 / 6 of the third
     derivative along the direction (of order one, h = 2^-6: 4e-5) and 2^-22 / h of the sum's magnitude."""
@@ -364,8 +379,8 @@ def norm_ref(x, w, eps, delta, f, dy=None, ds=None):
         return sd, serr, yd, yerr
     grads = torch.autograd.grad((s, y) if ds is not None else y, leaves + ([d] if d is not None else []),
                                 (ds.double(), dy.double()) if ds is not None else dy.double())
-    # the backward reads s rounded to x's type: relative error u of s, once in each factor s and r of the formula
-    u = (U[x.dtype] if delta is not None else 0.0) + rel
+    # the sum is that of the forward, unrounded: relative error u of s, once in each factor s and r of the formula
+    u = rel
     g = dy.double() * w.double()
     gs = (g * sd).abs().mean(-1, keepdim=True)
     dx_err = rd * (g.abs() * 2 * rel + 4 * u * sd.abs() * rd ** 2 * gs) + rel * grads[0].abs() + \

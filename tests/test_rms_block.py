@@ -180,7 +180,7 @@ def test_block_operators_have_schemas_and_fake_shapes():
         x, w = torch.empty((3, 5, 8), dtype=BF16), torch.empty((6, 8), dtype=BF16)
         res = torch.empty((3, 5, 6))
         out, z = ops.linear_fwd(x, w, None, "gelu", res)
-        assert out.shape == (3, 5, 6) and out.dtype == torch.float32 and z.shape == out.shape and z.dtype == BF16
+        assert out.shape == (3, 5, 6) and out.dtype == torch.float32 and z.shape == out.shape and z.dtype == torch.float16
         assert ops.linear_fwd(x, w, None, "relu", None)[1].numel() == 0
         dx, dw, db = ops.linear_bwd(out, z, x, w, None, "gelu")
         assert dx.shape == x.shape and dw.shape == w.shape and db.numel() == 0
