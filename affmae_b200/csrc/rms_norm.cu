@@ -512,24 +512,25 @@ __global__ void __launch_bounds__(1024) rms_dw_kernel(const float* __restrict__ 
 }
 
 constexpr int PIPE_BYTES = 54 * 1024;  // of a block: four on an SM
-constexpr int PIPE_MOST = 112 * 1024;  // two on an SM
+constexpr int PIPE_MOST = 200 * 1024;  // or one, for the widest rows
 
-// Threads that share a row, and chunks each holds (0: more than fit).
-// `row_bytes`: of the rows that come through shared memory; where two rounds of
-// sixteen rows would not fit there, a row of 33 to 48 chunks is shared by 32
-// threads instead of 16 (backward of 83888 x 384 fp32: 138 -> 115 us).
+// Threads that share a row, and chunks each holds (0: more than fit).  In the
+// backward, which keeps four or five arrays of a row, rows of 33 to 48 chunks
+// are shared by 32 threads instead of 16 (83888 x 384: fp32 138 -> 115 us,
+// bf16 101 -> 92) and rows of 65 to 128 by the block instead of a warp
+// (16384 x 1024: fp32 83 -> 57 us, bf16 134 -> 55).
 struct RowLayout {
   int tpr, nv;
 };
-static RowLayout rms_layout(int64_t C, int vec, int64_t row_bytes) {
+static RowLayout rms_layout(int64_t C, int vec, bool backward) {
   const int64_t n = (C + vec - 1) / vec;  // chunks of a row
   if (vec == 8) {
     if (n <= 8) return {8, 1};
     if (n <= 16) return {16, 1};
     if (n <= 32) return {32, 1};
-    if (n <= 48 && 32 * row_bytes <= PIPE_MOST) return {16, 3};
+    if (n <= 48 && !backward) return {16, 3};
     if (n <= 64) return {32, 2};
-    if (n <= 128) return {32, 4};
+    if (n <= 128 && !backward) return {32, 4};
   } else {
     if (n <= 32) return {32, 1};
     if (n <= 128) return {32, 4};
@@ -589,8 +590,7 @@ static cudaError_t rms_go(K kernel, unsigned blocks, int smem, const A& a, const
 
 template <typename TX, int VEC>
 static cudaError_t rms_fwd_launch(const RmsArgs& a, cudaStream_t st) {
-  const int64_t row_bytes = a.C * (int64_t)sizeof(TX) + (a.delta ? a.C * (a.delta_dtype == AFFB_F32 ? 4 : 2) : 0);
-  const RowLayout l = rms_layout(a.C, VEC, sizeof(TX) == 2 ? row_bytes : 0);
+  const RowLayout l = rms_layout(a.C, VEC, false);
   const int64_t rows = 256 / l.tpr, rounds = (a.R + rows - 1) / rows;
   // fp32 rows keep enough bytes on the way without the pipe (16384 x 4096: 129 us, 146 with it; bf16: 121 and 90)
   RowPipe p{};
@@ -612,7 +612,7 @@ template <typename TX, int VEC>
 static cudaError_t rms_bwd_launch(const RmsBwdArgs& a, int64_t* part_rows, cudaStream_t st) {
   const int64_t sx = a.C * (int64_t)sizeof(TX), sy = a.C * (a.y_dtype == AFFB_F32 ? 4 : 2);
   const int64_t sd = a.C * (a.delta_dtype == AFFB_F32 ? 4 : 2);
-  const RowLayout l = rms_layout(a.C, VEC, sx + (a.dy ? sy : 0) + (a.ds ? sx : 0) + (a.delta ? sd : 0));
+  const RowLayout l = rms_layout(a.C, VEC, true);
   const int64_t rows = 256 / l.tpr;
   int64_t blocks = rms_bwd_blocks(a.R, rows);
   const int sums = a.part && l.nv > 0 ? (int)(rows * a.C * 4) : 0;  // at most 32 KB
