@@ -576,13 +576,16 @@ struct Operand {
 };
 
 constexpr int PAIR_K = 6;
+constexpr int WIDEST_TWO_BUFFERS = 192;
 
 struct Shape {
   int cg, bn, nt, mt, splits;
 };
 
 // Tile and split of the contraction; `step`: multiple that the width of tiles
-// beside one another has to be (what one store covers).
+// beside one another has to be (what one store covers); `widest`: of a single
+// block's tile (two staging buffers a warp leave no room for two stages of 256
+// columns).
 //
 // Pairs of blocks (256-row tiles up to 256 columns wide) where there are
 // enough tiles, or enough k blocks to split, for all of them, and a tile's
@@ -598,7 +601,7 @@ struct Shape {
 // pairs of 128 columns instead of 42 of 192, 11.8 -> 10.9 us).
 constexpr int64_t SPLIT_COST = 2000;  // about 3 us
 
-static Shape choose_shape(int64_t M, int64_t N, int64_t total_k, int step) {
+static Shape choose_shape(int64_t M, int64_t N, int64_t total_k, int step, int widest) {
   const int64_t sms = sm_count();
   Shape s;
   const int64_t wide = (N + 255) / 256;
@@ -607,11 +610,12 @@ static Shape choose_shape(int64_t M, int64_t N, int64_t total_k, int step) {
   s.cg = M > TILE_M && total_k >= PAIR_K && pair_tiles * most_splits >= sms / 2 ? 2 : 1;
   const int64_t teams = sms / s.cg;
   s.mt = (int)((M + TILE_M * s.cg - 1) / (TILE_M * s.cg));
+  const int64_t most_bn = s.cg == 1 ? widest : 256;
   int64_t best = 0;
   for (int64_t nt = wide; nt <= 4 * wide + 3; ++nt) {
     const int64_t per = (N + nt - 1) / nt;
     const int64_t bn = round_up(per, nt > 1 ? step : s.cg == 1 ? 16 : 32);
-    if (bn > 256 || (nt > wide && bn < 64)) continue;
+    if (bn > most_bn || (nt > wide && bn < 64 && best)) continue;
     const int64_t tiles = s.mt * ((N + bn - 1) / bn);
     int64_t sp = teams / tiles < most_splits ? teams / tiles : most_splits;
     if (sp < 2) sp = 1;
@@ -633,8 +637,8 @@ static int store_step(bool direct, int out_dtype) { return direct || out_dtype =
 
 static int64_t partial_bytes(int64_t M, int64_t N, int64_t total_k) {
   int64_t most = 0;
-  for (int step = 32; step <= 64; step += 32) {
-    const Shape s = choose_shape(M, N, total_k, step);
+  for (int i = 0; i < 4; ++i) {
+    const Shape s = choose_shape(M, N, total_k, i & 1 ? 32 : 64, i & 2 ? 256 : WIDEST_TWO_BUFFERS);
     if (s.splits > 1) {
       const int64_t b = round_up((int64_t)s.splits * M * round_up(N, 4) * 4, 256);
       if (b > most) most = b;
@@ -689,7 +693,10 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
                 unsigned char* ws, cudaStream_t st) {
   const int64_t total_k = k_blocks(dtype, K);
   const bool plain = !(tma_rows(e.out, e.out_dtype, N) && (!e.z || tma_rows(e.z, e.z_dtype, N)));
-  const Shape s = choose_shape(M, N, total_k, store_step(plain, e.out_dtype == AFFB_F32 && e.z ? e.z_dtype : e.out_dtype));
+  const bool res_rows = e.residual && tma_rows(e.residual, e.residual_dtype, N);
+  const bool two_buffers = e.z || (res_rows && !plain);
+  const Shape s = choose_shape(M, N, total_k, store_step(plain, e.out_dtype == AFFB_F32 && e.z ? e.z_dtype : e.out_dtype),
+                               two_buffers ? WIDEST_TWO_BUFFERS : 256);
   const int et = dtype == AFFB_F32 ? AFFB_BF16 : dtype;  // element type in memory
   const int64_t planes = dtype == AFFB_F32 ? 3 : 1;
   GemmArgs p{};
@@ -713,7 +720,7 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
   }
   p.e = e;
   p.direct = s.splits > 1 ? 0 : plain;
-  p.res_rows = e.residual && tma_rows(e.residual, e.residual_dtype, p.N);
+  p.res_rows = e.residual && res_rows;  // not where partial products are written
   p.res_tma = p.res_rows && !e.z && !p.direct;
   p.bufs = e.z || p.res_tma ? 2 : 1;
   const int stage = A_BYTES + p.b_bytes;

@@ -259,6 +259,23 @@ def test_linear_on_a_side_stream_and_repeatable(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("shape", [(4000, 256, 96), (20000, 512, 64), (40000, 1024, 24), (100, 40000, 8), (120, 20000, 72)])
+def test_linear_wide_tiles_with_saved_sums_or_residual(cuda, dtype, shape):
+    """Tiles as wide as they get beside two staging buffers a warp, by single blocks and by pairs."""
+    M, N, K = shape
+    x, w, b = rnd(cuda, 1, M, K, dtype=dtype), rnd(cuda, 2, N, K, std=K ** -0.5, dtype=dtype), rnd(cuda, 3, N, dtype=dtype)
+    res = rnd(cuda, 4, M, N)
+    y = fused_linear(x.clone().requires_grad_(True), w, b, "gelu").detach()
+    z = fused_linear(x, w, b, "silu", res)
+    out, tol = linear_ref(x, w, b, "gelu", None)
+    within(y, out, tol, "gelu")
+    out, tol = linear_ref(x, w, b, "silu", res)
+    within(z, out, tol, "residual")
+    assert linear_status()
+
+
+@pytest.mark.gpu
 def test_linear_as_a_threads_first_call(cuda):
     """A thread that has made no CUDA call of its own yet (as autograd's have not) may begin with a product."""
     import threading
