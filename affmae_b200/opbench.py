@@ -23,6 +23,14 @@ GB/s; the same command under ``ncu -k <kernel>`` gives the kernel profiles.
   rel-bias    config 5 stage 1: in-kernel relative-position bias [16,3,32768,48], fwd+bwd
   head-layout config 5 stage 1: kv head split + output merge, [16,32768,3x32], fwd+bwd
   deform-nbidx  deformable attention with given 4-NN indices (non-fused path), fwd+bwd
+  linear      stage 1's first MLP product with GELU, 524288 x 96 -> 192 bf16, fwd+bwd
+  linear-e4m3 8-bit operands, 8192 x 4096 -> 8192 with GELU, forward
+  rms-norm    stage 1 pre-norm residual by root-mean-square norm, 524288 x 96, fwd+bwd
+  rms-norm-e4m3  16384 rows of 4096, bf16 stream, e4m3 output, forward
+  bucket-bias stage 1's bucketed position bias [16,3,32768,48] bf16, fwd+bwd
+  rms-block   one "rms" encoder block at stage 1 (16 x 32768 tokens, 96 channels, 3 heads, bf16 autocast), fwd+bwd
+  layer-block the default encoder block at the same shape, fwd+bwd
+  rms-block-eval / rms-block-e4m3  the "rms" block in eval mode, 16-bit and with 8-bit operands, forward
 
 Algorithmic bytes count every interface tensor once (inputs read, outputs
 written), as the roofline of a gather-bound operator.
@@ -281,7 +289,103 @@ def op_deform_nbidx():
     return step, fwd + bwd, {"BH": BH, "samples": S, "Nkv": Nkv, "C": C, "pass": "fwd+bwd"}
 
 
-OPS = {"knn": op_knn, "knn-brute": lambda: op_knn(brute=True), "deform": op_deform, "deform-mae": op_deform_mae,
+def op_linear():
+    from .kernels.linear import fused_linear
+    g = torch.Generator().manual_seed(0)
+    M, K, N = 524288, 96, 192
+    x, w, b = ((torch.randn(s, generator=g) * std).to("cuda", torch.bfloat16).requires_grad_(True)
+               for s, std in (((M, K), 1.0), ((N, K), 0.1), ((N,), 0.1)))
+    dout = torch.randn((M, N), generator=g).to("cuda", torch.bfloat16)
+
+    def step():
+        torch.autograd.grad(fused_linear(x, w, b, "gelu"), (x, w, b), dout)
+    return step, 2 * _nbytes(x, w, b) + 2 * _nbytes(dout), {"M": M, "K": K, "N": N, "act": "gelu", "dtype": "bf16",
+                                                           "pass": "fwd+bwd"}
+
+
+def op_linear_e4m3():
+    from .kernels.linear import linear_e4m3, quantize_e4m3
+    M, K, N = 8192, 4096, 8192
+    x, xs = quantize_e4m3(torch.randn((M, K), device="cuda"))
+    w, ws = quantize_e4m3(torch.randn((N, K), device="cuda"))
+    b = torch.randn(N, device="cuda")
+    out = linear_e4m3(x, xs, w, ws, b, "gelu")
+    return (lambda: linear_e4m3(x, xs, w, ws, b, "gelu")), _nbytes(x, xs, w, ws, b, out), {
+        "M": M, "K": K, "N": N, "act": "gelu", "dtype": "e4m3", "TFLOP": 2 * M * N * K / 1e12, "pass": "fwd"}
+
+
+def op_rms_norm(e4m3=False):
+    from .kernels.rms_norm import fused_rms_norm, rms_norm_e4m3
+    if e4m3:
+        x, d = (torch.randn((16384, 4096), device="cuda").to(torch.bfloat16) for _ in range(2))
+        w = torch.ones(4096, device="cuda")
+        out = rms_norm_e4m3(x, w, delta=d)
+        return (lambda: rms_norm_e4m3(x, w, delta=d)), _nbytes(x, d, w, *out), {"R": 16384, "C": 4096, "pass": "fwd"}
+    R, C = 524288, 96
+    x = torch.randn((R, C), device="cuda").requires_grad_(True)
+    d = torch.randn((R, C), device="cuda").to(torch.bfloat16).requires_grad_(True)
+    w = torch.ones(C, device="cuda").requires_grad_(True)
+    ds, dy = torch.randn((R, C), device="cuda"), torch.randn((R, C), device="cuda").to(torch.bfloat16)
+
+    def step():
+        torch.autograd.grad(fused_rms_norm(x, w, delta=d, out_dtype=torch.bfloat16), (x, w, d), (ds, dy))
+    return step, 2 * _nbytes(x, d, ds, dy), {"R": R, "C": C, "stream": "fp32", "branch": "bf16", "pass": "fwd+bwd"}
+
+
+def _stage1():
+    """Positions [16, 32768, 2] and neighbour lists of the first encoder stage."""
+    from .workloads import clustered_tokens, neighbourhoods
+    pos = clustered_tokens(16, 256, 0.5, 0, "cuda")
+    return pos, neighbourhoods(pos, 8, 48)
+
+
+def op_bucket_bias():
+    from .kernels.bucket_bias import bucket_bias, bucket_count
+    pos, (member, _) = _stage1()
+    edges = (1, 2, 3, 4, 7, 13, 24)
+    table = torch.randn((bucket_count(edges, 2), 3), device="cuda").to(torch.bfloat16).requires_grad_(True)
+    dout = torch.randn((16, 3, 32768, 48), device="cuda").to(torch.bfloat16)
+
+    def step():
+        torch.autograd.grad(bucket_bias(table, edges, pos, pos, member), table, dout)
+    return step, 2 * _nbytes(dout) + _nbytes(member, pos), {"B": 16, "H": 3, "N": 32768, "M": 48, "dtype": "bf16",
+                                                            "pass": "fwd+bwd"}
+
+
+def op_block(rms, mode="train"):
+    """One stage-1 encoder block under bf16 autocast; bytes: the stream in and out (and its gradients)."""
+    from .mae import ClusterBlock, RMSClusterBlock
+    torch.manual_seed(0)
+    pos, (member, pe_idx) = _stage1()
+    blk = (RMSClusterBlock(96, 3, 2.0, 0.0, (1, 2, 3, 4, 7, 13, 24)) if rms else ClusterBlock(96, 3, 2.0, 0.0)).to("cuda")
+    x = torch.randn((16, 32768, 96), device="cuda")
+    cfg = {"tokens": 16 * 32768, "C": 96, "heads": 3, "block": "rms" if rms else "layer", "mode": mode}
+    if mode != "train":
+        blk.eval()
+        if mode == "e4m3":
+            blk.quantize()
+
+        def answer():
+            with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+                blk(x, member, None, pos if rms else pe_idx)
+        return answer, 2 * _nbytes(x), cfg
+    x.requires_grad_(True)
+    dout = torch.randn_like(x)
+    params = [x, *blk.parameters()]
+
+    def step():
+        from .mae import add_pending
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            out = add_pending(*blk(x, member, None, pos if rms else pe_idx))
+        torch.autograd.grad(out, params, dout.to(out.dtype))
+    return step, 4 * _nbytes(x), cfg
+
+
+OPS = {"linear": op_linear, "linear-e4m3": op_linear_e4m3, "rms-norm": op_rms_norm,
+       "rms-norm-e4m3": lambda: op_rms_norm(e4m3=True), "bucket-bias": op_bucket_bias,
+       "rms-block": lambda: op_block(True), "layer-block": lambda: op_block(False),
+       "rms-block-eval": lambda: op_block(True, "eval"), "rms-block-e4m3": lambda: op_block(True, "e4m3"),
+       "knn": op_knn, "knn-brute": lambda: op_knn(brute=True), "deform": op_deform, "deform-mae": op_deform_mae,
        "deform-mae-raster": lambda: op_deform_mae(raster=True),
        "layer-norm-dec": lambda: op_layer_norm(C=384), "res-norm": op_residual_norm,
        "res-norm-s3": lambda: op_residual_norm(R=16 * 5243, C=384), "wfeat": op_wfeat,
