@@ -74,7 +74,8 @@ def linear_ref(x, w, b, act, res, dout=None):
 
 # (rows, out, in): single values, few rows, ragged tiles, several column tiles, a long sum over rows
 SHAPES = [(1, 1, 1), (1, 17, 33), (3, 64, 128), (8, 96, 200), (9, 16, 16), (9, 1, 5), (127, 24, 40), (128, 256, 64),
-          (129, 192, 96), (200, 100, 72), (300, 257, 65), (257, 768, 384), (70001, 32, 24), (1000, 520, 136)]
+          (129, 192, 96), (200, 100, 72), (300, 257, 65), (257, 768, 384), (70001, 32, 24), (1000, 520, 136),
+          (283, 2, 1), (65, 2, 2)]   # the last: sums of two terms, where the slope's own error shows
 
 
 @pytest.mark.gpu
