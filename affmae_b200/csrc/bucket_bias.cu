@@ -34,7 +34,9 @@ constexpr int BB_HEADS = 4;          // heads side by side in shared memory; hea
 constexpr int BB_MAX_EDGES = 64;
 constexpr int BB_LUT = 8192;         // distances answered by a byte table, else the edges are searched
 constexpr int BB_BITS = 19;          // 2^19 * 2048 terms stay below 2^31
-constexpr int BB_BLOCKS_PER_SM = 4;
+// Of the backward: a fifth block costs a few spilled registers and hides more
+// of the lists' latency (stage 1, bf16 158 -> 148 us with cold L2, fp32 165 -> 157; a sixth 152, 153).
+constexpr int BB_BLOCKS_PER_SM = 5;
 constexpr int BB_TABLE_SMEM = 64 * 1024;   // of one block's heads
 
 struct BucketArgs {

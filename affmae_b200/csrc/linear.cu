@@ -800,16 +800,18 @@ struct Arena {
     return used <= size ? p : nullptr;
   }
 };
+// `split`: an fp32 operand's copy is left to the caller's launch.
 static int make_operand(int dtype, const void* src, int64_t rows, int64_t cols, bool mn, Arena* ws, Operand* o,
-                        cudaStream_t st) {
+                        SplitRows* split, cudaStream_t st) {
   *o = Operand{src, rows, cols, cols, mn};
   if (!needs_copy(dtype, src, cols)) return AFFB_OK;
   o->ld = pitch(dtype, cols);
   void* dst = ws->take(rows * o->ld * (dtype == AFFB_F32 ? 6 : dtype_size(dtype)));
   AFFB_REQUIRE(dst, "linear: workspace too small (or an operand that is not 16-byte aligned)");
   o->p = dst;
-  return dtype == AFFB_F32 ? linear_split((const float*)src, rows, cols, dst, o->ld, st)
-                           : linear_pack(src, dtype_size(dtype), rows, cols, dst, o->ld, st);
+  if (dtype != AFFB_F32) return linear_pack(src, dtype_size(dtype), rows, cols, dst, o->ld, st);
+  *split = SplitRows{(const float*)src, rows, cols, dst, o->ld};
+  return AFFB_OK;
 }
 
 static int check_sizes(int64_t M, int64_t N, int64_t K) {
@@ -827,8 +829,10 @@ static int forward(const void* x, const void* w, int dtype, int64_t M, int64_t N
   Arena ws{(unsigned char*)workspace, 0, workspace ? workspace_bytes : 0};
   Operand a, b;
   int rc;
-  if ((rc = make_operand(dtype, x, M, K, false, &ws, &a, st))) return rc;
-  if ((rc = make_operand(dtype, w, N, K, false, &ws, &b, st))) return rc;
+  SplitRows sx{}, sw{};
+  if ((rc = make_operand(dtype, x, M, K, false, &ws, &a, &sx, st))) return rc;
+  if ((rc = make_operand(dtype, w, N, K, false, &ws, &b, &sw, st))) return rc;
+  if ((rc = linear_split(sx, sw, st))) return rc;
   const int64_t part = partial_bytes(M, N, k_blocks(dtype, K));
   unsigned char* pp = nullptr;
   if (part) AFFB_REQUIRE(pp = (unsigned char*)ws.take(part), "linear: workspace too small");
@@ -957,19 +961,20 @@ extern "C" int affb_linear_bwd(const void* dout, int dout_dtype, const void* z, 
   const int64_t p2 = dweight ? partial_bytes(N, K, k_blocks(dtype, M)) : 0;
   unsigned char* pp = nullptr;
   if (p1 || p2) AFFB_REQUIRE(pp = (unsigned char*)ws.take(p1 > p2 ? p1 : p2), "linear: workspace too small");
+  Operand w{}, xo{};
+  SplitRows sx{}, sw{};
+  if (dx && (rc = make_operand(dtype, weight, N, K, true, &ws, &w, &sw, st))) return rc;
+  if (dweight && (rc = make_operand(dtype, x, M, K, true, &ws, &xo, &sx, st))) return rc;
+  if ((rc = linear_split(sx, sw, st))) return rc;
   if (dx) {  // dx[m,k] = sum_n dz[m,n] w[n,k]
-    Operand b;
-    if ((rc = make_operand(dtype, weight, N, K, true, &ws, &b, st))) return rc;
     dz.mn = false;
     e.out = dx;
-    if ((rc = gemm(dtype, dz, b, M, K, N, e, pp, st))) return rc;
+    if ((rc = gemm(dtype, dz, w, M, K, N, e, pp, st))) return rc;
   }
   if (dweight) {  // dw[n,k] = sum_m dz[m,n] x[m,k]
-    Operand b;
-    if ((rc = make_operand(dtype, x, M, K, true, &ws, &b, st))) return rc;
     dz.mn = true;
     e.out = dweight;
-    if ((rc = gemm(dtype, dz, b, N, K, M, e, pp, st))) return rc;
+    if ((rc = gemm(dtype, dz, xo, N, K, M, e, pp, st))) return rc;
   }
   return AFFB_OK;
 }

@@ -54,8 +54,15 @@ cudaError_t rms_failed(int* failed);
 // linear_aux.cu
 // rows [R,C] -> [R,ld] of the same element size (the tail of a row is not written)
 int linear_pack(const void* src, int64_t elem, int64_t R, int64_t C, void* dst, int64_t ld, cudaStream_t st);
-// fp32 rows [R,C] -> three bf16 parts [3][R][ld] whose sum is the fp32 value
-int linear_split(const float* src, int64_t R, int64_t C, void* dst, int64_t ld, cudaStream_t st);
+// fp32 rows [R,C] -> three bf16 parts [3][R][ld] whose sum is the fp32 value,
+// for one or two arrays (R = 0: none) in one launch
+struct SplitRows {
+  const float* src;
+  int64_t R, C;
+  void* dst;
+  int64_t ld;
+};
+int linear_split(const SplitRows& a, const SplitRows& b, cudaStream_t st);
 // dz = dout * act'(z): dz (null: not wanted) [R,ld] of `dtype`, or the three
 // bf16 parts of it when dtype is fp32; column sums into part [strips][C] fp32
 // (null: not wanted).  strips = linear_dz_strips(R, C).

@@ -40,29 +40,29 @@ __device__ __forceinline__ void split3(float v, __nv_bfloat16* o) {
   o[2] = __float2bfloat16_rn(isfinite(r1) ? r1 - __bfloat162float(o[1]) : 0.f);
 }
 
-// A warp a row; a lane takes two columns, so that the parts are written in
-// words (rows of the parts are 16-byte aligned).
-__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, int64_t R, int64_t C,
-                                                         __nv_bfloat16* __restrict__ dst, int64_t ld) {
-  const int64_t part = R * ld;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < R; r += (int64_t)gridDim.x * 8) {
-    const float* s = src + r * C;
-    __nv_bfloat16* d = dst + r * ld;
+// A warp a row of either of two arrays; a lane takes two columns, so that the
+// parts are written in words (rows of the parts are 16-byte aligned).
+__global__ void __launch_bounds__(256) split_rows_kernel(SplitRows a, SplitRows b) {
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < a.R + b.R; i += (int64_t)gridDim.x * 8) {
+    const SplitRows& w = i < a.R ? a : b;
+    const int64_t r = i < a.R ? i : i - a.R, part = w.R * w.ld, C = w.C;
+    const float* s = w.src + r * C;
+    __nv_bfloat16* d = (__nv_bfloat16*)w.dst + r * w.ld;
 #pragma unroll 4
     for (int64_t c = (threadIdx.x & 31) * 2; c < C; c += 64) {
-      __nv_bfloat16 a[3], b[3];
-      split3(s[c], a);
-      split3(c + 1 < C ? s[c + 1] : 0.f, b);
+      __nv_bfloat16 p[3], q[3];
+      split3(s[c], p);
+      split3(c + 1 < C ? s[c + 1] : 0.f, q);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<__nv_bfloat162*>(d + c + k * part) = __nv_bfloat162(a[k], b[k]);
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<__nv_bfloat162*>(d + c + k * part) = __nv_bfloat162(p[k], q[k]);
     }
   }
 }
 
-int linear_split(const float* src, int64_t R, int64_t C, void* dst, int64_t ld, cudaStream_t st) {
-  if (R * C == 0) return AFFB_OK;
-  const unsigned blocks = (unsigned)imin64((R + 7) / 8, (int64_t)sm_count() * 16);
-  split_rows_kernel<<<blocks, 256, 0, st>>>(src, R, C, (__nv_bfloat16*)dst, ld);
+int linear_split(const SplitRows& a, const SplitRows& b, cudaStream_t st) {
+  if (a.R + b.R == 0) return AFFB_OK;
+  const unsigned blocks = (unsigned)imin64((a.R + b.R + 7) / 8, (int64_t)sm_count() * 16);
+  split_rows_kernel<<<blocks, 256, 0, st>>>(a, b);
   AFFB_LAUNCH_CHECK("linear: split");
   return AFFB_OK;
 }
