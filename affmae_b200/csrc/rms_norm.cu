@@ -100,7 +100,9 @@ struct AddOp { __device__ __forceinline__ float operator()(float a, float b) con
 struct MaxOp { __device__ __forceinline__ float operator()(float a, float b) const { return rms_max_nan(a, b); } };
 
 // Reduction over the TPR threads that share a row (all of them get it).  A
-// block-wide one writes to `red`, which the reduction before must not use.
+// block-wide one goes through `red` with one barrier between its writes and
+// its reads, so the block's next one may have begun before the last warp has
+// read: it must not use the same `red`.
 template <int TPR, typename Op>
 __device__ __forceinline__ float row_reduce(float v, float* red, Op op) {
 #pragma unroll
@@ -239,7 +241,8 @@ template <typename TX, int TPR, int NV, int VEC, bool PIPE>
 __global__ void __launch_bounds__(256) rms_fwd_kernel(const __grid_constant__ RmsArgs a,
                                                       const __grid_constant__ RowPipe pipe) {
   extern __shared__ __align__(128) unsigned char staged[];
-  __shared__ float red[3][8];  // sums of squares (two rows in turn), maxima
+  // sums of squares and maxima, two rows of each in turn: without the norm the maximum is a row's only reduction
+  __shared__ float red[4][8];
   constexpr int ROWS = 256 / TPR;
   constexpr int KEEP = NV > 0 ? NV : 1;
   const int t = threadIdx.x % TPR;
@@ -291,7 +294,6 @@ __global__ void __launch_bounds__(256) rms_fwd_kernel(const __grid_constant__ Rm
     float rstd = 1.f;
     if (a.w) {
       rstd = rsqrtf(row_reduce<TPR>(sq, red[flip], AddOp()) * inv_c + a.eps);
-      flip ^= 1;
       if (a.rstd && in && t == 0) a.rstd[r] = rstd;
     }
     // y: kept in place of the row
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(256) rms_fwd_kernel(const __grid_constant__ Rm
           for (int k = 0; k < VEC; ++k) top = rms_max_nan(top, fabsf(o[k]));
         }
       }
-      top = row_reduce<TPR>(top, red[2], MaxOp());
+      top = row_reduce<TPR>(top, red[2 + flip], MaxOp());
       const float scale = top == 0.f ? 1.f : top * (1.f / E4M3_MAX);
       inv = 1.f / scale;
       if (in && t == 0) a.scale[r] = scale;
@@ -344,6 +346,7 @@ __global__ void __launch_bounds__(256) rms_fwd_kernel(const __grid_constant__ Rm
         }
       }
     }
+    flip ^= 1;
     if constexpr (PIPE) reader->next(it);
   }
 }
