@@ -19,9 +19,13 @@
 //
 // Backward: bins in shared memory.  Float atomics would make the sums depend
 // on timing, so a block takes 2048 pairs at a time, scales their gradients by
-// a power of two of the tile's largest (19 bits are kept, an error below
-// 2^-20 of that largest value per term), adds them as integers, and then adds
-// the tile's sums to fp32 bins.  The blocks' bins are summed in block order.
+// a power of two of the tile's largest, adds the nearest integers (of 19
+// bits), adds what that rounding leaves in units 2^20 times as fine (few
+// 16-bit gradients leave anything), adds both sums to fp32 bins, and goes on
+// in the same way until nothing is left of any term.  The integer sums are
+// exact, so a row of the table is off by the fp32 additions of its own sums
+// alone, whatever the gradients of other rows are.  The blocks' bins are
+// summed in block order.
 #include "common.cuh"
 
 #include <type_traits>
@@ -34,9 +38,11 @@ constexpr int BB_HEADS = 4;          // heads side by side in shared memory; hea
 constexpr int BB_MAX_EDGES = 64;
 constexpr int BB_LUT = 8192;         // distances answered by a byte table, else the edges are searched
 constexpr int BB_BITS = 19;          // 2^19 * 2048 terms stay below 2^31
-// Of the backward: a fifth block costs a few spilled registers and hides more
-// of the lists' latency (stage 1, bf16 158 -> 148 us with cold L2, fp32 165 -> 157; a sixth 152, 153).
-constexpr int BB_BLOCKS_PER_SM = 5;
+// Blocks of the backward on an SM.  With 16-bit gradients the fifth costs a
+// few spilled registers and hides more of the lists' latency; fp32 ones take
+// twice the registers (stage 1: bf16 186 us with four, 178 with five; fp32
+// 246 and 270; with three 201 and 259).
+constexpr int BB_BLOCKS_PER_SM = 5, BB_BLOCKS_PER_SM_F32 = 4;
 constexpr int BB_TABLE_SMEM = 64 * 1024;   // of one block's heads
 
 struct BucketArgs {
@@ -297,9 +303,56 @@ __device__ __forceinline__ float bb_max_nan(float a, float b) {
   return y;
 }
 
+__device__ __forceinline__ float power_of_two(int t) { return __int_as_float((127 + t) << 23); }
+constexpr float ROUND = 12582912.f;      // 1.5 * 2^23: a sum with it is rounded to an integer, in the low mantissa bits
+constexpr int ROUND_BITS = 0x4B400000;
+constexpr int NO_POWER = -1000;
+// 2^t and 2^-t as products of two powers, since 2^t itself may pass fp32's range.
+struct Power {
+  float up, up2, down, down2;
+  __device__ __forceinline__ explicit Power(int t, bool whole = false) {  // whole: |t| < 127, in one power
+    const int a = whole ? t : t / 2, b = t - a;
+    up = power_of_two(a);
+    up2 = power_of_two(b);
+    down = power_of_two(-a);
+    down2 = power_of_two(-b);
+  }
+  // v 2^t rounded to an integer; v keeps the rest, which is exact and at most half a unit 2^-t.
+  __device__ __forceinline__ int round_off(float& v) const {
+    const float whole = fmaf(v * up, up2, ROUND);
+    v = fmaf((whole - ROUND) * -down, down2, v);
+    return __float_as_int(whole) - ROUND_BITS;
+  }
+  __device__ __forceinline__ float value(int n) const { return (float)n * down * down2; }
+};
+
+// A lane's gradients of one head as they were loaded.
+template <typename T, int PAIRS>
+struct Terms {
+  static constexpr int PER = sizeof(T) == 4 ? PAIRS : 1;  // words of a step
+  static constexpr int WORDS = BB_STEPS * PER;
+  static __device__ __forceinline__ void load(const T* p, bool in, int u, uint32_t* w) {
+    if constexpr (PER == 2) {
+      const uint2 v = in ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0u, 0u);
+      w[2 * u] = v.x;
+      w[2 * u + 1] = v.y;
+    } else if constexpr (sizeof(T) * PAIRS == 4) {
+      w[u] = in ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
+    } else {
+      w[u] = in ? __ldg(reinterpret_cast<const uint16_t*>(p)) : 0u;
+    }
+  }
+  static __device__ __forceinline__ float get(const uint32_t* w, int j) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+    const uint32_t half = PAIRS == 1 ? w[j] : j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(half << 16);
+    return __half2float(__ushort_as_half((unsigned short)half));
+  }
+};
+
 // Block (x: tiles taken in turn, y: group of BB_HEADS heads).
 template <typename T, typename P, int AXES, int PAIRS, bool BY_OFFSET>
-__global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
+__global__ void __launch_bounds__(BB_THREADS, sizeof(T) == 4 ? BB_BLOCKS_PER_SM_F32 : BB_BLOCKS_PER_SM)
     bucket_bwd_kernel(const __grid_constant__ BucketArgs a, const T* __restrict__ dout, float* __restrict__ part,
                       int resume) {
   constexpr int STEP = BB_THREADS * PAIRS, TILE = STEP * BB_STEPS, PER = BB_STEPS * PAIRS;
@@ -308,8 +361,8 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
   const int none = a.rows;
   const int stride = a.rows + 1;  // a bin more for pairs that have no row
   float* acc = reinterpret_cast<float*>(sm);                            // [BB_HEADS][stride]
-  int* bins = reinterpret_cast<int*>(acc + BB_HEADS * stride);          // [BB_HEADS][stride]
-  float* raw = reinterpret_cast<float*>(bins + BB_HEADS * stride);      // [TILE] values, only of an odd tile
+  int* bins = reinterpret_cast<int*>(acc + BB_HEADS * stride);          // [coarse, fine][BB_HEADS][stride]
+  float* raw = reinterpret_cast<float*>(bins + 2 * BB_HEADS * stride);  // [TILE] values, only of an odd tile
   uint16_t* raw_row = reinterpret_cast<uint16_t*>(raw + TILE);          // [TILE]
   // BY_OFFSET: the row of every combined clipped offset, and `none` last
   const int offsets = AXES == 2 ? a.span * a.span : a.span;
@@ -334,7 +387,7 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
     for (int i = threadIdx.x; i < stride; i += BB_THREADS) {
       // what the launch before (of more than 2^31 pairs) has summed
       acc[h * stride + i] = resume && h < nh && i < a.rows ? mine[h * a.rows + i] : 0.f;
-      bins[h * stride + i] = 0;
+      bins[h * stride + i] = bins[(BB_HEADS + h) * stride + i] = 0;
     }
   __syncthreads();
   const EntryOf<P, AXES, BY_OFFSET> entry(a, find);
@@ -343,7 +396,7 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
   for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
     const int b = total < (1ll << 31) ? (int)((uint32_t)t / per) : (int)(t / per);
     const int nm = (int)(t - (int64_t)b * per) * TILE + threadIdx.x * PAIRS;
-    float g[BB_HEADS][PER];
+    uint32_t g[BB_HEADS][Terms<T, PAIRS>::WORDS];
     const T* p0 = dout + ((int64_t)b * a.H + h0) * a.batch_pairs + nm;
 #pragma unroll
     for (int h = 0; h < BB_HEADS; ++h) {
@@ -351,22 +404,9 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
       const T* p = p0 + h * a.batch_pairs;
       float top = 0.f;
 #pragma unroll
-      for (int u = 0; u < BB_STEPS; ++u) {
-        const bool in = nm + u * STEP < a.NM;
-        if constexpr (PAIRS == 2 && sizeof(T) == 2) {
-          const uint32_t w = in ? __ldg(reinterpret_cast<const uint32_t*>(p + u * STEP)) : 0u;
-          g[h][2 * u] = ldf(reinterpret_cast<const T*>(&w));
-          g[h][2 * u + 1] = ldf(reinterpret_cast<const T*>(&w) + 1);
-        } else if constexpr (PAIRS == 2) {
-          const float2 w = in ? __ldg(reinterpret_cast<const float2*>(p + u * STEP)) : make_float2(0.f, 0.f);
-          g[h][2 * u] = w.x;
-          g[h][2 * u + 1] = w.y;
-        } else {
-          g[h][u] = in ? ldf(p + u * STEP) : 0.f;
-        }
-      }
+      for (int u = 0; u < BB_STEPS; ++u) Terms<T, PAIRS>::load(p + u * STEP, nm + u * STEP < a.NM, u, g[h]);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) top = bb_max_nan(top, fabsf(g[h][j]));
+      for (int j = 0; j < PER; ++j) top = bb_max_nan(top, fabsf(Terms<T, PAIRS>::get(g[h], j)));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = bb_max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
       if (lane == 0) wmax[h][warp] = top;
@@ -379,47 +419,84 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
       for (int j = 0; j < PER; ++j) row[j] = rows[row[j]];
     }
     __syncthreads();
-    float down[BB_HEADS];  // 2^-(t / 2) of the scale 2^t, 0: nothing to add
-    float rest[BB_HEADS];  // 2^-(t - t / 2)
-    bool odd = false;      // an infinity or NaN among the tile's gradients
+    int power[BB_HEADS];  // of a head's scale 2^power, NO_POWER: nothing to add
+    bool odd = false;     // an infinity or NaN among the tile's gradients
 #pragma unroll
     for (int h = 0; h < BB_HEADS; ++h) {
-      down[h] = 0.f;
+      power[h] = NO_POWER;
       if (h >= nh) continue;
       float top = 0.f;
 #pragma unroll
       for (int w = 0; w < BB_THREADS / 32; ++w) top = bb_max_nan(top, wmax[h][w]);
-      if (!isfinite(top)) {
-        odd = true;
-      } else if (top > 0.f) {
-        // top < 2^e: values times 2^t = 2^(BITS - e) stay below 2^BITS, and are
-        // rounded to integers by adding 1.5 * 2^23.  The power is taken in two
-        // halves where it may itself pass the range of fp32.
-        const int t = BB_BITS - (((__float_as_int(top) >> 23) & 255) - 126), t1 = t / 2;
-        const float up = __int_as_float((127 + t1) << 23), up2 = __int_as_float((127 + t - t1) << 23);
-        down[h] = __int_as_float((127 - t1) << 23);
-        rest[h] = __int_as_float((127 - t + t1) << 23);
-        int* bin = bins + h * stride;
-        if (t > -120 && t < 120) {
-          const float whole = up * up2;
+      if (!isfinite(top)) odd = true;
+      else if (top > 0.f) power[h] = BB_BITS - (((__float_as_int(top) >> 23) & 255) - 126);  // top < 2^e: 2^(BITS - e)
+    }
+    bool left = false;  // of any term after two roundings
 #pragma unroll
-          for (int j = 0; j < PER; ++j)
-            atomicAdd(bin + row[j], __float_as_int(fmaf(g[h][j], whole, 12582912.f)) - 0x4B400000);
-        } else {
+    for (int h = 0; h < BB_HEADS; ++h) {
+      if (power[h] == NO_POWER) continue;
+      int* bin = bins + h * stride;
+      int* fine = bin + BB_HEADS * stride;
+      const bool small = power[h] > -100 && power[h] < 100;  // the scales and their inverses stay in fp32's range
+      const Power one(power[h], small), two(power[h] + BB_BITS + 1, small);
+      // a term of at least 2^(mantissa) units is a whole number of them
+      const float whole_from = sizeof(T) == 4 ? INFINITY : (std::is_same<T, __half>::value ? 1024.f : 128.f) * one.down * one.down2;
 #pragma unroll
-          for (int j = 0; j < PER; ++j)
-            atomicAdd(bin + row[j], __float_as_int(fmaf(g[h][j] * up, up2, 12582912.f)) - 0x4B400000);
+      for (int j = 0; j < PER; ++j) {
+        float v = Terms<T, PAIRS>::get(g[h], j);
+        const bool rest = sizeof(T) == 4 || fabsf(v) < whole_from;
+        atomicAdd(bin + row[j], one.round_off(v));
+        if (rest) {
+          const int n = two.round_off(v);
+          if (n != 0) atomicAdd(fine + row[j], n);
+          left |= v != 0.f;
         }
       }
     }
-    __syncthreads();
+    const bool more = __syncthreads_or(left);
     for (int i = threadIdx.x; i <= a.rows; i += BB_THREADS) {
 #pragma unroll
       for (int h = 0; h < BB_HEADS; ++h) {
-        if (down[h] != 0.f) {
-          const int v = bins[h * stride + i];
-          bins[h * stride + i] = 0;
-          acc[h * stride + i] += (float)v * down[h] * rest[h];
+        if (power[h] != NO_POWER) {
+          int* bin = bins + h * stride + i;
+          int* fine = bin + BB_HEADS * stride;
+          acc[h * stride + i] += Power(power[h]).value(*bin) + Power(power[h] + BB_BITS + 1).value(*fine);
+          *bin = *fine = 0;
+        }
+      }
+    }
+    if (more) {  // head by head, a lane's rests and rows in its own places of raw
+#pragma unroll
+      for (int h = 0; h < BB_HEADS; ++h) {
+        int t = power[h];
+        if (t == NO_POWER) continue;
+        left = false;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          float v = Terms<T, PAIRS>::get(g[h], j);
+          Power(t).round_off(v);
+          Power(t + BB_BITS + 1).round_off(v);
+          raw[threadIdx.x * PER + j] = v;
+          raw_row[threadIdx.x * PER + j] = (uint16_t)row[j];
+          left |= v != 0.f;
+        }
+        int* bin = bins + h * stride;
+        for (t += 2 * (BB_BITS + 1); __syncthreads_or(left); t += BB_BITS + 1) {
+          left = false;
+          const Power unit(t);
+#pragma unroll 1
+          for (int j = threadIdx.x * PER; j < (int)(threadIdx.x + 1) * PER; ++j) {
+            float v = raw[j];
+            const int n = unit.round_off(v);
+            if (n != 0) atomicAdd(bin + raw_row[j], n);
+            raw[j] = v;
+            left |= v != 0.f;
+          }
+          __syncthreads();
+          for (int i = threadIdx.x; i <= a.rows; i += BB_THREADS) {
+            acc[h * stride + i] += unit.value(bin[i]);
+            bin[i] = 0;
+          }
         }
       }
     }
@@ -432,7 +509,7 @@ __global__ void __launch_bounds__(BB_THREADS, BB_BLOCKS_PER_SM)
           __syncthreads();
 #pragma unroll
           for (int j = 0; j < PER; ++j) {
-            raw[threadIdx.x * PER + j] = g[h][j];
+            raw[threadIdx.x * PER + j] = Terms<T, PAIRS>::get(g[h], j);
             raw_row[threadIdx.x * PER + j] = (uint16_t)row[j];
           }
           __syncthreads();
@@ -471,12 +548,12 @@ __global__ void __launch_bounds__(1024) bucket_table_kernel(const float* __restr
   }
 }
 
-// Blocks of the backward along x: sized for the narrower tile, so that it does
-// not depend on alignment.
-static int64_t bucket_bwd_blocks(int64_t B, int64_t H, int64_t NM) {
+// Blocks of the backward along x, `per_sm` of them on an SM: sized for the
+// narrower tile, so that it does not depend on alignment.
+static int64_t bucket_bwd_blocks(int64_t B, int64_t H, int64_t NM, int per_sm) {
   const int64_t tile = BB_THREADS * BB_STEPS;
   const int64_t tiles = (NM + tile - 1) / tile * B, groups = (H + BB_HEADS - 1) / BB_HEADS;
-  const int64_t want = ((int64_t)sm_count() * BB_BLOCKS_PER_SM + groups - 1) / groups;
+  const int64_t want = ((int64_t)sm_count() * per_sm + groups - 1) / groups;
   return tiles < want ? tiles : want;
 }
 
@@ -596,7 +673,7 @@ static cudaError_t bucket_bwd_launch(const BucketArgs& a, const void* dout, floa
   const int tile = BB_THREADS * PAIRS * BB_STEPS;
   BucketArgs c = a;
   c.use_lut = bb_use_lut(a, offsets, blocks);
-  const int smem = 2 * BB_HEADS * (a.rows + 1) * 4 + tile * 6 + (offsets ? (int)((offsets + 2) & ~1) * 2 : 0) +
+  const int smem = 3 * BB_HEADS * (a.rows + 1) * 4 + tile * 6 + (offsets ? (int)((offsets + 2) & ~1) * 2 : 0) +
                    BB_MAX_EDGES * 4 + (c.use_lut ? a.lut : 0);
   auto* k = offsets ? bucket_bwd_kernel<T, P, AXES, PAIRS, true> : bucket_bwd_kernel<T, P, AXES, PAIRS, false>;
   if (smem > 47 * 1024) {
@@ -654,7 +731,7 @@ extern "C" int64_t affb_bucket_bias_bwd_workspace_bytes(int n_edges, int one_sid
                                                         int64_t Nq, int64_t M) {
   if (B * Nq * M <= 0 || H < 1) return 0;
   const int64_t n = one_sided ? n_edges + 1 : 2 * n_edges + 1;
-  return bucket_bwd_blocks(B, H, Nq * M) * H * (axes == 1 ? n : n * n) * 4;
+  return bucket_bwd_blocks(B, H, Nq * M, BB_BLOCKS_PER_SM) * H * (axes == 1 ? n : n * n) * 4;
 }
 
 extern "C" int affb_bucket_bias_bwd(const void* dout, int dout_dtype, const int32_t* edges, int n_edges, int one_sided,
@@ -673,7 +750,7 @@ extern "C" int affb_bucket_bias_bwd(const void* dout, int dout_dtype, const int3
   int64_t blocks = 0;
   if (B * a.batch_pairs > 0 && Nk > 0) {
     AFFB_REQUIRE(dout, "bucket_bias: null pointer");
-    blocks = bucket_bwd_blocks(B, H, a.batch_pairs);
+    blocks = bucket_bwd_blocks(B, H, a.batch_pairs, dout_dtype == AFFB_F32 ? BB_BLOCKS_PER_SM_F32 : BB_BLOCKS_PER_SM);
     AFFB_REQUIRE(workspace && workspace_bytes >= blocks * n * 4, "bucket_bias: workspace too small");
     const bool two = bb_two(a, dout, dout_dtype == AFFB_F32 ? 4 : 2);
     cudaError_t e = cudaSuccess;

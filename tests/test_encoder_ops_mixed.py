@@ -5,8 +5,9 @@ test_encoder_ops.py."""
 import pytest
 import torch
 
+from affmae_b200.kernels.bucket_bias import bucket_bias, bucket_count, log_edges
 from affmae_b200.kernels.linear import quantize_e4m3
-from test_encoder_ops import BF16, FP16, FP32, check_e4m3, rnd
+from test_encoder_ops import BF16, E, FP16, FP32, TINY, U, bias_inputs, check_e4m3, rnd, rows_ref, within
 
 
 @pytest.mark.gpu
@@ -25,3 +26,44 @@ def test_quantize_e4m3_of_several_rows_a_block(cuda, dtype, shape):
         check_e4m3(q[i:i + 1000], scale[i:i + 1000], xd, torch.zeros_like(xd))
     again = quantize_e4m3(x)
     assert torch.equal(q.view(torch.uint8), again[0].view(torch.uint8)) and torch.equal(scale, again[1])
+
+
+WIDE = [  # B, H, Nq, Nk, M (0: all keys), axes, edges, one sided, position type
+    (2, 3, 2000, 2000, 48, 2, log_edges(7, 24), False, FP32),
+    (1, 5, 700, 700, 13, 2, (1, 4), False, torch.int32),
+    (2, 4, 33, 1001, 0, 1, log_edges(31, 512), True, torch.int64),
+    (1, 2, 400, 400, 64, 2, log_edges(32, 60), False, FP32),     # 65 x 65 rows
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("case", WIDE)
+@pytest.mark.parametrize("kind", ["spread", "outlier", "tiny", "huge"])
+def test_bucket_bias_gradients_of_mixed_size(cuda, dtype, case, kind):
+    """Every row of the table's gradient against its own terms, whatever the others are: a term is summed exactly
+    in integers within a tile; a tile's sum is formed of two to sixteen such sums, and up to eight tiles' and
+    blocks' sums are added one after the other, 32 additions in all."""
+    B, H, Nq, Nk, M, A, edges, one, _ = case
+    qp, kp, member = bias_inputs(cuda, case)
+    rows = bucket_count(edges, A, one)
+    table = torch.zeros((rows, H), device=cuda, dtype=dtype, requires_grad=True)
+    bias = bucket_bias(table, edges, qp, kp, member, one)
+    g = torch.Generator().manual_seed(7)
+    d = torch.randn(bias.shape, generator=g).double() * 10.0 ** (-8 * torch.rand(bias.shape, generator=g).double())
+    if kind == "outlier":
+        d = d * 1e-6
+        d[0, 0, 0, 0], d[-1, -1, -1, -1] = 3.0, -1e4
+    elif dtype != FP16 and kind != "spread":
+        d = d * (1e-34 if kind == "tiny" else 1e34)
+    dout = d.to(dtype).to(cuda)
+    (dt,) = torch.autograd.grad(bias, (table,), dout, retain_graph=True)
+    (again,) = torch.autograd.grad(bias, (table,), dout)
+    assert torch.equal(dt, again)
+    row = rows_ref(edges, qp, kp, member, one).reshape(-1)
+    ok = row >= 0
+    gd = dout.double().permute(0, 2, 3, 1).reshape(-1, H)[ok]
+    ref = torch.zeros((rows, H), dtype=torch.float64, device=cuda).index_add_(0, row[ok], gd)
+    mag = torch.zeros_like(ref).index_add_(0, row[ok], gd.abs())
+    # 2^-149: fp32's spacing next to zero (bf16's: 2^-133)
+    within(dt, ref, 32 * E * mag + U[dtype] * ref.abs() + TINY[dtype] + (2.0 ** -133 if dtype == BF16 else 32 * 2.0 ** -149))
