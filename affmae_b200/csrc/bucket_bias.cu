@@ -657,10 +657,8 @@ static cudaError_t bucket_fwd_launch(const BucketArgs& a, const void* table, voi
   c.use_lut = bb_use_lut(a, offsets, blocks);
   const int smem = (int)(groups * entries * v) + BB_MAX_EDGES * 4 + (c.use_lut ? a.lut : 0);
   auto* k = offsets ? bucket_fwd_kernel<T, TB, P, AXES, PAIRS, true> : bucket_fwd_kernel<T, TB, P, AXES, PAIRS, false>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-  }
+  const cudaError_t e = allow_dynamic_smem(k, smem);
+  if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)blocks, (unsigned)((all + groups - 1) / groups));
   k<<<grid, BB_THREADS, smem, st>>>(c, (const TB*)table, groups, (T*)out);
   return cudaGetLastError();
@@ -676,10 +674,8 @@ static cudaError_t bucket_bwd_launch(const BucketArgs& a, const void* dout, floa
   const int smem = 3 * BB_HEADS * (a.rows + 1) * 4 + tile * 6 + (offsets ? (int)((offsets + 2) & ~1) * 2 : 0) +
                    BB_MAX_EDGES * 4 + (c.use_lut ? a.lut : 0);
   auto* k = offsets ? bucket_bwd_kernel<T, P, AXES, PAIRS, true> : bucket_bwd_kernel<T, P, AXES, PAIRS, false>;
-  if (smem > 47 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-  }
+  const cudaError_t e = allow_dynamic_smem(k, smem);
+  if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)blocks, (unsigned)((a.H + BB_HEADS - 1) / BB_HEADS));
   k<<<grid, BB_THREADS, smem, st>>>(c, (const T*)dout, part, resume);
   return cudaGetLastError();

@@ -67,6 +67,15 @@ inline cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 bl
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// Lets a kernel launch with `smem` bytes of dynamic shared memory.  The limit
+// belongs to the kernel, not to the launch, and threads share it, so every
+// call raises it to the same value: 227 KB less 1 KB for static arrays.
+template <typename K>
+inline cudaError_t allow_dynamic_smem(K kernel, int smem) {
+  if (smem <= 47 * 1024) return cudaSuccess;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+}
+
 // ------------------------------------------------------------ conversions --
 template <typename T> struct io;
 template <> struct io<float> {

@@ -583,10 +583,8 @@ static int64_t rms_pipe_blocks(const RowPipe& p) { return imin64(4, 228 * 1024 /
 
 template <typename K, typename A>
 static cudaError_t rms_go(K kernel, unsigned blocks, int smem, const A& a, const RowPipe& p, cudaStream_t st) {
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-  }
+  const cudaError_t e = allow_dynamic_smem(kernel, smem);
+  if (e != cudaSuccess) return e;
   kernel<<<blocks, 256, smem, st>>>(a, p);
   return cudaGetLastError();
 }

@@ -2,9 +2,13 @@
 from one another: rows of other sizes in turn, gradients of mixed magnitude,
 infinities, forward-mode derivatives, several threads.  Bounds as in
 test_encoder_ops.py."""
+import ctypes
+import threading
+
 import pytest
 import torch
 
+from affmae_b200 import _native as nat
 from affmae_b200.kernels.bucket_bias import bucket_bias, bucket_count, log_edges
 from affmae_b200.kernels.linear import quantize_e4m3
 from test_encoder_ops import BF16, E, FP16, FP32, TINY, U, bias_inputs, check_e4m3, rnd, rows_ref, within
@@ -67,3 +71,44 @@ def test_bucket_bias_gradients_of_mixed_size(cuda, dtype, case, kind):
     mag = torch.zeros_like(ref).index_add_(0, row[ok], gd.abs())
     # 2^-149: fp32's spacing next to zero (bf16's: 2^-133)
     within(dt, ref, 32 * E * mag + U[dtype] * ref.abs() + TINY[dtype] + (2.0 ** -133 if dtype == BF16 else 32 * 2.0 ** -149))
+
+
+@pytest.mark.gpu
+def test_threads_that_launch_one_kernel_with_different_shared_memory(cuda):
+    """The norm with and without a residual branch and the bias gradient with two tables, each from a thread of its
+    own, each pair through one kernel: no launch depends on what another thread has asked for.  The library is
+    called directly, so that the threads are in it together."""
+    lib = nat.lib()
+    x, d, w = rnd(cuda, 1, 1800, 8192, dtype=BF16), rnd(cuda, 2, 1800, 8192, dtype=BF16), torch.ones(8192, device=cuda)
+    pos, dout = rnd(cuda, 3, 1, 8, 2, std=20.0), rnd(cuda, 4, 1, 4, 8, 8)
+    y, s = torch.empty_like(x), torch.empty_like(x)
+    ws = torch.empty(1 << 20, device=cuda, dtype=torch.uint8)
+    out = torch.empty((4225, 4), device=cuda)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    jobs = []
+    for k, delta in enumerate((None, d)):
+        jobs.append((lib.affb_rms_norm_fwd, (x.data_ptr(), 2, nat.ptr(delta), 2, None, 0, w.data_ptr(), 1e-6, 1800, 8192,
+                                             s.data_ptr() if k else None, None, y.data_ptr(), 2, None, None,
+                                             streams[k].cuda_stream)))
+    for k, n in enumerate((20, 32)):
+        e = (ctypes.c_int32 * n)(*log_edges(n, 9000))
+        jobs.append((lib.affb_bucket_bias_bwd, (dout.data_ptr(), 0, ctypes.addressof(e), n, 0, pos.data_ptr(), pos.data_ptr(),
+                                                0, 2, None, 1, 4, 8, 8, 8, out.data_ptr(), 0, ws.data_ptr(), ws.numel(),
+                                                streams[2 + k].cuda_stream)))
+        jobs[-1] += (e,)
+    errors = []
+
+    def work(f, args, stream, *_):
+        for i in range(4000):
+            if f(*args) != 0:
+                errors.append(lib.affb_last_error().decode())
+            if i % 100 == 99:
+                stream.synchronize()
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(j[0], j[1], s)) for j, s in zip(jobs, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, f"{len(errors)} calls failed: {errors[0]}"
