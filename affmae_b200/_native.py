@@ -13,6 +13,7 @@ import threading
 from pathlib import Path
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 _LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libaffmae_b200.so"
 _lock = threading.Lock()
@@ -211,6 +212,29 @@ def workspace(index: int, name: str, like, *args):
     current stream's pool."""
     n = _size(index, name, *args)
     return like.new_empty(n, dtype=torch.uint8) if n else None
+
+
+def differentiates(*tensors) -> bool:
+    """Whether autograd has to see a call on these tensors: one of them asks
+    for a gradient, or a forward-mode level is open (whose tangents do not;
+    an autograd.Function without a jvp refuses them, where a plain call would
+    drop them)."""
+    if getattr(_forward_ad, "_current_level", 0) >= 0:
+        return True
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """For the dispatcher's operators, which autograd passes by when nothing
+    asks for a gradient."""
+    if getattr(_forward_ad, "_current_level", 0) >= 0 and any(
+            t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def require_cuda(*tensors) -> None:

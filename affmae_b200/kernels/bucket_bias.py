@@ -163,7 +163,7 @@ def bucket_bias(table: torch.Tensor, edges, q_pos: torch.Tensor, k_pos: torch.Te
     Differentiable once in the table."""
     dtype = table.dtype if dtype is None else dtype
     edges = _check(table, edges, q_pos, k_pos, member_idx, one_sided, dtype)
-    if not (torch.is_grad_enabled() and table.requires_grad):
+    if not nat.differentiates(table):
         return bucket_bias_fwd(table.contiguous(), edges, nat.dense(q_pos), nat.dense(k_pos), _members(member_idx),
                                one_sided, dtype)
     return BucketBiasFunction.apply(table, edges, q_pos, k_pos, member_idx, one_sided, dtype)

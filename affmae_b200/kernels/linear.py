@@ -161,9 +161,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     "silu".  Differentiable once in x, weight, bias and residual."""
     code = ACTIVATIONS[act] if act in ACTIVATIONS else _act_code(act)
     _check_operands(x, weight, bias, residual)
-    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                         or (bias is not None and bias.requires_grad)
-                                         or (residual is not None and residual.requires_grad))):
+    if not nat.differentiates(x, weight, bias, residual):
         return linear_fwd(nat.dense(x), nat.dense(weight), bias, residual, code, False)[0]
     return FusedLinearFunction.apply(x, weight, bias, residual, code)
 

@@ -140,8 +140,7 @@ def fused_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, del
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in _FLOATS:
         raise RuntimeError(f"rms_norm: unsupported output dtype {out_dtype}")
-    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                         or (delta is not None and delta.requires_grad))):
+    if not nat.differentiates(x, weight, delta):
         _, _, _, s, _, y, _, _ = _launch(x, delta, row_scale, weight, eps, out_dtype, False)
         return y if s is None else (s, y)
     return FusedRMSNormFunction.apply(x, weight, delta, row_scale, eps, out_dtype)

@@ -191,6 +191,7 @@ def linear_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, resi
     """(out, z): z holds the pre-activation sums, empty where the backward needs none."""
     code = _li._act_code(act)
     _li._check_operands(x, weight, bias, residual)
+    _nat.refuse_tangents("affb200::linear_fwd", x, weight, bias, residual)
     out, z = _li.linear_fwd(_nat.dense(x), _nat.dense(weight), bias, residual, code, True)
     return out, (z if z is not None else x.new_empty(_EMPTY))
 
@@ -252,6 +253,7 @@ def rms_norm_fwd(x: Tensor, weight: Tensor, eps: float, delta: Optional[Tensor],
                  out_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
     """(s, y, rstd): s is empty without delta."""
     _rn._check(x, weight, delta, row_scale)
+    _nat.refuse_tangents("affb200::rms_norm_fwd", x, weight, delta)
     _, _, _, s, rstd, y, _, _ = _rn._launch(x, delta, row_scale, weight, eps, out_dtype, True)
     return (s if s is not None else x.new_empty(_EMPTY)), y, rstd
 
@@ -316,6 +318,7 @@ def _(x, weight, eps, delta, row_scale):
 def bucket_bias_fwd(table: Tensor, edges: list[int], q_pos: Tensor, k_pos: Tensor, member_idx: Optional[Tensor],
                     one_sided: bool, dtype: torch.dtype) -> Tensor:
     edges = _bb._check(table, edges, q_pos, k_pos, member_idx, one_sided, dtype)
+    _nat.refuse_tangents("affb200::bucket_bias_fwd", table)
     return _bb.bucket_bias_fwd(table.contiguous(), edges, _nat.dense(q_pos), _nat.dense(k_pos),
                                _bb._members(member_idx), one_sided, dtype)
 

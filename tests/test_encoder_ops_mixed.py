@@ -7,10 +7,12 @@ import threading
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from affmae_b200 import _native as nat
 from affmae_b200.kernels.bucket_bias import bucket_bias, bucket_count, log_edges
-from affmae_b200.kernels.linear import quantize_e4m3
+from affmae_b200.kernels.linear import fused_linear, quantize_e4m3
+from affmae_b200.kernels.rms_norm import fused_rms_norm
 from test_encoder_ops import BF16, E, FP16, FP32, TINY, U, bias_inputs, check_e4m3, rnd, rows_ref, within
 
 
@@ -112,3 +114,32 @@ def test_threads_that_launch_one_kernel_with_different_shared_memory(cuda):
         t.join()
     torch.cuda.synchronize()
     assert not errors, f"{len(errors)} calls failed: {errors[0]}"
+
+
+# ---------------------------------------------------- forward-mode -------
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(cuda):
+    """No operator has a forward-mode derivative: a tangent is refused, with and without a gradient asked for, by the
+    functions and by the dispatcher's operators; what has no tangent still runs inside a level."""
+    import affmae_b200.ops  # noqa: F401
+    ops = torch.ops.affb200
+    x, w, d = rnd(cuda, 1, 40, 24), rnd(cuda, 2, 16, 24), rnd(cuda, 3, 40, 24)
+    table, pos, ones = rnd(cuda, 4, 25, 3), rnd(cuda, 5, 1, 6, 2, std=3.0), torch.ones(24, device=cuda)
+    calls = [(lambda t: fused_linear(t, w), x), (lambda t: fused_linear(x, t, act="gelu"), w),
+             (lambda t: fused_linear(x, w, t), rnd(cuda, 6, 16)),
+             (lambda t: fused_linear(x, w, None, "none", t), rnd(cuda, 7, 40, 16)),
+             (lambda t: fused_rms_norm(t, ones), x), (lambda t: fused_rms_norm(x, t), ones),
+             (lambda t: fused_rms_norm(x, ones, delta=t)[0], d),
+             (lambda t: bucket_bias(t, (1, 3), pos, pos), table),
+             (lambda t: ops.linear_fwd(t, w, None, "none", None)[0], x),
+             (lambda t: ops.rms_norm_fwd(x, ones, 1e-6, t, None, FP32)[0], d),
+             (lambda t: ops.bucket_bias_fwd(t, [1, 3], pos, pos, None, False, FP32), table)]
+    for f, t in calls:
+        want = f(t)
+        with fwAD.dual_level():
+            assert torch.equal(f(t), want)
+            for leaf in (t, t.clone().requires_grad_(True)):
+                with pytest.raises((NotImplementedError, RuntimeError), match="jvp|forward-mode|forward mode"):
+                    f(fwAD.make_dual(leaf, torch.ones_like(t)))
+        assert torch.equal(f(t), want)
