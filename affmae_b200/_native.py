@@ -229,6 +229,24 @@ def differentiates(*tensors) -> bool:
     return False
 
 
+class _ForwardOnly(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, name, run, *tensors):
+        ctx.name = name
+        return run()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name} has no gradient: 8-bit values are for inference (torch.no_grad() leaves "
+                           "them out of the graph)")
+
+
+def forward_only(name: str, run, *tensors):
+    """``run()``; where autograd has to see the call, its outputs refuse a
+    gradient when one is asked of them, instead of passing for constants."""
+    return _ForwardOnly.apply(name, run, *tensors) if differentiates(*tensors) else run()
+
+
 def refuse_tangents(name: str, *tensors) -> None:
     """For the dispatcher's operators, which autograd passes by when nothing
     asks for a gradient."""

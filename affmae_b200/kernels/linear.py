@@ -191,10 +191,15 @@ class FusedLinear(nn.Linear):
 
 def quantize_e4m3(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows of x [..., C] as e4m3 values and the fp32 scale [...] of each row:
-    x ~ q * scale, scale = max|row| / 448 (1 for a zero row)."""
+    x ~ q * scale, scale = max|row| / 448 (1 for a zero row).  A gradient
+    through it is refused."""
     nat.require_cuda(x)
     if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in _FLOATS:
         raise RuntimeError("quantize_e4m3: needs fp32, fp16 or bf16 rows of at least one value")
+    return nat.forward_only("quantize_e4m3", lambda: _quantize(x), x)
+
+
+def _quantize(x):
     xc = nat.dense(x.detach())
     C = x.shape[-1]
     q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
@@ -209,19 +214,29 @@ def linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``act((x * x_scale) @ (weight * weight_scale).T + bias) + residual`` for
     e4m3 x [..., K] and weight [N, K] with fp32 scales per row ([...] and
-    [N]); bias fp32; residual of any float dtype; forward only."""
+    [N]); bias fp32; residual of any float dtype.  A gradient through it is
+    refused."""
     code = _act_code(act)
     _check(x, weight, bias, residual)
     if x.dtype != torch.float8_e4m3fn or weight.dtype != torch.float8_e4m3fn:
         raise RuntimeError("linear_e4m3: input and weight must be float8_e4m3fn")
     if out_dtype not in _FLOATS or (residual is not None and residual.dtype not in _FLOATS):
         raise RuntimeError("linear_e4m3: output and residual must be fp32, fp16 or bf16")
-    N, K = weight.shape
     index = x.get_device()
     if x_scale.shape != x.shape[:-1] or weight_scale.shape != weight.shape[:1]:
         raise RuntimeError("linear_e4m3: scales must have one value per row")
     if x_scale.get_device() != index or weight_scale.get_device() != index:
         raise RuntimeError("linear_e4m3: scales must be on the operands' device")
+    if nat.differentiates(x, x_scale, weight, weight_scale, bias, residual):
+        return nat.forward_only("linear_e4m3",
+                                lambda: _linear_e4m3(x, x_scale, weight, weight_scale, bias, code, residual, out_dtype),
+                                x, x_scale, weight, weight_scale, bias, residual)
+    return _linear_e4m3(x, x_scale, weight, weight_scale, bias, code, residual, out_dtype)
+
+
+def _linear_e4m3(x, x_scale, weight, weight_scale, bias, code, residual, out_dtype):
+    N, K = weight.shape
+    index = x.get_device()
     M = x.numel() // K
     x, weight = nat.dense(x), nat.dense(weight)
     x_scale, weight_scale = _f32(x_scale), _f32(weight_scale)
@@ -254,7 +269,7 @@ class LinearE4M3(nn.Module):
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None, act: str = "none"):
         super().__init__()
         _act_code(act)
-        q, scale = quantize_e4m3(weight)
+        q, scale = quantize_e4m3(weight.detach())
         self.act = act
         self.register_buffer("weight", q)
         self.register_buffer("weight_scale", scale)

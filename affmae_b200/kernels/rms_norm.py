@@ -150,10 +150,14 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, delt
                   row_scale: torch.Tensor | None = None):
     """(q, scale), or (s, q, scale) when ``delta`` is given: the norm with its
     output as e4m3 rows, ``y ~ q * scale``, ``scale = max|y| / 448`` of each
-    row (1 for a zero row).  No gradient."""
+    row (1 for a zero row).  A gradient through it, that of s included, is
+    refused."""
     _check(x, weight, delta, row_scale)
-    _, _, _, s, _, _, q, scale = _launch(x, delta, row_scale, weight, eps, None, False)
-    return (q, scale) if delta is None else (s, q, scale)
+
+    def run():
+        _, _, _, s, _, _, q, scale = _launch(x, delta, row_scale, weight, eps, None, False)
+        return (q, scale) if delta is None else (s, q, scale)
+    return nat.forward_only("rms_norm_e4m3", run, x, weight, delta)
 
 
 class FusedRMSNorm(nn.Module):

@@ -239,6 +239,7 @@ linear_fwd.register_autograd(_linear_backward, setup_context=_linear_setup)
 @custom_op("affb200::linear_e4m3", mutates_args=())
 def linear_e4m3(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor], act: str,
                 residual: Optional[Tensor], out_dtype: torch.dtype) -> Tensor:
+    _nat.refuse_tangents("affb200::linear_e4m3", x_scale, weight_scale, bias, residual)
     return _li.linear_e4m3(x, x_scale, weight, weight_scale, bias, act, residual, out_dtype)
 
 
@@ -303,6 +304,7 @@ rms_norm_fwd.register_autograd(_rms_backward, setup_context=_rms_setup)
 def rms_norm_e4m3(x: Tensor, weight: Tensor, eps: float, delta: Optional[Tensor], row_scale: Optional[Tensor]
                   ) -> tuple[Tensor, Tensor, Tensor]:
     """(s, q, scale): s is empty without delta."""
+    _nat.refuse_tangents("affb200::rms_norm_e4m3", x, weight, delta)
     got = _rn.rms_norm_e4m3(x, weight, eps, delta, row_scale)
     return got if delta is not None else (x.new_empty(_EMPTY), *got)
 

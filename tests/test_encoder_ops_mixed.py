@@ -11,8 +11,8 @@ import torch.autograd.forward_ad as fwAD
 
 from affmae_b200 import _native as nat
 from affmae_b200.kernels.bucket_bias import bucket_bias, bucket_count, log_edges
-from affmae_b200.kernels.linear import fused_linear, quantize_e4m3
-from affmae_b200.kernels.rms_norm import fused_rms_norm
+from affmae_b200.kernels.linear import LinearE4M3, fused_linear, linear_e4m3, quantize_e4m3
+from affmae_b200.kernels.rms_norm import fused_rms_norm, rms_norm_e4m3
 from test_encoder_ops import BF16, E, FP16, FP32, TINY, U, bias_inputs, check_e4m3, rnd, rows_ref, within
 
 
@@ -143,3 +143,48 @@ def test_forward_mode_is_refused(cuda):
                 with pytest.raises((NotImplementedError, RuntimeError), match="jvp|forward-mode|forward mode"):
                     f(fwAD.make_dual(leaf, torch.ones_like(t)))
         assert torch.equal(f(t), want)
+
+
+# ------------------------------------------------- 8-bit operands --------
+
+@pytest.mark.gpu
+def test_eight_bit_operators_refuse_a_gradient(cuda):
+    """Their outputs do not pass for constants: asking for a gradient is refused, also of the residual stream that the
+    norm returns, of a residual added to the product, and in forward mode; under no_grad nothing is recorded."""
+    x, w, d = (rnd(cuda, i, 40, 32).requires_grad_(True) for i in (1, 2, 3))
+    ones, b = torch.ones(32, device=cuda, requires_grad=True), torch.zeros(40, device=cuda, requires_grad=True)
+    res = rnd(cuda, 4, 40, 40).requires_grad_(True)
+    with torch.no_grad():
+        q, sc = quantize_e4m3(x)
+        wq, ws = quantize_e4m3(w)
+        want = rms_norm_e4m3(x, ones, delta=d)
+    assert not any(t.requires_grad for t in (q, sc, *want))
+    outs = [quantize_e4m3(w)[1], *rms_norm_e4m3(x, ones, delta=d)[::2], rms_norm_e4m3(x.detach(), ones)[1],
+            rms_norm_e4m3(x.detach(), ones.detach(), delta=d)[0], linear_e4m3(q, sc, wq, ws, b),
+            linear_e4m3(q, sc, wq, ws, None, "none", res), linear_e4m3(q, sc, *quantize_e4m3(w))]
+    for out in outs:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            out.float().sum().backward()
+    assert all(t.grad is None for t in (x, w, d, ones, b, res))
+    for p, r in zip(rms_norm_e4m3(x, ones, delta=d), want):
+        assert torch.equal(p.detach().float(), r.float())
+    with fwAD.dual_level():
+        t = fwAD.make_dual(x.detach(), torch.ones_like(x))
+        for f in (lambda: quantize_e4m3(t), lambda: rms_norm_e4m3(t, ones.detach())):
+            with pytest.raises((NotImplementedError, RuntimeError), match="jvp|forward-mode|forward mode"):
+                f()
+    layer = LinearE4M3(w, b)
+    assert not any(t.requires_grad for t in layer.state_dict().values())
+
+
+@pytest.mark.gpu
+def test_quantised_block_refuses_a_gradient(cuda):
+    from test_rms_block import _block, _inputs
+    blk = _block(cuda).eval().quantize()
+    pos, member, mask, feat = _inputs(cuda)
+    with torch.no_grad():
+        want, _ = blk(feat, member, mask, pos)
+    got, _ = blk(feat, member, mask, pos)
+    assert torch.equal(got.detach(), want)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        got.sum().backward()
