@@ -42,7 +42,7 @@ from .kernels.fused_deform_attn import (fused_knn_deformable_cross_attention,
 from .kernels.head_layout import merge_heads, split_heads
 from .kernels.knn import knn
 from .kernels.layer_norm import FusedLayerNorm
-from .kernels.linear import FusedLinear, LinearE4M3
+from .kernels.linear import FusedLinear, linear_e4m3, quantize_e4m3
 from .kernels.local_attn import FlashLocalAttentionFunction
 from .kernels.pos_bias import pos_bias_gather, rel_pos_bias
 from .kernels.relu_dropout import relu_dropout
@@ -334,8 +334,8 @@ class RMSClusterBlock(nn.Module):
 
     A branch that stochastic depth scales is added by the next norm, which
     takes the per-sample factor; any other is added to the stream by the
-    product's epilogue.  After ``quantize()`` (inference) the projections that
-    read a norm run on e4m3 operands."""
+    product's epilogue.  After ``quantize()`` the projections that read a norm
+    run on e4m3 operands in eval mode."""
 
     def __init__(self, dim: int, heads: int, mlp_ratio: float, drop_path: float, edges: tuple):
         super().__init__()
@@ -346,21 +346,28 @@ class RMSClusterBlock(nn.Module):
         self.fc1 = FusedLinear(dim, hidden, act="gelu")
         self.fc2 = FusedLinear(hidden, dim)
         self.drop_path = DropPath(drop_path)
-        self.eight_bit = None
+        self.eight_bit = False
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        # checkpoints of quantised blocks once held copies of the weights in e4m3
+        for k in [k for k in state_dict if k.startswith(prefix + "eight_bit.")]:
+            del state_dict[k]
+        super()._load_from_state_dict(state_dict, prefix, *args)
 
     def quantize(self):
-        """Keep e4m3 copies of the weights that read a norm and use them in
-        eval mode.  Returns self."""
-        self.eight_bit = nn.ModuleDict({n: LinearE4M3.from_linear(m) for n, m in
-                                        (("q", self.attn.q), ("kv", self.attn.kv), ("fc1", self.fc1))})
+        """Use e4m3 operands in eval mode.  No copies of the weights are kept:
+        each call rounds them as they are then (a fraction of a product's
+        time), so training or loading weights in between needs no care.
+        Returns self."""
+        self.eight_bit = True
         return self
 
-    def _project(self, norm, x, delta, factor, layers, names):
+    def _project(self, norm, x, delta, factor, *layers):
         """The stream (x, or x + factor * delta) and its norm through `layers`."""
         dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
-        if self.eight_bit is not None and not self.training:
+        if self.eight_bit and not self.training:
             *s, q, scale = norm.quantized(x, delta, factor)
-            outs = [self.eight_bit[n](q, scale, out_dtype=dt) for n in names]
+            outs = [linear_e4m3(q, scale, *quantize_e4m3(m.weight), m.bias, m.act, out_dtype=dt) for m in layers]
         else:
             y = norm(x, delta, factor, dt)
             s, y = ((), y) if delta is None else ((y[0],), y[1])
@@ -372,13 +379,13 @@ class RMSClusterBlock(nn.Module):
         if pending is None and torch.is_autocast_enabled("cuda"):
             feat = feat.float()  # the residual stream
         delta, f = (None, None) if pending is None else pending
-        feat, (q, kv) = self._project(self.norm1, feat, delta, f, (self.attn.q, self.attn.kv), ("q", "kv"))
+        feat, (q, kv) = self._project(self.norm1, feat, delta, f, self.attn.q, self.attn.kv)
         f = self.drop_path.factor(feat.shape[0], feat.device)
         if f is None:
             feat, delta = self.attn(q, kv, member_idx, mask, pos, global_attn, residual=feat), None
         else:
             delta = self.attn(q, kv, member_idx, mask, pos, global_attn)
-        feat, (h,) = self._project(self.norm2, feat, delta, f, (self.fc1,), ("fc1",))
+        feat, (h,) = self._project(self.norm2, feat, delta, f, self.fc1)
         f = self.drop_path.factor(feat.shape[0], feat.device)
         if f is None:
             return self.fc2(h, residual=feat), None
@@ -751,9 +758,9 @@ class AFFMaskedAutoEncoder(nn.Module):
         self.head_res2 = PredictionHead(D, out)
 
     def quantize_encoder(self):
-        """Inference with 8-bit operands: every "rms" encoder block keeps e4m3
-        copies of the projections that read a norm (used in eval mode; call
-        again after a change of the weights).  Returns self."""
+        """Inference with 8-bit operands: in eval mode the projections of every
+        "rms" encoder block that read a norm run on e4m3 operands.  Returns
+        self."""
         if self.cfg.block != "rms":
             raise RuntimeError('quantize_encoder needs MAEConfig(block="rms")')
         for mod in self.modules():

@@ -188,3 +188,64 @@ def test_quantised_block_refuses_a_gradient(cuda):
     assert torch.equal(got.detach(), want)
     with pytest.raises(RuntimeError, match="no gradient"):
         got.sum().backward()
+
+
+@pytest.mark.gpu
+def test_quantised_block_answers_with_the_weights_it_has(cuda):
+    """After a change of the weights by any way, a quantised block answers as one that is quantised then; its state
+    is that of the block itself."""
+    from test_rms_block import _block, _inputs
+    pos, member, mask, feat = _inputs(cuda)
+    blk, other = _block(cuda).eval(), _block(cuda, seed=9).eval()
+    names = list(blk.state_dict())
+    blk.quantize()
+    assert list(blk.state_dict()) == names
+    other.load_state_dict(blk.state_dict())
+
+    def answer(b):
+        with torch.no_grad():
+            return b(feat, member, mask, pos)[0]
+
+    def in_place(b):
+        with torch.no_grad():
+            for p in b.parameters():
+                p.mul_(1.25)
+
+    def behind(b):
+        for p in b.parameters():
+            p.data = p.data * 0.5 + 0.01
+            p.data.add_(0.01)
+
+    def replaced(b):
+        b.fc1.weight = torch.nn.Parameter(b.fc1.weight.detach().flip(0))
+
+    def loaded(b):
+        b.load_state_dict({k: v * 0.75 for k, v in _block(cuda, seed=11).state_dict().items()})
+
+    def trained(b):
+        b.train()
+        b(feat, member, mask, pos)[0].square().mean().backward()
+        with torch.no_grad():
+            for p in b.parameters():
+                p -= 0.1 * p.grad
+        b.eval()
+    before = answer(blk)
+    for change in (in_place, behind, replaced, loaded, trained):
+        change(blk)
+        change(other)
+        got = answer(blk)
+        want = answer(other.quantize())
+        assert torch.equal(got, want) and not torch.equal(got, before), change.__name__
+        before = got
+    fresh = _block(cuda, seed=12).eval()
+    fresh.load_state_dict(blk.state_dict())
+    assert torch.equal(answer(fresh.quantize()), before)
+
+
+def test_checkpoints_with_the_former_copies_load():
+    from affmae_b200.mae import RMSClusterBlock
+    blk = torch.nn.Sequential(RMSClusterBlock(8, 1, 2.0, 0.0, (1, 2)))
+    state = blk.state_dict()
+    blk.load_state_dict({**state, "0.eight_bit.q.weight": torch.zeros(8, 8), "0.eight_bit.q.bias": torch.zeros(8)})
+    with pytest.raises(RuntimeError, match="other"):
+        blk.load_state_dict({**state, "0.other.q.weight": torch.zeros(8, 8)})
