@@ -82,6 +82,7 @@ SIGNATURES = {
     "affb_linear_bwd": [_p, _i32, _p, _p, _p, _i32, _i32, _i64, _i64, _i64, _p, _p, _p, _i32, _p, _i64, _p],
     "affb_linear_e4m3": [_p, _p, _p, _p, _p, _p, _i32, _i32, _i64, _i64, _i64, _p, _i32, _p, _i64, _p],
     "affb_linear_status": [_p],
+    "affb_linear_wait_probe": [_i32, _p],
     "affb_rms_norm_fwd": [_p, _i32, _p, _i32, _p, _i64, _p, _f32, _i64, _i64, _p, _p, _p, _i32, _p, _p, _p],
     "affb_quantize_e4m3": [_p, _i32, _i64, _i64, _p, _p, _p],
     "affb_rms_norm_bwd": [_p, _i32, _p, _p, _i32, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _i32, _p, _p, _i64, _p],

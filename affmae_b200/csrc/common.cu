@@ -12,6 +12,36 @@ void set_error(const char* fmt, ...) {
   va_end(ap);
 }
 
+constexpr int MAX_DEVICES = 64;
+
+int* failure_word() {
+  // allocated once; relaxed, so that a thread that is capturing a graph may come first
+  static int* const words = [] {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    void* p = nullptr;
+    if (cudaHostAlloc(&p, MAX_DEVICES * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
+      cudaGetLastError();
+      p = nullptr;
+    } else {
+      memset(p, 0, MAX_DEVICES * sizeof(int));
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return (int*)p;
+  }();
+  int dev = 0;
+  if (!words || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return nullptr;
+  return words + dev;
+}
+
+int take_failure() {
+  int* word = failure_word();
+  AFFB_REQUIRE(word, "no host memory for the device's failure word");
+  if (__atomic_load_n(word, __ATOMIC_RELAXED) == 0 || __atomic_exchange_n(word, 0, __ATOMIC_RELAXED) == 0) return AFFB_OK;
+  set_error("an earlier product or norm on this device gave up a bounded wait: its output is incomplete");
+  return AFFB_ERR_CUDA;
+}
+
 int sm_count() {
   static int cached[64] = {0};
   int dev = 0;

@@ -76,6 +76,18 @@ inline cudaError_t allow_dynamic_smem(K kernel, int smem) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
 }
 
+// ------------------------------------------------------- waits that run out --
+// A kernel that gives up a bounded wait leaves its output incomplete.  It then
+// writes 1 to its device's word in host memory (report_failure), so that the
+// next call that may wait, or affb_linear_status, finds out without a
+// synchronisation; either clears the word as it reports it.
+int* failure_word();  // of the current device; null where there is none
+int take_failure();   // AFFB_OK, or an error (once) when the word is set
+__device__ __forceinline__ void report_failure(int* word) {
+  *reinterpret_cast<volatile int*>(word) = 1;
+  __threadfence_system();
+}
+
 // ------------------------------------------------------------ conversions --
 template <typename T> struct io;
 template <> struct io<float> {

@@ -47,9 +47,6 @@ constexpr int BUF_BYTES = WARP_ROWS * 128;  // staged rows of 128 bytes: 64 colu
 constexpr int BAR_BYTES = 512;
 constexpr int COLS_BYTES = EPI_WARPS * 2 * WARP_COLS * 4;  // each epilogue warp's bias and column scales
 
-// Set when a block's waits ran out; read by affb_linear_status.
-__device__ int g_linear_failed;
-
 struct GemmArgs {
   int M, N, bn, mt, nt, splits;
   int kblocks;       // 128-byte blocks of the contraction
@@ -63,6 +60,7 @@ struct GemmArgs {
   int res_rows;      // rows of the residual are 16-byte aligned
   int res_tma;       // the residual is brought into the second staging buffer while the products run
   int bufs;          // staging buffers of a warp: out, and z where it is wanted
+  int* failed;       // the device's failure word
   LinearEpilogue e;
 };
 
@@ -514,7 +512,7 @@ __global__ void __launch_bounds__(LIN_THREADS, 1)
     fence_after();
     tmem_free<CG>(tmem);
   }
-  if (threadIdx.x == 0 && *failed) atomicExch(&g_linear_failed, 1);
+  if (threadIdx.x == 0 && *failed) report_failure(p.failed);
 }
 
 // ------------------------------------------------------------------ host --
@@ -700,6 +698,8 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
   const int et = dtype == AFFB_F32 ? AFFB_BF16 : dtype;  // element type in memory
   const int64_t planes = dtype == AFFB_F32 ? 3 : 1;
   GemmArgs p{};
+  p.failed = failure_word();
+  AFFB_REQUIRE(p.failed, "linear: no host memory for the device's failure word");
   p.M = (int)M; p.N = (int)N;
   p.bn = s.bn; p.mt = s.mt; p.nt = s.nt; p.splits = s.splits;
   p.parts = dtype == AFFB_F32 ? 6 : 1;
@@ -825,10 +825,11 @@ static int check_sizes(int64_t M, int64_t N, int64_t K) {
 
 static int forward(const void* x, const void* w, int dtype, int64_t M, int64_t N, int64_t K, const LinearEpilogue& e,
                    void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+  int rc = take_failure();
+  if (rc) return rc;
   if (few_rows(dtype, M, N, K)) return linear_small(x, w, dtype, M, N, K, e, st);
   Arena ws{(unsigned char*)workspace, 0, workspace ? workspace_bytes : 0};
   Operand a, b;
-  int rc;
   SplitRows sx{}, sw{};
   if ((rc = make_operand(dtype, x, M, K, false, &ws, &a, &sx, st))) return rc;
   if ((rc = make_operand(dtype, w, N, K, false, &ws, &b, &sw, st))) return rc;
@@ -845,14 +846,32 @@ using namespace affb;
 
 extern "C" int affb_linear_status(int* failed) {
   AFFB_REQUIRE(failed, "affb_linear_status: null pointer");
-  int norms = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(failed, g_linear_failed, sizeof(int));
-  if (e == cudaSuccess) e = rms_failed(&norms);
-  *failed |= norms;
+  *failed = 0;
+  const cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) {
     set_error("affb_linear_status: %s", cudaGetErrorString(e));
     return AFFB_ERR_CUDA;
   }
+  *failed = take_failure() != AFFB_OK;
+  return AFFB_OK;
+}
+
+// One thread waits for a barrier that nothing completes, as the products do.
+__global__ void wait_probe_kernel(unsigned long long limit_ns, int* word) {
+  __shared__ __align__(8) unsigned long long bar;
+  __shared__ int failed;
+  failed = 0;
+  bar_init(smem_addr(&bar), 1);
+  bar_init_fence();
+  if (!bar_wait(smem_addr(&bar), 0, &failed, limit_ns)) report_failure(word);
+}
+
+extern "C" int affb_linear_wait_probe(int limit_ms, void* stream) {
+  AFFB_REQUIRE(limit_ms >= 1 && limit_ms <= 2000, "affb_linear_wait_probe: a limit of 1 to 2000 ms");
+  int* word = failure_word();
+  AFFB_REQUIRE(word, "affb_linear_wait_probe: no host memory for the device's failure word");
+  wait_probe_kernel<<<1, 1, 0, as_stream(stream)>>>(limit_ms * 1000000ull, word);
+  AFFB_LAUNCH_CHECK("affb_linear_wait_probe");
   return AFFB_OK;
 }
 
@@ -930,6 +949,7 @@ extern "C" int affb_linear_bwd(const void* dout, int dout_dtype, const void* z, 
   }
   AFFB_REQUIRE(dout && (act == AFFB_ACT_NONE || z) && (!dx || weight) && (!dweight || x), "linear: null pointer");
   AFFB_REQUIRE(workspace, "linear: workspace missing");
+  if ((rc = take_failure())) return rc;
   Arena ws{(unsigned char*)workspace, 0, workspace_bytes};
 
   // dz: the output gradient itself when nothing changes it

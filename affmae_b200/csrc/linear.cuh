@@ -48,9 +48,6 @@ inline bool few_rows(int dtype, int64_t M, int64_t N, int64_t K) {
 int linear_small(const void* x, const void* w, int dtype, int64_t M, int64_t N, int64_t K, const LinearEpilogue& e,
                  cudaStream_t st);
 
-// rms_norm.cu: 1 in *failed if one of its waits ran out
-cudaError_t rms_failed(int* failed);
-
 // linear_aux.cu
 // rows [R,C] -> [R,ld] of the same element size (the tail of a row is not written)
 int linear_pack(const void* src, int64_t elem, int64_t R, int64_t C, void* dst, int64_t ld, cudaStream_t st);

@@ -117,9 +117,6 @@ __device__ __forceinline__ float row_reduce(float v, float* red, Op op) {
   return v;
 }
 
-// Set when a wait on a copy ran out; read by rms_failed().
-__device__ int g_rms_failed;
-
 // Rounds of rows on their way into shared memory: up to four arrays with the
 // same rows, stage after stage.
 struct RowPipe {
@@ -128,6 +125,7 @@ struct RowPipe {
   int rows;           // of a round
   int stages;
   int stage_bytes;
+  int* failed;        // the device's failure word
 };
 constexpr int PIPE_HEAD = 128;  // barriers and the failure flag, before the stages
 
@@ -201,7 +199,7 @@ struct PipeReader {
         if (((int64_t)blockIdx.x + (it + i) * gridDim.x) * ROWS < R)
           tc5::bar_drain(bars + 8 * st, stage + i >= p.stages ? phase ^ 1 : phase);
       }
-      atomicExch(&g_rms_failed, 1);
+      report_failure(p.failed);
     }
   }
 };
@@ -568,7 +566,8 @@ static RowPipe rms_pipe(const RowLayout& l, int64_t R, int64_t blocks, const voi
             {(int)a_bytes, b ? (int)b_bytes : 0, c ? (int)c_bytes : 0, d ? (int)d_bytes : 0},
             256 / l.tpr,
             0,
-            0};
+            0,
+            failure_word()};
   if (l.nv == 0 || R < 3 * blocks * p.rows) return p;
   p.stage_bytes = p.rows * (p.row_bytes[0] + p.row_bytes[1] + p.row_bytes[2] + p.row_bytes[3]);
   p.stage_bytes = (p.stage_bytes + 127) / 128 * 128;
@@ -637,7 +636,6 @@ static int rms_status(cudaError_t e) {
   set_error("rms_norm: launch failed: %s", cudaGetErrorString(e));
   return AFFB_ERR_CUDA;
 }
-cudaError_t rms_failed(int* failed) { return cudaMemcpyFromSymbol(failed, g_rms_failed, sizeof(int)); }
 
 static bool rms_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -668,6 +666,7 @@ extern "C" int affb_rms_norm_fwd(const void* x, int x_dtype, const void* delta, 
   AFFB_REQUIRE(!s || delta, "rms_norm: the sum is written only with delta");
   if (R == 0) return AFFB_OK;
   AFFB_REQUIRE(x && weight, "rms_norm: null pointer");
+  if ((rc = take_failure())) return rc;
   RmsArgs a{x, delta, delta_dtype, row_scale, row_scale ? R / groups : 1, weight, eps, R, (int)C, s, rstd, y, y_dtype,
             (uint8_t*)q, q_scale};
   const bool vec = C % 8 == 0 && rms_aligned(x) && rms_aligned(delta) && rms_aligned(weight) && rms_aligned(s) &&
@@ -682,6 +681,7 @@ extern "C" int affb_quantize_e4m3(const void* x, int dtype, int64_t R, int64_t C
   if (rc) return rc;
   if (R == 0) return AFFB_OK;
   AFFB_REQUIRE(x && q && q_scale, "quantize_e4m3: null pointer");
+  if ((rc = take_failure())) return rc;
   RmsArgs a{x, nullptr, AFFB_F32, nullptr, 1, nullptr, 0.f, R, (int)C, nullptr, nullptr, nullptr, AFFB_F32, (uint8_t*)q, q_scale};
   const bool vec = C % 8 == 0 && rms_aligned(x) && ((uintptr_t)q & 7) == 0;
   cudaStream_t st = as_stream(stream);
@@ -715,6 +715,7 @@ extern "C" int affb_rms_norm_bwd(const void* dy, int y_dtype, const void* ds, co
                    rms_aligned(dx) && rms_aligned(ddelta) && rms_aligned(delta);
   AFFB_REQUIRE(!dweight || (workspace && workspace_bytes >= affb_rms_norm_bwd_workspace_bytes(R, C)),
                "rms_norm: workspace too small");
+  if ((rc = take_failure())) return rc;
   int64_t blocks = 0;
   RmsBwdArgs a{dy, y_dtype, ds, s, delta, rstd, weight, row_scale, row_scale ? R / groups : 1, R, (int)C, dx, ddelta, delta_dtype,
                dweight ? (float*)workspace : nullptr};

@@ -67,7 +67,8 @@ __device__ __forceinline__ bool bar_poll(uint32_t bar, uint32_t parity) {
 // block has failed or the wait ran out (which marks the block as failed).
 // The timer is read only by a wait that has already polled long: one read
 // takes longer than a stage of the pipeline does.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* failed,
+                                         unsigned long long limit = WAIT_NS) {
 #pragma unroll 1
   for (int i = 0; i < 4096; ++i)
     if (bar_poll(bar, parity)) return true;
@@ -77,7 +78,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     for (int i = 0; i < 256; ++i)
       if (bar_poll(bar, parity)) return true;
     if (*failed) return false;
-    if (now_ns() - t0 > WAIT_NS) break;
+    if (now_ns() - t0 > limit) break;
   }
   *failed = 1;
   return false;

@@ -285,7 +285,9 @@ class LinearE4M3(nn.Module):
 
 def linear_status() -> bool:
     """True unless a product or norm on the current device gave up a bounded wait
-    (which leaves its output incomplete).  Synchronises."""
+    (which leaves its output incomplete) that no call has reported yet: the
+    next product or norm called after that raises RuntimeError, once.  Waits
+    for the device."""
     import ctypes
     failed = ctypes.c_int(0)
     nat.call("affb_linear_status", ctypes.addressof(failed))

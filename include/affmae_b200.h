@@ -394,9 +394,15 @@ int64_t affb_linear_e4m3_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int affb_linear_e4m3(const void* x, const float* x_scale, const void* weight, const float* weight_scale,
                      const float* bias, const void* residual, int residual_dtype, int act, int64_t M, int64_t N,
                      int64_t K, void* out, int out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
-/* 1 in *failed if a product or norm on this device ever gave up one of its
- * bounded waits (its output is then incomplete), else 0.  Synchronises.     */
+/* A product or norm that gives up one of its bounded waits (seconds beyond any
+ * real one) leaves its output incomplete.  The next product or norm on the
+ * device that is called after that fails with AFFB_ERR_CUDA, once.
+ * affb_linear_status waits for the device and writes 1 to *failed if there has
+ * been such a wait that no call has reported yet, else 0; this reports it.  */
 int affb_linear_status(int* failed);
+/* A wait that nothing ends, given up after limit_ms (1 to 2000): what follows
+ * is what follows a real one.  To test a program's handling of it.          */
+int affb_linear_wait_probe(int limit_ms, void* stream);
 
 /* ------------------------------------------- root-mean-square norm --
  * s = x + f delta, y = s (mean(s^2) + eps)^-1/2 weight over rows of C.

@@ -11,7 +11,7 @@ import torch.autograd.forward_ad as fwAD
 
 from affmae_b200 import _native as nat
 from affmae_b200.kernels.bucket_bias import bucket_bias, bucket_count, log_edges
-from affmae_b200.kernels.linear import LinearE4M3, fused_linear, linear_e4m3, quantize_e4m3
+from affmae_b200.kernels.linear import LinearE4M3, fused_linear, linear_e4m3, linear_status, quantize_e4m3
 from affmae_b200.kernels.rms_norm import fused_rms_norm, rms_norm_e4m3
 from test_encoder_ops import BF16, E, FP16, FP32, TINY, U, bias_inputs, check_e4m3, rnd, rows_ref, within
 
@@ -249,3 +249,40 @@ def test_checkpoints_with_the_former_copies_load():
     blk.load_state_dict({**state, "0.eight_bit.q.weight": torch.zeros(8, 8), "0.eight_bit.q.bias": torch.zeros(8)})
     with pytest.raises(RuntimeError, match="other"):
         blk.load_state_dict({**state, "0.other.q.weight": torch.zeros(8, 8)})
+
+
+# ---------------------------------------------- waits that run out -------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["linear", "backward", "few rows", "e4m3", "norm", "norm backward", "quantize"])
+def test_a_wait_that_runs_out_is_reported_once(cuda, name):
+    """After it (here one of 50 ms that nothing ends, on a stream that blocks no other) the next call raises, and the
+    one after that runs; nothing is left behind."""
+    x, w = rnd(cuda, 1, 64, 64, dtype=BF16), rnd(cuda, 2, 32, 64, dtype=BF16)
+    ones = torch.ones(64, device=cuda)
+    q, s = quantize_e4m3(x)
+    leaf, vec = x.clone().requires_grad_(True), ones.clone().requires_grad_(True)
+    y, n = fused_linear(leaf, w), fused_rms_norm(x, vec)
+    f = {"linear": lambda: fused_linear(x, w), "few rows": lambda: fused_linear(x[:2], w),
+         "backward": lambda: torch.autograd.grad(y.sum(), leaf, retain_graph=True)[0],
+         "e4m3": lambda: linear_e4m3(q, s, q, s), "norm": lambda: fused_rms_norm(x, ones),
+         "norm backward": lambda: torch.autograd.grad(n.sum(), vec, retain_graph=True)[0],
+         "quantize": lambda: quantize_e4m3(x)[1]}[name]
+    want = f()
+    assert linear_status()
+    stream = torch.cuda.Stream()
+    nat.call("affb_linear_wait_probe", 50, stream.cuda_stream)
+    stream.synchronize()
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        f()
+    assert torch.equal(f(), want) and linear_status()
+
+
+@pytest.mark.gpu
+def test_status_waits_for_every_stream_and_reports_once(cuda):
+    assert linear_status()
+    nat.call("affb_linear_wait_probe", 200, torch.cuda.Stream().cuda_stream)
+    assert not linear_status()      # without waiting for that stream it would not know yet
+    assert linear_status()
+    with pytest.raises(RuntimeError, match="limit"):
+        nat.call("affb_linear_wait_probe", 0, None)
