@@ -19,7 +19,10 @@
 //
 // fp32 operands are split into three bf16 parts (8 mantissa bits each) and
 // the six leading products of parts are summed into the same accumulator,
-// smallest first; what is left out is of the order of 2^-24.
+// smallest first; what is left out is of the order of 2^-24.  A fourth plane
+// holds the first part with zeros for what is not finite: the products of an
+// infinity with the other operand's small parts, of either sign or zero, would
+// make NaN of it.
 //
 // Long contractions with few output tiles (the weight gradient sums over all
 // tokens) are split over blocks; partial products go to a workspace and are
@@ -65,9 +68,9 @@ struct GemmArgs {
 };
 
 // Parts of A and B of product i of an fp32 contraction, smallest first
-// (0: leading 8 bits, 1: next, 2: last).
-__device__ __forceinline__ int part_a(int i) { return (0x010120 >> (4 * i)) & 15; }
-__device__ __forceinline__ int part_b(int i) { return (0x001102 >> (4 * i)) & 15; }
+// (0: leading 8 bits, 1: next, 2: last, 3: leading ones of what is finite).
+__device__ __forceinline__ int part_a(int i) { return (0x013123 >> (4 * i)) & 15; }
+__device__ __forceinline__ int part_b(int i) { return (0x031132 >> (4 * i)) & 15; }
 
 // The units of work of a block or pair: (split, row tile, column tile), column
 // tiles fastest, every step-th.  Divides once, then steps by additions.
@@ -685,7 +688,7 @@ static bool tma_rows(const void* p, int dtype, int64_t N) {
 }
 
 // D = A B^T over a contraction of length K, then the epilogue.  `dtype` names
-// the operands' type as the caller has them (fp32: three bf16 planes each);
+// the operands' type as the caller has them (fp32: four bf16 planes each);
 // `ws` holds partial_bytes(...).
 static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K, LinearEpilogue e,
                 unsigned char* ws, cudaStream_t st) {
@@ -696,7 +699,7 @@ static int gemm(int dtype, const Operand& a, const Operand& b, int64_t M, int64_
   const Shape s = choose_shape(M, N, total_k, store_step(plain, e.out_dtype == AFFB_F32 && e.z ? e.z_dtype : e.out_dtype),
                                two_buffers ? WIDEST_TWO_BUFFERS : 256);
   const int et = dtype == AFFB_F32 ? AFFB_BF16 : dtype;  // element type in memory
-  const int64_t planes = dtype == AFFB_F32 ? 3 : 1;
+  const int64_t planes = dtype == AFFB_F32 ? SPLIT_PLANES : 1;
   GemmArgs p{};
   p.failed = failure_word();
   AFFB_REQUIRE(p.failed, "linear: no host memory for the device's failure word");
@@ -786,10 +789,12 @@ static int64_t pitch(int dtype, int64_t cols) { return round_up(cols, dtype == A
 static bool needs_copy(int dtype, const void* p, int64_t cols) {
   return dtype == AFFB_F32 || cols % (dtype == AFFB_E4M3 ? 16 : 8) != 0 || !aligned_to(p, 16);
 }
+// Bytes of a value in an operand's copy.
+static int64_t operand_size(int dtype) { return dtype == AFFB_F32 ? 2 * SPLIT_PLANES : dtype_size(dtype); }
 // Bytes of an operand's copy where its shape (or `any`: other reasons) needs one.
 static int64_t copy_bytes(int dtype, int64_t rows, int64_t cols, bool any) {
   if (!any && dtype != AFFB_F32 && cols % (dtype == AFFB_E4M3 ? 16 : 8) == 0) return 0;
-  return round_up(rows * pitch(dtype, cols) * (dtype == AFFB_F32 ? 6 : dtype_size(dtype)), 256);
+  return round_up(rows * pitch(dtype, cols) * operand_size(dtype), 256);
 }
 struct Arena {
   unsigned char* base;
@@ -806,7 +811,7 @@ static int make_operand(int dtype, const void* src, int64_t rows, int64_t cols, 
   *o = Operand{src, rows, cols, cols, mn};
   if (!needs_copy(dtype, src, cols)) return AFFB_OK;
   o->ld = pitch(dtype, cols);
-  void* dst = ws->take(rows * o->ld * (dtype == AFFB_F32 ? 6 : dtype_size(dtype)));
+  void* dst = ws->take(rows * o->ld * operand_size(dtype));
   AFFB_REQUIRE(dst, "linear: workspace too small (or an operand that is not 16-byte aligned)");
   o->p = dst;
   if (dtype != AFFB_F32) return linear_pack(src, dtype_size(dtype), rows, cols, dst, o->ld, st);
@@ -959,7 +964,7 @@ extern "C" int affb_linear_bwd(const void* dout, int dout_dtype, const void* z, 
   void* dzp = nullptr;
   if (want_dz && !as_is) {
     dz.ld = pitch(dtype, N);
-    dzp = ws.take(M * dz.ld * (dtype == AFFB_F32 ? 6 : dtype_size(dtype)));
+    dzp = ws.take(M * dz.ld * operand_size(dtype));
     AFFB_REQUIRE(dzp, "linear: workspace too small");
     dz.p = dzp;
   }

@@ -51,8 +51,10 @@ int linear_small(const void* x, const void* w, int dtype, int64_t M, int64_t N, 
 // linear_aux.cu
 // rows [R,C] -> [R,ld] of the same element size (the tail of a row is not written)
 int linear_pack(const void* src, int64_t elem, int64_t R, int64_t C, void* dst, int64_t ld, cudaStream_t st);
-// fp32 rows [R,C] -> three bf16 parts [3][R][ld] whose sum is the fp32 value,
-// for one or two arrays (R = 0: none) in one launch
+// fp32 rows [R,C] -> three bf16 parts [R][ld] whose sum is the fp32 value, and
+// a fourth plane: the first part, or 0 where the value is not finite; for one
+// or two arrays (R = 0: none) in one launch
+constexpr int SPLIT_PLANES = 4;
 struct SplitRows {
   const float* src;
   int64_t R, C;
@@ -60,8 +62,8 @@ struct SplitRows {
   int64_t ld;
 };
 int linear_split(const SplitRows& a, const SplitRows& b, cudaStream_t st);
-// dz = dout * act'(z): dz (null: not wanted) [R,ld] of `dtype`, or the three
-// bf16 parts of it when dtype is fp32; column sums into part [strips][C] fp32
+// dz = dout * act'(z): dz (null: not wanted) [R,ld] of `dtype`, or the four
+// bf16 planes of it when dtype is fp32; column sums into part [strips][C] fp32
 // (null: not wanted).  strips = linear_dz_strips(R, C).
 int64_t linear_dz_strips(int64_t R, int64_t C);
 int linear_dz(const void* dout, int dout_dtype, const void* z, int act, int dtype, int64_t R, int64_t C, void* dz,

@@ -29,8 +29,9 @@ int linear_pack(const void* src, int64_t elem, int64_t R, int64_t C, void* dst, 
 }
 
 // Three bf16 parts of an fp32 value: each takes the next 8 bits of the
-// mantissa, so their sum is the value (up to bf16's exponent range).
-__device__ __forceinline__ void split3(float v, __nv_bfloat16* o) {
+// mantissa, so their sum is the value (up to bf16's exponent range); o[3] is
+// the first of a finite value, else 0.
+__device__ __forceinline__ void split_value(float v, __nv_bfloat16* o) {
   o[0] = __float2bfloat16_rn(v);
   // the largest fp32 values would round up to infinity
   if (isfinite(v) && !isfinite(__bfloat162float(o[0]))) o[0] = __float2bfloat16_rz(v);
@@ -38,6 +39,7 @@ __device__ __forceinline__ void split3(float v, __nv_bfloat16* o) {
   const float r1 = isfinite(v) ? v - __bfloat162float(o[0]) : 0.f;
   o[1] = __float2bfloat16_rn(r1);
   o[2] = __float2bfloat16_rn(isfinite(r1) ? r1 - __bfloat162float(o[1]) : 0.f);
+  o[3] = isfinite(v) ? o[0] : __float2bfloat16_rn(0.f);
 }
 
 // A warp a row of either of two arrays; a lane takes two columns, so that the
@@ -50,11 +52,11 @@ __global__ void __launch_bounds__(256) split_rows_kernel(SplitRows a, SplitRows 
     __nv_bfloat16* d = (__nv_bfloat16*)w.dst + r * w.ld;
 #pragma unroll 4
     for (int64_t c = (threadIdx.x & 31) * 2; c < C; c += 64) {
-      __nv_bfloat16 p[3], q[3];
-      split3(s[c], p);
-      split3(c + 1 < C ? s[c + 1] : 0.f, q);
+      __nv_bfloat16 p[SPLIT_PLANES], q[SPLIT_PLANES];
+      split_value(s[c], p);
+      split_value(c + 1 < C ? s[c + 1] : 0.f, q);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<__nv_bfloat162*>(d + c + k * part) = __nv_bfloat162(p[k], q[k]);
+      for (int k = 0; k < SPLIT_PLANES; ++k) *reinterpret_cast<__nv_bfloat162*>(d + c + k * part) = __nv_bfloat162(p[k], q[k]);
     }
   }
 }
@@ -123,13 +125,18 @@ __global__ void __launch_bounds__(DZ_THREADS) dz_kernel(const TO* __restrict__ d
       if (dz) {
         if constexpr (SPLIT) {
           __nv_bfloat16* o = (__nv_bfloat16*)dz + r * ld + c;
+          union { __nv_bfloat16 v[VEC]; uint4 u; } plane[SPLIT_PLANES];
 #pragma unroll
           for (int k = 0; k < VEC; ++k) {
-            __nv_bfloat16 p[3];
-            split3(d[k], p);
-            o[k] = p[0];
-            o[k + R * ld] = p[1];
-            o[k + 2 * R * ld] = p[2];
+            __nv_bfloat16 p[SPLIT_PLANES];
+            split_value(d[k], p);
+#pragma unroll
+            for (int i = 0; i < SPLIT_PLANES; ++i) plane[i].v[k] = p[i];
+          }
+#pragma unroll
+          for (int i = 0; i < SPLIT_PLANES; ++i) {
+            if constexpr (VEC == 8) *reinterpret_cast<uint4*>(o + i * R * ld) = plane[i].u;
+            else o[i * R * ld] = plane[i].v[0];
           }
         } else {
           T* o = (T*)dz + r * ld + c;

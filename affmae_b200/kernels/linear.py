@@ -11,7 +11,8 @@
   ``LinearE4M3`` a layer that keeps its weight so.
 
 Sums are fp32.  Everything runs on the current stream; the gradients do not
-depend on timing.  In fp32 an infinite operand gives NaN.
+depend on timing.  In fp32, from 9 rows on, finite operands whose product is
+far beyond the type's range may give NaN in the place of an infinity.
 """
 from __future__ import annotations
 

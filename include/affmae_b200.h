@@ -371,7 +371,9 @@ int affb_cast_f32(const float* src, void* dst, int dtype, int64_t n, void* strea
  * bits more keep their rounding out of the gradients; past 65504 they are
  * infinite, where the gradient is constant.  N, K >= 1, M >= 0.  x and weight 16-byte aligned.
  * Sums are fp32; fp32 operands are multiplied as three bf16 parts each
- * (error of the order of 2^-24; an infinite operand gives NaN).
+ * (error of the order of 2^-24); infinities and NaNs give what fp32 products
+ * of them do, but finite operands whose product is far beyond fp32's range may
+ * give NaN in the place of an infinity.
  * workspace: affb_linear_fwd_workspace_bytes(...) bytes, 256-byte aligned, no
  * initial contents (NULL where that is 0).                                 */
 enum { AFFB_ACT_NONE = 0, AFFB_ACT_RELU = 1, AFFB_ACT_GELU = 2, AFFB_ACT_SILU = 3 };

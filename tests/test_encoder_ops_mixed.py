@@ -286,3 +286,43 @@ def test_status_waits_for_every_stream_and_reports_once(cuda):
     assert linear_status()
     with pytest.raises(RuntimeError, match="limit"):
         nat.call("affb_linear_wait_probe", 0, None)
+
+
+# ------------------------------------------------ infinities in fp32 -----
+
+def same_class(got, want, what):
+    """NaN where `want` (64 bits) is NaN, the same infinity where it is infinite, finite elsewhere."""
+    for f in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(f(got), f(want)), (what, f.__name__)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("shape", [(1, 24, 40), (8, 24, 40), (9, 24, 40), (9, 33, 200), (300, 200, 392), (3000, 24, 7)])
+@pytest.mark.parametrize("act", ["none", "relu"])
+def test_infinities_whatever_the_number_of_rows(cuda, dtype, shape, act):
+    """An infinite or NaN operand, gradient or weight gives what the definition gives, from one row to many; the
+    rest is as it is without them."""
+    M, N, K = shape
+    x, w, b = rnd(cuda, 1, M, K, dtype=dtype), rnd(cuda, 2, N, K, dtype=dtype), rnd(cuda, 3, N, dtype=dtype)
+    dout = rnd(cuda, 4, M, N, dtype=dtype)
+    w[1, 3], w[N - 1, 0] = 0, float("-inf")       # infinity times zero; a whole column of infinities
+    x[M // 2, 3] = float("inf")
+    x[M - 1, K - 1] = float("-inf") if M > 1 else x[M - 1, K - 1]
+    dout[0, 2] = float("inf")
+    if M > 2:
+        x[1, 0] = float("nan")
+        dout[M - 1, 0] = float("nan")
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    ref = [t.double().requires_grad_(True) for t in (x, w, b)]
+    y = fused_linear(*leaves, act=act)
+    z = ref[0] @ ref[1].T + ref[2]
+    yr = z.relu() if act == "relu" else z
+    same_class(y.detach(), yr.detach(), "y")
+    keep = yr.detach().isfinite()
+    tol = (U[dtype] * yr.abs() + (K + 18) * E * (torch.where(x.isfinite(), x, 0).double().abs()
+                                                  @ torch.where(w.isfinite(), w, 0).double().abs().T + 8)).detach()
+    within(torch.where(keep, y.detach(), 0), torch.where(keep, yr.detach(), 0), torch.where(keep, tol, 1))
+    if act == "none":
+        for n, p, q in zip("xwb", torch.autograd.grad(y, leaves, dout), torch.autograd.grad(yr, ref, dout.double())):
+            same_class(p, q, "d" + n)
