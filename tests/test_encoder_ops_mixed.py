@@ -326,3 +326,28 @@ def test_infinities_whatever_the_number_of_rows(cuda, dtype, shape, act):
     if act == "none":
         for n, p, q in zip("xwb", torch.autograd.grad(y, leaves, dout), torch.autograd.grad(yr, ref, dout.double())):
             same_class(p, q, "d" + n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("shape", [(700, 96), (64, 1000), (5, 8200), (2000, 2048), (33, 7)])
+def test_quantize_e4m3_is_its_definition(cuda, dtype, shape):
+    """Bit for bit: the row's maximum over 448 and the quotients, each rounded once to fp32, then to e4m3 (at most
+    448); rows from the smallest numbers of the type to the largest, zeros, and values on ties."""
+    R, C = shape
+    x = rnd(cuda, 2, R, C)
+    low, high = {BF16: (-133, 126), FP16: (-24, 14), FP32: (-149, 126)}[dtype]
+    x = x * torch.exp2(torch.linspace(low, high, R, device=cuda, dtype=torch.float64))[:, None].double()
+    x[R // 2] = 0
+    x[R // 2 + 1] = torch.randint(-896, 897, (C,), device=cuda) / 2     # whole and half steps of a scale of one
+    x[R // 2 + 1, 0] = 448
+    x = x.clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max).to(dtype)
+    assert x.isfinite().all()
+    q, scale = quantize_e4m3(x)
+    q, scale, x = q.cpu(), scale.cpu(), x.cpu()
+    top = x.float().abs().amax(1)
+    want = top / torch.full_like(top, 448)      # on the host, where both are IEEE divisions
+    want = torch.where(want == 0, 1.0, want)
+    assert torch.equal(scale, want)
+    quot = (x.float() / want[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+    assert torch.equal(q.view(torch.uint8), quot.view(torch.uint8))
