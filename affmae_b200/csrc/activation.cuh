@@ -112,10 +112,8 @@ __device__ __forceinline__ void activate_pair(float& x, float& y) {
 }
 
 template <int ACT>
-__device__ __forceinline__ float activate_grad(float z) {
-  if constexpr (ACT == AFFB_ACT_RELU) {
-    return z > 0.f ? 1.f : 0.f;
-  } else if constexpr (ACT == AFFB_ACT_GELU) {
+__device__ __forceinline__ float activate_grad(float z) {  // not of ReLU: see through_grad
+  if constexpr (ACT == AFFB_ACT_GELU) {
     const float a = min_nan(fabsf(z), 64.f);
     const float t = normal_tail(a);
     // Phi(z) + z phi(z)
@@ -128,6 +126,14 @@ __device__ __forceinline__ float activate_grad(float z) {
   } else {
     return 1.f;
   }
+}
+
+// The gradient d of act(z) as that of z.  ReLU selects: an infinite or NaN
+// gradient of a value it has cut off is no gradient.
+template <int ACT>
+__device__ __forceinline__ float through_grad(float d, float z) {
+  if constexpr (ACT == AFFB_ACT_RELU) return z <= 0.f ? 0.f : d;
+  return d * activate_grad<ACT>(z);
 }
 
 }  // namespace affb

@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(DZ_THREADS) dz_kernel(const TO* __restrict__ d
         float zz[VEC];
         ldn<TZ, VEC>(z + r * C + c, zz);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) d[k] *= activate_grad<ACT>(zz[k]);
+        for (int k = 0; k < VEC; ++k) d[k] = through_grad<ACT>(d[k], zz[k]);
       }
 #pragma unroll
       for (int k = 0; k < VEC; ++k) sum[k] += d[k];

@@ -351,3 +351,23 @@ def test_quantize_e4m3_is_its_definition(cuda, dtype, shape):
     assert torch.equal(scale, want)
     quot = (x.float() / want[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
     assert torch.equal(q.view(torch.uint8), quot.view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("shape", [(5, 24, 40), (300, 200, 64)])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_relu_cuts_off_gradients_that_are_not_finite(cuda, dtype, shape, with_residual):
+    """Where ReLU has cut a value off, an infinite or NaN gradient is none: the gradients are those of zeros there."""
+    M, N, K = shape
+    x, w, b = rnd(cuda, 1, M, K, dtype=dtype), rnd(cuda, 2, N, K, dtype=dtype), rnd(cuda, 3, N, dtype=dtype)
+    res = rnd(cuda, 4, M, N, dtype=dtype) if with_residual else None
+    dout = rnd(cuda, 5, M, N, dtype=dtype)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = fused_linear(*leaves, "relu", res)
+    off = fused_linear(x, w, b) <= 0
+    assert 0 < int(off.sum()) < off.numel()
+    bad = torch.where(torch.arange(N, device=cuda) % 2 == 0, float("nan"), float("-inf")).to(dtype).expand(M, N)
+    want = torch.autograd.grad(y, leaves, torch.where(off, 0, dout), retain_graph=True)
+    got = torch.autograd.grad(y, leaves, torch.where(off, bad, dout))
+    assert all(torch.equal(p, q) and p.isfinite().all() for p, q in zip(got, want))
