@@ -48,7 +48,11 @@ def bucket_count(edges, axes: int = 1, one_sided: bool = False) -> int:
 
 
 def _check_edges(edges) -> tuple[int, ...]:
-    return _checked(tuple(edges))
+    edges = tuple(edges)
+    for e in edges:
+        if type(e) is not int:  # a tensor, say, whose value may change while it stays the same key
+            return _checked.__wrapped__(edges)
+    return _checked(edges)
 
 
 @functools.lru_cache(maxsize=256)

@@ -371,3 +371,17 @@ def test_relu_cuts_off_gradients_that_are_not_finite(cuda, dtype, shape, with_re
     want = torch.autograd.grad(y, leaves, torch.where(off, 0, dout), retain_graph=True)
     got = torch.autograd.grad(y, leaves, torch.where(off, bad, dout))
     assert all(torch.equal(p, q) and p.isfinite().all() for p, q in zip(got, want))
+
+
+def test_edges_are_taken_by_value():
+    """Edges given as tensors or arrays are read at every call."""
+    from affmae_b200.kernels.bucket_bias import _check_edges
+    edges = [torch.tensor(1), torch.tensor(4)]
+    assert _check_edges(edges) == (1, 4) and _check_edges(torch.tensor([1, 4])) == (1, 4)
+    edges[1].fill_(6)
+    got = _check_edges(edges)
+    assert got == (1, 6) and all(type(e) is int for e in got)
+    edges[1].fill_(1)
+    with pytest.raises(RuntimeError, match="edges"):
+        _check_edges(edges)
+    assert _check_edges((1.0, 2.0)) == (1, 2) and _check_edges((1, 2)) == (1, 2)
