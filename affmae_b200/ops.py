@@ -225,9 +225,16 @@ def _linear_setup(ctx, inputs, output):
     code = _li._act_code(act)
     ctx.save_for_backward(x, weight, bias, z if _li.linear_saves(code, residual) or not code else out)
     ctx.act, ctx.residual = act, residual is not None
+    ctx.set_materialize_grads(False)
+
+
+def _refuse_gradient(grad, name):
+    if grad is not None:
+        raise RuntimeError(f"{name} is kept for the backward and has no gradient of its own")
 
 
 def _linear_backward(ctx, grad_out, grad_z):
+    _refuse_gradient(grad_z, "affb200::linear_fwd: z")
     x, weight, bias, z = ctx.saved_tensors
     dx, dw, db = linear_bwd(grad_out.contiguous(), z, x, weight, bias, ctx.act)
     return dx, dw, _none_if_empty(db), None, grad_out if ctx.residual else None
@@ -292,6 +299,7 @@ def _rms_setup(ctx, inputs, output):
 
 
 def _rms_backward(ctx, grad_s, grad_y, grad_rstd):
+    _refuse_gradient(grad_rstd, "affb200::rms_norm_fwd: rstd")
     s, rstd, weight, row_scale, delta = ctx.saved_tensors
     dx, dw, dd = rms_norm_bwd(grad_y, grad_s if delta is not None else None, s, rstd, weight, row_scale, delta)
     return dx, dw, None, _none_if_empty(dd), None, None

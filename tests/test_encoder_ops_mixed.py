@@ -385,3 +385,20 @@ def test_edges_are_taken_by_value():
     with pytest.raises(RuntimeError, match="edges"):
         _check_edges(edges)
     assert _check_edges((1.0, 2.0)) == (1, 2) and _check_edges((1, 2)) == (1, 2)
+
+
+@pytest.mark.gpu
+def test_dispatcher_refuses_gradients_of_what_is_kept(cuda):
+    """The sums and reciprocal roots that the dispatcher's operators return for the backward have no gradient, and say
+    so when one is asked for."""
+    import affmae_b200.ops  # noqa: F401
+    ops = torch.ops.affb200
+    x, w, ones = rnd(cuda, 1, 40, 24).requires_grad_(True), rnd(cuda, 2, 16, 24), torch.ones(24, device=cuda)
+    out, z = ops.linear_fwd(x, w, None, "gelu", None)
+    s, y, rstd = ops.rms_norm_fwd(x, ones, 1e-6, x.detach(), None, FP32)
+    for t in (z, out + z, rstd, y.sum(1) + rstd):
+        with pytest.raises(RuntimeError, match="no gradient of its own"):
+            t.sum().backward(retain_graph=True)
+    assert x.grad is None
+    (out.sum() + s.sum() + y.sum()).backward()
+    assert x.grad.isfinite().all() and x.grad.any()
