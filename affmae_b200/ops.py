@@ -186,45 +186,48 @@ deform_cross_fwd.register_autograd(_deform_backward, setup_context=_deform_setup
 
 # --------------------------------------------------------- matrix product --
 @custom_op("affb200::linear_fwd", mutates_args=())
-def linear_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, residual: Optional[Tensor]
-               ) -> tuple[Tensor, Tensor]:
-    """(out, z): z holds the pre-activation sums, empty where the backward needs none."""
+def linear_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, residual: Optional[Tensor],
+               save: bool = True) -> tuple[Tensor, Tensor]:
+    """(out, z): z holds the pre-activation sums, empty where the backward needs none, or without `save`
+    (inference), which saves their writing."""
     code = _li._act_code(act)
     _li._check_operands(x, weight, bias, residual)
     _nat.refuse_tangents("affb200::linear_fwd", x, weight, bias, residual)
-    out, z = _li.linear_fwd(_nat.dense(x), _nat.dense(weight), bias, residual, code, True)
+    out, z = _li.linear_fwd(_nat.dense(x), _nat.dense(weight), bias, residual, code, save)
     return out, (z if z is not None else x.new_empty(_EMPTY))
 
 
 @linear_fwd.register_fake
-def _(x, weight, bias, act, residual):
+def _(x, weight, bias, act, residual, save=True):
     shape = (*x.shape[:-1], weight.shape[0])
-    saves = _li.linear_saves(_li._act_code(act), residual)
+    saves = save and _li.linear_saves(_li._act_code(act), residual)
     return (x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype),
             x.new_empty(shape if saves else _EMPTY,
                         dtype=_li.z_dtype(x.dtype, _li._act_code(act)) if saves else x.dtype))
 
 
 @custom_op("affb200::linear_bwd", mutates_args=())
-def linear_bwd(dout: Tensor, z: Tensor, x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str
-               ) -> tuple[Tensor, Tensor, Tensor]:
+def linear_bwd(dout: Tensor, z: Tensor, x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str,
+               need_x: bool = True, need_w: bool = True) -> tuple[Tensor, Tensor, Tensor]:
+    """(dx, dweight, dbias), empty where not needed (dbias: without `bias`)."""
     dx, dw, db = _li.linear_bwd(_nat.dense(dout), _none_if_empty(z), _nat.dense(x), _nat.dense(weight),
-                                _li._act_code(act), True, True, bias.dtype if bias is not None else None)
-    return dx, dw, (db if db is not None else x.new_empty(_EMPTY))
+                                _li._act_code(act), need_x, need_w, bias.dtype if bias is not None else None)
+    return tuple(t if t is not None else x.new_empty(_EMPTY) for t in (dx, dw, db))
 
 
 @linear_bwd.register_fake
-def _(dout, z, x, weight, bias, act):
-    return (x.new_empty(x.shape), weight.new_empty(weight.shape),
+def _(dout, z, x, weight, bias, act, need_x=True, need_w=True):
+    return (x.new_empty(x.shape if need_x else _EMPTY), weight.new_empty(weight.shape if need_w else _EMPTY),
             bias.new_empty(bias.shape) if bias is not None else x.new_empty(_EMPTY))
 
 
 def _linear_setup(ctx, inputs, output):
-    x, weight, bias, act, residual = inputs
+    x, weight, bias, act, residual, save = inputs
     out, z = output
     code = _li._act_code(act)
     ctx.save_for_backward(x, weight, bias, z if _li.linear_saves(code, residual) or not code else out)
     ctx.act, ctx.residual = act, residual is not None
+    ctx.lacks_sums = not save and _li.linear_saves(code, residual)
     ctx.set_materialize_grads(False)
 
 
@@ -235,9 +238,15 @@ def _refuse_gradient(grad, name):
 
 def _linear_backward(ctx, grad_out, grad_z):
     _refuse_gradient(grad_z, "affb200::linear_fwd: z")
-    x, weight, bias, z = ctx.saved_tensors
-    dx, dw, db = linear_bwd(grad_out.contiguous(), z, x, weight, bias, ctx.act)
-    return dx, dw, _none_if_empty(db), None, grad_out if ctx.residual else None
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    dx = dw = db = None
+    if need_x or need_w or need_b:
+        if ctx.lacks_sums:
+            raise RuntimeError("affb200::linear_fwd: called without save, it has no gradient")
+        x, weight, bias, z = ctx.saved_tensors
+        got = linear_bwd(grad_out.contiguous(), z, x, weight, bias if need_b else None, ctx.act, need_x, need_w)
+        dx, dw, db = (t if need else None for t, need in zip(got, (need_x, need_w, need_b)))
+    return dx, dw, db, None, grad_out if ctx.residual else None, None
 
 
 linear_fwd.register_autograd(_linear_backward, setup_context=_linear_setup)
@@ -274,21 +283,25 @@ def _(x, weight, eps, delta, row_scale, out_dtype):
 
 @custom_op("affb200::rms_norm_bwd", mutates_args=())
 def rms_norm_bwd(dy: Optional[Tensor], ds: Optional[Tensor], s: Tensor, rstd: Tensor, weight: Tensor,
-                 row_scale: Optional[Tensor], delta: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
-    """s: the forward's sum in fp32; x itself in 16 bits or without delta."""
+                 row_scale: Optional[Tensor], delta: Optional[Tensor], need_x: bool = True, need_w: bool = True,
+                 need_delta: bool = True) -> tuple[Tensor, Tensor, Tensor]:
+    """(dx, dweight, ddelta), empty where not needed.  s: the forward's sum in fp32; x itself in 16 bits or without
+    delta."""
     dx, dw, dd = _rn.rms_norm_bwd(_nat.dense(dy) if dy is not None else None,
                                   _nat.dense(ds) if ds is not None else None, _nat.dense(s), rstd,
                                   _nat.dense(weight.float()),
-                                  row_scale.float().contiguous() if row_scale is not None else None, True, True,
-                                  delta.dtype if delta is not None else None,
+                                  row_scale.float().contiguous() if row_scale is not None else None, need_x, need_w,
+                                  delta.dtype if delta is not None and need_delta else None,
                                   _nat.dense(delta) if delta is not None and s.dtype != torch.float32 else None)
-    return dx, dw.to(weight.dtype), (dd if dd is not None else s.new_empty(_EMPTY))
+    return (dx if dx is not None else s.new_empty(_EMPTY),
+            dw.to(weight.dtype) if dw is not None else weight.new_empty(_EMPTY),
+            dd if dd is not None else s.new_empty(_EMPTY, dtype=delta.dtype if delta is not None else s.dtype))
 
 
 @rms_norm_bwd.register_fake
-def _(dy, ds, s, rstd, weight, row_scale, delta):
-    return s.new_empty(s.shape), weight.new_empty(weight.shape), \
-        (delta.new_empty(delta.shape) if delta is not None else s.new_empty(_EMPTY))
+def _(dy, ds, s, rstd, weight, row_scale, delta, need_x=True, need_w=True, need_delta=True):
+    return s.new_empty(s.shape if need_x else _EMPTY), weight.new_empty(weight.shape if need_w else _EMPTY), \
+        (delta.new_empty(delta.shape if need_delta else _EMPTY) if delta is not None else s.new_empty(_EMPTY))
 
 
 def _rms_setup(ctx, inputs, output):
@@ -301,8 +314,11 @@ def _rms_setup(ctx, inputs, output):
 def _rms_backward(ctx, grad_s, grad_y, grad_rstd):
     _refuse_gradient(grad_rstd, "affb200::rms_norm_fwd: rstd")
     s, rstd, weight, row_scale, delta = ctx.saved_tensors
-    dx, dw, dd = rms_norm_bwd(grad_y, grad_s if delta is not None else None, s, rstd, weight, row_scale, delta)
-    return dx, dw, None, _none_if_empty(dd), None, None
+    need_x, need_w, _, need_d = ctx.needs_input_grad[:4]
+    got = rms_norm_bwd(grad_y, grad_s if delta is not None else None, s, rstd, weight, row_scale, delta, need_x, need_w,
+                       need_d)
+    dx, dw, dd = (t if need else None for t, need in zip(got, (need_x, need_w, need_d)))
+    return dx, dw, None, dd, None, None
 
 
 rms_norm_fwd.register_autograd(_rms_backward, setup_context=_rms_setup)

@@ -402,3 +402,35 @@ def test_dispatcher_refuses_gradients_of_what_is_kept(cuda):
     assert x.grad is None
     (out.sum() + s.sum() + y.sum()).backward()
     assert x.grad.isfinite().all() and x.grad.any()
+
+
+@pytest.mark.gpu
+def test_dispatcher_computes_what_is_wanted(cuda):
+    """Gradients that nothing asks for come back empty from the backward operators, and the others are the same; the
+    forward writes no sums without `save`, and then has no gradient."""
+    import affmae_b200.ops  # noqa: F401
+    ops = torch.ops.affb200
+    x, w, b, ones = rnd(cuda, 1, 40, 24), rnd(cuda, 2, 16, 24), rnd(cuda, 3, 16), rnd(cuda, 4, 24)
+    dout, ds, d = rnd(cuda, 5, 40, 16), rnd(cuda, 6, 40, 24), rnd(cuda, 7, 40, 24)
+    out, z = ops.linear_fwd(x, w, b, "gelu", None)
+    bare, none = ops.linear_fwd(x, w, b, "gelu", None, False)
+    assert torch.equal(out, bare) and none.numel() == 0 and z.shape == out.shape
+    full = ops.linear_bwd(dout, z, x, w, b, "gelu")
+    s, y, rstd = ops.rms_norm_fwd(x, ones, 1e-6, d, None, FP32)
+    norm = ops.rms_norm_bwd(ds, ds, s, rstd, ones, None, d)
+    for i in range(3):
+        need = [i == j for j in range(3)]
+        got = ops.linear_bwd(dout, z, x, w, b if need[2] else None, "gelu", need[0], need[1])
+        assert torch.equal(got[i], full[i]) and sum(t.numel() for t in got) == full[i].numel()
+        got = ops.rms_norm_bwd(ds, ds, s, rstd, ones, None, d, *need)
+        assert torch.equal(got[i], norm[i]) and sum(t.numel() for t in got) == norm[i].numel()
+        leaves = [t.clone().requires_grad_(n) for t, n in zip((x, w, b), need)]
+        assert torch.equal(torch.autograd.grad(ops.linear_fwd(*leaves, "gelu", None)[0], leaves[i], dout)[0], full[i])
+        leaves = [t.clone().requires_grad_(n) for t, n in zip((x, ones, d), need)]
+        got = ops.rms_norm_fwd(leaves[0], leaves[1], 1e-6, leaves[2], None, FP32)
+        assert torch.equal(torch.autograd.grad((got[0], got[1]), leaves[i], (ds, ds))[0], norm[i])
+    leaf = x.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="without save"):
+        ops.linear_fwd(leaf, w, b, "gelu", None, False)[0].sum().backward()
+    ops.linear_fwd(leaf, w, b, "relu", None, False)[0].sum().backward()   # ReLU's output serves
+    assert leaf.grad.any()
