@@ -590,10 +590,12 @@ struct Shape {
 //
 // Pairs of blocks (256-row tiles up to 256 columns wide) where there are
 // enough tiles, or enough k blocks to split, for all of them, and a tile's
-// contraction is long enough to be worth the pair's handshakes (524288 x 96 ->
-// 192, two k blocks: 87 us by pairs, 57 by single blocks; 524288 x 384 -> 768,
-// six: 292 against 329; 8192 x 4096 -> 8192 e4m3, 32: 190 against 215); else
-// single blocks.
+// contraction is long enough to be worth the pair's handshakes; else single
+// blocks.  524288 rows of bf16 to 192, 384 and 768 columns, us by pairs against
+// single blocks: two k blocks 105, 180, 257 (74, 116, 173); three 119, 203, 293
+// (90, 146, 224); four 125, 212, 296 (100, 169, 257); five 131, 219, 291 (121,
+// 199, 311); six 123, 205, 305 (122, 207, 334); eight 133, 217, 364 (152, 263,
+// 405); e4m3 8192 x 4096 -> 8192, 32 blocks: 190 (215).
 // Tiles that leave SMs idle are split along the contraction, at least 4 k
 // blocks a part.  The width is the one that costs least, a k block of a tile
 // taken as its columns and 64 more for what does not depend on them, and a

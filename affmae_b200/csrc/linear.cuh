@@ -38,12 +38,18 @@ struct LinearEpilogue {
 };
 
 // linear_small.cu: out = epilogue(x w^T) for few rows (at most 8), one launch.
-// Against the tensor-core product, with w [8192,4096]: bf16 2 rows 14.6 us (17),
-// 3 rows 18.4 (17); e4m3 2 rows 11.5 (16.6), 4 rows 17.5 (16.6); with w
-// [4096,1024]: bf16 4 rows 7.0 (8.3), fp32 (six products of parts) 8 rows 15 (28).
+// Against the tensor-core product (in brackets; us, weights out of DRAM), bf16:
+// w [512,1024] 1 row 2.3 (7.3), 4 rows 6.6 (7.5); [4096,1024] 2 rows 6.7 (8.9),
+// 4 rows 8.6 (8.9); [4096,4096] 1 row 11.5 (14.6), 2 rows 19.8 (14.8), 4 rows
+// 28 (15); [16384,8192] 1 row 49 (64), 2 rows 90 (65).  e4m3: [4096,1024]
+// 4 rows 6.5 (6.9); [4096,4096] 1 row 7.7 (12), 2 rows 13.4 (12); [8192,4096]
+// 2 rows 14.9 (18.4), 4 rows 21.8 (18.1); [16384,8192] 1 row 29 (35), 2 rows 57
+// (35).  fp32, whose operands are split for six products: 8 rows 17 (22), 19
+// (30), 69 (97), 467 (605) with the same weights as bf16, 1 row 3.9 (22) to 85
+// (675).
 inline bool few_rows(int dtype, int64_t M, int64_t N, int64_t K) {
   if (dtype == AFFB_F32) return M <= 8;
-  return M <= 2 || (M <= 4 && M * N * K <= (64ll << 20));
+  return M == 1 || (M <= 4 && M * N * K <= (16ll << 20));
 }
 int linear_small(const void* x, const void* w, int dtype, int64_t M, int64_t N, int64_t K, const LinearEpilogue& e,
                  cudaStream_t st);

@@ -13,7 +13,7 @@ from affmae_b200 import _native as nat
 from affmae_b200.kernels.bucket_bias import bucket_bias, bucket_count, log_edges
 from affmae_b200.kernels.linear import LinearE4M3, fused_linear, linear_e4m3, linear_status, quantize_e4m3
 from affmae_b200.kernels.rms_norm import fused_rms_norm, rms_norm_e4m3
-from test_encoder_ops import BF16, E, FP16, FP32, TINY, U, bias_inputs, check_e4m3, rnd, rows_ref, within
+from test_encoder_ops import BF16, E, FP16, FP32, TINY, U, bias_inputs, check_e4m3, linear_ref, rnd, rows_ref, within
 
 
 @pytest.mark.gpu
@@ -434,3 +434,19 @@ def test_dispatcher_computes_what_is_wanted(cuda):
         ops.linear_fwd(leaf, w, b, "gelu", None, False)[0].sum().backward()
     ops.linear_fwd(leaf, w, b, "relu", None, False)[0].sum().backward()   # ReLU's output serves
     assert leaf.grad.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("N,K", [(4096, 1024), (4096, 1040), (2048, 4096), (1200, 4100)])
+def test_few_rows_on_both_sides_of_the_rule(cuda, M, N, K):
+    """Around the size from which two to four rows go to the tensor cores, 16-bit and e4m3 operands."""
+    x, w, b = rnd(cuda, 1, M, K, dtype=BF16), rnd(cuda, 2, N, K, std=K ** -0.5, dtype=BF16), rnd(cuda, 3, N, dtype=BF16)
+    out, tol = linear_ref(x, w, b, "gelu", None)
+    within(fused_linear(x, w, b, "gelu"), out, tol)
+    q, s = quantize_e4m3(x)
+    wq, ws = quantize_e4m3(w)
+    xd, wd = q.double() * s.double()[:, None], wq.double() * ws.double()[:, None]
+    z = xd @ wd.T + b.double()
+    zerr = (K + 16) * E * (xd.abs() @ wd.abs().T) + 4 * E * (z.abs() + b.double().abs())
+    within(linear_e4m3(q, s, wq, ws, b, out_dtype=FP32), z, zerr + E * z.abs())
