@@ -3,6 +3,8 @@ from one another: rows of other sizes in turn, gradients of mixed magnitude,
 infinities, forward-mode derivatives, several threads.  Bounds as in
 test_encoder_ops.py."""
 import ctypes
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -13,6 +15,7 @@ from affmae_b200 import _native as nat
 from affmae_b200.kernels.bucket_bias import bucket_bias, bucket_count, log_edges
 from affmae_b200.kernels.linear import LinearE4M3, fused_linear, linear_e4m3, linear_status, quantize_e4m3
 from affmae_b200.kernels.rms_norm import fused_rms_norm, rms_norm_e4m3
+from conftest import ROOT
 from test_encoder_ops import BF16, E, FP16, FP32, TINY, U, bias_inputs, check_e4m3, linear_ref, rnd, rows_ref, within
 
 
@@ -450,3 +453,44 @@ def test_few_rows_on_both_sides_of_the_rule(cuda, M, N, K):
     z = xd @ wd.T + b.double()
     zerr = (K + 16) * E * (xd.abs() @ wd.abs().T) + 4 * E * (z.abs() + b.double().abs())
     within(linear_e4m3(q, s, wq, ws, b, out_dtype=FP32), z, zerr + E * z.abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_bucket_bias_gradient_of_the_largest_table(cuda, dtype):
+    """65 x 65 rows beside the widest table of offsets: a block's whole shared memory."""
+    n, m, edges = 100000, 64, tuple(range(1, 32)) + (44,)
+    g = torch.Generator().manual_seed(5)
+    qp, kp = (torch.randint(0, 100, (1, k, 2), generator=g).float().to(cuda) for k in (n, 4096))
+    member = torch.randint(0, 4096, (1, n, m), generator=g).to(cuda, torch.int32)
+    table = torch.zeros((65 * 65, 2), device=cuda, dtype=dtype, requires_grad=True)
+    dout = rnd(cuda, 6, 1, 2, n, m, dtype=dtype)
+    bias = bucket_bias(table, edges, qp, kp, member)
+    (dt,) = torch.autograd.grad(bias, (table,), dout)
+    row = rows_ref(edges, qp, kp, member, False).reshape(-1)
+    gd = dout.double().permute(0, 2, 3, 1).reshape(-1, 2)
+    ref = torch.zeros((65 * 65, 2), dtype=torch.float64, device=cuda).index_add_(0, row, gd)
+    mag = torch.zeros_like(ref).index_add_(0, row, gd.abs())
+    # a block of an SM sums at most 16 tiles' sums, of two or three parts each; then 32 of up to 24 blocks' sums
+    within(dt, ref, 128 * E * mag + U[dtype] * ref.abs())
+
+
+@pytest.mark.gpu
+def test_a_captured_graph_may_hold_the_first_call(cuda):
+    """The first product and norm of a process may be those that a graph captures."""
+    code = """
+import torch
+from affmae_b200.kernels.linear import fused_linear, linear_status
+from affmae_b200.kernels.rms_norm import fused_rms_norm
+x, w = torch.randn(300, 64, device="cuda"), torch.randn(32, 64, device="cuda")
+ones = torch.ones(64, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.no_grad(), torch.cuda.graph(g):
+    y = fused_linear(fused_rms_norm(x, ones), w, act="gelu")
+g.replay()
+assert torch.equal(y, fused_linear(fused_rms_norm(x, ones), w, act="gelu")) and linear_status()
+print("captured")
+"""
+    got = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and "captured" in got.stdout, got.stderr[-2000:]
