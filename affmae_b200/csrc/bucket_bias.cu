@@ -37,7 +37,7 @@ constexpr int BB_STEPS = 4;          // steps of BB_THREADS * PAIRS pairs in a t
 constexpr int BB_HEADS = 4;          // heads side by side in shared memory; heads of one backward block
 constexpr int BB_MAX_EDGES = 64;
 constexpr int BB_LUT = 8192;         // distances answered by a byte table, else the edges are searched
-constexpr int BB_BITS = 19;          // 2^19 * 2048 terms stay below 2^31
+constexpr int BB_BITS = 19;          // of a rounded term: 2^19 * 2048 terms stay below 2^31
 // Blocks of the backward on an SM.  With 16-bit gradients the fifth costs a
 // few spilled registers and hides more of the lists' latency; fp32 ones take
 // twice the registers (stage 1: bf16 186 us with four, 178 with five; fp32

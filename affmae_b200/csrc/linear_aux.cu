@@ -93,7 +93,10 @@ __device__ __forceinline__ void ldn(const T* p, float* o) {
 
 // Block: DZ_COLS columns x one strip of rows.  A thread keeps VEC columns and
 // walks down the strip; the threads of a column group are summed in order, so
-// the sums do not depend on timing.  Bound by HBM, and by what is on the way:
+// the sums do not depend on timing (and are of the unrounded gradients).  dz is
+// rounded to the operands' type, since the products take operands of one type
+// (error of the gradients at 96 -> 192 bf16 GELU 2.3e-3 of their norm, 1.7e-3
+// from their own rounding alone).  Bound by HBM, and by what is on the way:
 // six blocks an SM, for which the strips are counted (131072 x 768 bf16 ReLU:
 // 92 us, 117 with the five that two registers more leave).
 template <typename TO, typename T, typename TZ, int ACT, int VEC>

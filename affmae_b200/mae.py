@@ -73,7 +73,7 @@ class MAEConfig:
     decoder_dropout: float = 0.1
     loss_weights: tuple = field(default=(0.05, 0.12, 1.0))  # res5, res4, res2 heads
     # encoder blocks: "layer" (the reference's) or "rms" (root-mean-square
-    # norms, fused matrix products, bucketed position bias)
+    # norms, fused matrix products, bucketed position bias; needs a GPU)
     block: str = "layer"
     bias_edges: tuple = (1, 2, 3, 4, 7, 13, 24)             # distances in tokens where a bias bucket begins
 

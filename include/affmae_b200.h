@@ -447,7 +447,8 @@ int affb_bucket_bias_fwd(const void* table, int table_dtype, const int32_t* edge
                          const void* q_pos, const void* k_pos, int pos_type, int axes, const int32_t* member_idx,
                          int64_t B, int64_t H, int64_t Nq, int64_t Nk, int64_t M, void* out, int out_dtype,
                          void* stream);
-/* dtable [n^axes, H] table_dtype (written).  Deterministic.                 */
+/* dtable [n^axes, H] table_dtype (written).  Deterministic; a row's sum is off
+ * by fp32 additions of its own terms, whatever the gradients of other rows.  */
 int64_t affb_bucket_bias_bwd_workspace_bytes(int n_edges, int one_sided, int axes, int64_t B, int64_t H, int64_t Nq,
                                              int64_t M);
 int affb_bucket_bias_bwd(const void* dout, int dout_dtype, const int32_t* edges, int n_edges, int one_sided,
