@@ -220,14 +220,11 @@ def differentiates(*tensors) -> bool:
     for a gradient, or a forward-mode level is open (whose tangents do not;
     an autograd.Function without a jvp refuses them, where a plain call would
     drop them)."""
-    if getattr(_forward_ad, "_current_level", 0) >= 0:
-        return True
-    if not torch.is_grad_enabled():
-        return False
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            return True
-    return False
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return getattr(_forward_ad, "_current_level", 0) >= 0
 
 
 class _ForwardOnly(torch.autograd.Function):
@@ -243,9 +240,10 @@ class _ForwardOnly(torch.autograd.Function):
 
 
 def forward_only(name: str, run, *tensors):
-    """``run()``; where autograd has to see the call, its outputs refuse a
-    gradient when one is asked of them, instead of passing for constants."""
-    return _ForwardOnly.apply(name, run, *tensors) if differentiates(*tensors) else run()
+    """``run()`` for a call that autograd has to see (``differentiates``): its
+    outputs refuse a gradient when one is asked of them, instead of passing for
+    constants."""
+    return _ForwardOnly.apply(name, run, *tensors)
 
 
 def refuse_tangents(name: str, *tensors) -> None:

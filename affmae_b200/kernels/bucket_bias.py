@@ -49,9 +49,8 @@ def bucket_count(edges, axes: int = 1, one_sided: bool = False) -> int:
 
 def _check_edges(edges) -> tuple[int, ...]:
     edges = tuple(edges)
-    for e in edges:
-        if type(e) is not int:  # a tensor, say, whose value may change while it stays the same key
-            return _checked.__wrapped__(edges)
+    if set(map(type, edges)) != {int}:  # tensors, say, whose values may change while they stay the same keys
+        return _checked.__wrapped__(edges)
     return _checked(edges)
 
 

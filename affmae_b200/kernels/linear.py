@@ -197,7 +197,9 @@ def quantize_e4m3(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     nat.require_cuda(x)
     if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in _FLOATS:
         raise RuntimeError("quantize_e4m3: needs fp32, fp16 or bf16 rows of at least one value")
-    return nat.forward_only("quantize_e4m3", lambda: _quantize(x), x)
+    if nat.differentiates(x):
+        return nat.forward_only("quantize_e4m3", lambda: _quantize(x), x)
+    return _quantize(x)
 
 
 def _quantize(x):

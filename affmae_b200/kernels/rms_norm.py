@@ -153,11 +153,14 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, delt
     row (1 for a zero row).  A gradient through it, that of s included, is
     refused."""
     _check(x, weight, delta, row_scale)
+    if nat.differentiates(x, weight, delta):
+        return nat.forward_only("rms_norm_e4m3", lambda: _rms_e4m3(x, weight, eps, delta, row_scale), x, weight, delta)
+    return _rms_e4m3(x, weight, eps, delta, row_scale)
 
-    def run():
-        _, _, _, s, _, _, q, scale = _launch(x, delta, row_scale, weight, eps, None, False)
-        return (q, scale) if delta is None else (s, q, scale)
-    return nat.forward_only("rms_norm_e4m3", run, x, weight, delta)
+
+def _rms_e4m3(x, weight, eps, delta, row_scale):
+    _, _, _, s, _, _, q, scale = _launch(x, delta, row_scale, weight, eps, None, False)
+    return (q, scale) if delta is None else (s, q, scale)
 
 
 class FusedRMSNorm(nn.Module):
